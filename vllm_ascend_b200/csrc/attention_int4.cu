@@ -1,0 +1,520 @@
+// Attention of few query rows over a 4-bit paged cache (format: kv_int4.cuh): decode, drafts to verify, any batch whose
+// sequences have few new tokens.
+//
+//   o_r = sum_j p_rj v_j / sum_j p_rj,   p_rj = exp(scale q_r k_j - m_r),   m_r the running maximum
+//
+// Bound: memory, 9/8 D bytes a stored token and head, and close behind it the instructions that unpack (three for two channels).
+// So nothing is unpacked to shared memory: a warp unpacks into the very registers that the tensor cores read, and both products have
+// the stored side as the rows of A, which takes 16 of them for 8 query rows:
+//   S^T = K Q^T     16 tokens x 8 rows, over D.  A lane holds 32 (D = 64: 16) adjacent channels of two tokens; the order of the
+//                   sum is free, so the query fragments follow what unpacking yields (channels j and j + 4 of eight)
+//   O^T = V^T P^T   D channels x 8 rows, over tokens.  A lane holds 16 (8) adjacent channels of four tokens; S^T's results
+//                   become P^T's fragments by transposing 8 x 8 blocks between the lanes
+// A block is one (sequence, KV head, part of the sequence); each of its warps walks tiles of TS tokens, one in W, through a
+// ring of its own that bulk copies fill (one per 16 tokens), with a running maximum of its own; they join at the end.  Parts join in
+// a second kernel.
+#include "kv_int4.cuh"
+
+namespace b200 {
+
+constexpr int D4_WARPS = 4;
+
+struct Int4Params {
+  const __nv_bfloat16* q;
+  const uint8_t *k_cache, *v_cache;
+  const int *cu, *seq_lens, *block_table;
+  __nv_bfloat16* out;
+  float *part_o, *part_lse;       // [tokens x heads][parts][D], [..][parts]: results of parts, normalised, with log2 of their sums
+  long q_stride, out_stride, num_blocks;
+  int num_seqs, max_blocks, block_size, G, Hkv, parts, row_blocks, causal, window;
+  float scale_log2;
+  int* status;
+};
+
+__device__ __forceinline__ float i4_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void i4_mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t i4_transpose(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void i4_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int D, int NT>
+struct Int4Cfg {
+  static constexpr int TS = 32;                          // tokens of a tile
+  static constexpr int UNITS = TS / KV4_TOKENS;
+  static constexpr int UNIT = kv4_unit_bytes(D);
+  static constexpr int STAGE = 2 * UNITS * UNIT;         // keys, then values
+  static constexpr int STAGES = D == 128 ? 3 : 6;
+  static constexpr int RING = STAGES * STAGE;
+  static constexpr int ROWS = 8 * NT;
+  static constexpr int SMEM = D4_WARPS * RING + 1024;    // barriers, maxima and sums behind the rings
+  static_assert(ROWS * D * 4 <= RING, "a warp's result takes its ring's place");
+  static_assert(D4_WARPS * (STAGES * 8 + ROWS * 8) + 16 <= 1024, "");
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(32 * D4_WARPS, NT == 1 ? 4 : 3) attn_int4_kernel(const Int4Params p) {
+  using Cfg = Int4Cfg<D, NT>;
+  constexpr int KW = D / 32;                    // words of a token's keys in a lane
+  constexpr int VW = D / 64;                    // words of a token's values in a lane
+  constexpr int MT = D / 16;                    // channel tiles of the result
+  constexpr int U = Cfg::UNITS, ROWS = Cfg::ROWS, TS = Cfg::TS;
+  extern __shared__ __align__(128) uint8_t i4_smem[];
+  const int warp = warp_index(), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  uint8_t* ring = i4_smem + warp * Cfg::RING;
+  uint64_t* bars = (uint64_t*)(i4_smem + D4_WARPS * Cfg::RING) + warp * Cfg::STAGES;
+  float* ms = (float*)(i4_smem + D4_WARPS * (Cfg::RING + Cfg::STAGES * 8));        // [warps][rows], sums behind
+  float* ls = ms + D4_WARPS * ROWS;
+  volatile int* abort_word = (volatile int*)(ls + D4_WARPS * ROWS);
+
+  const int seq = blockIdx.x / p.row_blocks, row0 = (blockIdx.x - seq * p.row_blocks) * ROWS, h = blockIdx.y, part = blockIdx.z;
+  const int q_start = p.cu[seq], q_len = p.cu[seq + 1] - q_start, len = p.seq_lens[seq], ctx = len - q_len;
+  const int rows = min(q_len * p.G - row0, ROWS);
+  if (rows <= 0) return;
+  if (lane == 0)
+    for (int s = 0; s < Cfg::STAGES; s++) mbar_init(&bars[s], 1);
+  if (threadIdx.x == 0) *abort_word = 0;
+  mbar_fence_init();
+  __syncthreads();
+
+  // keys that any row of the block sees, and those that all rows see
+  const int tok_first = row0 / p.G, tok_last = (row0 + rows - 1) / p.G;
+  const int hi = max(0, p.causal ? min(len, ctx + tok_last + 1) : len), all_hi = p.causal ? min(len, ctx + tok_first + 1) : len;
+  const int lo = p.window > 0 ? max(0, ctx + tok_first - p.window + 1) : 0, all_lo = p.window > 0 ? max(0, ctx + tok_last - p.window + 1) : 0;
+  const int t_lo = lo / TS, tiles = max(0, (hi + TS - 1) / TS - t_lo);
+  const int first = t_lo + (int)((long)tiles * part / p.parts), last = t_lo + (int)((long)tiles * (part + 1) / p.parts);
+
+  const int upp = p.block_size / KV4_TOKENS;
+  const int* bt = p.block_table + (long)seq * p.max_blocks;
+  const int lu = lane % U, lkv = lane / U;                     // lanes below 2 U copy: unit, keys or values
+  auto page_of = [&](int tile) -> int {
+    const int t = tile * TS + lu * KV4_TOKENS;
+    if (lkv >= 2 || tile >= last || t >= hi) return 0;
+    const int col = t / p.block_size;
+    return col < p.max_blocks ? bt[col] : -1;
+  };
+  bool bad = false;
+  auto issue = [&](int tile, int stage, int blk) {
+    const int n = min(U, (hi - tile * TS + KV4_TOKENS - 1) / KV4_TOKENS);
+    const bool mine = lkv < 2 && lu < n;
+    if (__any_sync(0xffffffffu, mine && (blk < 0 || blk >= p.num_blocks))) {
+      bad = true;
+      return;
+    }
+    if (lane == 0) mbar_expect_tx(&bars[stage], 2 * n * Cfg::UNIT);
+    __syncwarp();
+    if (mine) {
+      const int unit = (tile * U + lu) % upp;
+      const uint8_t* src = (lkv ? p.v_cache : p.k_cache) + (((long)blk * p.Hkv + h) * upp + unit) * Cfg::UNIT;
+      i4_bulk_load(ring + stage * Cfg::STAGE + (lkv * U + lu) * Cfg::UNIT, src, Cfg::UNIT, &bars[stage]);
+    }
+  };
+  int next = first + warp, blk_next = page_of(next);           // the next tile to copy
+  for (int s = 0; s < Cfg::STAGES && next < last && !bad; s++) {
+    issue(next, s, blk_next);
+    next += D4_WARPS;
+    blk_next = page_of(next);
+  }
+
+  // the rows' fragments: row r (+ 8 per tile), channels in the order of unpacking
+  uint32_t qf[NT][KW][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    const int row = row0 + nt * 8 + r, tok = row / p.G, g = row - tok * p.G;
+    const bool here = nt * 8 + r < rows;
+    const uint4* src = reinterpret_cast<const uint4*>(p.q + (long)(q_start + tok) * p.q_stride + (long)(h * p.G + g) * D + c * (D / 4));
+#pragma unroll
+    for (int w = 0; w < KW; w++) {
+      const uint4 x = here ? src[w] : make_uint4(0, 0, 0, 0);
+      qf[nt][w][0] = __byte_perm(x.x, x.z, 0x5410);
+      qf[nt][w][1] = __byte_perm(x.x, x.z, 0x7632);
+      qf[nt][w][2] = __byte_perm(x.y, x.w, 0x5410);
+      qf[nt][w][3] = __byte_perm(x.y, x.w, 0x7632);
+    }
+  }
+  // columns 2 c and 2 c + 1 of the score tiles
+  int k_lo[NT][2], k_hi[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int i = nt * 8 + 2 * c + e, pos = ctx + (row0 + i) / p.G;
+      k_hi[nt][e] = i < rows ? (p.causal ? min(len, pos + 1) : len) : 0;
+      k_lo[nt][e] = p.window > 0 ? pos - p.window + 1 : 0;
+    }
+
+  float o[NT][MT][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[nt][i][e] = 0.f;
+  }
+  const int kg = (c * (D / 4)) / KV4_GROUP, vg = (r * (D / 8)) / KV4_GROUP;
+
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int tile = first + warp; tile < last; tile += D4_WARPS) {
+    if (bad && tile >= next) break;              // pages behind a bad one were not fetched
+    if (!__all_sync(0xffffffffu, mbar_wait(&bars[stage], phase, abort_word))) break;
+    const uint8_t* ks = ring + stage * Cfg::STAGE;
+    const uint8_t* vs = ks + U * Cfg::UNIT;
+    const int t0 = tile * TS;
+    float s[U][NT][4];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint8_t* unit = ks + u * Cfg::UNIT;
+      uint32_t wa[KW], wb[KW];
+      const uint8_t* ra = unit + r * (D / 2) + c * (D / 8);
+      if constexpr (KW == 4) {
+        const uint4 a = *reinterpret_cast<const uint4*>(ra), b = *reinterpret_cast<const uint4*>(ra + 8 * (D / 2));
+        wa[0] = a.x; wa[1] = a.y; wa[2] = a.z; wa[3] = a.w;
+        wb[0] = b.x; wb[1] = b.y; wb[2] = b.z; wb[3] = b.w;
+      } else {
+        const uint2 a = *reinterpret_cast<const uint2*>(ra), b = *reinterpret_cast<const uint2*>(ra + 8 * (D / 2));
+        wa[0] = a.x; wa[1] = a.y;
+        wb[0] = b.x; wb[1] = b.y;
+      }
+      const uint16_t* sc = reinterpret_cast<const uint16_t*>(unit + 8 * D) + kg * KV4_TOKENS + r;
+      const __nv_bfloat162 sa = kv4_scale(sc[0] * 0x10001u), sb = kv4_scale(sc[8] * 0x10001u);
+      const __nv_bfloat162 sa24 = kv4_minus24(sa), sb24 = kv4_minus24(sb);
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[u][nt][e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < KW; w++) {
+        const uint32_t a0 = kv4_pair<0>(wa[w], sa, sa24), a1 = kv4_pair<1>(wa[w], sa, sa24);
+        const uint32_t b0 = kv4_pair<0>(wb[w], sb, sb24), b1 = kv4_pair<1>(wb[w], sb, sb24);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) i4_mma(s[u][nt], a0, b0, a1, b1, qf[nt][w][0], qf[nt][w][1]);
+        const uint32_t a2 = kv4_pair<2>(wa[w], sa, sa24), a3 = kv4_pair<3>(wa[w], sa, sa24);
+        const uint32_t b2 = kv4_pair<2>(wb[w], sb, sb24), b3 = kv4_pair<3>(wb[w], sb, sb24);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) i4_mma(s[u][nt], a2, b2, a3, b3, qf[nt][w][2], qf[nt][w][3]);
+      }
+    }
+    const bool masked = t0 + TS > all_hi || t0 < all_lo;
+    if (masked) {
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int t = t0 + u * KV4_TOKENS + r + (e >> 1) * 8;
+            if (t < k_lo[nt][e & 1] || t >= k_hi[nt][e & 1]) s[u][nt][e] = -INFINITY;
+          }
+    }
+    // running maxima: moved only where they grow by more than a factor of 2^8 (no probability then overflows bf16, and all
+    // of them shrink together otherwise)
+    bool grow = false;
+    float mt[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float x = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
+#pragma unroll
+        for (int u = 1; u < U; u++) x = fmaxf(x, fmaxf(s[u][nt][e], s[u][nt][e + 2]));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+        mt[nt][e] = x * p.scale_log2;
+        grow |= mt[nt][e] > m[nt][e] + 8.f;
+      }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const float now = fmaxf(m[nt][e], mt[nt][e]), f = m[nt][e] == -INFINITY ? 0.f : i4_exp2(m[nt][e] - now);
+          m[nt][e] = now;
+          l[nt][e] *= f;
+#pragma unroll
+          for (int i = 0; i < MT; i++) {
+            o[nt][i][e] *= f;
+            o[nt][i][e + 2] *= f;
+          }
+        }
+    }
+    uint32_t pf[U][NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const float n0 = m[nt][0] == -INFINITY ? 0.f : -m[nt][0], n1 = m[nt][1] == -INFINITY ? 0.f : -m[nt][1];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const float p0 = i4_exp2(fmaf(s[u][nt][0], p.scale_log2, n0)), p1 = i4_exp2(fmaf(s[u][nt][1], p.scale_log2, n1));
+        const float p2 = i4_exp2(fmaf(s[u][nt][2], p.scale_log2, n0)), p3 = i4_exp2(fmaf(s[u][nt][3], p.scale_log2, n1));
+        l[nt][0] += p0 + p2;
+        l[nt][1] += p1 + p3;
+        // bf16 probabilities for the tensor cores (the sums above are of the fp32 ones): half a step of 2^-8, with either sign
+        pf[u][nt][0] = i4_transpose(pack_bf16x2(p0, p1));
+        pf[u][nt][1] = i4_transpose(pack_bf16x2(p2, p3));
+      }
+    }
+    bool odd = false;                            // a scale that is no number, in a tile that not all rows see
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint8_t* unit = vs + u * Cfg::UNIT;
+      const uint32_t* sc = reinterpret_cast<const uint32_t*>(unit + 8 * D + vg * (KV4_TOKENS * 2)) + c;
+      uint32_t sw[2] = {sc[0], sc[4]};
+      if (masked) {                              // tokens that no row sees weigh nothing, whatever lies in their place
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const int t = t0 + u * KV4_TOKENS + 2 * c + 8 * i;
+          if (t < lo || t >= hi) sw[i] &= 0xffff0000u;
+          if (t + 1 < lo || t + 1 >= hi) sw[i] &= 0x0000ffffu;
+          if ((sw[i] & 0x7f80u) == 0x7f80u) { sw[i] &= 0xffff0000u; odd = true; }
+          if ((sw[i] & 0x7f800000u) == 0x7f800000u) { sw[i] &= 0x0000ffffu; odd = true; }
+        }
+      }
+      uint32_t x[2][VW][8];                      // [tokens 2 c, + 8][word][channel]: pairs of tokens
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const __nv_bfloat162 sv = kv4_scale(sw[i]), sv24 = kv4_minus24(sv);
+        const uint8_t* a = unit + (c + 8 * i) * (D / 2) + r * (D / 16);
+        uint32_t va[VW], vb[VW];
+        if constexpr (VW == 2) {
+          const uint2 e0 = *reinterpret_cast<const uint2*>(a), e1 = *reinterpret_cast<const uint2*>(a + 4 * (D / 2));
+          va[0] = e0.x; va[1] = e0.y;
+          vb[0] = e1.x; vb[1] = e1.y;
+        } else {
+          va[0] = *reinterpret_cast<const uint32_t*>(a);
+          vb[0] = *reinterpret_cast<const uint32_t*>(a + 4 * (D / 2));
+        }
+#pragma unroll
+        for (int w = 0; w < VW; w++) {
+          const uint32_t low = __byte_perm(va[w], vb[w], 0x5410), high = __byte_perm(va[w], vb[w], 0x7632);
+          x[i][w][0] = kv4_pair<0>(low, sv, sv24);
+          x[i][w][1] = kv4_pair<1>(low, sv, sv24);
+          x[i][w][2] = kv4_pair<2>(low, sv, sv24);
+          x[i][w][3] = kv4_pair<3>(low, sv, sv24);
+          x[i][w][4] = kv4_pair<0>(high, sv, sv24);
+          x[i][w][5] = kv4_pair<1>(high, sv, sv24);
+          x[i][w][6] = kv4_pair<2>(high, sv, sv24);
+          x[i][w][7] = kv4_pair<3>(high, sv, sv24);
+        }
+      }
+      // rows r of channel tile i: the lane's channel i, rows r + 8 its channel i + MT
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+        constexpr int last_w = VW - 1;
+        const int up = VW == 2 ? i : i + MT;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+          i4_mma(o[nt][i], x[0][0][i], x[0][last_w][up], x[1][0][i], x[1][last_w][up], pf[u][nt][0], pf[u][nt][1]);
+      }
+    }
+    if (masked && __any_sync(0xffffffffu, odd)) {
+      // values that are no numbers reach the rows that see them, and no others
+      for (int i = 0; i < TS; i++) {
+        const int t = t0 + i;
+        if (t < lo || t >= hi) continue;
+        const uint16_t sc = reinterpret_cast<const uint16_t*>(vs + (i / KV4_TOKENS) * Cfg::UNIT + 8 * D)[vg * KV4_TOKENS + i % KV4_TOKENS];
+        if ((sc & 0x7f80u) != 0x7f80u) continue;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+            if (t >= k_lo[nt][e] && t < k_hi[nt][e])
+#pragma unroll
+              for (int j = 0; j < MT; j++) o[nt][j][e] = o[nt][j][e + 2] = __int_as_float(0x7fc00000);
+      }
+    }
+    __syncwarp();                                // all lanes have read the stage
+    if (next < last && !bad) {
+      issue(next, stage, blk_next);
+      if (!bad) {
+        next += D4_WARPS;
+        blk_next = page_of(next);
+      }
+    }
+    if (++stage == Cfg::STAGES) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+
+  // ---------------- join the warps: results into the rings' place
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      float x = l[nt][e];
+      x += __shfl_xor_sync(0xffffffffu, x, 4);
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      if (r == 0) {
+        ms[warp * ROWS + nt * 8 + 2 * c + e] = m[nt][e];
+        ls[warp * ROWS + nt * 8 + 2 * c + e] = x;
+      }
+    }
+  if (bad && lane == 0) *abort_word = B200_BAD_INDEX;
+  float* res = (float*)ring;                     // [rows][D]
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      float* dst = res + (nt * 8 + 2 * c + e) * D + r * (D / 8);
+#pragma unroll
+      for (int i = 0; i < MT; i += 4) {
+        *reinterpret_cast<float4*>(dst + i) = make_float4(o[nt][i][e], o[nt][i + 1][e], o[nt][i + 2][e], o[nt][i + 3][e]);
+        *reinterpret_cast<float4*>(dst + MT + i) =
+            make_float4(o[nt][i][e + 2], o[nt][i + 1][e + 2], o[nt][i + 2][e + 2], o[nt][i + 3][e + 2]);
+      }
+    }
+  __syncthreads();
+  if (*abort_word != 0) {
+    if (*abort_word == B200_TIMEOUT) {           // copies still in flight land before the block's shared memory is released
+      const uint64_t t_start = globaltimer_ns();
+      while (globaltimer_ns() - t_start < 50000ull) __nanosleep(1000);
+    }
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, *abort_word);
+    __syncthreads();
+  }
+  for (int it = threadIdx.x; it < rows * (D / 8); it += 32 * D4_WARPS) {
+    const int i = it / (D / 8), ch = (it - i * (D / 8)) * 8;
+    float top = ms[i];
+#pragma unroll
+    for (int w = 1; w < D4_WARPS; w++) top = fmaxf(top, ms[w * ROWS + i]);
+    float sum = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < D4_WARPS; w++) {
+      const float mw = ms[w * ROWS + i];
+      if (mw == -INFINITY && ls[w * ROWS + i] == 0.f) continue;                // saw no key
+      const float f = i4_exp2(mw - top);
+      sum += ls[w * ROWS + i] * f;
+      const float4* src = reinterpret_cast<const float4*>(i4_smem + w * Cfg::RING) + (i * D + ch) / 4;
+      const float4 a = src[0], b = src[1];
+      acc[0] += a.x * f; acc[1] += a.y * f; acc[2] += a.z * f; acc[3] += a.w * f;
+      acc[4] += b.x * f; acc[5] += b.y * f; acc[6] += b.z * f; acc[7] += b.w * f;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;          // a row without keys: zeros
+    const int tok = (row0 + i) / p.G, g = row0 + i - tok * p.G;
+    if (p.parts == 1) {
+      uint4 v;
+      v.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+      v.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+      v.z = pack_bf16x2(acc[4] * inv, acc[5] * inv);
+      v.w = pack_bf16x2(acc[6] * inv, acc[7] * inv);
+      *reinterpret_cast<uint4*>(p.out + (long)(q_start + tok) * p.out_stride + (long)(h * p.G + g) * D + ch) = v;
+    } else {
+      const long at = ((long)(q_start + tok) * (p.Hkv * p.G) + h * p.G + g) * p.parts + part;
+      float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + ch);
+      dst[0] = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+      dst[1] = make_float4(acc[4] * inv, acc[5] * inv, acc[6] * inv, acc[7] * inv);
+      if (ch == 0) p.part_lse[at] = sum == 0.f ? -INFINITY : top + log2f(sum);
+    }
+  }
+}
+
+// Parts of a (token, head) joined: sum 2^(lse_i - max) o_i / sum 2^(lse_i - max).  A warp each; tokens of listed sequences only.
+template <int D>
+__global__ void __launch_bounds__(128) attn_int4_join_kernel(const float* part_o, const float* part_lse, const int* cu, int num_seqs, int heads,
+                                                             int parts, long rows, __nv_bfloat16* out, long out_stride) {
+  const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const long first = cu[0], end = cu[num_seqs];
+  const long tok = first + at / heads;
+  const int head = (int)(at % heads);
+  if (at >= rows || tok >= end) return;
+  const float* lse = part_lse + (tok * heads + head) * parts;
+  const float* o = part_o + (tok * heads + head) * parts * D;
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, lse[i]);
+  top = warp_reduce_max(top);
+  constexpr int V = D / 32;
+  float acc[V] = {}, sum = 0.f;
+  for (int i = 0; i < parts; i++) {
+    const float x = lse[i];
+    if (x == -INFINITY) continue;                // saw no key: nothing was written
+    const float f = i4_exp2(x - (top == -INFINITY ? 0.f : top));
+    sum += f;
+    if constexpr (V == 4) {
+      const float4 a = reinterpret_cast<const float4*>(o + (long)i * D)[lane];
+      acc[0] += a.x * f; acc[1] += a.y * f; acc[2] += a.z * f; acc[3] += a.w * f;
+    } else {
+      const float2 a = reinterpret_cast<const float2*>(o + (long)i * D)[lane];
+      acc[0] += a.x * f; acc[1] += a.y * f;
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(out + tok * out_stride + (long)head * D) + lane * (V / 2);
+  dst[0] = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  if constexpr (V == 4) dst[1] = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+}
+
+template <int D, int NT>
+static int launch_int4(Int4Params p, int max_rows, cudaStream_t stream) {
+  using Cfg = Int4Cfg<D, NT>;
+  cudaError_t e = allow_smem<attn_int4_kernel<D, NT>>(Cfg::SMEM);
+  if (e != cudaSuccess) return (int)e;
+  p.row_blocks = (max_rows + Cfg::ROWS - 1) / Cfg::ROWS;
+  const long x = (long)p.num_seqs * p.row_blocks;
+  if (x > 0x7fffffffl || p.Hkv > 65535 || p.parts > 65535) return 9886;
+  attn_int4_kernel<D, NT><<<dim3((unsigned)x, (unsigned)p.Hkv, (unsigned)p.parts), 32 * D4_WARPS, Cfg::SMEM, stream>>>(p);
+  return B200_CHECK_LAUNCH();
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+// q [*, Hq, D] and out rows with token strides; cu [num_seqs + 1] their row numbers; max_q_len: no sequence has more new tokens.
+// parts > 1: scratch of (rows of q) x Hq x parts x (D + 1) floats.
+B200_API int b200_attn_int4(const void* q, long q_stride, long q_rows, const void* k_cache, const void* v_cache, long num_blocks,
+                            int block_size, const void* cu, const void* seq_lens, const void* block_table, int max_blocks, int num_seqs,
+                            int max_q_len, int Hq, int Hkv, int D, float scale, int causal, int window, int parts, void* out,
+                            long out_stride, void* scratch, int* status, cudaStream_t stream) {
+  if (num_seqs <= 0 || q_rows <= 0 || max_q_len <= 0) return 0;
+  const int G = Hkv > 0 ? Hq / Hkv : 0;
+  if (G < 1 || G * Hkv != Hq || (D != 64 && D != 128)) return 9883;
+  if (block_size < KV4_TOKENS || block_size % KV4_TOKENS) return 9884;
+  if ((q_stride & 7) || (out_stride & 7) || parts < 1 || (parts > 1 && !scratch)) return 9885;
+  Int4Params p = {};
+  p.q = (const __nv_bfloat16*)q;
+  p.k_cache = (const uint8_t*)k_cache;
+  p.v_cache = (const uint8_t*)v_cache;
+  p.cu = (const int*)cu;
+  p.seq_lens = (const int*)seq_lens;
+  p.block_table = (const int*)block_table;
+  p.out = (__nv_bfloat16*)out;
+  p.part_o = (float*)scratch;
+  p.part_lse = p.part_o + q_rows * Hq * parts * D;
+  p.q_stride = q_stride; p.out_stride = out_stride; p.num_blocks = num_blocks;
+  p.num_seqs = num_seqs; p.max_blocks = max_blocks; p.block_size = block_size;
+  p.G = G; p.Hkv = Hkv; p.parts = parts; p.causal = causal; p.window = window;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.status = status;
+  const long rows = (long)max_q_len * G;
+  if (rows > 0x3fffffffl) return 9886;
+  int rc;
+  if (D == 128) rc = rows <= 8 ? launch_int4<128, 1>(p, (int)rows, stream) : launch_int4<128, 2>(p, (int)rows, stream);
+  else rc = rows <= 8 ? launch_int4<64, 1>(p, (int)rows, stream) : launch_int4<64, 2>(p, (int)rows, stream);
+  if (rc || parts == 1) return rc;
+  const long all = q_rows * Hq;
+  const unsigned blocks = (unsigned)((all + 3) / 4);
+  if (D == 128)
+    attn_int4_join_kernel<128><<<blocks, 128, 0, stream>>>(p.part_o, p.part_lse, p.cu, num_seqs, Hq, parts, all, p.out, out_stride);
+  else
+    attn_int4_join_kernel<64><<<blocks, 128, 0, stream>>>(p.part_o, p.part_lse, p.cu, num_seqs, Hq, parts, all, p.out, out_stride);
+  return B200_CHECK_LAUNCH();
+}

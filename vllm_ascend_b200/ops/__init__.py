@@ -968,3 +968,7 @@ def rms_norm_gated(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, eps: 
     _native.check(rc, "rms_norm_gated")
     launch_counter[0] += 1
     return out
+
+
+# ---------------------------------------------------------------- 4-bit cache
+from .kv_int4 import alloc_kv_cache_int4, paged_attention_int4, read_kv_int4, write_kv_int4  # noqa: E402,F401

@@ -1,0 +1,169 @@
+"""A paged cache of keys and values in 4 bits: allocation, the operators that fill and read it, attention over it.
+
+Groups of 32 adjacent channels of a token and head share a scale of five significant bits; a channel is a whole number in
+-7..7 times it, exact in bf16 (``reference.kv_int4_quantise``).  4.5 bits a channel: a GPU holds 3.5 times the tokens of a bf16
+cache, and decode reads 3.5 times fewer bytes.  A cache is one dense uint8 tensor [blocks, heads, bytes of
+a block] for the keys and one for the values (layout: csrc/kv_int4.cuh); head sizes 64 and 128, blocks of a multiple of 16 tokens.
+The reference quantises its cache to 8 bits with static scales (vllm_ascend/quantization/methods/kv_c8.py)."""
+from __future__ import annotations
+
+from ctypes import c_float, c_int, c_long, c_void_p
+from typing import Optional
+
+import torch
+
+from .. import _native
+from ..batch_invariant import fixed_sums
+from . import reference as ref
+from .scratch import Scratch
+
+_P, _I, _L, _F = c_void_p, c_int, c_long, c_float
+_native.register_signature("b200_kv_int4_write", [_P, _L, _P, _L, _L, _P, _P, _P, _L, _I, _I, _I, _P, _P])
+_native.register_signature("b200_kv_int4_read", [_P, _P, _L, _P, _P, _P, _L, _I, _I, _I, _P, _P])
+_native.register_signature("b200_attn_int4", [_P, _L, _L, _P, _P, _L, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P, _L, _P, _P, _P])
+
+HEAD_SIZES = (64, 128)
+
+_scratch = Scratch(torch.float32)
+
+
+def block_bytes(block_size: int, dim: int) -> int:
+    """Bytes of a block of one head, of the keys or of the values."""
+    if dim not in HEAD_SIZES:
+        raise ValueError(f"a 4-bit cache takes heads of {HEAD_SIZES}, not {dim}")
+    if block_size < 1 or block_size % ref.KV_INT4_TOKENS:
+        raise ValueError(f"a 4-bit cache takes blocks of a multiple of {ref.KV_INT4_TOKENS} tokens, not {block_size}")
+    return block_size // ref.KV_INT4_TOKENS * 9 * dim
+
+
+def alloc_kv_cache_int4(num_blocks: int, block_size: int, heads: int, dim: int, device, arena=None) -> torch.Tensor:
+    """Zero-filled cache [blocks, heads, bytes]; ``arena`` as in ``alloc_kv_cache``."""
+    shape = (num_blocks, heads, block_bytes(block_size, dim))
+    return arena.take(shape, torch.uint8) if arena is not None else torch.zeros(shape, dtype=torch.uint8, device=device)
+
+
+def _check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dim: int, device) -> int:
+    """Block size of a pair of caches that belong together."""
+    if dim not in HEAD_SIZES:
+        raise ValueError(f"a 4-bit cache takes heads of {HEAD_SIZES}, not {dim}")
+    bs = ref.kv_int4_block_size(k_cache, dim)
+    if v_cache.shape != k_cache.shape or ref.kv_int4_block_size(v_cache, dim) != bs:
+        raise ValueError(f"keys {tuple(k_cache.shape)} and values {tuple(v_cache.shape)} are caches of different sizes")
+    if k_cache.device != device or v_cache.device != device:
+        raise ValueError(f"caches on {k_cache.device} and {v_cache.device}, rows on {device}")
+    return bs
+
+
+def _check_slots(slots: torch.Tensor, rows: int, device) -> torch.Tensor:
+    if slots.dim() != 1 or slots.shape[0] != rows or slots.device != device or slots.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"slots: {rows} whole numbers on {device}, not {slots.dtype} {tuple(slots.shape)} on {slots.device}")
+    return slots.to(torch.int64).contiguous()
+
+
+def _dense_heads(x: torch.Tensor) -> torch.Tensor:
+    """x [T, H, D] as the kernels read rows: heads dense, rows and the first element on 16-byte boundaries."""
+    T, H, D = x.shape
+    if x.stride(2) == 1 and (x.stride(1) == D or H == 1) and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def write_kv_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """Rows of k and v [T, heads, D] quantised into their slots (block * block size + offset) of a 4-bit cache; rows whose slot
+    is below zero are not stored.  A slot may be listed once only."""
+    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or not k.is_floating_point() or k.device != v.device:
+        raise ValueError(f"keys {k.dtype} {tuple(k.shape)} and values {v.dtype} {tuple(v.shape)} are not rows [T, heads, D] of one type")
+    T, H, D = k.shape
+    bs = _check_caches(k_cache, v_cache, D, k.device)
+    if H != k_cache.shape[1]:
+        raise ValueError(f"rows of {H} heads, a cache of {k_cache.shape[1]}")
+    slots = _check_slots(slot_mapping, T, k.device)
+    if T == 0:
+        return
+    if not k.is_cuda or k.dtype != torch.bfloat16:
+        return ref.write_kv_int4(k, v, k_cache, v_cache, slots)
+    k, v = _dense_heads(k), _dense_heads(v)
+    with torch.cuda.device(k.device):
+        rc = _native.lib().b200_kv_int4_write(
+            k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), T, slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_cache.shape[0] * bs, H, D, bs, _native.status_word(k.device).data_ptr(), _native.stream_ptr())
+    _native.check(rc, "kv_int4_write")
+    _native.count_launch()
+
+
+def read_kv_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, dim: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """What slots of a 4-bit cache of heads of ``dim`` stand for: keys and values [slots, heads, dim] in bf16, exact.  Slots below zero
+    read as zeros; a slot may be listed any number of times."""
+    bs = _check_caches(k_cache, v_cache, dim, k_cache.device)
+    n, H, dev = slots.shape[0] if slots.dim() else 0, k_cache.shape[1], k_cache.device
+    slots = _check_slots(slots, n, dev)
+    if not k_cache.is_cuda:
+        return ref.read_kv_int4(k_cache, v_cache, slots, dim)
+    k = torch.empty((n, H, dim), dtype=torch.bfloat16, device=dev)
+    v = torch.empty_like(k)
+    if n == 0:
+        return k, v
+    with torch.cuda.device(dev):
+        rc = _native.lib().b200_kv_int4_read(
+            k.data_ptr(), v.data_ptr(), n, slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0] * bs, H, dim, bs,
+            _native.status_word(dev).data_ptr(), _native.stream_ptr())
+    _native.check(rc, "kv_int4_read")
+    _native.count_launch()
+    return k, v
+
+
+def _parts(blocks: int, max_len: int, sms: int) -> int:
+    """Parts that every sequence's keys are split into."""
+    if fixed_sums():
+        return 1
+    return max(1, min(4 * sms // max(1, blocks), -(-max_len // 128), 64))
+
+
+def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta, scale: float,
+                         out: Optional[torch.Tensor] = None, causal: bool = True, window: int = 0) -> torch.Tensor:
+    """``paged_attention`` over a 4-bit cache: q [T, Hq, D], every new token over its sequence's pages.  Rows of ``out`` behind the last
+    sequence are left as they are; a token that sees no key gets zeros."""
+    if q.dim() != 3:
+        raise ValueError(f"queries are [T, heads, D], not {tuple(q.shape)}")
+    T, Hq, D = q.shape
+    bs = _check_caches(k_cache, v_cache, D, q.device)
+    NB, Hkv, _ = k_cache.shape
+    if Hkv == 0 or Hq % Hkv or Hq == 0:
+        raise ValueError(f"{Hq} query heads do not share {Hkv} heads of a cache evenly")
+    if not scale > 0:
+        raise ValueError(f"scale {scale} is not above zero")
+    if window < 0:
+        raise ValueError(f"window {window} is below zero")
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError(f"out: {q.dtype} {tuple(q.shape)} on {q.device}, not {out.dtype} {tuple(out.shape)} on {out.device}")
+    if not q.is_cuda or q.dtype != torch.bfloat16:
+        return ref.paged_attention_int4(q, k_cache, v_cache, meta.query_start_loc_cpu, meta.seq_lens_cpu, meta.block_table, scale,
+                                        causal, window, out=out)
+    n = meta.num_reqs
+    if n == 0 or T == 0:
+        return out
+    given, q = out, _dense_heads(q)
+    if out.stride(2) != 1 or out.stride(1) != D or out.stride(0) % 8 or out.data_ptr() % 16:
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+        out.copy_(given)
+    with torch.cuda.device(q.device):
+        _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, n, meta.max_query_len)
+    return out if out is given else given.copy_(out)
+
+
+def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, n, max_q) -> None:
+    """The first ``n`` sequences of the batch, none with more than ``max_q`` new tokens."""
+    T, Hq, D = q.shape
+    NB, Hkv, _ = k_cache.shape
+    rows = max_q * (Hq // Hkv)
+    blocks = n * Hkv * (1 if rows <= 8 else -(-rows // 16))
+    parts = _parts(blocks, meta.max_seq_len, _native.sm_count(q.device))
+    scratch = _scratch.get(q.device, T * Hq * parts * (D + 1)) if parts > 1 else None
+    rc = _native.lib().b200_attn_int4(
+        q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(),
+        meta.block_table.data_ptr(), meta.block_table.stride(0), n, max_q, Hq, Hkv, D, scale, int(causal), int(window), parts,
+        out.data_ptr(), out.stride(0), _native.ptr(scratch), _native.status_word(q.device).data_ptr(), _native.stream_ptr())
+    _native.check(rc, "attn_int4")
+    _native.count_launch(1 + int(parts > 1))

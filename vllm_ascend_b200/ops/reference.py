@@ -258,6 +258,87 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     return out
 
 
+# ---------------------------------------------------------------- 4-bit cache
+KV_INT4_GROUP, KV_INT4_TOKENS = 32, 16
+
+
+def kv_int4_quantise(x: torch.Tensor):
+    """x [..., D] -> whole numbers in -7..7 (int8) [..., D] and scales (bf16) [..., D / 32].  A scale is the smallest number
+    of five significant bits (zero, or a multiple of 2^-130 up to 2^122) with 7 scale >= max |x| over its 32 channels; a group
+    that holds a NaN or an infinity is NaN."""
+    g = x.float().unflatten(-1, (-1, KV_INT4_GROUP))
+    top = g.abs().amax(-1, keepdim=True)
+    finite = torch.isfinite(top)
+    top = torch.where(finite, top, 0.0)
+    low = top / torch.full_like(top, 7.0)
+    s = ((low.view(torch.int32) + 0x7ffff) & ~0x7ffff).view(torch.float32).clamp_max(2.0 ** 122)
+    n = torch.where(finite & (s > 0), g / torch.where(s > 0, s, 1.0), 0.0).clamp(-7, 7).round()
+    nan = torch.tensor(0x7fc0, dtype=torch.int16, device=x.device).view(torch.bfloat16)      # the same bits everywhere
+    s = torch.where(finite, s.to(torch.bfloat16), nan)
+    return n.flatten(-2).to(torch.int8), s.squeeze(-1)
+
+
+def kv_int4_block_size(cache: torch.Tensor, dim: int) -> int:
+    """Tokens of a block of a 4-bit cache [blocks, heads, bytes]; raises where the bytes do not fit heads of ``dim``."""
+    unit = 9 * dim
+    if cache.dtype != torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or cache.shape[2] == 0 or cache.shape[2] % unit:
+        raise ValueError(f"not a dense 4-bit cache [blocks, heads, bytes] of heads of {dim}: {cache.dtype} {tuple(cache.shape)}")
+    return cache.shape[2] // unit * KV_INT4_TOKENS
+
+
+def _kv_int4_views(cache: torch.Tensor, dim: int):
+    """Rows [blocks, heads, units, 16, dim / 2] and scales [blocks, heads, units, dim / 32, 16] of a cache."""
+    B, H, _ = cache.shape
+    units = kv_int4_block_size(cache, dim) // KV_INT4_TOKENS
+    rows = cache.view(B, H, units, 9 * dim)[..., :8 * dim].unflatten(-1, (KV_INT4_TOKENS, dim // 2))
+    scales = cache.view(torch.bfloat16).view(B, H, units, 9 * dim // 2)[..., 4 * dim:]
+    return rows, scales.unflatten(-1, (dim // KV_INT4_GROUP, KV_INT4_TOKENS))
+
+
+def _kv_int4_row(t: torch.Tensor, values: bool) -> torch.Tensor:
+    """Row of token t of a unit: keys lie in order, values with the even tokens of each eight first."""
+    return (t & 8) | ((t & 1) << 2) | ((t >> 1) & 3) if values else t
+
+
+def write_kv_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor) -> None:
+    dim = k.shape[-1]
+    bs = kv_int4_block_size(k_cache, dim)
+    valid = slots >= 0
+    at = slots[valid]
+    blk, off = at // bs, at % bs
+    unit, t = off // KV_INT4_TOKENS, off % KV_INT4_TOKENS
+    for x, cache, values in ((k, k_cache, False), (v, v_cache, True)):
+        rows, scales = _kv_int4_views(cache, dim)
+        n, s = kv_int4_quantise(x[valid])
+        n = (n + 8).to(torch.uint8)
+        rows[blk, :, unit, _kv_int4_row(t, values)] = n[..., 0::2] | (n[..., 1::2] << 4)
+        scales[blk, :, unit, :, t] = s
+
+
+def read_kv_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, dim: int, dtype=torch.bfloat16):
+    bs = kv_int4_block_size(k_cache, dim)
+    at = slots.clamp(min=0)
+    blk, off = at // bs, at % bs
+    unit, t = off // KV_INT4_TOKENS, off % KV_INT4_TOKENS
+    out = []
+    for cache, values in ((k_cache, False), (v_cache, True)):
+        rows, scales = _kv_int4_views(cache, dim)
+        w = rows[blk, :, unit, _kv_int4_row(t, values)]
+        n = torch.stack((w & 15, w >> 4), -1).flatten(-2).float() - 8
+        x = (n.unflatten(-1, (-1, KV_INT4_GROUP)) * scales[blk, :, unit, :, t].float().unsqueeze(-1)).flatten(-2)
+        out.append(torch.where((slots >= 0).view(-1, 1, 1), x, 0.0).to(dtype))
+    return tuple(out)
+
+
+def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, query_start_loc, seq_lens,
+                         block_table: torch.Tensor, scale: float, causal: bool = True, window: int = 0, out: Optional[torch.Tensor] = None):
+    dim = q.shape[-1]
+    B, bs = k_cache.shape[0], kv_int4_block_size(k_cache, dim)
+    dense = read_kv_int4(k_cache, v_cache, torch.arange(B * bs, device=q.device), dim, torch.float32)
+    return paged_attention(q, *(t.view(B, bs, -1, dim) for t in dense), query_start_loc, seq_lens, block_table, scale, causal,
+                           window, out=out)
+
+
 def merge_attn_states(o1, lse1, o2, lse2):
     """LSE merge of two partial attention results ([T,H,D], [T,H])."""
     m = torch.maximum(lse1, lse2)
