@@ -3,7 +3,7 @@
 Attention is compared with fp64 attention over the values that the cache stands for.  Bound of an element, from the number types: the
 kernels round probabilities to bf16 (half a step, 2^-8) before they weight values, and the result (2^-8); scores are fp32 sums of D
 products (D 2^-24 of the largest sum of magnitudes, doubled for the products of the exponent's argument), which moves a probability by
-as much times log 2 and is counted as it is."""
+as much, and the sum that it is divided by by as much again."""
 import numpy as np
 import pytest
 import torch
@@ -71,7 +71,7 @@ def _want(q, kc, vc, meta, scale, window=0, causal=True):
             p = torch.softmax(s, -1)
             p = torch.where(off.all(-1, keepdim=True), 0.0, p)
             o = p @ vh
-            moved = 2 * (D + 4) * 2.0 ** -24 * float((x.abs() @ kh.abs().T).max()) * scale
+            moved = 2 * (D + 4) * 2.0 ** -24 * float((x.abs() @ kh.nan_to_num(0.0).abs().T).max()) * scale
             out[cu[b]:cu[b + 1], h] = o
             tol[cu[b]:cu[b + 1], h] = (2.0 ** -8 + 2 * moved) * (p @ vh.abs()) * (1 + 2.0 ** -7) + 2.0 ** -8 * o.abs() + 1e-30
     return out, tol

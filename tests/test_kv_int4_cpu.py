@@ -21,7 +21,8 @@ def _definition(group):
     while Fraction(31) * Fraction(2) ** e * 7 < top:              # scales of five bits: m 2^e, 16 <= m <= 31
         e += 1
     s = next(m * Fraction(2) ** e for m in range(1, 32) if 7 * m * Fraction(2) ** e >= top)
-    return s, [round(v / s) for v in x]                           # round(): ties to even
+    s = min(max(s, Fraction(2) ** -80), Fraction(2) ** 36)
+    return s, [min(max(round(v / s), -7), 7) for v in x]          # round(): ties to even
 
 
 def _meta(new, lens, table, Hq, Hkv, D):
@@ -51,9 +52,8 @@ def test_quantiser_at_the_edges_of_the_type():
     n, s = ref.kv_int4_quantise(x)
     assert s[0, 0].isnan() and not n[0].any() and s[0, 1] == 0
     assert s[1, 1].isnan() and s[1, 0] == 0
-    assert (s[2] == 2.0 ** 122).all() and (n[2] == 7).all()
-    # scales are multiples of 2^-130 (the five bits of a subnormal float that are kept), so n may be 0, within half a scale still
-    assert s[3, 0].float() == 2.0 ** -130 and 7 * s[3, 0].float() >= x[3, 0].float()
+    assert (s[2] == 2.0 ** 36).all() and (n[2] == 7).all()
+    assert s[3, 0].float() == 2.0 ** -80                                  # the smallest scale: n is 0, within half a scale still
     assert (x[3, 0].double() - n[3, 0] * s[3, 0].double()).abs() <= s[3, 0].double() / 2
     assert s[5].eq(0).all() and not n[5].any() and n[4, 1] == -7
 
@@ -70,16 +70,20 @@ def test_page_layout(D, page, H):
     ops.write_kv_int4(k, v, kc, vc, slots)
     for x, cache, values in ((k, kc, False), (v, vc, True)):
         n, s = ref.kv_int4_quantise(x)
-        for t in (0, 1, T - 1):
+        for t in (0, 1, 3, 4, T - 2, T - 1):
             blk, off = divmod(int(slots[t]), page)
             unit, i = divmod(off, 16)
-            row = [0, 4, 1, 5, 2, 6, 3, 7, 8, 12, 9, 13, 10, 14, 11, 15][i] if values else i
             for h in (0, H - 1):
-                mem = cache[blk, h, unit * 9 * D:(unit + 1) * 9 * D]
-                data = mem[row * D // 2:(row + 1) * D // 2]
-                assert data.tolist() == [int(n[t, h, 2 * c]) + 8 + 16 * (int(n[t, h, 2 * c + 1]) + 8) for c in range(D // 2)]
-                scales = mem[8 * D:].view(torch.bfloat16)
-                assert [float(scales[16 * c + i]) for c in range(D // 32)] == s[t, h].tolist()
+                mem = cache[blk, h, unit * 9 * D:(unit + 1) * 9 * D].tolist()
+                scales = cache[blk, h, unit * 9 * D + 8 * D:(unit + 1) * 9 * D].view(torch.bfloat16)
+                for ch in range(0, D, 2):
+                    byte = int(n[t, h, ch]) + 8 + 16 * (int(n[t, h, ch + 1]) + 8)
+                    if values:
+                        chunk = ch // 16 ^ (2 * (i // 2 % 4) if D == 128 else i // 2 & 2)
+                        assert mem[i // 2 * D + chunk * 16 + ch % 16 // 4 * 4 + i % 2 * 2 + ch % 4 // 2] == byte
+                    else:
+                        assert mem[i * D // 2 + ch // 2] == byte
+                    assert scales[ch // 32 * 16 + i] == s[t, h, ch // 32]
     got = ops.read_kv_int4(kc, vc, slots, D)
     for x, y in zip((k, v), got):
         n, s = ref.kv_int4_quantise(x)

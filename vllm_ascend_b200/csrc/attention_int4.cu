@@ -10,10 +10,12 @@
 //                   sum is free, so the query fragments follow what unpacking yields (channels j and j + 4 of eight)
 //   O^T = V^T P^T   D channels x 8 rows, over tokens.  A lane holds 16 (8) adjacent channels of four tokens; S^T's results
 //                   become P^T's fragments by transposing 8 x 8 blocks between the lanes
-// A block is one (sequence, KV head, part of the sequence); each of its warps walks tiles of TS tokens, one in W, through a
-// ring of its own that bulk copies fill (one per 16 tokens), with a running maximum of its own; they join at the end.  Parts join in
-// a second kernel.
+// A block is one (sequence, KV head, part of the sequence); each of its warps walks a stretch of it, in tiles of 64 (32) tokens where
+// all rows see them and 16 at a time at the edges, through a ring of its own that bulk copies fill, with a running maximum of
+// its own; they join at the end.  Parts join in a second kernel.
 #include "kv_int4.cuh"
+
+#include <type_traits>
 
 namespace b200 {
 
@@ -37,13 +39,13 @@ __device__ __forceinline__ float i4_exp2(float x) {
   return y;
 }
 __device__ __forceinline__ void i4_mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t i4_transpose(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ void i4_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -54,11 +56,10 @@ __device__ __forceinline__ void i4_bulk_load(void* dst, const void* src, uint32_
 
 template <int D, int NT>
 struct Int4Cfg {
-  static constexpr int TS = 32;                          // tokens of a tile
-  static constexpr int UNITS = TS / KV4_TOKENS;
+  static constexpr int U = NT == 1 ? 4 : 2;              // units of a tile
   static constexpr int UNIT = kv4_unit_bytes(D);
-  static constexpr int STAGE = 2 * UNITS * UNIT;         // keys, then values
-  static constexpr int STAGES = D == 128 ? 3 : 6;
+  static constexpr int STAGE = 2 * U * UNIT;             // keys, then values
+  static constexpr int STAGES = 2 * (128 / D) * (NT == 1 ? 1 : 2);
   static constexpr int RING = STAGES * STAGE;
   static constexpr int ROWS = 8 * NT;
   static constexpr int SMEM = D4_WARPS * RING + 1024;    // barriers, maxima and sums behind the rings
@@ -67,12 +68,12 @@ struct Int4Cfg {
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * D4_WARPS, NT == 1 ? 4 : 3) attn_int4_kernel(const Int4Params p) {
+__global__ void __launch_bounds__(32 * D4_WARPS, 3) attn_int4_kernel(const Int4Params p) {
   using Cfg = Int4Cfg<D, NT>;
-  constexpr int KW = D / 32;                    // words of a token's keys in a lane
-  constexpr int VW = D / 64;                    // words of a token's values in a lane
+  constexpr int KW = D / 32;                    // groups: words of a token's keys in a lane
+  constexpr int VX = D / 32;                    // words of two tokens' values in a lane
   constexpr int MT = D / 16;                    // channel tiles of the result
-  constexpr int U = Cfg::UNITS, ROWS = Cfg::ROWS, TS = Cfg::TS;
+  constexpr int U = Cfg::U, ROWS = Cfg::ROWS;
   extern __shared__ __align__(128) uint8_t i4_smem[];
   const int warp = warp_index(), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   uint8_t* ring = i4_smem + warp * Cfg::RING;
@@ -95,42 +96,61 @@ __global__ void __launch_bounds__(32 * D4_WARPS, NT == 1 ? 4 : 3) attn_int4_kern
   const int tok_first = row0 / p.G, tok_last = (row0 + rows - 1) / p.G;
   const int hi = max(0, p.causal ? min(len, ctx + tok_last + 1) : len), all_hi = p.causal ? min(len, ctx + tok_first + 1) : len;
   const int lo = p.window > 0 ? max(0, ctx + tok_first - p.window + 1) : 0, all_lo = p.window > 0 ? max(0, ctx + tok_last - p.window + 1) : 0;
-  const int t_lo = lo / TS, tiles = max(0, (hi + TS - 1) / TS - t_lo);
-  const int first = t_lo + (int)((long)tiles * part / p.parts), last = t_lo + (int)((long)tiles * (part + 1) / p.parts);
+  // the block's units, and the warp's among them
+  const int u_lo = lo / KV4_TOKENS, units = max(0, (hi + KV4_TOKENS - 1) / KV4_TOKENS - u_lo);
+  const int b0 = (int)((long)units * part / p.parts), b1 = (int)((long)units * (part + 1) / p.parts);
+  const int first = u_lo + b0 + (b1 - b0) * warp / D4_WARPS, last = u_lo + b0 + (b1 - b0) * (warp + 1) / D4_WARPS;
 
+  // the next tile to copy: lanes below U know the page of a unit each, and the unit's place there, walked by additions
   const int upp = p.block_size / KV4_TOKENS;
   const int* bt = p.block_table + (long)seq * p.max_blocks;
-  const int lu = lane % U, lkv = lane / U;                     // lanes below 2 U copy: unit, keys or values
-  auto page_of = [&](int tile) -> int {
-    const int t = tile * TS + lu * KV4_TOKENS;
-    if (lkv >= 2 || tile >= last || t >= hi) return 0;
-    const int col = t / p.block_size;
-    return col < p.max_blocks ? bt[col] : -1;
+  int next = first, col = (first + lane) / upp, at = first + lane - col * upp, blk = 0;
+  const int step = U / upp, rest = U - step * upp;
+  auto look_up = [&]() {
+    if (lane < U && next + lane < last) blk = col < p.max_blocks ? bt[col] : -1;
   };
+  look_up();
   bool bad = false;
-  auto issue = [&](int tile, int stage, int blk) {
-    const int n = min(U, (hi - tile * TS + KV4_TOKENS - 1) / KV4_TOKENS);
-    const bool mine = lkv < 2 && lu < n;
-    if (__any_sync(0xffffffffu, mine && (blk < 0 || blk >= p.num_blocks))) {
+  auto issue = [&](int stage) {
+    const int n = min(U, last - next);
+    if (__any_sync(0xffffffffu, lane < n && (blk < 0 || blk >= p.num_blocks))) {
       bad = true;
       return;
     }
-    if (lane == 0) mbar_expect_tx(&bars[stage], 2 * n * Cfg::UNIT);
-    __syncwarp();
-    if (mine) {
-      const int unit = (tile * U + lu) % upp;
-      const uint8_t* src = (lkv ? p.v_cache : p.k_cache) + (((long)blk * p.Hkv + h) * upp + unit) * Cfg::UNIT;
-      i4_bulk_load(ring + stage * Cfg::STAGE + (lkv * U + lu) * Cfg::UNIT, src, Cfg::UNIT, &bars[stage]);
+    const long from = (((long)blk * p.Hkv + h) * upp + at) * Cfg::UNIT;
+    uint8_t* to = ring + stage * Cfg::STAGE;
+    if (upp >= U) {                              // one run of a page, or two
+      const int n0 = min(n, upp - __shfl_sync(0xffffffffu, at, 0));
+      const long from0 = __shfl_sync(0xffffffffu, from, 0), from1 = __shfl_sync(0xffffffffu, from, n0 % U);
+      if (elect_one()) {
+        mbar_expect_tx(&bars[stage], 2 * n * Cfg::UNIT);
+        i4_bulk_load(to, p.k_cache + from0, n0 * Cfg::UNIT, &bars[stage]);
+        i4_bulk_load(to + U * Cfg::UNIT, p.v_cache + from0, n0 * Cfg::UNIT, &bars[stage]);
+        if (n0 < n) {
+          i4_bulk_load(to + n0 * Cfg::UNIT, p.k_cache + from1, (n - n0) * Cfg::UNIT, &bars[stage]);
+          i4_bulk_load(to + (U + n0) * Cfg::UNIT, p.v_cache + from1, (n - n0) * Cfg::UNIT, &bars[stage]);
+        }
+      }
+    } else {
+      if (lane == 0) mbar_expect_tx(&bars[stage], 2 * n * Cfg::UNIT);
+      __syncwarp();
+      if (lane < n) {
+        i4_bulk_load(to + lane * Cfg::UNIT, p.k_cache + from, Cfg::UNIT, &bars[stage]);
+        i4_bulk_load(to + (U + lane) * Cfg::UNIT, p.v_cache + from, Cfg::UNIT, &bars[stage]);
+      }
     }
+    next += U;
+    col += step;
+    at += rest;
+    if (at >= upp) {
+      at -= upp;
+      col++;
+    }
+    look_up();
   };
-  int next = first + warp, blk_next = page_of(next);           // the next tile to copy
-  for (int s = 0; s < Cfg::STAGES && next < last && !bad; s++) {
-    issue(next, s, blk_next);
-    next += D4_WARPS;
-    blk_next = page_of(next);
-  }
+  for (int s = 0; s < Cfg::STAGES && next < last && !bad; s++) issue(s);
 
-  // the rows' fragments: row r (+ 8 per tile), channels in the order of unpacking
+  // the rows' fragments: row r (+ 8 per tile), channels in the order of unpacking (j and j + 4 of a word's eight)
   uint32_t qf[NT][KW][4];
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
@@ -146,7 +166,7 @@ __global__ void __launch_bounds__(32 * D4_WARPS, NT == 1 ? 4 : 3) attn_int4_kern
       qf[nt][w][3] = __byte_perm(x.y, x.w, 0x7632);
     }
   }
-  // columns 2 c and 2 c + 1 of the score tiles
+  // keys that columns 2 c and 2 c + 1 see
   int k_lo[NT][2], k_hi[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; nt++)
@@ -169,20 +189,16 @@ __global__ void __launch_bounds__(32 * D4_WARPS, NT == 1 ? 4 : 3) attn_int4_kern
   }
   const int kg = (c * (D / 4)) / KV4_GROUP, vg = (r * (D / 8)) / KV4_GROUP;
 
-  int stage = 0;
-  uint32_t phase = 0;
-  for (int tile = first + warp; tile < last; tile += D4_WARPS) {
-    if (bad && tile >= next) break;              // pages behind a bad one were not fetched
-    if (!__all_sync(0xffffffffu, mbar_wait(&bars[stage], phase, abort_word))) break;
-    const uint8_t* ks = ring + stage * Cfg::STAGE;
-    const uint8_t* vs = ks + U * Cfg::UNIT;
-    const int t0 = tile * TS;
-    float s[U][NT][4];
+  // N units from ks and vs on, tokens from t0 on.  EDGE: some rows do not see all of them
+  auto tokens = [&](auto n_units, auto edge, const uint8_t* ks, const uint8_t* vs, int t0) {
+    constexpr int N = decltype(n_units)::value;
+    constexpr bool EDGE = decltype(edge)::value;
+    float s[N][NT][4];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
+    for (int u = 0; u < N; u++) {
       const uint8_t* unit = ks + u * Cfg::UNIT;
-      uint32_t wa[KW], wb[KW];
-      const uint8_t* ra = unit + r * (D / 2) + c * (D / 8);
+      uint32_t wa[KW], wb[KW];                   // words of tokens r and r + 8
+      const uint8_t* ra = unit + kv4_key_word(D, r, c * (D / 4));
       if constexpr (KW == 4) {
         const uint4 a = *reinterpret_cast<const uint4*>(ra), b = *reinterpret_cast<const uint4*>(ra + 8 * (D / 2));
         wa[0] = a.x; wa[1] = a.y; wa[2] = a.z; wa[3] = a.w;
@@ -192,29 +208,26 @@ __global__ void __launch_bounds__(32 * D4_WARPS, NT == 1 ? 4 : 3) attn_int4_kern
         wa[0] = a.x; wa[1] = a.y;
         wb[0] = b.x; wb[1] = b.y;
       }
-      const uint16_t* sc = reinterpret_cast<const uint16_t*>(unit + 8 * D) + kg * KV4_TOKENS + r;
-      const __nv_bfloat162 sa = kv4_scale(sc[0] * 0x10001u), sb = kv4_scale(sc[8] * 0x10001u);
-      const __nv_bfloat162 sa24 = kv4_minus24(sa), sb24 = kv4_minus24(sb);
+      const uint16_t* sc = reinterpret_cast<const uint16_t*>(unit + kv4_scale(D, r, kg));
+      const Kv4Scale sa(sc[0] * 0x10001u), sb(sc[8] * 0x10001u);
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int e = 0; e < 4; e++) s[u][nt][e] = 0.f;
 #pragma unroll
       for (int w = 0; w < KW; w++) {
-        const uint32_t a0 = kv4_pair<0>(wa[w], sa, sa24), a1 = kv4_pair<1>(wa[w], sa, sa24);
-        const uint32_t b0 = kv4_pair<0>(wb[w], sb, sb24), b1 = kv4_pair<1>(wb[w], sb, sb24);
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) i4_mma(s[u][nt], a0, b0, a1, b1, qf[nt][w][0], qf[nt][w][1]);
-        const uint32_t a2 = kv4_pair<2>(wa[w], sa, sa24), a3 = kv4_pair<3>(wa[w], sa, sa24);
-        const uint32_t b2 = kv4_pair<2>(wb[w], sb, sb24), b3 = kv4_pair<3>(wb[w], sb, sb24);
+        for (int j = 0; j < 2; j++) {            // channels 0, 1, 4, 5: the word's own low bytes; 2, 3, 6, 7
+          const uint32_t xa = j ? wa[w] >> 8 : wa[w], xb = j ? wb[w] >> 8 : wb[w];
+          const uint32_t a0 = kv4_pair(0, xa, sa), a1 = kv4_pair(0, xb, sb), a2 = kv4_pair(1, xa, sa), a3 = kv4_pair(1, xb, sb);
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) i4_mma(s[u][nt], a2, b2, a3, b3, qf[nt][w][2], qf[nt][w][3]);
+          for (int nt = 0; nt < NT; nt++) i4_mma(s[u][nt], a0, a1, a2, a3, qf[nt][w][2 * j], qf[nt][w][2 * j + 1]);
+        }
       }
     }
-    const bool masked = t0 + TS > all_hi || t0 < all_lo;
-    if (masked) {
+    if constexpr (EDGE) {
 #pragma unroll
-      for (int u = 0; u < U; u++)
+      for (int u = 0; u < N; u++)
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -223,8 +236,8 @@ __global__ void __launch_bounds__(32 * D4_WARPS, NT == 1 ? 4 : 3) attn_int4_kern
             if (t < k_lo[nt][e & 1] || t >= k_hi[nt][e & 1]) s[u][nt][e] = -INFINITY;
           }
     }
-    // running maxima: moved only where they grow by more than a factor of 2^8 (no probability then overflows bf16, and all
-    // of them shrink together otherwise)
+    // running maxima: moved only where a score outgrows them by more than a factor of 2^8 (no probability then overflows bf16, and
+    // all of them shrink together otherwise), so most tiles need a vote and no exchange
     bool grow = false;
     float mt[NT][2];
 #pragma unroll
@@ -233,19 +246,20 @@ __global__ void __launch_bounds__(32 * D4_WARPS, NT == 1 ? 4 : 3) attn_int4_kern
       for (int e = 0; e < 2; e++) {
         float x = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
 #pragma unroll
-        for (int u = 1; u < U; u++) x = fmaxf(x, fmaxf(s[u][nt][e], s[u][nt][e + 2]));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        mt[nt][e] = x * p.scale_log2;
-        grow |= mt[nt][e] > m[nt][e] + 8.f;
+        for (int u = 1; u < N; u++) x = fmaxf(x, fmaxf(s[u][nt][e], s[u][nt][e + 2]));
+        mt[nt][e] = x;
+        grow |= x * p.scale_log2 > m[nt][e] + 8.f;
       }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          const float now = fmaxf(m[nt][e], mt[nt][e]), f = m[nt][e] == -INFINITY ? 0.f : i4_exp2(m[nt][e] - now);
+          float x = mt[nt][e];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          const float now = fmaxf(m[nt][e], x * p.scale_log2), f = m[nt][e] == -INFINITY ? 0.f : i4_exp2(m[nt][e] - now);
           m[nt][e] = now;
           l[nt][e] *= f;
 #pragma unroll
@@ -255,12 +269,12 @@ __global__ void __launch_bounds__(32 * D4_WARPS, NT == 1 ? 4 : 3) attn_int4_kern
           }
         }
     }
-    uint32_t pf[U][NT][2];
+    uint32_t pf[N][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       const float n0 = m[nt][0] == -INFINITY ? 0.f : -m[nt][0], n1 = m[nt][1] == -INFINITY ? 0.f : -m[nt][1];
 #pragma unroll
-      for (int u = 0; u < U; u++) {
+      for (int u = 0; u < N; u++) {
         const float p0 = i4_exp2(fmaf(s[u][nt][0], p.scale_log2, n0)), p1 = i4_exp2(fmaf(s[u][nt][1], p.scale_log2, n1));
         const float p2 = i4_exp2(fmaf(s[u][nt][2], p.scale_log2, n0)), p3 = i4_exp2(fmaf(s[u][nt][3], p.scale_log2, n1));
         l[nt][0] += p0 + p2;
@@ -270,13 +284,13 @@ __global__ void __launch_bounds__(32 * D4_WARPS, NT == 1 ? 4 : 3) attn_int4_kern
         pf[u][nt][1] = i4_transpose(pack_bf16x2(p2, p3));
       }
     }
-    bool odd = false;                            // a scale that is no number, in a tile that not all rows see
+    bool odd = false;                            // a scale that is no number
 #pragma unroll
-    for (int u = 0; u < U; u++) {
+    for (int u = 0; u < N; u++) {
       const uint8_t* unit = vs + u * Cfg::UNIT;
-      const uint32_t* sc = reinterpret_cast<const uint32_t*>(unit + 8 * D + vg * (KV4_TOKENS * 2)) + c;
+      const uint32_t* sc = reinterpret_cast<const uint32_t*>(unit + kv4_scale(D, 2 * c, vg));
       uint32_t sw[2] = {sc[0], sc[4]};
-      if (masked) {                              // tokens that no row sees weigh nothing, whatever lies in their place
+      if constexpr (EDGE) {                      // tokens that no row sees weigh nothing, whatever lies in their place
 #pragma unroll
         for (int i = 0; i < 2; i++) {
           const int t = t0 + u * KV4_TOKENS + 2 * c + 8 * i;
@@ -286,49 +300,41 @@ __global__ void __launch_bounds__(32 * D4_WARPS, NT == 1 ? 4 : 3) attn_int4_kern
           if ((sw[i] & 0x7f800000u) == 0x7f800000u) { sw[i] &= 0x0000ffffu; odd = true; }
         }
       }
-      uint32_t x[2][VW][8];                      // [tokens 2 c, + 8][word][channel]: pairs of tokens
+      const Kv4Scale sv[2] = {Kv4Scale(sw[0]), Kv4Scale(sw[1])};
+      uint32_t x[2][2 * VX];                     // [tokens 2 c, + 8][two channels]: low bytes of a word, then its high ones
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        const __nv_bfloat162 sv = kv4_scale(sw[i]), sv24 = kv4_minus24(sv);
-        const uint8_t* a = unit + (c + 8 * i) * (D / 2) + r * (D / 16);
-        uint32_t va[VW], vb[VW];
-        if constexpr (VW == 2) {
-          const uint2 e0 = *reinterpret_cast<const uint2*>(a), e1 = *reinterpret_cast<const uint2*>(a + 4 * (D / 2));
-          va[0] = e0.x; va[1] = e0.y;
-          vb[0] = e1.x; vb[1] = e1.y;
+        const uint8_t* a = unit + kv4_value_word(D, 2 * c + 8 * i, r * (D / 8));
+        uint32_t v[VX];
+        if constexpr (VX == 4) {
+          const uint4 e = *reinterpret_cast<const uint4*>(a);
+          v[0] = e.x; v[1] = e.y; v[2] = e.z; v[3] = e.w;
         } else {
-          va[0] = *reinterpret_cast<const uint32_t*>(a);
-          vb[0] = *reinterpret_cast<const uint32_t*>(a + 4 * (D / 2));
+          const uint2 e = *reinterpret_cast<const uint2*>(a);
+          v[0] = e.x; v[1] = e.y;
         }
 #pragma unroll
-        for (int w = 0; w < VW; w++) {
-          const uint32_t low = __byte_perm(va[w], vb[w], 0x5410), high = __byte_perm(va[w], vb[w], 0x7632);
-          x[i][w][0] = kv4_pair<0>(low, sv, sv24);
-          x[i][w][1] = kv4_pair<1>(low, sv, sv24);
-          x[i][w][2] = kv4_pair<2>(low, sv, sv24);
-          x[i][w][3] = kv4_pair<3>(low, sv, sv24);
-          x[i][w][4] = kv4_pair<0>(high, sv, sv24);
-          x[i][w][5] = kv4_pair<1>(high, sv, sv24);
-          x[i][w][6] = kv4_pair<2>(high, sv, sv24);
-          x[i][w][7] = kv4_pair<3>(high, sv, sv24);
+        for (int w = 0; w < VX; w++) {
+          x[i][2 * w] = v[w];
+          x[i][2 * w + 1] = v[w] >> 8;
         }
       }
       // rows r of channel tile i: the lane's channel i, rows r + 8 its channel i + MT
 #pragma unroll
       for (int i = 0; i < MT; i++) {
-        constexpr int last_w = VW - 1;
-        const int up = VW == 2 ? i : i + MT;
+        const int j = i & 1, at = i >> 1, up = at + MT / 2;
+        const uint32_t a0 = kv4_pair(j, x[0][at], sv[0]), a1 = kv4_pair(j, x[0][up], sv[0]);
+        const uint32_t a2 = kv4_pair(j, x[1][at], sv[1]), a3 = kv4_pair(j, x[1][up], sv[1]);
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-          i4_mma(o[nt][i], x[0][0][i], x[0][last_w][up], x[1][0][i], x[1][last_w][up], pf[u][nt][0], pf[u][nt][1]);
+        for (int nt = 0; nt < NT; nt++) i4_mma(o[nt][i], a0, a1, a2, a3, pf[u][nt][0], pf[u][nt][1]);
       }
     }
-    if (masked && __any_sync(0xffffffffu, odd)) {
+    if (EDGE && __any_sync(0xffffffffu, odd)) {
       // values that are no numbers reach the rows that see them, and no others
-      for (int i = 0; i < TS; i++) {
+      for (int i = 0; i < N * KV4_TOKENS; i++) {
         const int t = t0 + i;
         if (t < lo || t >= hi) continue;
-        const uint16_t sc = reinterpret_cast<const uint16_t*>(vs + (i / KV4_TOKENS) * Cfg::UNIT + 8 * D)[vg * KV4_TOKENS + i % KV4_TOKENS];
+        const uint16_t sc = *reinterpret_cast<const uint16_t*>(vs + (i / KV4_TOKENS) * Cfg::UNIT + kv4_scale(D, i % KV4_TOKENS, vg));
         if ((sc & 0x7f80u) != 0x7f80u) continue;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
@@ -339,14 +345,26 @@ __global__ void __launch_bounds__(32 * D4_WARPS, NT == 1 ? 4 : 3) attn_int4_kern
               for (int j = 0; j < MT; j++) o[nt][j][e] = o[nt][j][e + 2] = __int_as_float(0x7fc00000);
       }
     }
-    __syncwarp();                                // all lanes have read the stage
-    if (next < last && !bad) {
-      issue(next, stage, blk_next);
-      if (!bad) {
-        next += D4_WARPS;
-        blk_next = page_of(next);
-      }
+  };
+  auto inside = [&](int u, int n) { return u * KV4_TOKENS >= all_lo && (u + n) * KV4_TOKENS <= all_hi; };
+
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int u0 = first; u0 < last; u0 += U) {
+    if (bad && u0 >= next) break;                // tiles from a bad page on were not fetched
+    if (!__all_sync(0xffffffffu, mbar_wait(&bars[stage], phase, abort_word))) break;
+    const uint8_t* ks = ring + stage * Cfg::STAGE;
+    const uint8_t* vs = ks + U * Cfg::UNIT;
+    const int n = min(U, last - u0);
+    if (n == U && inside(u0, U)) {
+      tokens(std::integral_constant<int, U>(), std::false_type(), ks, vs, u0 * KV4_TOKENS);
+    } else {
+#pragma unroll 1
+      for (int u = 0; u < n; u++)
+        tokens(std::integral_constant<int, 1>(), std::true_type(), ks + u * Cfg::UNIT, vs + u * Cfg::UNIT, (u0 + u) * KV4_TOKENS);
     }
+    __syncwarp();                                // all lanes have read the stage
+    if (next < last && !bad) issue(stage);
     if (++stage == Cfg::STAGES) {
       stage = 0;
       phase ^= 1;
@@ -407,7 +425,7 @@ __global__ void __launch_bounds__(32 * D4_WARPS, NT == 1 ? 4 : 3) attn_int4_kern
       acc[0] += a.x * f; acc[1] += a.y * f; acc[2] += a.z * f; acc[3] += a.w * f;
       acc[4] += b.x * f; acc[5] += b.y * f; acc[6] += b.z * f; acc[7] += b.w * f;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;          // a row without keys: zeros
+    const float inv = sum == 0.f ? 0.f : KV4_UNDO / sum;     // a row without keys: zeros
     const int tok = (row0 + i) / p.G, g = row0 + i - tok * p.G;
     if (p.parts == 1) {
       uint4 v;
@@ -502,7 +520,7 @@ B200_API int b200_attn_int4(const void* q, long q_stride, long q_rows, const voi
   p.q_stride = q_stride; p.out_stride = out_stride; p.num_blocks = num_blocks;
   p.num_seqs = num_seqs; p.max_blocks = max_blocks; p.block_size = block_size;
   p.G = G; p.Hkv = Hkv; p.parts = parts; p.causal = causal; p.window = window;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.scale_log2 = scale * 1.4426950408889634f * KV4_UNDO;
   p.status = status;
   const long rows = (long)max_q_len * G;
   if (rows > 0x3fffffffl) return 9886;

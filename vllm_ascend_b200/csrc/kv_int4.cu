@@ -45,8 +45,8 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4Rows p) {
     unit = (keys ? p.k_cache : p.v_cache) +
            ((blk * p.heads + h) * (p.block_size / KV4_TOKENS) + off / KV4_TOKENS) * (long)kv4_unit_bytes(p.D);
   }
-  const int data = (keys ? t : kv4_value_row(t)) * (p.D >> 1) + c8 * 4;
-  const int scale = 8 * p.D + ((c8 >> 2) * KV4_TOKENS + t) * 2;
+  const int data = keys ? kv4_key_word(p.D, t, c8 * 8) : kv4_value_word(p.D, t, c8 * 8) + 2 * (t & 1);
+  const int scale = kv4_scale(p.D, t, c8 >> 2);
   __nv_bfloat16* dense = (__nv_bfloat16*)(keys ? p.k : p.v) + row * (keys ? p.k_stride : p.v_stride) + h * p.D + c8 * 8;
   if (WRITE) {
     uint4 x = make_uint4(0, 0, 0, 0);
@@ -61,12 +61,12 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4Rows p) {
       s16 = 0x7fc0u;                                           // not finite: the whole group is NaN
     } else if (top > 0) {
       uint32_t sb = (__float_as_uint(__fdiv_rn(__uint_as_float(top << 16), 7.f)) + 0x7ffffu) & ~0x7ffffu;
-      sb = min(sb, 0x7c800000u);                               // 2^122: 24 s is finite; larger magnitudes saturate
+      sb = min(max(sb, 0x17800000u), 0x51800000u);             // 2^-80 and 2^36; larger magnitudes saturate
       s16 = sb >> 16;
       const float s = __uint_as_float(sb);
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
       word = 0;
-      if (s >= 1e-30f && sb < 0x7c800000u) {
+      if (sb < 0x51800000u) {
         const float r = 1.f / s;
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -80,13 +80,19 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4Rows p) {
         }
       }
     }
-    *reinterpret_cast<uint32_t*>(unit + data) = word;
+    if (keys) {
+      *reinterpret_cast<uint32_t*>(unit + data) = word;
+    } else {
+      *reinterpret_cast<uint16_t*>(unit + data) = (uint16_t)word;
+      *reinterpret_cast<uint16_t*>(unit + data + 4) = (uint16_t)(word >> 16);
+    }
     if ((c8 & 3) == 0) *reinterpret_cast<uint16_t*>(unit + scale) = (uint16_t)s16;
   } else {
     if (!here) return;
     uint4 x = make_uint4(0, 0, 0, 0);
     if (stored) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(unit + data);
+      const uint32_t w = keys ? *reinterpret_cast<const uint32_t*>(unit + data)
+                              : *reinterpret_cast<const uint16_t*>(unit + data) | (uint32_t)*reinterpret_cast<const uint16_t*>(unit + data + 4) << 16;
       const float s = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(unit + scale) << 16);
       uint32_t o[4];
 #pragma unroll

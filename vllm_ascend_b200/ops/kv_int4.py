@@ -116,7 +116,7 @@ def _parts(blocks: int, max_len: int, sms: int) -> int:
     """Parts that every sequence's keys are split into."""
     if fixed_sums():
         return 1
-    return max(1, min(4 * sms // max(1, blocks), -(-max_len // 128), 64))
+    return max(1, min(3 * sms // max(1, blocks), -(-max_len // 128), 64))
 
 
 def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta, scale: float,

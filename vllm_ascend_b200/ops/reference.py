@@ -264,14 +264,15 @@ KV_INT4_GROUP, KV_INT4_TOKENS = 32, 16
 
 def kv_int4_quantise(x: torch.Tensor):
     """x [..., D] -> whole numbers in -7..7 (int8) [..., D] and scales (bf16) [..., D / 32].  A scale is the smallest number
-    of five significant bits (zero, or a multiple of 2^-130 up to 2^122) with 7 scale >= max |x| over its 32 channels; a group
-    that holds a NaN or an infinity is NaN."""
+    of five significant bits with 7 scale >= max |x| over its 32 channels, between 2^-80 and 2^36 (larger magnitudes saturate), or zero
+    for a group of zeros; a group that holds a NaN or an infinity is NaN."""
     g = x.float().unflatten(-1, (-1, KV_INT4_GROUP))
     top = g.abs().amax(-1, keepdim=True)
     finite = torch.isfinite(top)
     top = torch.where(finite, top, 0.0)
     low = top / torch.full_like(top, 7.0)
-    s = ((low.view(torch.int32) + 0x7ffff) & ~0x7ffff).view(torch.float32).clamp_max(2.0 ** 122)
+    s = ((low.view(torch.int32) + 0x7ffff) & ~0x7ffff).view(torch.float32).clamp(2.0 ** -80, 2.0 ** 36)
+    s = torch.where(top > 0, s, 0.0)
     n = torch.where(finite & (s > 0), g / torch.where(s > 0, s, 1.0), 0.0).clamp(-7, 7).round()
     nan = torch.tensor(0x7fc0, dtype=torch.int16, device=x.device).view(torch.bfloat16)      # the same bits everywhere
     s = torch.where(finite, s.to(torch.bfloat16), nan)
@@ -286,18 +287,21 @@ def kv_int4_block_size(cache: torch.Tensor, dim: int) -> int:
     return cache.shape[2] // unit * KV_INT4_TOKENS
 
 
-def _kv_int4_views(cache: torch.Tensor, dim: int):
-    """Rows [blocks, heads, units, 16, dim / 2] and scales [blocks, heads, units, dim / 32, 16] of a cache."""
+def _kv_int4_views(cache: torch.Tensor, dim: int, values: bool):
+    """Bytes and scales of a cache, [blocks, heads, units, ...] each (csrc/kv_int4.cuh has the layout).  Keys: [token, byte], values:
+    [pair of tokens, chunk, word, token of the pair, byte]; scales [group, token]."""
     B, H, _ = cache.shape
     units = kv_int4_block_size(cache, dim) // KV_INT4_TOKENS
-    rows = cache.view(B, H, units, 9 * dim)[..., :8 * dim].unflatten(-1, (KV_INT4_TOKENS, dim // 2))
+    data = cache.view(B, H, units, 9 * dim)[..., :8 * dim]
     scales = cache.view(torch.bfloat16).view(B, H, units, 9 * dim // 2)[..., 4 * dim:]
-    return rows, scales.unflatten(-1, (dim // KV_INT4_GROUP, KV_INT4_TOKENS))
+    data = data.unflatten(-1, (8, dim // 16, 4, 2, 2) if values else (KV_INT4_TOKENS, dim // 2))
+    return data, scales.unflatten(-1, (dim // KV_INT4_GROUP, KV_INT4_TOKENS))
 
 
-def _kv_int4_row(t: torch.Tensor, values: bool) -> torch.Tensor:
-    """Row of token t of a unit: keys lie in order, values with the even tokens of each eight first."""
-    return (t & 8) | ((t & 1) << 2) | ((t >> 1) & 3) if values else t
+def _kv_int4_chunks(pair: torch.Tensor, dim: int) -> torch.Tensor:
+    """Where chunk 0, 1, ... of a pair's values lie: [tokens, chunks]."""
+    swizzle = 2 * (pair & 3) if dim == 128 else pair & 2
+    return torch.arange(dim // 16, device=pair.device) ^ swizzle.unsqueeze(-1)
 
 
 def write_kv_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor) -> None:
@@ -307,11 +311,17 @@ def write_kv_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     at = slots[valid]
     blk, off = at // bs, at % bs
     unit, t = off // KV_INT4_TOKENS, off % KV_INT4_TOKENS
+    heads = torch.arange(k.shape[1], device=k.device).view(1, -1, 1)
     for x, cache, values in ((k, k_cache, False), (v, v_cache, True)):
-        rows, scales = _kv_int4_views(cache, dim)
+        data, scales = _kv_int4_views(cache, dim, values)
         n, s = kv_int4_quantise(x[valid])
         n = (n + 8).to(torch.uint8)
-        rows[blk, :, unit, _kv_int4_row(t, values)] = n[..., 0::2] | (n[..., 1::2] << 4)
+        n = n[..., 0::2] | (n[..., 1::2] << 4)                                   # bytes of two channels, in order
+        if values:
+            b, u, pair, half = (i.view(-1, 1, 1) for i in (blk, unit, t >> 1, t & 1))
+            data[b, heads, u, pair, _kv_int4_chunks(t >> 1, dim).unsqueeze(1), :, half] = n.unflatten(-1, (dim // 16, 4, 2))
+        else:
+            data[blk, :, unit, t] = n
         scales[blk, :, unit, :, t] = s
 
 
@@ -321,11 +331,17 @@ def read_kv_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tens
     blk, off = at // bs, at % bs
     unit, t = off // KV_INT4_TOKENS, off % KV_INT4_TOKENS
     out = []
+    heads = torch.arange(k_cache.shape[1], device=slots.device).view(1, -1, 1)
     for cache, values in ((k_cache, False), (v_cache, True)):
-        rows, scales = _kv_int4_views(cache, dim)
-        w = rows[blk, :, unit, _kv_int4_row(t, values)]
+        data, scales = _kv_int4_views(cache, dim, values)
+        if values:
+            b, u, pair, half = (i.view(-1, 1, 1) for i in (blk, unit, t >> 1, t & 1))
+            w = data[b, heads, u, pair, _kv_int4_chunks(t >> 1, dim).unsqueeze(1), :, half].flatten(-3)
+        else:
+            w = data[blk, :, unit, t]
+        s = scales[blk, :, unit, :, t]
         n = torch.stack((w & 15, w >> 4), -1).flatten(-2).float() - 8
-        x = (n.unflatten(-1, (-1, KV_INT4_GROUP)) * scales[blk, :, unit, :, t].float().unsqueeze(-1)).flatten(-2)
+        x = (n.unflatten(-1, (-1, KV_INT4_GROUP)) * s.float().unsqueeze(-1)).flatten(-2)
         out.append(torch.where((slots >= 0).view(-1, 1, 1), x, 0.0).to(dtype))
     return tuple(out)
 
