@@ -303,3 +303,77 @@ def test_graph_replay_with_other_lengths_and_another_stream():
         again = ops.paged_attention_int4(q, kc, vc, meta, 0.09)
     side.synchronize()
     assert torch.equal(again, out)
+
+
+# ---------------------------------------------------------------- prompts
+@pytest.mark.parametrize("Hq,Hkv,D,page,window,causal", [
+    (8, 2, 128, 128, 0, True), (4, 4, 128, 16, 0, True), (28, 4, 64, 16, 0, True), (16, 1, 128, 48, 0, True), (6, 2, 64, 128, 0, True),
+    (8, 1, 128, 64, 100, True), (8, 2, 64, 32, 1, True), (4, 2, 128, 256, 0, False), (5, 1, 128, 32, 300, True), (2, 2, 64, 128, 77, True)])
+def test_prompts(Hq, Hkv, D, page, window, causal):
+    tile = 128 // (Hq // Hkv)
+    new = [20, tile - 1, tile, tile + 1, 2 * tile, 2 * tile + 1, 300, 17, 3]
+    old = [0, 5, 0, 200, 129, 0, 77, 640, 250]
+    q, kc, vc, meta = _setup(new, [a + b for a, b in zip(new, old)], page, Hq, Hkv, D, Hq + page + window)
+    scale = 1.3 * D ** -0.5
+    out = ops.paged_attention_int4(q, kc, vc, meta, scale, causal=causal, window=window)
+    _check(out, *_want(q, kc, vc, meta, scale, window, causal))
+    _native.check_status(torch.device(DEV))
+
+
+@pytest.mark.parametrize("D,Hq,Hkv", [(128, 8, 2), (64, 16, 4)])
+def test_mixed_batches(D, Hq, Hkv):
+    """Decodes in front of prompts, a short sequence behind them, tokens behind the last sequence."""
+    new, old = [1, 1, 1, 2, 130, 1, 700, 9], [5, 300, 1000, 64, 0, 90, 333, 2000]
+    q, kc, vc, meta = _setup(new, [a + b for a, b in zip(new, old)], 32, Hq, Hkv, D, 21)
+    want, tol = _want(q, kc, vc, meta, 0.1)
+    q = torch.cat([q, torch.full((5, Hq, D), float("nan"), device=DEV, dtype=torch.bfloat16)])
+    out = torch.full_like(q, 3.0)
+    ops.paged_attention_int4(q, kc, vc, meta, 0.1, out=out)
+    _check(out[:-5], want, tol)
+    assert out[-5:].eq(3).all()
+
+
+def test_a_long_portion_behind_a_long_context():
+    q, kc, vc, meta = _setup([333], [20333], 128, 8, 2, 128, 22)
+    _check(ops.paged_attention_int4(q, kc, vc, meta, 0.09), *_want(q, kc, vc, meta, 0.09))
+
+
+def test_prompt_tokens_that_see_no_key():
+    """More new tokens than keys: those in front of the first key get zeros."""
+    q, kc, vc, meta = _setup([300, 40, 64], [20, 0, 64], 16, 8, 2, 128, 23)
+    out = ops.paged_attention_int4(q, kc, vc, meta, 0.1)
+    assert not out[:280].any() and not out[300:340].any()
+    _check(out, *_want(q, kc, vc, meta, 0.1))
+
+
+@pytest.mark.parametrize("window,D", [(0, 128), (200, 128), (0, 64)])
+def test_nan_values_reach_the_prompt_rows_that_see_them(window, D):
+    new, old, page = [260, 70], [500, 3], 32
+    q, kc, vc, meta = _setup(new, [a + b for a, b in zip(new, old)], page, 8, 2, D, 24)
+    spots = [(0, 10), (0, 300), (0, 500), (0, 640), (0, 758), (1, 2), (1, 60)]
+    slots = torch.stack([meta.block_table[b, t // page].long() * page + t % page for b, t in spots])
+    ones = torch.ones(len(spots), 2, D, device=DEV, dtype=torch.bfloat16)
+    ops.write_kv_int4(ones, ones, kc, vc, slots)
+    want, tol = _want(q, kc, vc, meta, 0.1, window)
+    bad = ones.clone()
+    bad[:, 1, 37] = float("nan")
+    ops.write_kv_int4(ones, bad, kc, vc, slots)
+    out = ops.paged_attention_int4(q, kc, vc, meta, 0.1, window=window)
+    hit = torch.zeros_like(want, dtype=torch.bool)
+    starts = [0, 260]
+    for b, t in spots:
+        pos = torch.arange(old[b], old[b] + new[b], device=DEV)
+        sees = (pos >= t) & ((pos < t + window) if window else True)
+        hit[starts[b]:starts[b] + new[b], 4:, 32:64] |= sees.view(-1, 1, 1)
+    assert out.isnan().equal(hit)
+    _check(torch.where(hit, 0.0, out), torch.where(hit, 0.0, want), tol)
+
+
+def test_prompt_pages_outside_of_the_cache_are_reported():
+    q, kc, vc, meta = _setup([200, 100], [300, 100], 16, 8, 2, 128, 25)
+    good = ops.paged_attention_int4(q, kc, vc, meta, 0.1)
+    meta.block_table[0, 7] = -3
+    out = ops.paged_attention_int4(q, kc, vc, meta, 0.1)
+    with pytest.raises(_native.NativeError, match="BAD_INDEX"):
+        _native.check_status(torch.device(DEV))
+    assert torch.equal(out[200:], good[200:])

@@ -13,7 +13,7 @@
 // A block is one (sequence, KV head, part of the sequence); each of its warps walks a stretch of it, in tiles of 64 (32) tokens where
 // all rows see them and 16 at a time at the edges, through a ring of its own that bulk copies fill, with a running maximum of
 // its own; they join at the end.  Parts join in a second kernel.
-#include "kv_int4.cuh"
+#include "attention_int4.cuh"
 
 #include <type_traits>
 
@@ -21,23 +21,6 @@ namespace b200 {
 
 constexpr int D4_WARPS = 4;
 
-struct Int4Params {
-  const __nv_bfloat16* q;
-  const uint8_t *k_cache, *v_cache;
-  const int *cu, *seq_lens, *block_table;
-  __nv_bfloat16* out;
-  float *part_o, *part_lse;       // [tokens x heads][parts][D], [..][parts]: results of parts, normalised, with log2 of their sums
-  long q_stride, out_stride, num_blocks;
-  int num_seqs, max_blocks, block_size, G, Hkv, parts, row_blocks, causal, window;
-  float scale_log2;
-  int* status;
-};
-
-__device__ __forceinline__ float i4_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void i4_mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -48,12 +31,6 @@ __device__ __forceinline__ uint32_t i4_transpose(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ void i4_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
-               "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
 template <int D, int NT>
 struct Int4Cfg {
   static constexpr int U = NT == 1 ? 4 : 2;              // units of a tile
@@ -487,8 +464,43 @@ static int launch_int4(Int4Params p, int max_rows, cudaStream_t stream) {
   if (e != cudaSuccess) return (int)e;
   p.row_blocks = (max_rows + Cfg::ROWS - 1) / Cfg::ROWS;
   const long x = (long)p.num_seqs * p.row_blocks;
-  if (x > 0x7fffffffl || p.Hkv > 65535 || p.parts > 65535) return 9886;
+  if (x > 0x7fffffffl || p.Hkv > 65535) return 9886;
   attn_int4_kernel<D, NT><<<dim3((unsigned)x, (unsigned)p.Hkv, (unsigned)p.parts), 32 * D4_WARPS, Cfg::SMEM, stream>>>(p);
+  return B200_CHECK_LAUNCH();
+}
+
+int int4_params(Int4Params* p, const void* q, long q_stride, long q_rows, const void* k_cache, const void* v_cache, long num_blocks, int block_size,
+                const void* cu, const void* seq_lens, const void* block_table, int max_blocks, int num_seqs, int Hq, int Hkv, int D,
+                float scale, int causal, int window, int parts, void* out, long out_stride, void* scratch, int* status) {
+  const int G = Hkv > 0 ? Hq / Hkv : 0;
+  if (G < 1 || G * Hkv != Hq || (D != 64 && D != 128)) return 9883;
+  if (block_size < KV4_TOKENS || block_size % KV4_TOKENS) return 9884;
+  if ((q_stride & 7) || (out_stride & 7) || parts < 1 || parts > 65535 || (parts > 1 && !scratch)) return 9885;
+  *p = Int4Params{};
+  p->q = (const __nv_bfloat16*)q;
+  p->k_cache = (const uint8_t*)k_cache;
+  p->v_cache = (const uint8_t*)v_cache;
+  p->cu = (const int*)cu;
+  p->seq_lens = (const int*)seq_lens;
+  p->block_table = (const int*)block_table;
+  p->out = (__nv_bfloat16*)out;
+  p->part_o = (float*)scratch;
+  p->part_lse = p->part_o + q_rows * Hq * parts * D;
+  p->q_stride = q_stride; p->out_stride = out_stride; p->num_blocks = num_blocks;
+  p->num_seqs = num_seqs; p->max_blocks = max_blocks; p->block_size = block_size;
+  p->G = G; p->Hkv = Hkv; p->parts = parts; p->causal = causal; p->window = window;
+  p->scale_log2 = scale * 1.4426950408889634f * KV4_UNDO;
+  p->status = status;
+  return 0;
+}
+
+int int4_join(const Int4Params& p, int D, long q_rows, cudaStream_t stream) {
+  const int heads = p.G * p.Hkv;
+  const long all = q_rows * heads;
+  if ((all + 3) / 4 > 0x7fffffffl) return 9886;
+  const unsigned blocks = (unsigned)((all + 3) / 4);
+  if (D == 128) attn_int4_join_kernel<128><<<blocks, 128, 0, stream>>>(p.part_o, p.part_lse, p.cu, p.num_seqs, heads, p.parts, all, p.out, p.out_stride);
+  else attn_int4_join_kernel<64><<<blocks, 128, 0, stream>>>(p.part_o, p.part_lse, p.cu, p.num_seqs, heads, p.parts, all, p.out, p.out_stride);
   return B200_CHECK_LAUNCH();
 }
 
@@ -503,36 +515,13 @@ B200_API int b200_attn_int4(const void* q, long q_stride, long q_rows, const voi
                             int max_q_len, int Hq, int Hkv, int D, float scale, int causal, int window, int parts, void* out,
                             long out_stride, void* scratch, int* status, cudaStream_t stream) {
   if (num_seqs <= 0 || q_rows <= 0 || max_q_len <= 0) return 0;
-  const int G = Hkv > 0 ? Hq / Hkv : 0;
-  if (G < 1 || G * Hkv != Hq || (D != 64 && D != 128)) return 9883;
-  if (block_size < KV4_TOKENS || block_size % KV4_TOKENS) return 9884;
-  if ((q_stride & 7) || (out_stride & 7) || parts < 1 || (parts > 1 && !scratch)) return 9885;
-  Int4Params p = {};
-  p.q = (const __nv_bfloat16*)q;
-  p.k_cache = (const uint8_t*)k_cache;
-  p.v_cache = (const uint8_t*)v_cache;
-  p.cu = (const int*)cu;
-  p.seq_lens = (const int*)seq_lens;
-  p.block_table = (const int*)block_table;
-  p.out = (__nv_bfloat16*)out;
-  p.part_o = (float*)scratch;
-  p.part_lse = p.part_o + q_rows * Hq * parts * D;
-  p.q_stride = q_stride; p.out_stride = out_stride; p.num_blocks = num_blocks;
-  p.num_seqs = num_seqs; p.max_blocks = max_blocks; p.block_size = block_size;
-  p.G = G; p.Hkv = Hkv; p.parts = parts; p.causal = causal; p.window = window;
-  p.scale_log2 = scale * 1.4426950408889634f * KV4_UNDO;
-  p.status = status;
-  const long rows = (long)max_q_len * G;
+  Int4Params p;
+  int rc = int4_params(&p, q, q_stride, q_rows, k_cache, v_cache, num_blocks, block_size, cu, seq_lens, block_table, max_blocks, num_seqs,
+                       Hq, Hkv, D, scale, causal, window, parts, out, out_stride, scratch, status);
+  if (rc) return rc;
+  const long rows = (long)max_q_len * p.G;
   if (rows > 0x3fffffffl) return 9886;
-  int rc;
   if (D == 128) rc = rows <= 8 ? launch_int4<128, 1>(p, (int)rows, stream) : launch_int4<128, 2>(p, (int)rows, stream);
   else rc = rows <= 8 ? launch_int4<64, 1>(p, (int)rows, stream) : launch_int4<64, 2>(p, (int)rows, stream);
-  if (rc || parts == 1) return rc;
-  const long all = q_rows * Hq;
-  const unsigned blocks = (unsigned)((all + 3) / 4);
-  if (D == 128)
-    attn_int4_join_kernel<128><<<blocks, 128, 0, stream>>>(p.part_o, p.part_lse, p.cu, num_seqs, Hq, parts, all, p.out, out_stride);
-  else
-    attn_int4_join_kernel<64><<<blocks, 128, 0, stream>>>(p.part_o, p.part_lse, p.cu, num_seqs, Hq, parts, all, p.out, out_stride);
-  return B200_CHECK_LAUNCH();
+  return rc || parts == 1 ? rc : int4_join(p, D, q_rows, stream);
 }

@@ -10,6 +10,7 @@ from __future__ import annotations
 from ctypes import c_float, c_int, c_long, c_void_p
 from typing import Optional
 
+import numpy as np
 import torch
 
 from .. import _native
@@ -22,7 +23,12 @@ _native.register_signature("b200_kv_int4_write", [_P, _L, _P, _L, _L, _P, _P, _P
 _native.register_signature("b200_kv_int4_read", [_P, _P, _L, _P, _P, _P, _L, _I, _I, _I, _P, _P])
 _native.register_signature("b200_attn_int4", [_P, _L, _L, _P, _P, _L, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P, _L, _P, _P, _P])
 
+_native.register_signature("b200_attn_int4_prefill",
+                           [_P, _L, _L, _P, _P, _L, _I, _P, _P, _P, _I, _I, _L, _I, _I, _I, _F, _I, _I, _I, _P, _L, _P, _P, _P])
+
 HEAD_SIZES = (64, 128)
+#: rows (new tokens times heads of a group) of a sequence up to which the kernel for few rows takes it
+FEW_ROWS = 16
 
 _scratch = Scratch(torch.float32)
 
@@ -148,8 +154,17 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     if out.stride(2) != 1 or out.stride(1) != D or out.stride(0) % 8 or out.data_ptr() % 16:
         out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
         out.copy_(given)
+    G = Hq // Hkv
     with torch.cuda.device(q.device):
-        _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, n, meta.max_query_len)
+        few = n
+        if meta.max_query_len * G > FEW_ROWS and G <= 128:
+            new = np.diff(meta.query_start_loc_cpu[:n + 1])
+            many = new * G > FEW_ROWS
+            few = int(many.argmax()) if many.any() else n      # sequences in front of the first that the other kernel takes
+        if few:
+            _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, few, meta.max_query_len if few == n else int(new[:few].max()))
+        if few < n:
+            _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, few, new[few:])
     return out if out is given else given.copy_(out)
 
 
@@ -166,4 +181,21 @@ def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, n, max_
         meta.block_table.data_ptr(), meta.block_table.stride(0), n, max_q, Hq, Hkv, D, scale, int(causal), int(window), parts,
         out.data_ptr(), out.stride(0), _native.ptr(scratch), _native.status_word(q.device).data_ptr(), _native.stream_ptr())
     _native.check(rc, "attn_int4")
+    _native.count_launch(1 + int(parts > 1))
+
+
+def _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, new) -> None:
+    """The sequences from ``first`` on, with ``new`` new tokens."""
+    T, Hq, D = q.shape
+    NB, Hkv, _ = k_cache.shape
+    row, pair = int(meta.query_start_loc_cpu[first]), 2 * (128 // (Hq // Hkv))
+    blocks = int((-(-new // pair)).sum()) * Hkv
+    parts = 1 if fixed_sums() else max(1, min(_native.sm_count(q.device) // max(1, blocks), meta.max_seq_len // 512))
+    scratch = _scratch.get(q.device, T * Hq * parts * (D + 1)) if parts > 1 else None
+    rc = _native.lib().b200_attn_int4_prefill(
+        q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, meta.query_start_loc[first:].data_ptr(),
+        meta.seq_lens[first:].data_ptr(), meta.block_table[first:].data_ptr(), meta.block_table.stride(0), meta.num_reqs - first, T - row,
+        Hq, Hkv, D, scale, int(causal), int(window), parts, out.data_ptr(), out.stride(0), _native.ptr(scratch),
+        _native.status_word(q.device).data_ptr(), _native.stream_ptr())
+    _native.check(rc, "attn_int4_prefill")
     _native.count_launch(1 + int(parts > 1))
