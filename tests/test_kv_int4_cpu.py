@@ -21,7 +21,7 @@ def _definition(group):
     while Fraction(31) * Fraction(2) ** e * 7 < top:              # scales of five bits: m 2^e, 16 <= m <= 31
         e += 1
     s = next(m * Fraction(2) ** e for m in range(1, 32) if 7 * m * Fraction(2) ** e >= top)
-    s = min(max(s, Fraction(2) ** -80), Fraction(2) ** 36)
+    s = min(max(s, Fraction(2) ** -80), Fraction(2) ** 34)
     return s, [min(max(round(v / s), -7), 7) for v in x]          # round(): ties to even
 
 
@@ -52,7 +52,7 @@ def test_quantiser_at_the_edges_of_the_type():
     n, s = ref.kv_int4_quantise(x)
     assert s[0, 0].isnan() and not n[0].any() and s[0, 1] == 0
     assert s[1, 1].isnan() and s[1, 0] == 0
-    assert (s[2] == 2.0 ** 36).all() and (n[2] == 7).all()
+    assert (s[2] == 2.0 ** 34).all() and (n[2] == 7).all()
     assert s[3, 0].float() == 2.0 ** -80                                  # the smallest scale: n is 0, within half a scale still
     assert (x[3, 0].double() - n[3, 0] * s[3, 0].double()).abs() <= s[3, 0].double() / 2
     assert s[5].eq(0).all() and not n[5].any() and n[4, 1] == -7

@@ -3,8 +3,8 @@
 // Two query tiles of 128 rows (row = token * G + head of the group) share every tile of 128 keys, a warpgroup each, as in the kernel over
 // bf16 pages (attention_prefill.cu, which has the reasons for that split).  Keys and values come packed by bulk copies, a quarter of
 // the bytes, and a third warpgroup unpacks them into the swizzled tiles that the tensor cores read:
-//   warps 0..3, 4..7   softmax and epilogue of query tile 0, 1 (one thread per row)
-//   warps 8..11        queries into shared memory, then keys and values out of the packed ring into their tiles
+//   warps 0..3, 4..7   queries, softmax and epilogue of query tile 0, 1 (one thread per row)
+//   warps 8..11        keys and values out of the packed ring into their tiles
 //   warp 12            packed tiles into the ring;  warp 13  MMA issuer
 // Unpacking 128 keys and values costs the four warps some 480 instructions each, next to the 128 exponentials a thread that bound the
 // softmax warps; without it those pages would cost a pass of their own that writes and reads four times the bytes.
@@ -42,38 +42,9 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
   using Cfg = Int4PrefillCfg<D>;
   constexpr int NK = Cfg::NK, TILE = Cfg::TILE, UNIT = Cfg::UNIT, O_COL = 256;
 
-  // ---------------- work item: a pair of query tiles and a part of their keys; late pairs see more keys and come first
-  const int h = blockIdx.x, G = p.G, tpt = 128 / G, part = blockIdx.z;
-  const int wi = gridDim.y - 1 - blockIdx.y, pair = 2 * tpt, base = p.cu[0];
-  int lo_s = 0, hi_s = p.num_seqs - 1;
-  while (lo_s < hi_s) {
-    const int mid = (lo_s + hi_s + 1) >> 1;
-    if ((p.cu[mid] - base) / pair + mid <= wi) lo_s = mid; else hi_s = mid - 1;
-  }
-  const int seq = lo_s;
-  const int tok0 = (wi - ((p.cu[seq] - base) / pair + seq)) * pair;
-  const int q_start = p.cu[seq], q_len = p.cu[seq + 1] - q_start, seq_len = p.seq_lens[seq], ctx = seq_len - q_len;
-  if (tok0 >= q_len) return;
-  int ntok[2], t_end[2];
-#pragma unroll
-  for (int w = 0; w < 2; w++) {
-    ntok[w] = max(0, min(tpt, q_len - tok0 - w * tpt));
-    const int end = p.causal ? min(seq_len, ctx + tok0 + w * tpt + ntok[w]) : seq_len;
-    t_end[w] = ntok[w] > 0 ? max(0, end + 127) >> 7 : 0;
-  }
-  const int key_lo = p.window > 0 ? max(0, ctx + tok0 - p.window + 1) : 0;                     // keys that any row sees
-  const int key_hi = p.causal ? min(seq_len, ctx + tok0 + ntok[0] + ntok[1]) : seq_len;
-  const int t_lo = key_lo >> 7, all = max(0, max(t_end[0], t_end[1]) - t_lo);
-  const int t_a = t_lo + (int)((long)all * part / p.parts), t_b = t_lo + (int)((long)all * (part + 1) / p.parts);
-  const int n = t_b - t_a;
-  const int n0 = max(0, min(t_b, t_end[0]) - t_a), n1 = max(0, min(t_b, t_end[1]) - t_a);      // key tiles of each query tile
-  auto note_slot = [&](int tile) {            // where a tile's values that are no numbers are noted; -1: nowhere
-    const int i = tile - t_lo;
-    return i < P4_EDGE ? i : i >= all - P4_EDGE ? i - (all - 2 * P4_EDGE) : -1;
-  };
-
-  const int warp = warp_index(), lane = threadIdx.x & 31;
   extern __shared__ uint8_t smem_raw[];
+  __shared__ int item[4];                     // sequence, its first query row, query rows, keys
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* Qs = smem;
   uint8_t* Ks = Qs + 2 * TILE;
@@ -94,8 +65,22 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
   uint32_t* tmem_ptr = (uint32_t*)(bars + 21);
   volatile int* abort_word = (volatile int*)(tmem_ptr + 1);
   volatile int* noted = (volatile int*)(tmem_ptr + 2);
+
+  // ---------------- work item: a pair of query tiles and a part of their keys; late pairs see more keys and come first.  Pairs of
+  // sequence i begin at (cu[i] - base) / pair + i; the thread whose sequence has this one says so
+  const int h = blockIdx.x, G = p.G, tpt = 128 / G, part = blockIdx.z;
+  const int wi = gridDim.y - 1 - blockIdx.y, pair = 2 * tpt, base = p.cu[0];
+  for (int i = threadIdx.x; i < p.num_seqs; i += P4_THREADS) {
+    const int from = p.cu[i], to = p.cu[i + 1], keys = p.seq_lens[i];
+    if ((from - base) / pair + i <= wi && (i + 1 == p.num_seqs || (to - base) / pair + i + 1 > wi)) {
+      item[0] = i;
+      item[1] = from;
+      item[2] = to - from;
+      item[3] = keys;
+    }
+  }
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 4);
+    mbar_init(q_full, 8);
     for (int b = 0; b < 2; b++) {
       mbar_init(&k_full[b], 4);
       mbar_init(&k_empty[b], 1);
@@ -122,6 +107,29 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = warp_uniform(*tmem_ptr);
+  const int seq = item[0], q_start = item[1], q_len = item[2], seq_len = item[3], ctx = seq_len - q_len;
+  const int tok0 = (wi - ((q_start - base) / pair + seq)) * pair;
+  if (tok0 >= q_len) {                        // the grid has a pair more than some sequences
+    if (warp == 13) tmem_dealloc(tmem_base, 512);
+    return;
+  }
+  int ntok[2], t_end[2];
+#pragma unroll
+  for (int w = 0; w < 2; w++) {
+    ntok[w] = max(0, min(tpt, q_len - tok0 - w * tpt));
+    const int end = p.causal ? min(seq_len, ctx + tok0 + w * tpt + ntok[w]) : seq_len;
+    t_end[w] = ntok[w] > 0 ? max(0, end + 127) >> 7 : 0;
+  }
+  const int key_lo = p.window > 0 ? max(0, ctx + tok0 - p.window + 1) : 0;                     // keys that any row sees
+  const int key_hi = p.causal ? min(seq_len, ctx + tok0 + ntok[0] + ntok[1]) : seq_len;
+  const int t_lo = key_lo >> 7, all = max(0, max(t_end[0], t_end[1]) - t_lo);
+  const int t_a = t_lo + (int)((long)all * part / p.parts), t_b = t_lo + (int)((long)all * (part + 1) / p.parts);
+  const int n = t_b - t_a;
+  const int n0 = max(0, min(t_b, t_end[0]) - t_a), n1 = max(0, min(t_b, t_end[1]) - t_a);      // key tiles of each query tile
+  auto note_slot = [&](int tile) {            // where a tile's values that are no numbers are noted; -1: nowhere
+    const int i = tile - t_lo;
+    return i < P4_EDGE ? i : i >= all - P4_EDGE ? i - (all - 2 * P4_EDGE) : -1;
+  };
 
   // 512 threads of 128 registers; 256 x 184 + 128 x 96 + 128 x 40 are no more than that
   if (warp >= 12) {
@@ -203,28 +211,10 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
       }
     }
   } else if (warp >= 8) {
-    // ------------------------------------------------------------ queries, then unpacking
+    // ------------------------------------------------------------ unpacking
     p4_fewer_registers<96>();
     if (n > 0) {
-      const int wl = warp - 8, tid = threadIdx.x - 256;
-#pragma unroll 4
-      for (int i = tid; i < 256 * (D / 8); i += 128) {
-        const int row = i / (D / 8), c8 = i - row * (D / 8), w = row >> 7, rr = row & 127;
-        const int tok = rr / G, g = rr - tok * G;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (tok < ntok[w])
-          x = *reinterpret_cast<const uint4*>(p.q + (long)(q_start + tok0 + w * tpt + tok) * p.q_stride + (long)(h * G + g) * D + c8 * 8);
-        uint4 y;                                 // channels j and j + 4 side by side
-        y.x = __byte_perm(x.x, x.z, 0x5410);
-        y.y = __byte_perm(x.x, x.z, 0x7632);
-        y.z = __byte_perm(x.y, x.w, 0x5410);
-        y.w = __byte_perm(x.y, x.w, 0x7632);
-        *reinterpret_cast<uint4*>(Qs + w * TILE + (c8 >> 3) * P4_HALF + rr * 128 + (((c8 & 7) ^ (rr & 7)) << 4)) = y;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-
+      const int wl = warp - 8;
       for (int j = 0; j < n; j++) {
         const int st = j & 1, slot_n = note_slot(t_a + j);
 #pragma unroll 1
@@ -239,7 +229,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
             constexpr int Q = D / 32, RP = 32 / Q;          // lanes of a row, rows of a warp's pass
             const int q = lane % Q;
             uint8_t* dst = Ks + st * TILE + (q >> 1) * P4_HALF;
-#pragma unroll
+#pragma unroll 2
             for (int pass = 0; pass < 128 / (4 * RP); pass++) {
               const int row = (pass * 4 + wl) * RP + lane / Q, t = row & 15;
               const uint8_t* unit = src + (row >> 4) * UNIT;
@@ -260,7 +250,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
             constexpr int Q = D / 16, RP = 32 / Q;          // lanes of a pair, pairs of a warp's pass
             const int q = lane % Q;
             uint8_t* dst = Vs + st * TILE + (q >> 2) * P4_HALF;
-#pragma unroll
+#pragma unroll 2
             for (int pass = 0; pass < 64 / (4 * RP); pass++) {
               const int pr = (pass * 4 + wl) * RP + lane / Q, t = 2 * (pr & 7), row = 2 * pr, key = (t_a + j) * 128 + row;
               const uint8_t* unit = src + (row >> 4) * UNIT;
@@ -312,6 +302,35 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
     p4_more_registers<184>();
     const int w = warp >> 2;
     const int nw = w == 0 ? n0 : n1, nt = w == 0 ? ntok[0] : ntok[1];
+    {
+      // its queries, channels j and j + 4 side by side; eight lanes take a slab's row
+      uint8_t* dst = Qs + w * TILE;
+      const int c8 = lane & 7;
+#pragma unroll
+      for (int s = 0; s < NK; s++) {
+        uint4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int rr = (warp & 3) * 32 + i * 4 + (lane >> 3), tok = rr / G, g = rr - tok * G;
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (tok < nt)
+            x[i] = *reinterpret_cast<const uint4*>(p.q + (long)(q_start + tok0 + w * tpt + tok) * p.q_stride + (long)(h * G + g) * D + s * 64 + c8 * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int rr = (warp & 3) * 32 + i * 4 + (lane >> 3);
+          uint4 y;
+          y.x = __byte_perm(x[i].x, x[i].z, 0x5410);
+          y.y = __byte_perm(x[i].x, x[i].z, 0x7632);
+          y.z = __byte_perm(x[i].y, x[i].w, 0x5410);
+          y.w = __byte_perm(x[i].y, x[i].w, 0x7632);
+          *reinterpret_cast<uint4*>(dst + s * P4_HALF + rr * 128 + ((c8 ^ (rr & 7)) << 4)) = y;
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
     if (nt > 0) {
       const int row = (warp & 3) * 32 + lane;
       const int tok = row / G, g = row - tok * G;
@@ -337,12 +356,15 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
         tmem_ld_32x32b_x32(t_s + 96, sreg + 96);
         tmem_ld_wait();
         const int key0 = (t_a + j) << 7;
-        if (key0 + 128 > all_hi || key0 < all_lo) {
+        if (key0 + 128 > all_hi) {
+          const int end = k_hi - key0;
 #pragma unroll
-          for (int i = 0; i < 128; i++) {
-            const int key = key0 + i;
-            if (key < k_lo || key >= k_hi) sreg[i] = 0xff800000u;   // -inf
-          }
+          for (int i = 0; i < 128; i++) if (i >= end) sreg[i] = 0xff800000u;   // -inf
+        }
+        if (key0 < all_lo) {
+          const int start = k_lo - key0;
+#pragma unroll
+          for (int i = 0; i < 128; i++) if (i < start) sreg[i] = 0xff800000u;
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll

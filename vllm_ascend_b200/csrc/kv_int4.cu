@@ -1,118 +1,177 @@
 // Rows of keys and values into a 4-bit cache and back (format: kv_int4.cuh).
 //
-// Bound: memory.  A thread takes 8 channels of a row (16 bytes dense, 4 packed), four threads share a group and find its
-// largest magnitude as whole numbers (the bits of |bf16| order as its values do, NaN and infinities above all numbers).
+// Bound: memory.  A thread keeps to 8 channels (16 bytes dense, 4 packed) and walks rows, keys and values of two rows in flight at once; what
+// a row's slot means is found once for the block.  Four threads share a group and find its largest magnitude as whole
+// numbers (the bits of |bf16| order as its values do, NaN and infinities above all numbers).
 #include "kv_int4.cuh"
 
 namespace b200 {
+
+constexpr int KV4_ROWS_THREADS = 256;
+constexpr int KV4_ROWS_MAX = 256;           // of a block
 
 struct Kv4Rows {
   void *k, *v;                    // [rows, heads, D] bf16, heads dense; written by the read
   uint8_t *k_cache, *v_cache;
   const long long* slots;
   long k_stride, v_stride, rows, num_slots;
-  int heads, D, block_size;
+  int heads, D, block_size, rows_per_block;
   int* status;
 };
 
-// x / s for a group's scale, to the nearest whole number, ties to even.  With 8 significant bits of x and 5 of s a quotient that is no
-// tie lies at least 2^-11 from one, so the product with the reciprocal (off by less than 2^-20) is first rounded to a multiple of
-// 2^-13, which puts ties back where they are.
+// x / s to the nearest whole number, ties to even, plus 8.  With 8 significant bits of x and 5 of s a quotient that is no
+// tie lies at least 2^-11 from one, so the product with an approximate reciprocal (off by less than 2^-18) is first rounded to a
+// multiple of 2^-13, which puts ties back where they are.
 __device__ __forceinline__ uint32_t kv4_code(float x, float r) {
   const float q = fmaf(x, r, 1536.f) - 1536.f;
   return __float_as_uint(q + 12582920.f) & 15u;      // 1.5 2^23 + 8
 }
 
-template <bool WRITE>
-__global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4Rows p) {
-  const int per_head = p.D >> 3, per_row = p.heads * per_head;
-  const long first = (long)blockIdx.x * 256;
-  const long row0 = first / per_row;                           // the same in all threads
-  const int in_row = (int)(first - row0 * per_row) + threadIdx.x;
-  const long row = row0 + in_row / per_row;
-  const int item = in_row % per_row, h = item / per_head, c8 = item - h * per_head;
-  const bool here = row < p.rows;
-  const bool keys = blockIdx.y == 0;
-  const long long slot = here ? p.slots[row] : -1;
-  const bool stored = slot >= 0 && slot < p.num_slots;
-  if (here && slot >= p.num_slots && p.status) atomicExch(p.status, B200_BAD_INDEX);
-  uint8_t* unit = nullptr;
-  int t = 0;
-  if (stored) {
-    const long blk = slot / p.block_size;
-    const int off = (int)(slot - blk * p.block_size);
-    t = off % KV4_TOKENS;
-    unit = (keys ? p.k_cache : p.v_cache) +
-           ((blk * p.heads + h) * (p.block_size / KV4_TOKENS) + off / KV4_TOKENS) * (long)kv4_unit_bytes(p.D);
+// Eight channels (x) of a group to a word; s16 receives the group's scale as bf16.  All lanes of a warp call it.
+__device__ __forceinline__ uint32_t kv4_quantise(const uint4& x, uint32_t& s16) {
+  uint32_t top = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+  top = max(top & 0xffffu, top >> 16);
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  s16 = top >= 0x7f80u ? 0x7fc0u : 0u;                         // not finite: the whole group is NaN
+  if (top == 0 || top >= 0x7f80u) return 0x88888888u;
+  // top = m 2^(e - 134), m of eight bits; the smallest five-bit number from m / 7 on is ceil(m / 7) up to 31, an even one above
+  const uint32_t e = top >> 7, m = (top & 0x7fu) | 0x80u;
+  uint32_t k = ((m + 6) * 9363u) >> 16;
+  if (k > 31) k = (((m + 13) * 4682u) >> 16) * 2;
+  float s = __uint_as_float((e > 7 ? e - 7 : 1) << 23) * (float)k;
+  s = fminf(fmaxf(s, 0x1p-80f), 0x1p34f);                      // larger magnitudes saturate
+  s16 = __float_as_uint(s) >> 16;
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t word = 0;
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  if (s < 0x1p34f) {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      word |= kv4_code(__uint_as_float(w[i] << 16), r) << (8 * i) | kv4_code(__uint_as_float(w[i] & 0xffff0000u), r) << (8 * i + 4);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float v = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+      word |= (uint32_t)((int)rintf(fminf(fmaxf(v * 0x1p-34f, -7.f), 7.f)) + 8) << (4 * i);
+    }
   }
-  const int data = keys ? kv4_key_word(p.D, t, c8 * 8) : kv4_value_word(p.D, t, c8 * 8) + 2 * (t & 1);
-  const int scale = kv4_scale(p.D, t, c8 >> 2);
-  __nv_bfloat16* dense = (__nv_bfloat16*)(keys ? p.k : p.v) + row * (keys ? p.k_stride : p.v_stride) + h * p.D + c8 * 8;
-  if (WRITE) {
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (stored) x = *reinterpret_cast<const uint4*>(dense);
-    uint32_t top = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
-    top = max(top & 0xffffu, top >> 16);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));      // groups of four lanes: a row has a multiple of four items
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    if (!stored) return;
-    uint32_t word = 0x88888888u, s16 = 0;
-    if (top >= 0x7f80u) {
-      s16 = 0x7fc0u;                                           // not finite: the whole group is NaN
-    } else if (top > 0) {
-      uint32_t sb = (__float_as_uint(__fdiv_rn(__uint_as_float(top << 16), 7.f)) + 0x7ffffu) & ~0x7ffffu;
-      sb = min(max(sb, 0x17800000u), 0x51800000u);             // 2^-80 and 2^36; larger magnitudes saturate
-      s16 = sb >> 16;
-      const float s = __uint_as_float(sb);
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-      word = 0;
-      if (sb < 0x51800000u) {
-        const float r = 1.f / s;
+  return word;
+}
+
+// A word next to its scale as eight bf16 channels.
+__device__ __forceinline__ uint4 kv4_unpack(uint32_t w, uint32_t s16) {
+  const Kv4Scale s(s16 * 0x10001u);
+  uint32_t v[4] = {kv4_pair(0, w, s), kv4_pair(1, w, s), kv4_pair(0, w >> 8, s), kv4_pair(1, w >> 8, s)};
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          word |= kv4_code(__uint_as_float(w[i] << 16), r) << (8 * i) | kv4_code(__uint_as_float(w[i] & 0xffff0000u), r) << (8 * i + 4);
-      } else {
+  for (int i = 0; i < 4; i++) {
+    const __nv_bfloat162 u = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v[i]), __floats2bfloat162_rn(KV4_UNDO, KV4_UNDO));
+    v[i] = *reinterpret_cast<const uint32_t*>(&u);
+  }
+  return make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
+                    __byte_perm(v[2], v[3], 0x7632));
+}
+
+template <bool WRITE, int D>
+__global__ void __launch_bounds__(KV4_ROWS_THREADS) kv4_rows_kernel(const Kv4Rows p) {
+  __shared__ long unit_of[KV4_ROWS_MAX];        // unit of the row's token within head 0 of its block, token of the unit in the low bits; -1: none
+  const long row0 = (long)blockIdx.x * p.rows_per_block;
+  const int rows = (int)min((long)p.rows_per_block, p.rows - row0), upp = p.block_size / KV4_TOKENS;
+  for (int i = threadIdx.x; i < rows; i += KV4_ROWS_THREADS) {
+    const long long slot = p.slots[row0 + i];
+    long at = -1;
+    if (slot >= 0 && slot < p.num_slots) {
+      const long blk = slot / p.block_size;
+      const int off = (int)(slot - blk * p.block_size);
+      at = (blk * p.heads * upp + off / KV4_TOKENS) * KV4_TOKENS + off % KV4_TOKENS;
+    } else if (slot >= 0 && p.status) {
+      atomicExch(p.status, B200_BAD_INDEX);
+    }
+    unit_of[i] = at;
+  }
+  __syncthreads();
+  const int per_row = p.heads * (D / 8), together = max(1, KV4_ROWS_THREADS / per_row);        // items of a row, rows at once
+  for (int item0 = 0; item0 < per_row; item0 += KV4_ROWS_THREADS) {
+    const int sub = per_row > KV4_ROWS_THREADS ? 0 : threadIdx.x / per_row;
+    const int item = per_row > KV4_ROWS_THREADS ? item0 + threadIdx.x : threadIdx.x - sub * per_row;
+    const bool mine = sub < together && item < per_row;
+    const int h = item / (D / 8), c8 = item - h * (D / 8), head = h * upp;
+    const __nv_bfloat16 *ks = (const __nv_bfloat16*)p.k + h * D + c8 * 8, *vs = (const __nv_bfloat16*)p.v + h * D + c8 * 8;
+    for (int i0 = 0; i0 < rows; i0 += 2 * together) {
+      uint4 x[2][2];
+      long at[2];
+      uint32_t w[2][2], s16[2][2];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float v = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
-          const int n = (int)rintf(fminf(fmaxf(__fdiv_rn(v, s), -7.f), 7.f));
-          word |= (uint32_t)(n + 8) << (4 * i);
+      for (int u = 0; u < 2; u++) {
+        const int i = i0 + u * together + sub;
+        at[u] = mine && i < rows ? unit_of[i] : -1;
+        x[u][0] = x[u][1] = make_uint4(0, 0, 0, 0);
+        w[u][0] = w[u][1] = s16[u][0] = s16[u][1] = 0;
+        if (at[u] < 0) continue;
+        if (WRITE) {
+          x[u][0] = *reinterpret_cast<const uint4*>(ks + (row0 + i) * p.k_stride);
+          x[u][1] = *reinterpret_cast<const uint4*>(vs + (row0 + i) * p.v_stride);
+        } else {
+          const int t = (int)(at[u] & (KV4_TOKENS - 1));
+          const long unit = ((at[u] >> 4) + head) * kv4_unit_bytes(D);
+          const uint8_t *ku = p.k_cache + unit, *vu = p.v_cache + unit;
+          const int vw = kv4_value_word(D, t, c8 * 8) + 2 * (t & 1), sc = kv4_scale(D, t, c8 >> 2);
+          w[u][0] = *reinterpret_cast<const uint32_t*>(ku + kv4_key_word(D, t, c8 * 8));
+          w[u][1] = *reinterpret_cast<const uint16_t*>(vu + vw) | (uint32_t)*reinterpret_cast<const uint16_t*>(vu + vw + 4) << 16;
+          s16[u][0] = *reinterpret_cast<const uint16_t*>(ku + sc);
+          s16[u][1] = *reinterpret_cast<const uint16_t*>(vu + sc);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const int i = i0 + u * together + sub;
+        if (WRITE) {
+#pragma unroll
+          for (int kv = 0; kv < 2; kv++) w[u][kv] = kv4_quantise(x[u][kv], s16[u][kv]);
+          if (at[u] < 0) continue;
+          const int t = (int)(at[u] & (KV4_TOKENS - 1));
+          const long unit = ((at[u] >> 4) + head) * kv4_unit_bytes(D);
+          uint8_t *ku = p.k_cache + unit, *vu = p.v_cache + unit;
+          const int vw = kv4_value_word(D, t, c8 * 8) + 2 * (t & 1), sc = kv4_scale(D, t, c8 >> 2);
+          *reinterpret_cast<uint32_t*>(ku + kv4_key_word(D, t, c8 * 8)) = w[u][0];
+          *reinterpret_cast<uint16_t*>(vu + vw) = (uint16_t)w[u][1];
+          *reinterpret_cast<uint16_t*>(vu + vw + 4) = (uint16_t)(w[u][1] >> 16);
+          if ((c8 & 3) == 0) {
+            *reinterpret_cast<uint16_t*>(ku + sc) = (uint16_t)s16[u][0];
+            *reinterpret_cast<uint16_t*>(vu + sc) = (uint16_t)s16[u][1];
+          }
+        } else if (mine && i < rows) {
+          uint4 *ko = (uint4*)((__nv_bfloat16*)p.k + (row0 + i) * p.k_stride + h * D + c8 * 8);
+          uint4 *vo = (uint4*)((__nv_bfloat16*)p.v + (row0 + i) * p.v_stride + h * D + c8 * 8);
+          *ko = at[u] < 0 ? make_uint4(0, 0, 0, 0) : kv4_unpack(w[u][0], s16[u][0]);
+          *vo = at[u] < 0 ? make_uint4(0, 0, 0, 0) : kv4_unpack(w[u][1], s16[u][1]);
         }
       }
     }
-    if (keys) {
-      *reinterpret_cast<uint32_t*>(unit + data) = word;
-    } else {
-      *reinterpret_cast<uint16_t*>(unit + data) = (uint16_t)word;
-      *reinterpret_cast<uint16_t*>(unit + data + 4) = (uint16_t)(word >> 16);
-    }
-    if ((c8 & 3) == 0) *reinterpret_cast<uint16_t*>(unit + scale) = (uint16_t)s16;
-  } else {
-    if (!here) return;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (stored) {
-      const uint32_t w = keys ? *reinterpret_cast<const uint32_t*>(unit + data)
-                              : *reinterpret_cast<const uint16_t*>(unit + data) | (uint32_t)*reinterpret_cast<const uint16_t*>(unit + data + 4) << 16;
-      const float s = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(unit + scale) << 16);
-      uint32_t o[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        o[i] = pack_bf16x2((float)((int)(w >> (8 * i) & 15u) - 8) * s, (float)((int)(w >> (8 * i + 4) & 15u) - 8) * s);
-      x = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-    *reinterpret_cast<uint4*>(dense) = x;
   }
 }
 
-static int kv4_rows(bool write, const Kv4Rows& p, cudaStream_t stream) {
+static int kv4_rows(bool write, Kv4Rows p, cudaStream_t stream) {
   if (p.rows <= 0) return 0;
-  if ((p.D != 64 && p.D != 128) || p.heads < 1 || p.heads > 4096 || p.block_size < KV4_TOKENS || p.block_size % KV4_TOKENS) return 9880;
+  if ((p.D != 64 && p.D != 128) || p.heads < 1 || p.heads > 65536 || p.block_size < KV4_TOKENS || p.block_size % KV4_TOKENS) return 9880;
   if ((p.k_stride & 7) || (p.v_stride & 7)) return 9881;
-  const long blocks = (p.rows * p.heads * (p.D >> 3) + 255) / 256;
+  // two rows a thread at least, more where that leaves eight blocks an SM
+  const int per_row = p.heads * (p.D / 8), together = per_row < KV4_ROWS_THREADS ? KV4_ROWS_THREADS / per_row : 1;
+  const long most = KV4_ROWS_MAX / (2 * together) > 0 ? KV4_ROWS_MAX / (2 * together) : 1;
+  long passes = p.rows / ((long)2 * together * 8 * num_sms());
+  passes = passes < 1 ? 1 : passes > most ? most : passes;
+  p.rows_per_block = (int)(passes * 2 * together < KV4_ROWS_MAX ? passes * 2 * together : KV4_ROWS_MAX);
+  const long blocks = (p.rows + p.rows_per_block - 1) / p.rows_per_block;
   if (blocks > 0x7fffffffl) return 9882;
-  const dim3 grid((unsigned)blocks, 2);
-  if (write) kv4_rows_kernel<true><<<grid, 256, 0, stream>>>(p);
-  else kv4_rows_kernel<false><<<grid, 256, 0, stream>>>(p);
+  const unsigned g = (unsigned)blocks;
+  if (p.D == 128) {
+    if (write) kv4_rows_kernel<true, 128><<<g, KV4_ROWS_THREADS, 0, stream>>>(p);
+    else kv4_rows_kernel<false, 128><<<g, KV4_ROWS_THREADS, 0, stream>>>(p);
+  } else {
+    if (write) kv4_rows_kernel<true, 64><<<g, KV4_ROWS_THREADS, 0, stream>>>(p);
+    else kv4_rows_kernel<false, 64><<<g, KV4_ROWS_THREADS, 0, stream>>>(p);
+  }
   return B200_CHECK_LAUNCH();
 }
 
@@ -124,7 +183,7 @@ using namespace b200;
 B200_API int b200_kv_int4_write(const void* k, long k_stride, const void* v, long v_stride, long rows, const void* slots, void* k_cache,
                                 void* v_cache, long num_slots, int heads, int D, int block_size, int* status, cudaStream_t stream) {
   Kv4Rows p = {const_cast<void*>(k), const_cast<void*>(v), (uint8_t*)k_cache, (uint8_t*)v_cache, (const long long*)slots, k_stride, v_stride,
-               rows, num_slots, heads, D, block_size, status};
+               rows, num_slots, heads, D, block_size, 0, status};
   return kv4_rows(true, p, stream);
 }
 
@@ -133,6 +192,6 @@ B200_API int b200_kv_int4_read(void* k, void* v, long rows, const void* slots, c
                                int heads, int D, int block_size, int* status, cudaStream_t stream) {
   const long stride = (long)heads * D;
   Kv4Rows p = {k, v, (uint8_t*)const_cast<void*>(k_cache), (uint8_t*)const_cast<void*>(v_cache), (const long long*)slots, stride, stride,
-               rows, num_slots, heads, D, block_size, status};
+               rows, num_slots, heads, D, block_size, 0, status};
   return kv4_rows(false, p, stream);
 }

@@ -1,7 +1,7 @@
 // Keys and values in 4 bits: how a page lies in memory, and how it is unpacked.
 //
 // Groups of 32 adjacent channels of a (token, head) share a scale s: the smallest number of five significant bits with
-// 7 s no less than the group's largest magnitude, between 2^-80 and 2^36, held as bf16.  A channel x is the whole number
+// 7 s no less than the group's largest magnitude, between 2^-80 and 2^34, held as bf16.  A channel x is the whole number
 // n = rint(x / s) (ties to even), -7..7, held as n + 8, and stands for n s, three bits times five: exact in bf16.
 //
 // A bf16 whose low byte alone is set has the value (low byte) 2^-133, through subnormals and the first exponent alike.  So a nibble that

@@ -28,7 +28,7 @@ _native.register_signature("b200_attn_int4_prefill",
 
 HEAD_SIZES = (64, 128)
 #: rows (new tokens times heads of a group) of a sequence up to which the kernel for few rows takes it
-FEW_ROWS = 16
+FEW_ROWS = 32
 
 _scratch = Scratch(torch.float32)
 
@@ -184,13 +184,18 @@ def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, n, max_
     _native.count_launch(1 + int(parts > 1))
 
 
+def _prompt_parts(blocks: int, max_len: int, sms: int) -> int:
+    """Parts of a prompt's keys: where its blocks (one per SM) leave half of the GPU idle, and a part keeps 512 keys."""
+    return max(1, min(sms // max(1, blocks), max_len // 512, 16))
+
+
 def _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, new) -> None:
     """The sequences from ``first`` on, with ``new`` new tokens."""
     T, Hq, D = q.shape
     NB, Hkv, _ = k_cache.shape
     row, pair = int(meta.query_start_loc_cpu[first]), 2 * (128 // (Hq // Hkv))
     blocks = int((-(-new // pair)).sum()) * Hkv
-    parts = 1 if fixed_sums() else max(1, min(_native.sm_count(q.device) // max(1, blocks), meta.max_seq_len // 512))
+    parts = 1 if fixed_sums() else _prompt_parts(blocks, meta.max_seq_len, _native.sm_count(q.device))
     scratch = _scratch.get(q.device, T * Hq * parts * (D + 1)) if parts > 1 else None
     rc = _native.lib().b200_attn_int4_prefill(
         q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, meta.query_start_loc[first:].data_ptr(),

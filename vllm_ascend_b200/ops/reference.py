@@ -264,14 +264,14 @@ KV_INT4_GROUP, KV_INT4_TOKENS = 32, 16
 
 def kv_int4_quantise(x: torch.Tensor):
     """x [..., D] -> whole numbers in -7..7 (int8) [..., D] and scales (bf16) [..., D / 32].  A scale is the smallest number
-    of five significant bits with 7 scale >= max |x| over its 32 channels, between 2^-80 and 2^36 (larger magnitudes saturate), or zero
+    of five significant bits with 7 scale >= max |x| over its 32 channels, between 2^-80 and 2^34 (larger magnitudes saturate), or zero
     for a group of zeros; a group that holds a NaN or an infinity is NaN."""
     g = x.float().unflatten(-1, (-1, KV_INT4_GROUP))
     top = g.abs().amax(-1, keepdim=True)
     finite = torch.isfinite(top)
     top = torch.where(finite, top, 0.0)
     low = top / torch.full_like(top, 7.0)
-    s = ((low.view(torch.int32) + 0x7ffff) & ~0x7ffff).view(torch.float32).clamp(2.0 ** -80, 2.0 ** 36)
+    s = ((low.view(torch.int32) + 0x7ffff) & ~0x7ffff).view(torch.float32).clamp(2.0 ** -80, 2.0 ** 34)
     s = torch.where(top > 0, s, 0.0)
     n = torch.where(finite & (s > 0), g / torch.where(s > 0, s, 1.0), 0.0).clamp(-7, 7).round()
     nan = torch.tensor(0x7fc0, dtype=torch.int16, device=x.device).view(torch.bfloat16)      # the same bits everywhere
