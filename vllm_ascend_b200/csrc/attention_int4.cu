@@ -14,6 +14,7 @@
 // all rows see them and 16 at a time at the edges, through a ring of its own that bulk copies fill, with a running maximum of
 // its own; they join at the end.  Parts join in a second kernel.
 #include "attention_int4.cuh"
+#include "cluster_sum.cuh"
 
 #include <type_traits>
 
@@ -40,8 +41,8 @@ struct Int4Cfg {
   static constexpr int RING = STAGES * STAGE;
   static constexpr int ROWS = 8 * NT;
   static constexpr int SMEM = D4_WARPS * RING + 1024;    // barriers, maxima and sums behind the rings
-  static_assert(ROWS * D * 4 <= RING, "a warp's result takes its ring's place");
-  static_assert(D4_WARPS * (STAGES * 8 + ROWS * 8) + 16 <= 1024, "");
+  static_assert(2 * ROWS * D * 4 <= RING, "a warp's result takes its ring's place, and the block's that behind the first warp's");
+  static_assert(D4_WARPS * (STAGES * 8 + ROWS * 8) + ROWS * 8 + 16 <= 1024, "");
 };
 
 template <int D, int NT>
@@ -57,9 +58,12 @@ __global__ void __launch_bounds__(32 * D4_WARPS, 3) attn_int4_kernel(const Int4P
   uint64_t* bars = (uint64_t*)(i4_smem + D4_WARPS * Cfg::RING) + warp * Cfg::STAGES;
   float* ms = (float*)(i4_smem + D4_WARPS * (Cfg::RING + Cfg::STAGES * 8));        // [warps][rows], sums behind
   float* ls = ms + D4_WARPS * ROWS;
-  volatile int* abort_word = (volatile int*)(ls + D4_WARPS * ROWS);
+  float* block_m = ls + D4_WARPS * ROWS;                                           // [rows] of the block, sums behind
+  float* block_l = block_m + ROWS;
+  volatile int* abort_word = (volatile int*)(block_l + ROWS);
 
-  const int seq = blockIdx.x / p.row_blocks, row0 = (blockIdx.x - seq * p.row_blocks) * ROWS, h = blockIdx.y, part = blockIdx.z;
+  const int seq = p.row_blocks == 1 ? blockIdx.x : blockIdx.x / p.row_blocks, row0 = (blockIdx.x - seq * p.row_blocks) * ROWS;
+  const int h = blockIdx.y, part = blockIdx.z;
   const int q_start = p.cu[seq], q_len = p.cu[seq + 1] - q_start, len = p.seq_lens[seq], ctx = len - q_len;
   const int rows = min(q_len * p.G - row0, ROWS);
   if (rows <= 0) return;
@@ -70,19 +74,23 @@ __global__ void __launch_bounds__(32 * D4_WARPS, 3) attn_int4_kernel(const Int4P
   __syncthreads();
 
   // keys that any row of the block sees, and those that all rows see
-  const int tok_first = row0 / p.G, tok_last = (row0 + rows - 1) / p.G;
+  const int tok_first = int4_div(row0, p.G, p.g_inv), tok_last = int4_div(row0 + rows - 1, p.G, p.g_inv);
   const int hi = max(0, p.causal ? min(len, ctx + tok_last + 1) : len), all_hi = p.causal ? min(len, ctx + tok_first + 1) : len;
   const int lo = p.window > 0 ? max(0, ctx + tok_first - p.window + 1) : 0, all_lo = p.window > 0 ? max(0, ctx + tok_last - p.window + 1) : 0;
   // the block's units, and the warp's among them
   const int u_lo = lo / KV4_TOKENS, units = max(0, (hi + KV4_TOKENS - 1) / KV4_TOKENS - u_lo);
-  const int b0 = (int)((long)units * part / p.parts), b1 = (int)((long)units * (part + 1) / p.parts);
+  int b0 = 0, b1 = units;
+  if (p.parts > 1) {
+    b0 = (int)((uint32_t)units * part / (uint32_t)p.parts);
+    b1 = (int)((uint32_t)units * (part + 1) / (uint32_t)p.parts);
+  }
   const int first = u_lo + b0 + (b1 - b0) * warp / D4_WARPS, last = u_lo + b0 + (b1 - b0) * (warp + 1) / D4_WARPS;
 
   // the next tile to copy: lanes below U know the page of a unit each, and the unit's place there, walked by additions
   const int upp = p.block_size / KV4_TOKENS;
   const int* bt = p.block_table + (long)seq * p.max_blocks;
-  int next = first, col = (first + lane) / upp, at = first + lane - col * upp, blk = 0;
-  const int step = U / upp, rest = U - step * upp;
+  int next = first, col = int4_div(first + lane, upp, p.upp_inv), at = first + lane - col * upp, blk = 0;
+  const int step = int4_div(U, upp, p.upp_inv), rest = U - step * upp;
   auto look_up = [&]() {
     if (lane < U && next + lane < last) blk = col < p.max_blocks ? bt[col] : -1;
   };
@@ -131,7 +139,7 @@ __global__ void __launch_bounds__(32 * D4_WARPS, 3) attn_int4_kernel(const Int4P
   uint32_t qf[NT][KW][4];
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
-    const int row = row0 + nt * 8 + r, tok = row / p.G, g = row - tok * p.G;
+    const int row = row0 + nt * 8 + r, tok = int4_div(row, p.G, p.g_inv), g = row - tok * p.G;
     const bool here = nt * 8 + r < rows;
     const uint4* src = reinterpret_cast<const uint4*>(p.q + (long)(q_start + tok) * p.q_stride + (long)(h * p.G + g) * D + c * (D / 4));
 #pragma unroll
@@ -149,7 +157,7 @@ __global__ void __launch_bounds__(32 * D4_WARPS, 3) attn_int4_kernel(const Int4P
   for (int nt = 0; nt < NT; nt++)
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      const int i = nt * 8 + 2 * c + e, pos = ctx + (row0 + i) / p.G;
+      const int i = nt * 8 + 2 * c + e, pos = ctx + int4_div(row0 + i, p.G, p.g_inv);
       k_hi[nt][e] = i < rows ? (p.causal ? min(len, pos + 1) : len) : 0;
       k_lo[nt][e] = p.window > 0 ? pos - p.window + 1 : 0;
     }
@@ -337,8 +345,15 @@ __global__ void __launch_bounds__(32 * D4_WARPS, 3) attn_int4_kernel(const Int4P
       tokens(std::integral_constant<int, U>(), std::false_type(), ks, vs, u0 * KV4_TOKENS);
     } else {
 #pragma unroll 1
-      for (int u = 0; u < n; u++)
-        tokens(std::integral_constant<int, 1>(), std::true_type(), ks + u * Cfg::UNIT, vs + u * Cfg::UNIT, (u0 + u) * KV4_TOKENS);
+      for (int u = 0; u < n;) {
+        if (U > 2 && n - u >= 2 && inside(u0 + u, 2)) {
+          tokens(std::integral_constant<int, 2>(), std::false_type(), ks + u * Cfg::UNIT, vs + u * Cfg::UNIT, (u0 + u) * KV4_TOKENS);
+          u += 2;
+        } else {
+          tokens(std::integral_constant<int, 1>(), std::true_type(), ks + u * Cfg::UNIT, vs + u * Cfg::UNIT, (u0 + u) * KV4_TOKENS);
+          u++;
+        }
+      }
     }
     __syncwarp();                                // all lanes have read the stage
     if (next < last && !bad) issue(stage);
@@ -385,6 +400,7 @@ __global__ void __launch_bounds__(32 * D4_WARPS, 3) attn_int4_kernel(const Int4P
     if (threadIdx.x == 0 && p.status) atomicExch(p.status, *abort_word);
     __syncthreads();
   }
+  float* block_o = (float*)i4_smem + ROWS * D;
   for (int it = threadIdx.x; it < rows * (D / 8); it += 32 * D4_WARPS) {
     const int i = it / (D / 8), ch = (it - i * (D / 8)) * 8;
     float top = ms[i];
@@ -403,8 +419,16 @@ __global__ void __launch_bounds__(32 * D4_WARPS, 3) attn_int4_kernel(const Int4P
       acc[4] += b.x * f; acc[5] += b.y * f; acc[6] += b.z * f; acc[7] += b.w * f;
     }
     const float inv = sum == 0.f ? 0.f : KV4_UNDO / sum;     // a row without keys: zeros
-    const int tok = (row0 + i) / p.G, g = row0 + i - tok * p.G;
-    if (p.parts == 1) {
+    const int tok = int4_div(row0 + i, p.G, p.g_inv), g = row0 + i - tok * p.G;
+    if (p.cluster) {
+      float4* dst = reinterpret_cast<float4*>(block_o + i * D + ch);
+      dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      if (ch == 0) {
+        block_m[i] = top;
+        block_l[i] = sum;
+      }
+    } else if (p.parts == 1) {
       uint4 v;
       v.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
       v.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
@@ -418,6 +442,38 @@ __global__ void __launch_bounds__(32 * D4_WARPS, 3) attn_int4_kernel(const Int4P
       dst[1] = make_float4(acc[4] * inv, acc[5] * inv, acc[6] * inv, acc[7] * inv);
       if (ch == 0) p.part_lse[at] = sum == 0.f ? -INFINITY : top + log2f(sum);
     }
+  }
+  if (p.cluster) {
+    // the parts' blocks form a cluster: each joins every parts-th piece of the rows out of all blocks' shared memory
+    sg_cluster_sync();
+    for (int it = part * 32 * D4_WARPS + threadIdx.x; it < rows * (D / 4); it += p.parts * 32 * D4_WARPS) {
+      const int i = it / (D / 4), ch = (it - i * (D / 4)) * 4;
+      float pm[I4_CLUSTER], pl[I4_CLUSTER], top = -INFINITY, sum = 0.f;
+      float4 po[I4_CLUSTER], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int q = 0; q < I4_CLUSTER; q++) {
+        pm[q] = -INFINITY;
+        pl[q] = 0.f;
+        if (q < p.parts) {
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pm[q]) : "r"(sg_map(smem_u32(block_m + i), q)) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pl[q]) : "r"(sg_map(smem_u32(block_l + i), q)) : "memory");
+          po[q] = sg_ld(sg_map(smem_u32(block_o + i * D + ch), q));
+        }
+        top = fmaxf(top, pm[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < I4_CLUSTER; q++) {
+        if (q >= p.parts || (pm[q] == -INFINITY && pl[q] == 0.f)) continue;     // saw no key
+        const float f = i4_exp2(pm[q] - top);
+        sum += pl[q] * f;
+        acc.x += po[q].x * f; acc.y += po[q].y * f; acc.z += po[q].z * f; acc.w += po[q].w * f;
+      }
+      const float inv = sum == 0.f ? 0.f : KV4_UNDO / sum;
+      const int tok = int4_div(row0 + i, p.G, p.g_inv), g = row0 + i - tok * p.G;
+      *reinterpret_cast<uint2*>(p.out + (long)(q_start + tok) * p.out_stride + (long)(h * p.G + g) * D + ch) =
+          make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    }
+    sg_cluster_sync();                           // no block leaves while others read it
   }
 }
 
@@ -433,22 +489,37 @@ __global__ void __launch_bounds__(128) attn_int4_join_kernel(const float* part_o
   if (at >= rows || tok >= end) return;
   const float* lse = part_lse + (tok * heads + head) * parts;
   const float* o = part_o + (tok * heads + head) * parts * D;
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, lse[i]);
-  top = warp_reduce_max(top);
+  // a lane's weights: of parts lane and lane + 32
+  const float x0 = lane < parts ? lse[lane] : -INFINITY, x1 = lane + 32 < parts ? lse[lane + 32] : -INFINITY;
+  float top = warp_reduce_max(fmaxf(x0, x1));
+  if (top == -INFINITY) top = 0.f;
+  const float w0 = x0 == -INFINITY ? 0.f : i4_exp2(x0 - top), w1 = x1 == -INFINITY ? 0.f : i4_exp2(x1 - top);
+  const uint32_t here0 = __ballot_sync(0xffffffffu, x0 != -INFINITY), here1 = __ballot_sync(0xffffffffu, x1 != -INFINITY);
+  const float sum = warp_reduce_sum(w0 + w1);
   constexpr int V = D / 32;
-  float acc[V] = {}, sum = 0.f;
-  for (int i = 0; i < parts; i++) {
-    const float x = lse[i];
-    if (x == -INFINITY) continue;                // saw no key: nothing was written
-    const float f = i4_exp2(x - (top == -INFINITY ? 0.f : top));
-    sum += f;
-    if constexpr (V == 4) {
-      const float4 a = reinterpret_cast<const float4*>(o + (long)i * D)[lane];
-      acc[0] += a.x * f; acc[1] += a.y * f; acc[2] += a.z * f; acc[3] += a.w * f;
-    } else {
-      const float2 a = reinterpret_cast<const float2*>(o + (long)i * D)[lane];
-      acc[0] += a.x * f; acc[1] += a.y * f;
+  float acc[V] = {};
+  for (int i0 = 0; i0 < parts; i0 += 8) {
+    float a[8][V];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const int i = i0 + k;
+#pragma unroll
+      for (int v = 0; v < V; v++) a[k][v] = 0.f;
+      if ((i < 32 ? here0 >> i : here1 >> (i - 32)) & 1u) {      // others saw no key, and nothing was written
+        if constexpr (V == 4) {
+          const float4 x = reinterpret_cast<const float4*>(o + (long)i * D)[lane];
+          a[k][0] = x.x; a[k][1] = x.y; a[k][2] = x.z; a[k][3] = x.w;
+        } else {
+          const float2 x = reinterpret_cast<const float2*>(o + (long)i * D)[lane];
+          a[k][0] = x.x; a[k][1] = x.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const float f = __shfl_sync(0xffffffffu, i0 < 32 ? w0 : w1, (i0 + k) & 31);
+#pragma unroll
+      for (int v = 0; v < V; v++) acc[v] += a[k][v] * f;
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -465,8 +536,19 @@ static int launch_int4(Int4Params p, int max_rows, cudaStream_t stream) {
   p.row_blocks = (max_rows + Cfg::ROWS - 1) / Cfg::ROWS;
   const long x = (long)p.num_seqs * p.row_blocks;
   if (x > 0x7fffffffl || p.Hkv > 65535) return 9886;
-  attn_int4_kernel<D, NT><<<dim3((unsigned)x, (unsigned)p.Hkv, (unsigned)p.parts), 32 * D4_WARPS, Cfg::SMEM, stream>>>(p);
-  return B200_CHECK_LAUNCH();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)x, (unsigned)p.Hkv, (unsigned)p.parts);
+  cfg.blockDim = dim3(32 * D4_WARPS);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = p.parts;
+  cfg.attrs = &attr;
+  cfg.numAttrs = p.cluster;
+  e = cudaLaunchKernelEx(&cfg, attn_int4_kernel<D, NT>, p);
+  return e != cudaSuccess ? (int)e : B200_CHECK_LAUNCH();
 }
 
 int int4_params(Int4Params* p, const void* q, long q_stride, long q_rows, const void* k_cache, const void* v_cache, long num_blocks, int block_size,
@@ -475,7 +557,7 @@ int int4_params(Int4Params* p, const void* q, long q_stride, long q_rows, const 
   const int G = Hkv > 0 ? Hq / Hkv : 0;
   if (G < 1 || G * Hkv != Hq || (D != 64 && D != 128)) return 9883;
   if (block_size < KV4_TOKENS || block_size % KV4_TOKENS) return 9884;
-  if ((q_stride & 7) || (out_stride & 7) || parts < 1 || parts > 65535 || (parts > 1 && !scratch)) return 9885;
+  if ((q_stride & 7) || (out_stride & 7) || parts < 1 || parts > I4_PARTS) return 9885;
   *p = Int4Params{};
   p->q = (const __nv_bfloat16*)q;
   p->k_cache = (const uint8_t*)k_cache;
@@ -489,6 +571,10 @@ int int4_params(Int4Params* p, const void* q, long q_stride, long q_rows, const 
   p->q_stride = q_stride; p->out_stride = out_stride; p->num_blocks = num_blocks;
   p->num_seqs = num_seqs; p->max_blocks = max_blocks; p->block_size = block_size;
   p->G = G; p->Hkv = Hkv; p->parts = parts; p->causal = causal; p->window = window;
+  const int upp = block_size / KV4_TOKENS;
+  if ((long)max_blocks * upp * upp > 0xffffffffl || (long)max_blocks * upp > 0xffffffffl / 65536) return 9888;      // 1M tokens a sequence and more
+  p->g_inv = (uint32_t)((0x100000000ll + G - 1) / G);
+  p->upp_inv = (uint32_t)((0x100000000ll + upp - 1) / upp);
   p->scale_log2 = scale * 1.4426950408889634f * KV4_UNDO;
   p->status = status;
   return 0;
@@ -509,7 +595,7 @@ int int4_join(const Int4Params& p, int D, long q_rows, cudaStream_t stream) {
 using namespace b200;
 
 // q [*, Hq, D] and out rows with token strides; cu [num_seqs + 1] their row numbers; max_q_len: no sequence has more new tokens.
-// parts > 1: scratch of (rows of q) x Hq x parts x (D + 1) floats.
+// parts > 1: joined in a cluster (up to I4_CLUSTER), or, where scratch of (rows of q) x Hq x parts x (D + 1) floats is given, there.
 B200_API int b200_attn_int4(const void* q, long q_stride, long q_rows, const void* k_cache, const void* v_cache, long num_blocks,
                             int block_size, const void* cu, const void* seq_lens, const void* block_table, int max_blocks, int num_seqs,
                             int max_q_len, int Hq, int Hkv, int D, float scale, int causal, int window, int parts, void* out,
@@ -520,8 +606,10 @@ B200_API int b200_attn_int4(const void* q, long q_stride, long q_rows, const voi
                        Hq, Hkv, D, scale, causal, window, parts, out, out_stride, scratch, status);
   if (rc) return rc;
   const long rows = (long)max_q_len * p.G;
-  if (rows > 0x3fffffffl) return 9886;
+  if (rows * p.G > 0x7fffffffl) return 9886;
+  p.cluster = parts > 1 && !scratch;
+  if (p.cluster && parts > I4_CLUSTER) return 9885;
   if (D == 128) rc = rows <= 8 ? launch_int4<128, 1>(p, (int)rows, stream) : launch_int4<128, 2>(p, (int)rows, stream);
   else rc = rows <= 8 ? launch_int4<64, 1>(p, (int)rows, stream) : launch_int4<64, 2>(p, (int)rows, stream);
-  return rc || parts == 1 ? rc : int4_join(p, D, q_rows, stream);
+  return rc || parts == 1 || p.cluster ? rc : int4_join(p, D, q_rows, stream);
 }

@@ -4,6 +4,9 @@
 
 namespace b200 {
 
+constexpr int I4_CLUSTER = 8;      // blocks of a cluster at most
+constexpr int I4_PARTS = 64;       // parts at most
+
 struct Int4Params {
   const __nv_bfloat16* q;
   const uint8_t *k_cache, *v_cache;
@@ -11,10 +14,14 @@ struct Int4Params {
   __nv_bfloat16* out;
   float *part_o, *part_lse;       // [tokens x heads][parts][D], [..][parts]: results of parts, normalised, with log2 of their sums
   long q_stride, out_stride, num_blocks;
-  int num_seqs, max_blocks, block_size, G, Hkv, parts, row_blocks, causal, window;
+  int num_seqs, max_blocks, block_size, G, Hkv, parts, cluster, row_blocks, causal, window;
+  uint32_t g_inv, upp_inv;        // ceil(2^32 / .) of G and of the units of a page (int4_div)
   float scale_log2;               // of scores over unpacked keys, which carry 2^-40
   int* status;
 };
+
+// x / d for x d < 2^32 with inv = ceil(2^32 / d)
+__device__ __forceinline__ int int4_div(int x, int d, uint32_t inv) { return d == 1 ? x : (int)__umulhi((uint32_t)x, inv); }
 
 __device__ __forceinline__ float i4_exp2(float x) {
   float y;

@@ -510,6 +510,7 @@ B200_API int b200_attn_int4_prefill(const void* q, long q_stride, long q_rows, c
                        Hq, Hkv, D, scale, causal, window, parts, out, out_stride, scratch, status);
   if (rc) return rc;
   if (p.G > 128) return 9883;
+  if (parts > 1 && !scratch) return 9885;
   rc = D == 128 ? launch_int4_prefill<128>(p, tokens, stream) : launch_int4_prefill<64>(p, tokens, stream);
   return rc || parts == 1 ? rc : int4_join(p, D, q_rows, stream);
 }

@@ -1,6 +1,6 @@
 // Rows of keys and values into a 4-bit cache and back (format: kv_int4.cuh).
 //
-// Bound: memory.  A thread keeps to 8 channels (16 bytes dense, 4 packed) and walks rows, keys and values of two rows in flight at once; what
+// Bound: memory.  A thread keeps to 8 channels (16 bytes dense, 4 packed) and walks rows, keys and values of several rows in flight at once; what
 // a row's slot means is found once for the block.  Four threads share a group and find its largest magnitude as whole
 // numbers (the bits of |bf16| order as its values do, NaN and infinities above all numbers).
 #include "kv_int4.cuh"
@@ -9,6 +9,7 @@ namespace b200 {
 
 constexpr int KV4_ROWS_THREADS = 256;
 constexpr int KV4_ROWS_MAX = 256;           // of a block
+constexpr int KV4_FLIGHT = 2;               // rows of a thread whose loads are under way together
 
 struct Kv4Rows {
   void *k, *v;                    // [rows, heads, D] bf16, heads dense; written by the read
@@ -73,7 +74,7 @@ __device__ __forceinline__ uint4 kv4_unpack(uint32_t w, uint32_t s16) {
                     __byte_perm(v[2], v[3], 0x7632));
 }
 
-template <bool WRITE, int D>
+template <bool WRITE, int D, int U>
 __global__ void __launch_bounds__(KV4_ROWS_THREADS) kv4_rows_kernel(const Kv4Rows p) {
   __shared__ long unit_of[KV4_ROWS_MAX];        // unit of the row's token within head 0 of its block, token of the unit in the low bits; -1: none
   const long row0 = (long)blockIdx.x * p.rows_per_block;
@@ -98,12 +99,12 @@ __global__ void __launch_bounds__(KV4_ROWS_THREADS) kv4_rows_kernel(const Kv4Row
     const bool mine = sub < together && item < per_row;
     const int h = item / (D / 8), c8 = item - h * (D / 8), head = h * upp;
     const __nv_bfloat16 *ks = (const __nv_bfloat16*)p.k + h * D + c8 * 8, *vs = (const __nv_bfloat16*)p.v + h * D + c8 * 8;
-    for (int i0 = 0; i0 < rows; i0 += 2 * together) {
-      uint4 x[2][2];
-      long at[2];
-      uint32_t w[2][2], s16[2][2];
+    for (int i0 = 0; i0 < rows; i0 += U * together) {
+      uint4 x[U][2];
+      long at[U];
+      uint32_t w[U][2], s16[U][2];
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
+      for (int u = 0; u < U; u++) {
         const int i = i0 + u * together + sub;
         at[u] = mine && i < rows ? unit_of[i] : -1;
         x[u][0] = x[u][1] = make_uint4(0, 0, 0, 0);
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(KV4_ROWS_THREADS) kv4_rows_kernel(const Kv4Row
         }
       }
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
+      for (int u = 0; u < U; u++) {
         const int i = i0 + u * together + sub;
         if (WRITE) {
 #pragma unroll
@@ -156,22 +157,26 @@ static int kv4_rows(bool write, Kv4Rows p, cudaStream_t stream) {
   if (p.rows <= 0) return 0;
   if ((p.D != 64 && p.D != 128) || p.heads < 1 || p.heads > 65536 || p.block_size < KV4_TOKENS || p.block_size % KV4_TOKENS) return 9880;
   if ((p.k_stride & 7) || (p.v_stride & 7)) return 9881;
-  // two rows a thread at least, more where that leaves eight blocks an SM
+  // KV4_FLIGHT rows a thread at least, more where that leaves eight blocks an SM; single rows where few are asked for
   const int per_row = p.heads * (p.D / 8), together = per_row < KV4_ROWS_THREADS ? KV4_ROWS_THREADS / per_row : 1;
-  const long most = KV4_ROWS_MAX / (2 * together) > 0 ? KV4_ROWS_MAX / (2 * together) : 1;
-  long passes = p.rows / ((long)2 * together * 8 * num_sms());
+  const bool many = p.rows >= (long)KV4_FLIGHT * together * num_sms();
+  const int step = (many ? KV4_FLIGHT : 1) * together, most = KV4_ROWS_MAX / step > 0 ? KV4_ROWS_MAX / step : 1;
+  long passes = p.rows / ((long)step * 8 * num_sms());
   passes = passes < 1 ? 1 : passes > most ? most : passes;
-  p.rows_per_block = (int)(passes * 2 * together < KV4_ROWS_MAX ? passes * 2 * together : KV4_ROWS_MAX);
+  p.rows_per_block = (int)(passes * step < KV4_ROWS_MAX ? passes * step : KV4_ROWS_MAX);
   const long blocks = (p.rows + p.rows_per_block - 1) / p.rows_per_block;
   if (blocks > 0x7fffffffl) return 9882;
   const unsigned g = (unsigned)blocks;
+  const dim3 block(KV4_ROWS_THREADS);
+#define KV4_ROWS(W, D, U) kv4_rows_kernel<W, D, U><<<g, block, 0, stream>>>(p)
   if (p.D == 128) {
-    if (write) kv4_rows_kernel<true, 128><<<g, KV4_ROWS_THREADS, 0, stream>>>(p);
-    else kv4_rows_kernel<false, 128><<<g, KV4_ROWS_THREADS, 0, stream>>>(p);
+    if (write) many ? KV4_ROWS(true, 128, KV4_FLIGHT) : KV4_ROWS(true, 128, 1);
+    else many ? KV4_ROWS(false, 128, KV4_FLIGHT) : KV4_ROWS(false, 128, 1);
   } else {
-    if (write) kv4_rows_kernel<true, 64><<<g, KV4_ROWS_THREADS, 0, stream>>>(p);
-    else kv4_rows_kernel<false, 64><<<g, KV4_ROWS_THREADS, 0, stream>>>(p);
+    if (write) many ? KV4_ROWS(true, 64, KV4_FLIGHT) : KV4_ROWS(true, 64, 1);
+    else many ? KV4_ROWS(false, 64, KV4_FLIGHT) : KV4_ROWS(false, 64, 1);
   }
+#undef KV4_ROWS
   return B200_CHECK_LAUNCH();
 }
 

@@ -118,11 +118,16 @@ def read_kv_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tens
     return k, v
 
 
+#: parts whose blocks form a cluster and join in it
+CLUSTER = 8
+
+
 def _parts(blocks: int, max_len: int, sms: int) -> int:
-    """Parts that every sequence's keys are split into."""
+    """Parts that every sequence's keys are split into, by the blocks (three per SM) without a split."""
     if fixed_sums():
         return 1
-    return max(1, min(3 * sms // max(1, blocks), -(-max_len // 128), 64))
+    most = min(3 * sms // max(1, blocks), -(-max_len // 128), 64)
+    return max(1, most if most <= CLUSTER or max_len >= 8192 else CLUSTER)
 
 
 def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta, scale: float,
@@ -175,13 +180,13 @@ def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, n, max_
     rows = max_q * (Hq // Hkv)
     blocks = n * Hkv * (1 if rows <= 8 else -(-rows // 16))
     parts = _parts(blocks, meta.max_seq_len, _native.sm_count(q.device))
-    scratch = _scratch.get(q.device, T * Hq * parts * (D + 1)) if parts > 1 else None
+    scratch = _scratch.get(q.device, T * Hq * parts * (D + 1)) if parts > CLUSTER else None
     rc = _native.lib().b200_attn_int4(
         q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(),
         meta.block_table.data_ptr(), meta.block_table.stride(0), n, max_q, Hq, Hkv, D, scale, int(causal), int(window), parts,
         out.data_ptr(), out.stride(0), _native.ptr(scratch), _native.status_word(q.device).data_ptr(), _native.stream_ptr())
     _native.check(rc, "attn_int4")
-    _native.count_launch(1 + int(parts > 1))
+    _native.count_launch(1 + int(parts > CLUSTER))
 
 
 def _prompt_parts(blocks: int, max_len: int, sms: int) -> int:
