@@ -377,3 +377,49 @@ def test_prompt_pages_outside_of_the_cache_are_reported():
     with pytest.raises(_native.NativeError, match="BAD_INDEX"):
         _native.check_status(torch.device(DEV))
     assert torch.equal(out[200:], good[200:])
+
+
+# ---------------------------------------------------------------- as the engine uses it
+def test_norm_rotation_and_store():
+    """The model's call: rows are normed and rotated as for a bf16 cache, what the slots stand for is the quantised result."""
+    T, Hq, Hkv, D = 37, 8, 2, 128
+    g = torch.Generator().manual_seed(31)
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, generator=g).to(DEV, torch.bfloat16)
+    wq, wk = (torch.rand(D, generator=g).to(DEV, torch.bfloat16) + 0.5 for _ in "qk")
+    pos, slots = torch.arange(T, device=DEV) + 11, torch.randperm(128, generator=g)[:T].to(DEV)
+    slots[5] = -1
+    ang = torch.outer(torch.arange(64.0), 10000.0 ** (-torch.arange(0, D, 2) / D))
+    cos_sin = torch.cat([ang.cos(), ang.sin()], -1).to(DEV)
+    args = (pos, cos_sin, D, wq, wk, 1e-6)
+    dense, rows = qkv.clone(), qkv.clone()
+    kc, vc = (ops.alloc_kv_cache(4, 32, Hkv, D, torch.bfloat16, DEV) for _ in "kv")
+    ops.qknorm_rope_kvwrite(dense, *args, kc, vc, slots, Hq, Hkv, D)
+    k4, v4 = _caches(4, 32, Hkv, D)
+    ops.qknorm_rope_kvwrite(rows, *args, k4, v4, slots, Hq, Hkv, D)
+    assert torch.equal(rows, dense)
+    want = _caches(4, 32, Hkv, D)
+    k, v = (dense[:, a * D:(a + Hkv) * D].view(T, Hkv, D) for a in (Hq, Hq + Hkv))
+    ops.write_kv_int4(k, v, *want, slots)
+    assert torch.equal(k4, want[0]) and torch.equal(v4, want[1]) and k4.any()
+
+
+@pytest.mark.parametrize("eager", [True, False])
+def test_engine_over_a_4_bit_cache(eager):
+    from vllm_ascend_b200.config import ModelConfig
+    from vllm_ascend_b200.engine.llm import LLM
+    from vllm_ascend_b200.engine.request import SamplingParams
+    cfg = ModelConfig(name="t", architecture="Qwen3ForCausalLM", vocab_size=2048, hidden_size=512, intermediate_size=1024,
+                      num_hidden_layers=3, num_attention_heads=8, num_key_value_heads=2, head_dim=128, qk_norm=True, rope_theta=1e6,
+                      dtype="bfloat16", init_std=0.05)
+    rng = np.random.default_rng(0)
+    prompts = [rng.integers(0, 2048, size=n).tolist() for n in (150, 40, 333, 129)]
+    llm = LLM(cfg, device="cuda", max_model_len=512, max_num_seqs=8, max_num_batched_tokens=256, num_gpu_blocks_override=40,
+              enforce_eager=eager, cudagraph_capture_sizes=[2, 4, 8], kv_cache_dtype="int4")
+    outs = llm.generate(prompts, SamplingParams(temperature=0.0, max_tokens=12, ignore_eos=True))
+    assert all(len(o.outputs[0].token_ids) == 12 for o in outs)
+    again = llm.generate(prompts, SamplingParams(temperature=0.0, max_tokens=12, ignore_eos=True))
+    assert [o.outputs[0].token_ids for o in again] == [o.outputs[0].token_ids for o in outs]
+    runner = llm.engine.runner
+    assert eager or runner.stats["graph_replays"] > 0
+    assert all(t.dtype == torch.uint8 and t.any() for pair in runner.kv_caches for t in pair)
+    _native.check_status(torch.device(DEV))

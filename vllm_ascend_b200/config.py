@@ -601,7 +601,7 @@ class CacheConfig:
     gpu_memory_utilization: float = 0.92
     num_gpu_blocks: Optional[int] = None   # override; else profiled
     enable_prefix_caching: bool = False
-    kv_cache_dtype: str = "auto"
+    kv_cache_dtype: str = "auto"       # int4: ops/kv_int4.py; others: the model's type
     kv_layout: str = "HND"             # physical order inside a block: HND (per-head pages) | NHD
 
 

@@ -389,7 +389,7 @@ class LLM:
                  decode_context_parallel_size: int = 1, prefill_context_parallel_size: int = 1,
                  enable_lora: bool = False, max_loras: int = 4,
                  max_lora_rank: int = 64, async_scheduling: Optional[bool] = None, load_format: str = "auto",
-                 model_loader_extra_config: Optional[dict] = None, **unused):
+                 model_loader_extra_config: Optional[dict] = None, kv_cache_dtype: str = "auto", **unused):
         mcfg = model if isinstance(model, ModelConfig) else get_model_config(model)
         if dtype:
             mcfg.dtype = dtype
@@ -409,7 +409,7 @@ class LLM:
             model=mcfg,
             cache=CacheConfig(block_size=block_size, gpu_memory_utilization=gpu_memory_utilization,
                               num_gpu_blocks=num_gpu_blocks_override,
-                              enable_prefix_caching=enable_prefix_caching),
+                              enable_prefix_caching=enable_prefix_caching, kv_cache_dtype=kv_cache_dtype),
             scheduler=SchedulerConfig(max_num_seqs=max_num_seqs,
                                       max_num_batched_tokens=max(max_num_batched_tokens, 1),
                                       max_model_len=max_model_len,

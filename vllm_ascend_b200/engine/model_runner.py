@@ -229,7 +229,27 @@ class ModelRunner:
         shapes = attn.sequence_state_shapes(self.max_seqs + 1) if hasattr(attn, "sequence_state_shapes") else []
         return [s if isinstance(s[0], tuple) else (s, self.kv_dtype) for s in shapes]
 
+    def _kv_int4(self) -> bool:
+        """Whether keys and values are cached in 4 bits; raises for what cannot be."""
+        if self.cfg.cache.kv_cache_dtype != "int4":
+            return False
+        from ..batch_invariant import is_training_consistent
+        c, par = self.mcfg, self.cfg.parallel
+        for bad, what in ((c.use_mla, "latent attention"), (bool(c.layer_plan), "plan-built models"),
+                          (bool(self.cfg.kv_transfer_config), "KV transfer"),
+                          (par.decode_context_parallel_size > 1 or par.prefill_context_parallel_size > 1, "context parallelism"),
+                          (is_training_consistent(), "training-consistent attention")):
+            if bad:
+                raise NotImplementedError(f"kv_cache_dtype 'int4' with {what}")
+        from ..ops.kv_int4 import block_bytes
+        block_bytes(self.block_size, self._attn_layer().D)         # head and block sizes that such a cache takes
+        return True
+
     def kv_bytes_per_block(self) -> int:
+        if self._kv_int4():
+            from ..ops.kv_int4 import block_bytes
+            a = self._attn_layer()
+            return self._num_kv_layers() * 2 * a.Hkv * block_bytes(self.block_size, a.D)
         itemsize = torch.tensor([], dtype=self.kv_dtype).element_size()
         if self.mcfg.layer_plan:             # every layer has sizes of its own
             per_tok = sum(sum(h * d for h, d in L.self_attn.kv_cache_heads()) for L in self.model.layers
@@ -312,6 +332,7 @@ class ModelRunner:
                 shapes = [(num_blocks, self.block_size, a.Hkv, a.D)] * 2
             per_layer.append(shapes)
         layout = self.cfg.cache.kv_layout if self.is_cuda else "NHD"
+        int4 = self._kv_int4()
         self.kv_arena = None
         if self.cfg.kv_transfer_config and any(self._extra_states(L.self_attn) for L in self.model.layers):
             raise NotImplementedError("KV transfer of layers that keep a state beside their pages")
@@ -344,6 +365,9 @@ class ModelRunner:
                 else:
                     self.kv_caches.append((torch.zeros(cs, dtype=self.kv_dtype, device=self.device),
                                            torch.zeros(ss, dtype=torch.float32, device=self.device)))
+                continue
+            if int4:
+                self.kv_caches.append(tuple(ops.alloc_kv_cache_int4(s[0], s[1], s[2], s[3], self.device) for s in shapes))
                 continue
             self.kv_caches.append(tuple(
                 ops.alloc_kv_cache(s[0], s[1], s[2], s[3], self.kv_dtype, self.device, layout,

@@ -138,7 +138,16 @@ def qknorm_rope_kvwrite(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: tor
                         mrope_axis: Optional[torch.Tensor] = None) -> None:
     """Split-QKV + per-head q/k RMSNorm + neox RoPE + paged KV-cache write, one pass, in place.
     With ``mrope_axis`` (int32 [rot_dim/2]) positions is [3, N] and each rotary pair follows the
-    temporal / height / width position its table entry names (multimodal rotary embedding)."""
+    temporal / height / width position its table entry names (multimodal rotary embedding).  4-bit caches take the rows as
+    ``write_kv_int4`` quantises them, behind the norm and the rotation."""
+    if k_cache is not None and k_cache.dtype == torch.uint8:
+        if rot_dim or q_norm_w is not None or k_norm_w is not None:
+            qknorm_rope_kvwrite(qkv, positions, cos_sin, rot_dim, q_norm_w, k_norm_w, eps, None, None, None, Hq, Hkv, D, mrope_axis)
+        if slot_mapping is not None:
+            T = qkv.shape[0]
+            write_kv_int4(qkv[:, Hq * D:(Hq + Hkv) * D].view(T, Hkv, D), qkv[:, (Hq + Hkv) * D:(Hq + 2 * Hkv) * D].view(T, Hkv, D),
+                          k_cache, v_cache, slot_mapping[:T])
+        return
     native_ok = (_use_native(qkv) and D in (32, 64, 96, 128, 256) and rot_dim <= D
                  and (rot_dim == 0 or (rot_dim // 2) % 32 == 0)
                  and (k_cache is None or k_cache.dtype == _BF16))
@@ -657,6 +666,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     scale: float, out: Optional[torch.Tensor] = None, causal: bool = True,
                     window: int = 0) -> torch.Tensor:
     """Attention of every scheduled token over its sequence's paged KV."""
+    if k_cache.dtype == torch.uint8:
+        return paged_attention_int4(q, k_cache, v_cache, meta, scale, out, causal, window)
     T, Hq, D = q.shape
     if out is None:
         out = torch.empty((T, Hq, v_cache.shape[-1]), dtype=q.dtype, device=q.device)

@@ -7,6 +7,7 @@ a block] for the keys and one for the values (layout: csrc/kv_int4.cuh); head si
 The reference quantises its cache to 8 bits with static scales (vllm_ascend/quantization/methods/kv_c8.py)."""
 from __future__ import annotations
 
+import functools
 from ctypes import c_float, c_int, c_long, c_void_p
 from typing import Optional
 
@@ -48,51 +49,62 @@ def alloc_kv_cache_int4(num_blocks: int, block_size: int, heads: int, dim: int, 
     return arena.take(shape, torch.uint8) if arena is not None else torch.zeros(shape, dtype=torch.uint8, device=device)
 
 
-def _check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dim: int, device) -> int:
-    """Block size of a pair of caches that belong together."""
+def _check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dim: int, device: int) -> int:
+    """Block size of a pair of caches that belong together, on the device of that index (-1: the host)."""
+    shape = k_cache.shape
+    if dim in HEAD_SIZES and len(shape) == 3 and shape[2] and shape[2] % (9 * dim) == 0 and v_cache.shape == shape \
+            and k_cache.dtype is v_cache.dtype is torch.uint8 and k_cache.is_contiguous() and v_cache.is_contiguous() \
+            and k_cache.get_device() == v_cache.get_device() == device:
+        return shape[2] // (9 * dim) * ref.KV_INT4_TOKENS
     if dim not in HEAD_SIZES:
         raise ValueError(f"a 4-bit cache takes heads of {HEAD_SIZES}, not {dim}")
     bs = ref.kv_int4_block_size(k_cache, dim)
-    if v_cache.shape != k_cache.shape or ref.kv_int4_block_size(v_cache, dim) != bs:
-        raise ValueError(f"keys {tuple(k_cache.shape)} and values {tuple(v_cache.shape)} are caches of different sizes")
-    if k_cache.device != device or v_cache.device != device:
-        raise ValueError(f"caches on {k_cache.device} and {v_cache.device}, rows on {device}")
-    return bs
+    if v_cache.shape != shape or ref.kv_int4_block_size(v_cache, dim) != bs:
+        raise ValueError(f"keys {tuple(shape)} and values {tuple(v_cache.shape)} are caches of different sizes")
+    raise ValueError(f"caches on {k_cache.device} and {v_cache.device}, rows on device {device}")
 
 
-def _check_slots(slots: torch.Tensor, rows: int, device) -> torch.Tensor:
-    if slots.dim() != 1 or slots.shape[0] != rows or slots.device != device or slots.dtype not in (torch.int64, torch.int32):
-        raise ValueError(f"slots: {rows} whole numbers on {device}, not {slots.dtype} {tuple(slots.shape)} on {slots.device}")
-    return slots.to(torch.int64).contiguous()
+def _check_slots(slots: torch.Tensor, rows: int, device: int) -> torch.Tensor:
+    if slots.dim() != 1 or slots.shape[0] != rows or slots.get_device() != device or slots.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"slots: {rows} whole numbers on device {device}, not {slots.dtype} {tuple(slots.shape)} on {slots.device}")
+    return slots if slots.dtype is torch.int64 and slots.is_contiguous() else slots.to(torch.int64).contiguous()
 
 
 def _dense_heads(x: torch.Tensor) -> torch.Tensor:
     """x [T, H, D] as the kernels read rows: heads dense, rows and the first element on 16-byte boundaries."""
-    T, H, D = x.shape
-    if x.stride(2) == 1 and (x.stride(1) == D or H == 1) and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
+    row, head, channel = x.stride()
+    if channel == 1 and (head == x.shape[2] or x.shape[1] == 1) and row % 8 == 0 and x.data_ptr() % 16 == 0:
         return x
     return x.clone(memory_format=torch.contiguous_format)
+
+
+def _elsewhere(device: int) -> bool:
+    """Whether tensors of that device index are on a GPU that is not the current one."""
+    return device >= 0 and device != torch.cuda.current_device()
 
 
 def write_kv_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
     """Rows of k and v [T, heads, D] quantised into their slots (block * block size + offset) of a 4-bit cache; rows whose slot
     is below zero are not stored.  A slot may be listed once only."""
-    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or not k.is_floating_point() or k.device != v.device:
+    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or not k.is_floating_point() or k.get_device() != v.get_device():
         raise ValueError(f"keys {k.dtype} {tuple(k.shape)} and values {v.dtype} {tuple(v.shape)} are not rows [T, heads, D] of one type")
     T, H, D = k.shape
-    bs = _check_caches(k_cache, v_cache, D, k.device)
+    device = k.get_device()
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return write_kv_int4(k, v, k_cache, v_cache, slot_mapping)
+    bs = _check_caches(k_cache, v_cache, D, device)
     if H != k_cache.shape[1]:
         raise ValueError(f"rows of {H} heads, a cache of {k_cache.shape[1]}")
-    slots = _check_slots(slot_mapping, T, k.device)
+    slots = _check_slots(slot_mapping, T, device)
     if T == 0:
         return
-    if not k.is_cuda or k.dtype != torch.bfloat16:
+    if device < 0 or k.dtype is not torch.bfloat16:
         return ref.write_kv_int4(k, v, k_cache, v_cache, slots)
     k, v = _dense_heads(k), _dense_heads(v)
-    with torch.cuda.device(k.device):
-        rc = _native.lib().b200_kv_int4_write(
-            k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), T, slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            k_cache.shape[0] * bs, H, D, bs, _native.status_word(k.device).data_ptr(), _native.stream_ptr())
+    rc = _native.lib().b200_kv_int4_write(
+        k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), T, slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_cache.shape[0] * bs, H, D, bs, _native.status_word(k.device).data_ptr(), _native.stream_ptr())
     _native.check(rc, "kv_int4_write")
     _native.count_launch()
 
@@ -100,19 +112,22 @@ def write_kv_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
 def read_kv_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, dim: int) -> tuple[torch.Tensor, torch.Tensor]:
     """What slots of a 4-bit cache of heads of ``dim`` stand for: keys and values [slots, heads, dim] in bf16, exact.  Slots below zero
     read as zeros; a slot may be listed any number of times."""
-    bs = _check_caches(k_cache, v_cache, dim, k_cache.device)
-    n, H, dev = slots.shape[0] if slots.dim() else 0, k_cache.shape[1], k_cache.device
-    slots = _check_slots(slots, n, dev)
-    if not k_cache.is_cuda:
+    device = k_cache.get_device()
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return read_kv_int4(k_cache, v_cache, slots, dim)
+    bs = _check_caches(k_cache, v_cache, dim, device)
+    n, H = slots.shape[0] if slots.dim() else 0, k_cache.shape[1]
+    slots = _check_slots(slots, n, device)
+    if device < 0:
         return ref.read_kv_int4(k_cache, v_cache, slots, dim)
-    k = torch.empty((n, H, dim), dtype=torch.bfloat16, device=dev)
-    v = torch.empty_like(k)
+    k = k_cache.new_empty((n, H, dim), dtype=torch.bfloat16)
+    v = k_cache.new_empty((n, H, dim), dtype=torch.bfloat16)
     if n == 0:
         return k, v
-    with torch.cuda.device(dev):
-        rc = _native.lib().b200_kv_int4_read(
-            k.data_ptr(), v.data_ptr(), n, slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0] * bs, H, dim, bs,
-            _native.status_word(dev).data_ptr(), _native.stream_ptr())
+    rc = _native.lib().b200_kv_int4_read(
+        k.data_ptr(), v.data_ptr(), n, slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0] * bs, H, dim, bs,
+        _native.status_word(k.device).data_ptr(), _native.stream_ptr())
     _native.check(rc, "kv_int4_read")
     _native.count_launch()
     return k, v
@@ -126,7 +141,7 @@ def _parts(blocks: int, max_len: int, sms: int) -> int:
     """Parts that every sequence's keys are split into, by the blocks (three per SM) without a split."""
     if fixed_sums():
         return 1
-    most = min(3 * sms // max(1, blocks), -(-max_len // 128), 64)
+    most = min(3 * sms // max(1, blocks), -(-max_len // 128), 18)
     return max(1, most if most <= CLUSTER or max_len >= 8192 else CLUSTER)
 
 
@@ -137,8 +152,12 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     if q.dim() != 3:
         raise ValueError(f"queries are [T, heads, D], not {tuple(q.shape)}")
     T, Hq, D = q.shape
-    bs = _check_caches(k_cache, v_cache, D, q.device)
-    NB, Hkv, _ = k_cache.shape
+    device = q.get_device()
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return paged_attention_int4(q, k_cache, v_cache, meta, scale, out, causal, window)
+    bs = _check_caches(k_cache, v_cache, D, device)
+    Hkv = k_cache.shape[1]
     if Hkv == 0 or Hq % Hkv or Hq == 0:
         raise ValueError(f"{Hq} query heads do not share {Hkv} heads of a cache evenly")
     if not scale > 0:
@@ -146,31 +165,41 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     if window < 0:
         raise ValueError(f"window {window} is below zero")
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        out = q.new_empty((T, Hq, D))
+    elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device:
         raise ValueError(f"out: {q.dtype} {tuple(q.shape)} on {q.device}, not {out.dtype} {tuple(out.shape)} on {out.device}")
-    if not q.is_cuda or q.dtype != torch.bfloat16:
+    if device < 0 or q.dtype is not torch.bfloat16:
         return ref.paged_attention_int4(q, k_cache, v_cache, meta.query_start_loc_cpu, meta.seq_lens_cpu, meta.block_table, scale,
                                         causal, window, out=out)
     n = meta.num_reqs
     if n == 0 or T == 0:
         return out
     given, q = out, _dense_heads(q)
-    if out.stride(2) != 1 or out.stride(1) != D or out.stride(0) % 8 or out.data_ptr() % 16:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+    row, head, channel = out.stride()
+    if channel != 1 or head != D or row % 8 or out.data_ptr() % 16:
+        out = q.new_empty((T, Hq, D))
         out.copy_(given)
-    G = Hq // Hkv
-    with torch.cuda.device(q.device):
-        few = n
-        if meta.max_query_len * G > FEW_ROWS and G <= 128:
-            new = np.diff(meta.query_start_loc_cpu[:n + 1])
-            many = new * G > FEW_ROWS
-            few = int(many.argmax()) if many.any() else n      # sequences in front of the first that the other kernel takes
+    max_q, G = meta.max_query_len, Hq // Hkv
+    if max_q * G <= FEW_ROWS or G > 128:
+        _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, n, max_q)
+    else:
+        few, max_q, row, pairs = _plan(np.ascontiguousarray(meta.query_start_loc_cpu, dtype=np.int32)[:n + 1].tobytes(), G)
         if few:
-            _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, few, meta.max_query_len if few == n else int(new[:few].max()))
+            _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, few, max_q)
         if few < n:
-            _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, few, new[few:])
+            _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, few, row, pairs * Hkv)
     return out if out is given else given.copy_(out)
+
+
+@functools.lru_cache(maxsize=256)
+def _plan(cu: bytes, G: int) -> tuple[int, int, int, int]:
+    """Of sequences that begin at these int32 row numbers: how many in front the kernel for few rows takes, the most new tokens of one of
+    those, the first row of the others, and their pairs of query tiles."""
+    starts = np.frombuffer(cu, dtype=np.int32)
+    new = np.diff(starts)
+    many = new * G > FEW_ROWS
+    few = int(many.argmax()) if many.any() else len(new)
+    return few, int(new[:few].max(initial=0)), int(starts[few]), int((-(-new[few:] // (2 * (128 // G)))).sum())
 
 
 def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, n, max_q) -> None:
@@ -179,7 +208,9 @@ def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, n, max_
     NB, Hkv, _ = k_cache.shape
     rows = max_q * (Hq // Hkv)
     blocks = n * Hkv * (1 if rows <= 8 else -(-rows // 16))
-    parts = _parts(blocks, meta.max_seq_len, _native.sm_count(q.device))
+    # a captured graph is replayed with other lengths, up to what the table holds
+    longest = meta.block_table.shape[1] * bs if torch.cuda.is_current_stream_capturing() else meta.max_seq_len
+    parts = _parts(blocks, longest, _native.sm_count(q.get_device()))
     scratch = _scratch.get(q.device, T * Hq * parts * (D + 1)) if parts > CLUSTER else None
     rc = _native.lib().b200_attn_int4(
         q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(),
@@ -194,18 +225,18 @@ def _prompt_parts(blocks: int, max_len: int, sms: int) -> int:
     return max(1, min(sms // max(1, blocks), max_len // 512, 16))
 
 
-def _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, new) -> None:
-    """The sequences from ``first`` on, with ``new`` new tokens."""
+def _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, row, blocks) -> None:
+    """The sequences from ``first`` on, whose tokens begin at ``row``: ``blocks`` pairs of query tiles and heads."""
     T, Hq, D = q.shape
     NB, Hkv, _ = k_cache.shape
-    row, pair = int(meta.query_start_loc_cpu[first]), 2 * (128 // (Hq // Hkv))
-    blocks = int((-(-new // pair)).sum()) * Hkv
-    parts = 1 if fixed_sums() else _prompt_parts(blocks, meta.max_seq_len, _native.sm_count(q.device))
+    parts = 1 if fixed_sums() else _prompt_parts(blocks, meta.max_seq_len, _native.sm_count(q.get_device()))
     scratch = _scratch.get(q.device, T * Hq * parts * (D + 1)) if parts > 1 else None
+    cu, lens, table = meta.query_start_loc, meta.seq_lens, meta.block_table
+    if first:
+        cu, lens, table = cu[first:], lens[first:], table[first:]
     rc = _native.lib().b200_attn_int4_prefill(
-        q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, meta.query_start_loc[first:].data_ptr(),
-        meta.seq_lens[first:].data_ptr(), meta.block_table[first:].data_ptr(), meta.block_table.stride(0), meta.num_reqs - first, T - row,
-        Hq, Hkv, D, scale, int(causal), int(window), parts, out.data_ptr(), out.stride(0), _native.ptr(scratch),
-        _native.status_word(q.device).data_ptr(), _native.stream_ptr())
+        q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, cu.data_ptr(), lens.data_ptr(), table.data_ptr(),
+        table.stride(0), meta.num_reqs - first, T - row, Hq, Hkv, D, scale, int(causal), int(window), parts, out.data_ptr(), out.stride(0),
+        _native.ptr(scratch), _native.status_word(q.device).data_ptr(), _native.stream_ptr())
     _native.check(rc, "attn_int4_prefill")
     _native.count_launch(1 + int(parts > 1))
