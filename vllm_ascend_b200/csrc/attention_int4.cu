@@ -10,7 +10,7 @@
 //                   sum is free, so the query fragments follow what unpacking yields (channels j and j + 4 of eight)
 //   O^T = V^T P^T   D channels x 8 rows, over tokens.  A lane holds 16 (8) adjacent channels of four tokens; S^T's results
 //                   become P^T's fragments by transposing 8 x 8 blocks between the lanes
-// A block is one (sequence, KV head, part of the sequence); each of its warps walks a stretch of it, in tiles of 64 (32) tokens where
+// A block is one (sequence, KV head, part of the sequence); each of its warps walks a stretch of it, in tiles of 64 tokens where
 // all rows see them and 16 at a time at the edges, through a ring of its own that bulk copies fill, with a running maximum of
 // its own; they join at the end.  Parts join in a second kernel.
 #include "attention_int4.cuh"
@@ -32,12 +32,16 @@ __device__ __forceinline__ uint32_t i4_transpose(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+// NT tiles of 8 query rows: one with three blocks on an SM, two with two, whose warps have the registers for them (40 sequences of 2304
+// tokens, 32 rows of 4 heads: 56 us with three blocks and tiles of 32 tokens, 49 us).  More rows are blocks of their own that read
+// the pages again: four tiles (255 registers, spills, rows' fragments in shared memory) took 55 us there.
 template <int D, int NT>
 struct Int4Cfg {
-  static constexpr int U = NT == 1 ? 4 : 2;              // units of a tile
+  static constexpr int U = 4;                            // units of a tile
+  static constexpr int BLOCKS = NT == 1 ? 3 : 2;         // of an SM
   static constexpr int UNIT = kv4_unit_bytes(D);
   static constexpr int STAGE = 2 * U * UNIT;             // keys, then values
-  static constexpr int STAGES = 2 * (128 / D) * (NT == 1 ? 1 : 2);
+  static constexpr int STAGES = 2 * (128 / D);
   static constexpr int RING = STAGES * STAGE;
   static constexpr int ROWS = 8 * NT;
   static constexpr int SMEM = D4_WARPS * RING + 1024;    // barriers, maxima and sums behind the rings
@@ -46,7 +50,7 @@ struct Int4Cfg {
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * D4_WARPS, 3) attn_int4_kernel(const Int4Params p) {
+__global__ void __launch_bounds__(32 * D4_WARPS, Int4Cfg<D, NT>::BLOCKS) attn_int4_kernel(const Int4Params p) {
   using Cfg = Int4Cfg<D, NT>;
   constexpr int KW = D / 32;                    // groups: words of a token's keys in a lane
   constexpr int VX = D / 32;                    // words of two tokens' values in a lane
@@ -346,7 +350,7 @@ __global__ void __launch_bounds__(32 * D4_WARPS, 3) attn_int4_kernel(const Int4P
     } else {
 #pragma unroll 1
       for (int u = 0; u < n;) {
-        if (U > 2 && n - u >= 2 && inside(u0 + u, 2)) {
+        if (n - u >= 2 && inside(u0 + u, 2)) {
           tokens(std::integral_constant<int, 2>(), std::false_type(), ks + u * Cfg::UNIT, vs + u * Cfg::UNIT, (u0 + u) * KV4_TOKENS);
           u += 2;
         } else {

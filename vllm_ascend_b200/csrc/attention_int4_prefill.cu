@@ -343,8 +343,10 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
       int k_hi = seq_len;                      // keys [k_lo, k_hi) are visible to this row
       if (p.causal) k_hi = min(k_hi, q_pos + 1);
       const int k_lo = p.window > 0 ? max(0, q_pos - p.window + 1) : 0;
-      const int all_hi = p.causal ? min(seq_len, ctx + t_first + 1) : seq_len;                  // seen by every row of the tile
-      const int all_lo = p.window > 0 ? max(0, ctx + t_first + nt - p.window) : 0;
+      // seen by every row of the warp that there is
+      const int tok_a = (warp & 3) * 32 / G, tok_b = min(nt - 1, ((warp & 3) * 32 + 31) / G);
+      const int all_hi = p.causal ? min(seq_len, ctx + t_first + tok_a + 1) : seq_len;
+      const int all_lo = p.window > 0 ? max(0, ctx + t_first + tok_b - p.window + 1) : 0;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < nw; j++) {
         if (!__all_sync(0xffffffffu, mbar_wait(&s_full[w], (uint32_t)j & 1u, abort_word))) goto done;
@@ -356,15 +358,19 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
         tmem_ld_32x32b_x32(t_s + 96, sreg + 96);
         tmem_ld_wait();
         const int key0 = (t_a + j) << 7;
-        if (key0 + 128 > all_hi) {
-          const int end = k_hi - key0;
+        if (key0 + 128 > all_hi || key0 < all_lo) {
+          const int end = k_hi - key0, start = k_lo - key0;
 #pragma unroll
-          for (int i = 0; i < 128; i++) if (i >= end) sreg[i] = 0xff800000u;   // -inf
-        }
-        if (key0 < all_lo) {
-          const int start = k_lo - key0;
+          for (int c = 0; c < 4; c++) {          // 32 keys at a time, where some row of the warp does not see them all
+            if (key0 + 32 * c + 32 > all_hi) {
 #pragma unroll
-          for (int i = 0; i < 128; i++) if (i < start) sreg[i] = 0xff800000u;
+              for (int i = 32 * c; i < 32 * c + 32; i++) if (i >= end) sreg[i] = 0xff800000u;   // -inf
+            }
+            if (key0 + 32 * c < all_lo) {
+#pragma unroll
+              for (int i = 32 * c; i < 32 * c + 32; i++) if (i < start) sreg[i] = 0xff800000u;
+            }
+          }
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll

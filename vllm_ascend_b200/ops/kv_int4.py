@@ -137,11 +137,11 @@ def read_kv_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tens
 CLUSTER = 8
 
 
-def _parts(blocks: int, max_len: int, sms: int) -> int:
-    """Parts that every sequence's keys are split into, by the blocks (three per SM) without a split."""
+def _parts(blocks: int, max_len: int, at_once: int) -> int:
+    """Parts that every sequence's keys are split into, by the blocks without a split and those that run at once."""
     if fixed_sums():
         return 1
-    most = min(3 * sms // max(1, blocks), -(-max_len // 128), 18)
+    most = min(at_once // max(1, blocks), -(-max_len // 128), 18)
     return max(1, most if most <= CLUSTER or max_len >= 8192 else CLUSTER)
 
 
@@ -210,7 +210,7 @@ def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, n, max_
     blocks = n * Hkv * (1 if rows <= 8 else -(-rows // 16))
     # a captured graph is replayed with other lengths, up to what the table holds
     longest = meta.block_table.shape[1] * bs if torch.cuda.is_current_stream_capturing() else meta.max_seq_len
-    parts = _parts(blocks, longest, _native.sm_count(q.get_device()))
+    parts = _parts(blocks, longest, (3 if rows <= 8 else 2) * _native.sm_count(q.get_device()))
     scratch = _scratch.get(q.device, T * Hq * parts * (D + 1)) if parts > CLUSTER else None
     rc = _native.lib().b200_attn_int4(
         q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(),
