@@ -17,7 +17,7 @@
 
 namespace b200 {
 
-constexpr int P4_THREADS = 512;
+constexpr int P4_THREADS = 448;
 constexpr int P4_HALF = 128 * 128;          // 128 rows x 64 bf16
 constexpr int P4_RING = 3;                  // packed tiles
 constexpr int P4_EDGE = 3;                  // tiles at either end that a pair of query tiles (256 tokens at most) may see in part
@@ -32,11 +32,6 @@ struct Int4PrefillCfg {
   static constexpr int SMEM_BYTES = 6 * TILE + P4_RING * PACKED + NOTES + 1024 + 512;
 };
 
-template <int R>
-__device__ __forceinline__ void p4_fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
-template <int R>
-__device__ __forceinline__ void p4_more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
-
 template <int D>
 __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const Int4Params p) {
   using Cfg = Int4PrefillCfg<D>;
@@ -45,7 +40,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
   extern __shared__ uint8_t smem_raw[];
   __shared__ int item[4];                     // sequence, its first query row, query rows, keys
   const int warp = warp_index(), lane = threadIdx.x & 31;
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);      // still known to be shared memory
   uint8_t* Qs = smem;
   uint8_t* Ks = Qs + 2 * TILE;
   uint8_t* Vs = Ks + 2 * TILE;
@@ -131,9 +126,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
     return i < P4_EDGE ? i : i >= all - P4_EDGE ? i - (all - 2 * P4_EDGE) : -1;
   };
 
-  // 512 threads of 128 registers; 256 x 184 + 128 x 96 + 128 x 40 are no more than that
   if (warp >= 12) {
-    p4_fewer_registers<40>();
     if (warp == 12) {
       // ---------------------------------------------------------- packed tiles
       const int upp = p.block_size / KV4_TOKENS;
@@ -200,7 +193,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
               tc_fence_after();
 #pragma unroll
               for (int kk = 0; kk < 8; kk++)
-                umma_f16_ts(tmem_base + O_COL + w * 128, tmem_base + w * 128 + kk * 8, dv + kk * 128, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+                umma_f16_ts(tmem_base + O_COL + w * 128, tmem_base + w * 128 + (kk & 3) * 8 + (kk >> 2) * 64, dv + kk * 128, idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
               if (j == nw - 1) umma_commit(&o_full[w]);
               if (j + 1 < nw) issue_s(w, j + 1);
             }
@@ -212,7 +205,6 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
     }
   } else if (warp >= 8) {
     // ------------------------------------------------------------ unpacking
-    p4_fewer_registers<96>();
     if (n > 0) {
       const int wl = warp - 8;
       for (int j = 0; j < n; j++) {
@@ -299,7 +291,6 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
     }
   } else {
     // ------------------------------------------------------------ softmax / epilogue of query tile w
-    p4_more_registers<184>();
     const int w = warp >> 2;
     const int nw = w == 0 ? n0 : n1, nt = w == 0 ? ntok[0] : ntok[1];
     {
@@ -351,33 +342,40 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
       for (int j = 0; j < nw; j++) {
         if (!__all_sync(0xffffffffu, mbar_wait(&s_full[w], (uint32_t)j & 1u, abort_word))) goto done;
         tc_fence_after();
-        uint32_t sreg[128];
-        tmem_ld_32x32b_x32(t_s, sreg);
-        tmem_ld_32x32b_x32(t_s + 32, sreg + 32);
-        tmem_ld_32x32b_x32(t_s + 64, sreg + 64);
-        tmem_ld_32x32b_x32(t_s + 96, sreg + 96);
-        tmem_ld_wait();
+        // 64 scores at a time: the maximum of all, then the second half's probabilities out of the registers that still hold it, then the
+        // first half's.  A half's probabilities replace its own scores (keys 64 on: column 64 on), two to a column
         const int key0 = (t_a + j) << 7;
-        if (key0 + 128 > all_hi || key0 < all_lo) {
-          const int end = k_hi - key0, start = k_lo - key0;
+        uint32_t sr[64];
+        auto half = [&](int hf) {
+          tmem_ld_32x32b_x32(t_s + 64 * hf, sr);
+          tmem_ld_32x32b_x32(t_s + 64 * hf + 32, sr + 32);
+          tmem_ld_wait();
+          const int first = key0 + 64 * hf;
+          if (first + 64 > all_hi || first < all_lo) {
+            const int end = k_hi - first, start = k_lo - first;
 #pragma unroll
-          for (int c = 0; c < 4; c++) {          // 32 keys at a time, where some row of the warp does not see them all
-            if (key0 + 32 * c + 32 > all_hi) {
+            for (int c = 0; c < 2; c++) {        // 32 keys at a time, where some row of the warp does not see them all
+              if (first + 32 * c + 32 > all_hi) {
 #pragma unroll
-              for (int i = 32 * c; i < 32 * c + 32; i++) if (i >= end) sreg[i] = 0xff800000u;   // -inf
-            }
-            if (key0 + 32 * c < all_lo) {
+                for (int i = 32 * c; i < 32 * c + 32; i++) if (i >= end) sr[i] = 0xff800000u;   // -inf
+              }
+              if (first + 32 * c < all_lo) {
 #pragma unroll
-              for (int i = 32 * c; i < 32 * c + 32; i++) if (i < start) sreg[i] = 0xff800000u;
+                for (int i = 32 * c; i < 32 * c + 32; i++) if (i < start) sr[i] = 0xff800000u;
+              }
             }
           }
-        }
+        };
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 128; i += 8)
+        for (int hf = 0; hf < 2; hf++) {
+          half(hf);
 #pragma unroll
-          for (int q = 0; q < 4; q++)
-            mx[q] = fmaxf(mx[q], fmaxf(__uint_as_float(sreg[i + 2 * q]), __uint_as_float(sreg[i + 2 * q + 1])));
+          for (int i = 0; i < 64; i += 8)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+              mx[q] = fmaxf(mx[q], fmaxf(__uint_as_float(sr[i + 2 * q]), __uint_as_float(sr[i + 2 * q + 1])));
+        }
         const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         // O is rescaled only when the running maximum moved by more than 2^8 (powers of two: exact)
         float alpha = 1.f;
@@ -403,17 +401,21 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
         const float nmb = m == -INFINITY ? 0.f : -m * sl2;
         float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          uint32_t pk[16];
+        for (int hf = 1; hf >= 0; hf--) {
+          if (hf == 0) half(0);
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const float p0 = i4_exp2(fmaf(__uint_as_float(sreg[c * 32 + 2 * i]), sl2, nmb));
-            const float p1 = i4_exp2(fmaf(__uint_as_float(sreg[c * 32 + 2 * i + 1]), sl2, nmb));
-            rs[(i & 1) * 2] += p0;
-            rs[(i & 1) * 2 + 1] += p1;
-            pk[i] = pack_bf16x2(p0, p1);
+          for (int c = 0; c < 2; c++) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const float p0 = i4_exp2(fmaf(__uint_as_float(sr[c * 32 + 2 * i]), sl2, nmb));
+              const float p1 = i4_exp2(fmaf(__uint_as_float(sr[c * 32 + 2 * i + 1]), sl2, nmb));
+              rs[(i & 1) * 2] += p0;
+              rs[(i & 1) * 2 + 1] += p1;
+              pk[i] = pack_bf16x2(p0, p1);
+            }
+            tmem_st_32x32b_x16(t_s + 64 * hf + c * 16, pk);
           }
-          tmem_st_32x32b_x16(t_s + c * 16, pk);
         }
         l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
         tmem_st_wait();
