@@ -283,6 +283,62 @@ def test_modes_with_a_fixed_order_of_sums(monkeypatch):
         assert torch.equal(ops.paged_attention_int4(q[b:b + 1], kc, vc, one, 0.1), out[b:b + 1])
 
 
+def test_modes_with_a_fixed_order_of_sums_over_mixed_batches(monkeypatch):
+    """Neither do short sequences behind long ones change with their neighbours."""
+    new, lens = [1, 200, 3, 1, 90], [700, 200, 503, 64, 1000]
+    q, kc, vc, meta = _setup(new, lens, 32, 8, 2, 128, 15)
+    monkeypatch.setattr("vllm_ascend_b200.ops.kv_int4.fixed_sums", lambda: True)
+    out = ops.paged_attention_int4(q, kc, vc, meta, 0.1)
+    _check(out, *_want(q, kc, vc, meta, 0.1))
+    cu = meta.query_start_loc_cpu
+    for b in range(5):
+        one = _meta(new[b:b + 1], lens[b:b + 1], meta.block_table[b:b + 1], 8, 2, 128)
+        assert torch.equal(ops.paged_attention_int4(q[cu[b]:cu[b + 1]], kc, vc, one, 0.1), out[cu[b]:cu[b + 1]])
+
+
+@pytest.mark.parametrize("new,lens", [([1], [40000]), ([300], [9000])])
+def test_calls_on_two_streams_at_once(new, lens):
+    """Sequences in parts that join through memory: every call, and every graph, has its own."""
+    sets = [_setup(new, lens, 128, 8, 2, 128, seed) for seed in (16, 17)]
+    want = [ops.paged_attention_int4(*s, 0.09) for s in sets]
+    torch.cuda.synchronize()
+    sides, graphs, got, replayed = [torch.cuda.Stream() for _ in sets], [], [[], []], []
+    for _ in range(20):
+        for i, s in enumerate(sets):
+            with torch.cuda.stream(sides[i]):
+                got[i].append(ops.paged_attention_int4(*s, 0.09))
+    torch.cuda.synchronize()
+    for i, s in enumerate(sets):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            replayed.append(ops.paged_attention_int4(*s, 0.09))
+    for x in replayed:
+        x.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, graph in enumerate(graphs):
+            with torch.cuda.stream(sides[i]):
+                graph.replay()
+    torch.cuda.synchronize()
+    # a captured call may split a sequence otherwise (by what its table holds)
+    for x, s in zip(replayed, sets):
+        _check(x, *_want(*s, 0.09))
+
+
+@pytest.mark.parametrize("new", [[1, 1], [100, 60]])
+def test_row_numbers_beyond_the_rows_are_reported(new):
+    q, kc, vc, meta = _setup(new, [200, 300], 32, 8, 2, 128, 18)
+    want, tol = _want(q, kc, vc, meta, 0.1)
+    meta.query_start_loc[2] += 1
+    out = torch.full_like(q, 5.0)
+    ops.paged_attention_int4(q, kc, vc, meta, 0.1, out=out)
+    _check(out[:new[0]], want[:new[0]], tol[:new[0]])
+    assert out[new[0]:].eq(5).all()
+    with pytest.raises(_native.NativeError, match="BAD_INDEX"):
+        _native.check_status(torch.device(DEV))
+
+
 def test_graph_replay_with_other_lengths_and_another_stream():
     lens = [700, 1, 2000]
     q, kc, vc, meta = _setup([1] * 3, lens, 128, 32, 8, 128, 14)

@@ -1,5 +1,6 @@
 """4-bit cache on the host: the quantiser against its definition in whole numbers, the page layout byte by byte, what the operators
 refuse, attention over the cache."""
+import dataclasses
 from fractions import Fraction
 
 import numpy as np
@@ -145,6 +146,18 @@ def test_refusals():
                     (dict(out=q.double()), "out"), (dict(q=torch.zeros(2, 4, 96)), "takes heads")):
         with pytest.raises(ValueError, match=why):
             ops.paged_attention_int4(**{**dict(q=q, k_cache=kc, v_cache=vc, meta=meta, scale=0.125), **kw})
+    for kw in (dict(seq_lens=meta.seq_lens.long()), dict(block_table=meta.block_table[:1]), dict(query_start_loc=meta.query_start_loc[:2])):
+        with pytest.raises(ValueError, match="metadata of 2 sequences"):
+            ops.paged_attention_int4(q, kc, vc, dataclasses.replace(meta, **kw), 0.125)
+
+
+def test_which_sequences_share_a_launch():
+    from vllm_ascend_b200.ops.kv_int4 import _plan
+    cu = np.cumsum([0, 1, 8, 9, 1, 0, 300, 2]).astype(np.int32).tobytes()
+    assert _plan(cu, 4, False) == ((True, 0, 2, (8,)), (False, 2, 7, (312, 8)))
+    assert _plan(cu, 4, True) == ((True, 0, 2, (8,)), (False, 2, 3, (9, 1)), (True, 3, 5, (1,)), (False, 5, 6, (300, 5)), (True, 6, 7, (2,)))
+    assert _plan(cu, 128, False) == ((False, 0, 7, (321, 162)),)
+    assert _plan(np.array([0, 1, 3], dtype=np.int32).tobytes(), 4, False) == ((True, 0, 2, (2,)),)
 
 
 def test_nothing_to_do():

@@ -64,3 +64,25 @@ def test_refusals():
         LLM(get_model_config("tiny-deepseek"), **small)
     with pytest.raises(NotImplementedError, match="plan-built"):
         LLM(get_model_config("tiny-nevotar"), **small)
+    runner = LLM(_cfg(), **small).engine.runner
+    runner.is_cuda = True                        # float32: its rows would go through the host's definitions, which no graph can hold
+    with pytest.raises(NotImplementedError, match="float32 on a GPU"):
+        runner.kv_bytes_per_block()
+
+
+def test_dispatcher_schema_and_copied_blocks():
+    import vllm_ascend_b200.ops.torch_bindings as tb
+    from vllm_ascend_b200.attention.backend import B200AttentionBackend
+    from vllm_ascend_b200.attention.metadata import metadata_from_tensors
+    tb.register()
+    g = torch.Generator().manual_seed(5)
+    kc, vc = (ops.alloc_kv_cache_int4(4, 16, 2, 64, "cpu") for _ in "kv")
+    ops.write_kv_int4(*(torch.randn(32, 2, 64, generator=g) for _ in "kv"), kc, vc, torch.arange(32))
+    q = torch.randn(3, 4, 64, generator=g)
+    cu, lens = torch.tensor([0, 1, 3], dtype=torch.int32), torch.tensor([16, 9], dtype=torch.int32)
+    table = torch.tensor([[0], [1]], dtype=torch.int32)
+    out = ops.paged_attention(q, kc, vc, metadata_from_tensors(cu, lens, table, 2, 16, 4, 2, 64), 0.125)
+    assert torch.equal(getattr(torch.ops, tb.NAMESPACE).paged_attention(q, kc, vc, table, lens, cu, 2, 16, 0.125, True, 0), out)
+    B200AttentionBackend.copy_blocks([(kc, vc)], torch.tensor([[0, 3], [1, 2]]))
+    moved = metadata_from_tensors(cu, lens, 3 - table, 2, 16, 4, 2, 64)
+    assert torch.equal(ops.paged_attention(q, kc, vc, moved, 0.125), out)

@@ -6,6 +6,8 @@ choose it from the batch, and what the mode does there:
 * the split-KV factor of decode attention (grouped, latent, variants): 1.  Where a context-parallel rank needs the log-sum-exp
   of latent attention, which two splits give, or a caller names a factor, the splits are even parts of each sequence by itself
   (latent attention cuts by the lengths of all sequences of the step in other modes);
+* attention over 4-bit caches: one part, and the kernel for few rows or that for many by a sequence's own rows, in a launch for every
+  run of either;
 * the collective algorithm: a fixed one;
 * products of few rows, which split K over the blocks of a cluster (bf16 and block-scaled fp8): not
   taken.  The other GEMM kernels accumulate every output element over K in one fixed order whatever

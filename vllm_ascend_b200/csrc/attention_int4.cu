@@ -71,6 +71,10 @@ __global__ void __launch_bounds__(32 * D4_WARPS, Int4Cfg<D, NT>::BLOCKS) attn_in
   const int q_start = p.cu[seq], q_len = p.cu[seq + 1] - q_start, len = p.seq_lens[seq], ctx = len - q_len;
   const int rows = min(q_len * p.G - row0, ROWS);
   if (rows <= 0) return;
+  if (q_start < 0 || q_start + (long)q_len > p.q_rows) {         // reported; nothing lies there
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, B200_BAD_INDEX);
+    return;
+  }
   if (lane == 0)
     for (int s = 0; s < Cfg::STAGES; s++) mbar_init(&bars[s], 1);
   if (threadIdx.x == 0) *abort_word = 0;
@@ -490,7 +494,7 @@ __global__ void __launch_bounds__(128) attn_int4_join_kernel(const float* part_o
   const long first = cu[0], end = cu[num_seqs];
   const long tok = first + at / heads;
   const int head = (int)(at % heads);
-  if (at >= rows || tok >= end) return;
+  if (at >= rows || tok < 0 || tok >= end || tok * heads >= rows) return;
   const float* lse = part_lse + (tok * heads + head) * parts;
   const float* o = part_o + (tok * heads + head) * parts * D;
   // a lane's weights: of parts lane and lane + 32
@@ -573,6 +577,7 @@ int int4_params(Int4Params* p, const void* q, long q_stride, long q_rows, const 
   p->part_o = (float*)scratch;
   p->part_lse = p->part_o + q_rows * Hq * parts * D;
   p->q_stride = q_stride; p->out_stride = out_stride; p->num_blocks = num_blocks;
+  p->q_rows = q_rows;
   p->num_seqs = num_seqs; p->max_blocks = max_blocks; p->block_size = block_size;
   p->G = G; p->Hkv = Hkv; p->parts = parts; p->causal = causal; p->window = window;
   const int upp = block_size / KV4_TOKENS;

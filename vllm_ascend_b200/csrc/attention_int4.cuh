@@ -13,7 +13,7 @@ struct Int4Params {
   const int *cu, *seq_lens, *block_table;
   __nv_bfloat16* out;
   float *part_o, *part_lse;       // [tokens x heads][parts][D], [..][parts]: results of parts, normalised, with log2 of their sums
-  long q_stride, out_stride, num_blocks;
+  long q_stride, out_stride, num_blocks, q_rows;
   int num_seqs, max_blocks, block_size, G, Hkv, parts, cluster, row_blocks, causal, window;
   uint32_t g_inv, upp_inv;        // ceil(2^32 / .) of G and of the units of a page (int4_div)
   float scale_log2;               // of scores over unpacked keys, which carry 2^-40

@@ -104,7 +104,9 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
   const uint32_t tmem_base = warp_uniform(*tmem_ptr);
   const int seq = item[0], q_start = item[1], q_len = item[2], seq_len = item[3], ctx = seq_len - q_len;
   const int tok0 = (wi - ((q_start - base) / pair + seq)) * pair;
-  if (tok0 >= q_len) {                        // the grid has a pair more than some sequences
+  const bool beyond = q_start < 0 || q_start + (long)q_len > p.q_rows;          // reported; nothing lies there
+  if (tok0 >= q_len || beyond) {              // the grid has a pair more than some sequences
+    if (beyond && threadIdx.x == 0 && p.status) atomicExch(p.status, B200_BAD_INDEX);
     if (warp == 13) tmem_dealloc(tmem_base, 512);
     return;
   }

@@ -238,7 +238,8 @@ class ModelRunner:
         for bad, what in ((c.use_mla, "latent attention"), (bool(c.layer_plan), "plan-built models"),
                           (bool(self.cfg.kv_transfer_config), "KV transfer"),
                           (par.decode_context_parallel_size > 1 or par.prefill_context_parallel_size > 1, "context parallelism"),
-                          (is_training_consistent(), "training-consistent attention")):
+                          (is_training_consistent(), "training-consistent attention"),
+                          (self.is_cuda and self.kv_dtype != torch.bfloat16, f"models in {self.kv_dtype} on a GPU")):
             if bad:
                 raise NotImplementedError(f"kv_cache_dtype 'int4' with {what}")
         from ..ops.kv_int4 import block_bytes

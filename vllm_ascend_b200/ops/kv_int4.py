@@ -17,7 +17,6 @@ import torch
 from .. import _native
 from ..batch_invariant import fixed_sums
 from . import reference as ref
-from .scratch import Scratch
 
 _P, _I, _L, _F = c_void_p, c_int, c_long, c_float
 _native.register_signature("b200_kv_int4_write", [_P, _L, _P, _L, _L, _P, _P, _P, _L, _I, _I, _I, _P, _P])
@@ -30,8 +29,6 @@ _native.register_signature("b200_attn_int4_prefill",
 HEAD_SIZES = (64, 128)
 #: rows (new tokens times heads of a group) of a sequence up to which the kernel for few rows takes it
 FEW_ROWS = 32
-
-_scratch = Scratch(torch.float32)
 
 
 def block_bytes(block_size: int, dim: int) -> int:
@@ -168,10 +165,15 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         out = q.new_empty((T, Hq, D))
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device:
         raise ValueError(f"out: {q.dtype} {tuple(q.shape)} on {q.device}, not {out.dtype} {tuple(out.shape)} on {out.device}")
+    n = meta.num_reqs
+    cu, lens, table = meta.query_start_loc, meta.seq_lens, meta.block_table
+    if not (cu.dtype is lens.dtype is table.dtype is torch.int32 and cu.get_device() == lens.get_device() == table.get_device() == device
+            and cu.shape[0] > n and lens.shape[0] >= n and table.shape[0] >= n and table.stride(1) == 1):
+        raise ValueError(f"metadata of {n} sequences: row numbers {cu.dtype} {tuple(cu.shape)}, lengths {lens.dtype} {tuple(lens.shape)}, "
+                         f"pages {table.dtype} {tuple(table.shape)}, not int32 on device {device}")
     if device < 0 or q.dtype is not torch.bfloat16:
         return ref.paged_attention_int4(q, k_cache, v_cache, meta.query_start_loc_cpu, meta.seq_lens_cpu, meta.block_table, scale,
                                         causal, window, out=out)
-    n = meta.num_reqs
     if n == 0 or T == 0:
         return out
     given, q = out, _dense_heads(q)
@@ -180,44 +182,67 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         out = q.new_empty((T, Hq, D))
         out.copy_(given)
     max_q, G = meta.max_query_len, Hq // Hkv
+    window = min(window, 2 ** 31 - 1)
+    args = (q, k_cache, v_cache, meta, scale, out, causal, window, bs)
     if max_q * G <= FEW_ROWS or G > 128:
-        _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, n, max_q)
+        _few_rows(*args, 0, n, max_q)
     else:
-        few, max_q, row, pairs = _plan(np.ascontiguousarray(meta.query_start_loc_cpu, dtype=np.int32)[:n + 1].tobytes(), G)
-        if few:
-            _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, few, max_q)
-        if few < n:
-            _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, few, row, pairs * Hkv)
+        for few, first, end, what in _plan(np.ascontiguousarray(meta.query_start_loc_cpu, dtype=np.int32)[:n + 1].tobytes(), G, fixed_sums()):
+            if few:
+                _few_rows(*args, first, end, what[0])
+            else:
+                _prompts(*args, first, end, *what)
     return out if out is given else given.copy_(out)
 
 
 @functools.lru_cache(maxsize=256)
-def _plan(cu: bytes, G: int) -> tuple[int, int, int, int]:
-    """Of sequences that begin at these int32 row numbers: how many in front the kernel for few rows takes, the most new tokens of one of
-    those, the first row of the others, and their pairs of query tiles."""
+def _plan(cu: bytes, G: int, fixed: bool) -> tuple:
+    """Launches for sequences that begin at these int32 row numbers: (whether of the kernel for few rows, first sequence, end, and the most new
+    tokens of one, or their rows and pairs of query tiles).  Sequences of few rows in front of the others go to the kernel for them; those
+    behind go with the others, except (``fixed``) where which kernel a sequence gets must not depend on its neighbours."""
     starts = np.frombuffer(cu, dtype=np.int32)
     new = np.diff(starts)
-    many = new * G > FEW_ROWS
-    few = int(many.argmax()) if many.any() else len(new)
-    return few, int(new[:few].max(initial=0)), int(starts[few]), int((-(-new[few:] // (2 * (128 // G)))).sum())
+    many = new.astype(np.int64) * G > FEW_ROWS
+    ends = np.flatnonzero(np.diff(many)) + 1 if fixed else np.flatnonzero(many)[:1]
+    plan = []
+    for first, end in zip([0, *ends.tolist()], [*ends.tolist(), len(new)]):
+        if first < end:
+            n = new[first:end]
+            few = not (many[first:end].any())
+            plan.append((few, first, end, (int(n.max()),) if few else (int(n.sum()), int((-(-n // (2 * (128 // G)))).sum()))))
+    return tuple(plan)
 
 
-def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, n, max_q) -> None:
-    """The first ``n`` sequences of the batch, none with more than ``max_q`` new tokens."""
+def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, end, max_q) -> None:
+    """Sequences ``first`` to ``end``, none with more than ``max_q`` new tokens."""
     T, Hq, D = q.shape
+    n = end - first
     NB, Hkv, _ = k_cache.shape
     rows = max_q * (Hq // Hkv)
     blocks = n * Hkv * (1 if rows <= 8 else -(-rows // 16))
     # a captured graph is replayed with other lengths, up to what the table holds
     longest = meta.block_table.shape[1] * bs if torch.cuda.is_current_stream_capturing() else meta.max_seq_len
     parts = _parts(blocks, longest, (3 if rows <= 8 else 2) * _native.sm_count(q.get_device()))
-    scratch = _scratch.get(q.device, T * Hq * parts * (D + 1)) if parts > CLUSTER else None
+    scratch = _results(q, parts) if parts > CLUSTER else None
+    cu, lens, table = _of(meta, first)
     rc = _native.lib().b200_attn_int4(
-        q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(),
-        meta.block_table.data_ptr(), meta.block_table.stride(0), n, max_q, Hq, Hkv, D, scale, int(causal), int(window), parts,
+        q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, cu.data_ptr(), lens.data_ptr(),
+        table.data_ptr(), table.stride(0), n, max_q, Hq, Hkv, D, scale, int(causal), int(window), parts,
         out.data_ptr(), out.stride(0), _native.ptr(scratch), _native.status_word(q.device).data_ptr(), _native.stream_ptr())
     _native.check(rc, "attn_int4")
     _native.count_launch(1 + int(parts > CLUSTER))
+
+
+def _of(meta, first: int):
+    """Row numbers, lengths and pages of the sequences from ``first`` on."""
+    cu, lens, table = meta.query_start_loc, meta.seq_lens, meta.block_table
+    return (cu[first:], lens[first:], table[first:]) if first else (cu, lens, table)
+
+
+def _results(q, parts: int) -> torch.Tensor:
+    """Memory for the results of parts.  Each call has its own: calls on two streams, or two graphs, may run at once."""
+    T, Hq, D = q.shape
+    return torch.empty(T * Hq * parts * (D + 1), dtype=torch.float32, device=q.device)
 
 
 def _prompt_parts(blocks: int, max_len: int, sms: int) -> int:
@@ -225,18 +250,16 @@ def _prompt_parts(blocks: int, max_len: int, sms: int) -> int:
     return max(1, min(sms // max(1, blocks), max_len // 512, 16))
 
 
-def _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, row, blocks) -> None:
-    """The sequences from ``first`` on, whose tokens begin at ``row``: ``blocks`` pairs of query tiles and heads."""
+def _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, end, tokens, pairs) -> None:
+    """Sequences ``first`` to ``end`` with so many new tokens and pairs of query tiles."""
     T, Hq, D = q.shape
     NB, Hkv, _ = k_cache.shape
-    parts = 1 if fixed_sums() else _prompt_parts(blocks, meta.max_seq_len, _native.sm_count(q.get_device()))
-    scratch = _scratch.get(q.device, T * Hq * parts * (D + 1)) if parts > 1 else None
-    cu, lens, table = meta.query_start_loc, meta.seq_lens, meta.block_table
-    if first:
-        cu, lens, table = cu[first:], lens[first:], table[first:]
+    parts = 1 if fixed_sums() else _prompt_parts(pairs * Hkv, meta.max_seq_len, _native.sm_count(q.get_device()))
+    scratch = _results(q, parts) if parts > 1 else None
+    cu, lens, table = _of(meta, first)
     rc = _native.lib().b200_attn_int4_prefill(
         q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, cu.data_ptr(), lens.data_ptr(), table.data_ptr(),
-        table.stride(0), meta.num_reqs - first, T - row, Hq, Hkv, D, scale, int(causal), int(window), parts, out.data_ptr(), out.stride(0),
+        table.stride(0), end - first, tokens, Hq, Hkv, D, scale, int(causal), int(window), parts, out.data_ptr(), out.stride(0),
         _native.ptr(scratch), _native.status_word(q.device).data_ptr(), _native.stream_ptr())
     _native.check(rc, "attn_int4_prefill")
     _native.count_launch(1 + int(parts > 1))

@@ -97,7 +97,7 @@ def _impls():
         from .. import envs
         from ..attention.metadata import metadata_from_tensors
         meta = metadata_from_tensors(query_start_loc, seq_lens, block_table, max_query_len, max_seq_len, q.shape[1],
-                                     k_cache.shape[2], q.shape[2],
+                                     k_cache.shape[1 if k_cache.dtype == torch.uint8 else 2], q.shape[2],
                                      decode_kernel=envs.VLLM_B200_DECODE_ATTN == "native")
         return ops.paged_attention(q, k_cache, v_cache, meta, scale, None, causal, window)
 
