@@ -34,7 +34,8 @@ def _greedy(llm, prompt, n, page=16):
     return ids[len(prompt):]
 
 
-@pytest.mark.parametrize("kw", [{}, {"enable_prefix_caching": True}, {"max_num_batched_tokens": 32}])
+@pytest.mark.parametrize("kw", [{}, {"enable_prefix_caching": True}, {"max_num_batched_tokens": 32},
+                                {"speculative_config": {"method": "ngram", "num_speculative_tokens": 2}}])
 def test_generation_over_a_4_bit_cache(kw):
     rng = np.random.default_rng(1)
     prompts = [rng.integers(0, 256, size=n).tolist() for n in (5, 40, 17)]

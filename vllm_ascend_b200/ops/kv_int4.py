@@ -162,13 +162,13 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     if window < 0:
         raise ValueError(f"window {window} is below zero")
     if out is None:
-        out = q.new_empty((T, Hq, D))
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((T, Hq, D))
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device:
         raise ValueError(f"out: {q.dtype} {tuple(q.shape)} on {q.device}, not {out.dtype} {tuple(out.shape)} on {out.device}")
     n = meta.num_reqs
     cu, lens, table = meta.query_start_loc, meta.seq_lens, meta.block_table
     if not (cu.dtype is lens.dtype is table.dtype is torch.int32 and cu.get_device() == lens.get_device() == table.get_device() == device
-            and cu.shape[0] > n and lens.shape[0] >= n and table.shape[0] >= n and table.stride(1) == 1):
+            and cu.numel() > n and lens.numel() >= n and table.shape[0] >= n and table.stride()[1] == 1):
         raise ValueError(f"metadata of {n} sequences: row numbers {cu.dtype} {tuple(cu.shape)}, lengths {lens.dtype} {tuple(lens.shape)}, "
                          f"pages {table.dtype} {tuple(table.shape)}, not int32 on device {device}")
     if device < 0 or q.dtype is not torch.bfloat16:
