@@ -272,6 +272,16 @@ def test_given_outputs_strides_and_other_types():
     assert f32.dtype == torch.float32 and float((f32.double() - want).abs().max()) < 1e-4
 
 
+@pytest.fixture(params=["prompts", "few rows"])
+def kernel(request, monkeypatch):
+    """Sequences that could go to either kernel go to this one."""
+    from vllm_ascend_b200.ops import kv_int4
+    monkeypatch.setattr(kv_int4, "_prompt_us", lambda *a: 1e9 if request.param == "few rows" else -1e9)
+    kv_int4._plan.cache_clear()
+    yield request.param
+    kv_int4._plan.cache_clear()
+
+
 def test_modes_with_a_fixed_order_of_sums(monkeypatch):
     """A sequence's row has the same bits alone and in a batch."""
     lens = [1000, 64, 513]
@@ -297,7 +307,7 @@ def test_modes_with_a_fixed_order_of_sums_over_mixed_batches(monkeypatch):
 
 
 @pytest.mark.parametrize("new,lens", [([1], [40000]), ([300], [9000])])
-def test_calls_on_two_streams_at_once(new, lens):
+def test_calls_on_two_streams_at_once(new, lens, kernel):
     """Sequences in parts that join through memory: every call, and every graph, has its own."""
     sets = [_setup(new, lens, 128, 8, 2, 128, seed) for seed in (16, 17)]
     want = [ops.paged_attention_int4(*s, 0.09) for s in sets]
@@ -327,7 +337,7 @@ def test_calls_on_two_streams_at_once(new, lens):
 
 
 @pytest.mark.parametrize("new", [[1, 1], [100, 60]])
-def test_row_numbers_beyond_the_rows_are_reported(new):
+def test_row_numbers_beyond_the_rows_are_reported(new, kernel):
     q, kc, vc, meta = _setup(new, [200, 300], 32, 8, 2, 128, 18)
     want, tol = _want(q, kc, vc, meta, 0.1)
     meta.query_start_loc[2] += 1
@@ -365,7 +375,7 @@ def test_graph_replay_with_other_lengths_and_another_stream():
 @pytest.mark.parametrize("Hq,Hkv,D,page,window,causal", [
     (8, 2, 128, 128, 0, True), (4, 4, 128, 16, 0, True), (28, 4, 64, 16, 0, True), (16, 1, 128, 48, 0, True), (6, 2, 64, 128, 0, True),
     (8, 1, 128, 64, 100, True), (8, 2, 64, 32, 1, True), (4, 2, 128, 256, 0, False), (5, 1, 128, 32, 300, True), (2, 2, 64, 128, 77, True)])
-def test_prompts(Hq, Hkv, D, page, window, causal):
+def test_prompts(Hq, Hkv, D, page, window, causal, kernel):
     tile = 128 // (Hq // Hkv)
     new = [20, tile - 1, tile, tile + 1, 2 * tile, 2 * tile + 1, 300, 17, 3]
     old = [0, 5, 0, 200, 129, 0, 77, 640, 250]
@@ -377,7 +387,7 @@ def test_prompts(Hq, Hkv, D, page, window, causal):
 
 
 @pytest.mark.parametrize("D,Hq,Hkv", [(128, 8, 2), (64, 16, 4)])
-def test_mixed_batches(D, Hq, Hkv):
+def test_mixed_batches(D, Hq, Hkv, kernel):
     """Decodes in front of prompts, a short sequence behind them, tokens behind the last sequence."""
     new, old = [1, 1, 1, 2, 130, 1, 700, 9], [5, 300, 1000, 64, 0, 90, 333, 2000]
     q, kc, vc, meta = _setup(new, [a + b for a, b in zip(new, old)], 32, Hq, Hkv, D, 21)
@@ -389,12 +399,12 @@ def test_mixed_batches(D, Hq, Hkv):
     assert out[-5:].eq(3).all()
 
 
-def test_a_long_portion_behind_a_long_context():
+def test_a_long_portion_behind_a_long_context(kernel):
     q, kc, vc, meta = _setup([333], [20333], 128, 8, 2, 128, 22)
     _check(ops.paged_attention_int4(q, kc, vc, meta, 0.09), *_want(q, kc, vc, meta, 0.09))
 
 
-def test_prompt_tokens_that_see_no_key():
+def test_prompt_tokens_that_see_no_key(kernel):
     """More new tokens than keys: those in front of the first key get zeros."""
     q, kc, vc, meta = _setup([300, 40, 64], [20, 0, 64], 16, 8, 2, 128, 23)
     out = ops.paged_attention_int4(q, kc, vc, meta, 0.1)
@@ -403,7 +413,7 @@ def test_prompt_tokens_that_see_no_key():
 
 
 @pytest.mark.parametrize("window,D", [(0, 128), (200, 128), (0, 64)])
-def test_nan_values_reach_the_prompt_rows_that_see_them(window, D):
+def test_nan_values_reach_the_prompt_rows_that_see_them(window, D, kernel):
     new, old, page = [260, 70], [500, 3], 32
     q, kc, vc, meta = _setup(new, [a + b for a, b in zip(new, old)], page, 8, 2, D, 24)
     spots = [(0, 10), (0, 300), (0, 500), (0, 640), (0, 758), (1, 2), (1, 60)]
@@ -425,7 +435,7 @@ def test_nan_values_reach_the_prompt_rows_that_see_them(window, D):
     _check(torch.where(hit, 0.0, out), torch.where(hit, 0.0, want), tol)
 
 
-def test_prompt_pages_outside_of_the_cache_are_reported():
+def test_prompt_pages_outside_of_the_cache_are_reported(kernel):
     q, kc, vc, meta = _setup([200, 100], [300, 100], 16, 8, 2, 128, 25)
     good = ops.paged_attention_int4(q, kc, vc, meta, 0.1)
     meta.block_table[0, 7] = -3

@@ -154,10 +154,20 @@ def test_refusals():
 def test_which_sequences_share_a_launch():
     from vllm_ascend_b200.ops.kv_int4 import _plan
     cu = np.cumsum([0, 1, 8, 9, 1, 0, 300, 2]).astype(np.int32).tobytes()
-    assert _plan(cu, 4, False) == ((True, 0, 2, (8,)), (False, 2, 7, (312, 8)))
-    assert _plan(cu, 4, True) == ((True, 0, 2, (8,)), (False, 2, 3, (9, 1)), (True, 3, 5, (1,)), (False, 5, 6, (300, 5)), (True, 6, 7, (2,)))
-    assert _plan(cu, 128, False) == ((False, 0, 7, (321, 162)),)
-    assert _plan(np.array([0, 1, 3], dtype=np.int32).tobytes(), 4, False) == ((True, 0, 2, (2,)),)
+    def plan(cu, lens, G, fixed=False, window=0):
+        return _plan(cu, "i", np.array(lens + [7], dtype=np.int64).tobytes(), "l", len(lens), window, G, 8, 128, 148, fixed)
+    lens = [5000] * 7
+    assert plan(cu, lens, 4) == ((True, 0, 2, (8,)), (False, 2, 7, (312, 8)))
+    assert plan(cu, lens, 4, True) == ((True, 0, 2, (8,)), (False, 2, 3, (9, 1)), (True, 3, 5, (1,)), (False, 5, 6, (300, 5)), (True, 6, 7, (2,)))
+    assert plan(cu, lens, 128) == ((False, 0, 7, (321, 162)),)
+    assert plan(np.array([0, 1, 3], dtype=np.int32).tobytes(), [9, 9], 4) == ((True, 0, 2, (2,)),)
+    # what lies behind the first ones may take less time in that kernel too: all in one launch, unless that leaves most of its blocks idle
+    short = np.array([0, 1, 2, 40], dtype=np.int32).tobytes()
+    assert plan(short, [600, 500, 38], 4) == ((True, 0, 3, (38,)),)
+    assert plan(short, [600, 500, 38], 4, True) == ((True, 0, 2, (1,)), (False, 2, 3, (38, 1)))
+    many = np.concatenate([np.arange(201), [300]]).astype(np.int32).tobytes()
+    assert plan(many, [600] * 200 + [100], 4) == ((True, 0, 200, (1,)), (True, 200, 201, (100,)))
+    assert plan(many, [600] * 200 + [0], 4, window=10)[0] == (True, 0, 200, (1,))
 
 
 def test_nothing_to_do():

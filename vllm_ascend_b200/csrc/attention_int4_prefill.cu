@@ -14,7 +14,7 @@
 // zeros, are noted, and put into the rows that see them at the end.
 // All waits are bounded.
 // Measured, 32 heads on 8 of 128: 8 prompts of 1000 tokens 137 us (bf16 pages: 127), one of 4096 tokens 162 us (149), 0.85 PFLOP/s; 137 tokens
-// 11.3 us.  28 heads on 4 of 64, three portions of 667 tokens behind 9000, window 4096: 143 us, where the exponentials alone take
+// 11.3 us (those go to the kernel for few rows: 7.7).  28 heads on 4 of 64, three portions of 667 tokens behind 9000, window 4096: 143 us, where the exponentials alone take
 // 52 us of the multifunction units.  Scores in halves of 64 keep a row in registers without spills: 128 at once with the registers
 // moved to the softmax warps (setmaxnreg) took 150 us there.  A block that works through several items, to hide the 8 us of a
 // block's start and end, lost more to uneven shares (147 -> 198 us).

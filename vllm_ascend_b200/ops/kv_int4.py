@@ -27,7 +27,7 @@ _native.register_signature("b200_attn_int4_prefill",
                            [_P, _L, _L, _P, _P, _L, _I, _P, _P, _P, _I, _I, _L, _I, _I, _I, _F, _I, _I, _I, _P, _L, _P, _P, _P])
 
 HEAD_SIZES = (64, 128)
-#: rows (new tokens times heads of a group) of a sequence up to which the kernel for few rows takes it
+#: rows (new tokens times heads of a group) of a sequence up to which the kernel for few rows always takes it
 FEW_ROWS = 32
 
 
@@ -187,7 +187,9 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     if max_q * G <= FEW_ROWS or G > 128:
         _few_rows(*args, 0, n, max_q)
     else:
-        for few, first, end, what in _plan(np.ascontiguousarray(meta.query_start_loc_cpu, dtype=np.int32)[:n + 1].tobytes(), G, fixed_sums()):
+        starts, keys = meta.query_start_loc_cpu, meta.seq_lens_cpu
+        for few, first, end, what in _plan(starts.tobytes(), starts.dtype.char, keys.tobytes(), keys.dtype.char, n, window, G, Hkv, D,
+                                           _native.sm_count(device), fixed_sums()):
             if few:
                 _few_rows(*args, first, end, what[0])
             else:
@@ -195,21 +197,56 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     return out if out is given else given.copy_(out)
 
 
+def _few_us(new, keys, G: int, Hkv: int, D: int, sms: int) -> float:
+    """About what a launch of the kernel for few rows takes in us for sequences with so many new tokens and keys: a block of 16 rows (two an
+    SM at once) costs its start and its units of 16 keys, and every sequence has as many blocks as the longest.  Fitted like ``_prompt_us`` to
+    prompts, portions and drafts of 8 to 1000 tokens."""
+    blocks = -(-new * G // 16)
+    units = float((blocks * ((keys - new / 2).clip(0) / 16 + 1)).sum()) * Hkv * (1 if D == 128 else 0.65)
+    idle = (len(new) * int(blocks.max()) - int(blocks.sum())) * Hkv
+    return 4 + (1.75 * int(blocks.sum()) * Hkv + 0.4 * idle + 0.1 * units) / sms
+
+
+def _prompt_us(new, keys, G: int, Hkv: int, D: int, sms: int) -> float:
+    """The same for the kernel for prompts: a pair of query tiles, one an SM, costs its start and its tiles of 128 keys.  32 heads on 8 of 128: 137
+    tokens 7.7 us there, 11.6 here; 300 tokens 16.5 and 14.9; 30 behind 4000 17 and 24; 8 x 100 30 and 14; 40 x 8 behind 2000 80 and 112.
+    64 on 8: 137 tokens 12.3 and 11.8, 40 x 8 behind 2000 126 and 112."""
+    pairs = -(-new // (2 * (128 // G)))
+    blocks = int(pairs.sum()) * Hkv
+    parts = _prompt_parts(blocks, int(keys.max()), sms)
+    tile = 1.9 if D == 128 else 1.5
+    us = 7.5 + tile / parts * ((keys - new / 2).clip(0) / 128 + 0.5) * np.where(new * G > 128, 1.25, 1)
+    return 1 + 5 * (parts > 1) + (float(us.max()) if blocks <= sms else (blocks / sms + 0.5) * float((us * pairs).sum()) * Hkv / blocks)
+
+
 @functools.lru_cache(maxsize=256)
-def _plan(cu: bytes, G: int, fixed: bool) -> tuple:
-    """Launches for sequences that begin at these int32 row numbers: (whether of the kernel for few rows, first sequence, end, and the most new
-    tokens of one, or their rows and pairs of query tiles).  Sequences of few rows in front of the others go to the kernel for them; those
-    behind go with the others, except (``fixed``) where which kernel a sequence gets must not depend on its neighbours."""
-    starts = np.frombuffer(cu, dtype=np.int32)
-    new = np.diff(starts)
-    many = new.astype(np.int64) * G > FEW_ROWS
-    ends = np.flatnonzero(np.diff(many)) + 1 if fixed else np.flatnonzero(many)[:1]
+def _plan(cu: bytes, cu_type: str, lens: bytes, lens_type: str, n: int, window: int, G: int, Hkv: int, D: int, sms: int, fixed: bool) -> tuple:
+    """Launches for ``n`` sequences that begin at these row numbers and have so many keys: (whether of the kernel for few rows, first sequence, end,
+    and the most new tokens of one, or their rows and pairs of query tiles).  Sequences of few rows in front of the others go to the kernel for
+    them; those behind go with the others, to the kernel that takes less time for them, or all go to that for few rows in one launch.  With
+    sums in a fixed order (``fixed``) a sequence's kernel follows from its own rows alone."""
+    new = np.diff(np.frombuffer(cu, dtype=cu_type)[:n + 1].astype(np.int64))
+    many = new * G > FEW_ROWS
+    if fixed:
+        ends = (np.flatnonzero(np.diff(many)) + 1).tolist()
+        runs = [(not many[a], a, b) for a, b in zip([0, *ends], [*ends, len(new)])]
+    else:
+        first = int(many.argmax()) if many.any() else n
+        runs = [(True, 0, first)] if first else []
+        if int(new[first:].sum()) * G * Hkv > 256 * sms:              # 16 blocks of 16 rows an SM: never near
+            runs.append((False, first, n))
+        elif first < n:
+            shape, keys = (G, Hkv, D, sms), np.maximum(np.frombuffer(lens, dtype=lens_type)[:n].astype(np.int64), 0)
+            if window:
+                keys = np.minimum(keys, window + new)
+            few, rest = _few_us(new[first:], keys[first:], *shape), _prompt_us(new[first:], keys[first:], *shape)
+            runs.append((few < rest, first, n))
+            if first and _few_us(new, keys, *shape) < min(few, rest) + _few_us(new[:first], keys[:first], *shape):
+                runs = [(True, 0, n)]
     plan = []
-    for first, end in zip([0, *ends.tolist()], [*ends.tolist(), len(new)]):
-        if first < end:
-            n = new[first:end]
-            few = not (many[first:end].any())
-            plan.append((few, first, end, (int(n.max()),) if few else (int(n.sum()), int((-(-n // (2 * (128 // G)))).sum()))))
+    for few, a, b in runs:
+        x = new[a:b]
+        plan.append((few, a, b, (int(x.max()),) if few else (int(x.sum()), int((-(-x // (2 * (128 // G)))).sum()))))
     return tuple(plan)
 
 
