@@ -13,11 +13,11 @@
 // A value whose scale is no number would reach rows that do not see it (0 x NaN): near a mask's edges such groups enter as
 // zeros, are noted, and put into the rows that see them at the end.
 // All waits are bounded.
-// Measured, 32 heads on 8 of 128: 8 prompts of 1000 tokens 137 us (bf16 pages: 127), one of 4096 tokens 162 us (149), 0.85 PFLOP/s; 137 tokens
-// 11.3 us (those go to the kernel for few rows: 7.7).  28 heads on 4 of 64, three portions of 667 tokens behind 9000, window 4096: 143 us, where the exponentials alone take
-// 52 us of the multifunction units.  Scores in halves of 64 keep a row in registers without spills: 128 at once with the registers
-// moved to the softmax warps (setmaxnreg) took 150 us there.  A block that works through several items, to hide the 8 us of a
-// block's start and end, lost more to uneven shares (147 -> 198 us).
+// Measured, 32 heads on 8 of 128: 8 prompts of 1000 tokens 135 us (bf16 pages: 127), one of 4096 tokens 153 us (149), 0.90 PFLOP/s; 137 tokens
+// 11.3 us (those go to the kernel for few rows: 7.7).  28 heads on 4 of 64, three portions of 667 tokens behind 9000, window 4096: 143 us,
+// where the exponentials alone take 52 us of the multifunction units.  Scores in halves of 64 keep a row in registers without spills: 128
+// at once with the registers moved to the softmax warps (setmaxnreg) took 150 us there.  A block that works through several items (the
+// next one's tiles unpacked while the last one's results are written) gained nothing: 143 us, or 198 with every 148th item fixed.
 #include "attention_int4.cuh"
 
 namespace b200 {
@@ -404,6 +404,8 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
             for (int i = 0; i < 32; i++) r[i] = __float_as_uint(__uint_as_float(r[i]) * a);
             tmem_st_32x32b_x32(t_o + c * 32, r);
           }
+          // the second half once more, rather than in registers across this rare case: 4096 tokens 162 -> 153 us (D = 64: 142 -> 146)
+          if constexpr (D == 128) half(1);
         }
         const float nmb = m == -INFINITY ? 0.f : -m * sl2;
         float rs[4] = {0.f, 0.f, 0.f, 0.f};
