@@ -132,6 +132,9 @@ def read_kv_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tens
 
 #: parts whose blocks form a cluster and join in it
 CLUSTER = 8
+#: us that a pair of query tiles takes to start and end, and a tile of 128 keys of one query tile (two: a quarter more), by head size
+PAIR_US = 7.5
+TILE_US = {128: 1.9, 64: 1.5}
 
 
 def _parts(blocks: int, max_len: int, at_once: int) -> int:
@@ -213,10 +216,10 @@ def _prompt_us(new, keys, G: int, Hkv: int, D: int, sms: int) -> float:
     64 on 8: 137 tokens 12.3 and 11.8, 40 x 8 behind 2000 126 and 112."""
     pairs = -(-new // (2 * (128 // G)))
     blocks = int(pairs.sum()) * Hkv
-    parts = _prompt_parts(blocks, int(keys.max()), sms)
-    tile = 1.9 if D == 128 else 1.5
-    us = 7.5 + tile / parts * ((keys - new / 2).clip(0) / 128 + 0.5) * np.where(new * G > 128, 1.25, 1)
-    return 1 + 5 * (parts > 1) + (float(us.max()) if blocks <= sms else (blocks / sms + 0.5) * float((us * pairs).sum()) * Hkv / blocks)
+    parts = _prompt_parts(blocks, int(keys.max()), int(new.sum()), G * Hkv, D, sms)
+    us = PAIR_US + TILE_US[D] / parts * ((keys - new / 2).clip(0) / 128 + 0.5) * np.where(new * G > 128, 1.25, 1)
+    rounds = blocks * parts / sms
+    return 1 + 5 * (parts > 1) + (float(us.max()) if rounds <= 1 else (rounds + 0.5) * float((us * pairs).sum()) * Hkv / blocks)
 
 
 @functools.lru_cache(maxsize=256)
@@ -282,16 +285,27 @@ def _results(q, parts: int) -> torch.Tensor:
     return torch.empty(T * Hq * parts * (D + 1), dtype=torch.float32, device=q.device)
 
 
-def _prompt_parts(blocks: int, max_len: int, sms: int) -> int:
-    """Parts of a prompt's keys: where its blocks (one per SM) leave half of the GPU idle, and a part keeps 512 keys."""
-    return max(1, min(sms // max(1, blocks), max_len // 512, 16))
+@functools.lru_cache(maxsize=1024)
+def _prompt_parts(blocks: int, max_len: int, tokens: int, heads: int, D: int, sms: int) -> int:
+    """Parts of a prompt's keys, of 512 at least: those that take least time in rounds of one block an SM, each of ``PAIR_US`` and its tiles, with
+    a join that writes and reads the parts' fp32 results.  32 heads on 8 of 128, 1300 tokens behind 8000 (168 blocks): 278 us whole, 252 in three;
+    600 behind 20000 (80 blocks): 339, 253; 64 on 8, 700 behind 20000 (176 blocks): 652, 498 in four; 28 on 4 of 64, 2000 behind 9000 in a window of
+    4096 (232 blocks): 142, 168."""
+    tiles, tile = max_len / 128, 1.25 * TILE_US[D]
+
+    def us(parts):
+        join = 5 + tokens * heads * D * 8 * parts / 4e6
+        whole = -(-blocks * parts // sms) * (PAIR_US + tile * tiles / parts)
+        return 1.08 * whole + join if parts > 1 else whole           # sequences of unequal lengths gain less
+    return min(range(1, max(1, min(max_len // 512, 16)) + 1), key=us)
 
 
 def _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, end, tokens, pairs) -> None:
     """Sequences ``first`` to ``end`` with so many new tokens and pairs of query tiles."""
     T, Hq, D = q.shape
     NB, Hkv, _ = k_cache.shape
-    parts = 1 if fixed_sums() else _prompt_parts(pairs * Hkv, meta.max_seq_len, _native.sm_count(q.get_device()))
+    longest = min(meta.max_seq_len, window + meta.max_query_len) if window else meta.max_seq_len
+    parts = 1 if fixed_sums() else _prompt_parts(pairs * Hkv, longest, tokens, Hq, D, _native.sm_count(q.get_device()))
     scratch = _results(q, parts) if parts > 1 else None
     cu, lens, table = _of(meta, first)
     rc = _native.lib().b200_attn_int4_prefill(
