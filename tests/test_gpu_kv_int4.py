@@ -336,6 +336,25 @@ def test_calls_on_two_streams_at_once(new, lens, kernel):
         _check(x, *_want(*s, 0.09))
 
 
+@pytest.mark.parametrize("D,window", [(64, 0), (128, 0), (64, 5000)])
+def test_many_sequences_of_all_lengths(D, window):
+    """In parts where the host knows the lengths, whole in a graph that is replayed with others."""
+    lens = [6500, 1, 100, 2047, 2048, 4095, 4096, 4097, 6145, 6500, 0] * 3
+    q, kc, vc, meta = _setup([1] * 33, lens, 128, 8, 8, D, 19)
+    out = ops.paged_attention_int4(q, kc, vc, meta, 0.1, window=window)
+    _check(out, *_want(q, kc, vc, meta, 0.1, window))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_attention_int4(q, kc, vc, meta, 0.1, window=window)
+    other = torch.tensor([max(0, n - 3 * i) for i, n in enumerate(lens)], dtype=torch.int32)
+    meta.seq_lens.copy_(other)
+    meta.seq_lens_cpu = other.numpy()
+    graph.replay()
+    torch.cuda.synchronize()
+    _check(out, *_want(q, kc, vc, meta, 0.1, window))
+    _native.check_status(torch.device(DEV))
+
+
 @pytest.mark.parametrize("new", [[1, 1], [100, 60]])
 def test_row_numbers_beyond_the_rows_are_reported(new, kernel):
     q, kc, vc, meta = _setup(new, [200, 300], 32, 8, 2, 128, 18)
