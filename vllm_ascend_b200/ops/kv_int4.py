@@ -137,12 +137,16 @@ PAIR_US = 7.5
 TILE_US = {128: 1.9, 64: 1.5}
 
 
-def _parts(blocks: int, max_len: int, at_once: int) -> int:
-    """Parts that every sequence's keys are split into, by the blocks without a split and those that run at once."""
+def _parts(blocks: int, max_len: int, at_once: int, known: bool) -> int:
+    """Parts that every sequence's keys are split into, by the blocks without a split and those that run at once.  More than a cluster's join in
+    a second kernel, 6 us more, which parts of few long sequences win back: 32 heads on 8, one sequence of 1337 tokens 6.2 us in 8 parts and 12 in
+    18, of 12000 13.4 and 15.9, of 40000 31 and 25.  In a graph ``max_len`` is what the table holds; a quarter of it counts there."""
     if fixed_sums():
         return 1
     most = min(at_once // max(1, blocks), -(-max_len // 128), 18)
-    return max(1, most if most <= CLUSTER or max_len >= 8192 else CLUSTER)
+    if most > CLUSTER and (max_len if known else max_len / 4) * (1 / CLUSTER - 1 / most) < 1300:
+        most = CLUSTER
+    return max(1, most)
 
 
 def _parts_of_rounds(blocks: int, max_len: int, mean: float, at_once: int, D: int) -> int:
@@ -280,7 +284,7 @@ def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, 
     if window:
         longest = min(longest, window + max_q)
     if 2 * blocks <= at_once or longest < 2048 or capturing or fixed_sums():
-        parts = _parts(blocks, longest, at_once)
+        parts = _parts(blocks, longest, at_once, not capturing)
     else:
         parts = _parts_of_rounds(blocks, longest, min(float(meta.seq_lens_cpu[first:end].mean()), longest), at_once, D)
     scratch = _results(q, parts) if parts > CLUSTER else None
