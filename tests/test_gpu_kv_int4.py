@@ -182,6 +182,15 @@ def test_one_long_sequence():
     _check(out, *_want(q, kc, vc, meta, 128 ** -0.5))
 
 
+@pytest.mark.parametrize("lens,Hq,Hkv,D,each", [([9000], 8, 2, 128, 1), ([8001], 4, 1, 64, 1), ([12345, 3], 16, 8, 128, 1), ([9000, 0, 8100], 16, 8, 64, 1),
+                                                ([9001], 16, 2, 128, 2)])
+def test_wide_clusters(lens, Hq, Hkv, D, each):
+    """Few long sequences: 14 or 16 parts, some without keys, joined by eight at a time."""
+    q, kc, vc, meta = _setup([each] * len(lens), lens, 128, Hq, Hkv, D, 30)
+    _check(ops.paged_attention_int4(q, kc, vc, meta, 0.1), *_want(q, kc, vc, meta, 0.1))
+    _native.check_status(torch.device(DEV))
+
+
 def test_growing_and_peaked_scores():
     """Keys whose scores climb along the sequence (every tile moves the maximum), and a score that outweighs all others."""
     D, n = 128, 1500

@@ -172,8 +172,9 @@ def test_which_sequences_share_a_launch():
 
 def test_parts_of_few_rows():
     from vllm_ascend_b200.ops.kv_int4 import _parts, _parts_of_rounds
-    assert [_parts(8, n, 444, True) for n in (0, 100, 1000, 12000, 40000)] == [1, 1, 8, 8, 18]
-    assert [_parts(8, n, 444, False) for n in (40000, 80000)] == [8, 18]          # a graph's table
+    assert [_parts(8, n, 444, True) for n in (0, 100, 1000, 7000, 12000, 40001)] == [1, 1, 8, 8, 16, 18]
+    assert [_parts(8, n, 444, False) for n in (30000, 40001)] == [8, 16]          # a graph's table
+    assert [_parts(b, 20000, 444, True) for b in (24, 25, 32, 44)] == [14, 8, 8, 8]
     assert [_parts(b, 8000, 444, True) for b in (100, 222, 300)] == [4, 2, 1]
     assert [_parts_of_rounds(b, 11000, 8000.0, 444, 128) for b in (240, 2048)] == [4, 1]
     assert all(1 <= _parts_of_rounds(b, n, n / 2, 444, D) <= 8 for b in (223, 444, 10 ** 6) for n in (2048, 10 ** 6) for D in (64, 128))

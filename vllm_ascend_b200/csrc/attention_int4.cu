@@ -12,8 +12,8 @@
 //                   become P^T's fragments by transposing 8 x 8 blocks between the lanes
 // A block is one (sequence, KV head, part of the sequence); each of its warps walks a stretch of it, in tiles of 64 tokens where
 // all rows see them and 16 at a time at the edges, through a ring of its own that bulk copies fill, with a running maximum of
-// its own; they join at the end.  Up to eight parts are a cluster whose blocks join through each other's shared memory; more (few long
-// sequences) join in a second kernel.
+// its own; they join at the end.  Up to sixteen parts are a cluster whose blocks join through each other's shared memory; more (few very
+// long sequences) join in a second kernel.
 // Measured: 256 sequences of 1152 tokens, 32 heads on 8 of 128: 76 us, 4.4 TB/s (the copies alone, nothing unpacked: 6.5; unpacking and
 // products alone: 46 us; twelve warps of an SM overlap the two that far, and 16 with fewer registers no further; the last blocks of
 // unequal sequences take some 10 of the 76); bf16 pages take 187 us.  3 of 60001 tokens, 64 heads: 57 us, 3.6 TB/s, 4 of it the second
@@ -461,25 +461,37 @@ __global__ void __launch_bounds__(32 * D4_WARPS, Int4Cfg<D, NT>::BLOCKS) attn_in
     sg_cluster_sync();
     for (int it = part * 32 * D4_WARPS + threadIdx.x; it < rows * (D / 4); it += p.parts * 32 * D4_WARPS) {
       const int i = it / (D / 4), ch = (it - i * (D / 4)) * 4;
-      float pm[I4_CLUSTER], pl[I4_CLUSTER], top = -INFINITY, sum = 0.f;
-      float4 po[I4_CLUSTER], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      // eight parts at a time, whose loads are under way together
+      float top = -INFINITY, sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int q0 = 0; q0 < p.parts; q0 += 8) {
+        float pm[8], pl[8], now = top;
+        float4 po[8];
 #pragma unroll
-      for (int q = 0; q < I4_CLUSTER; q++) {
-        pm[q] = -INFINITY;
-        pl[q] = 0.f;
-        if (q < p.parts) {
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pm[q]) : "r"(sg_map(smem_u32(block_m + i), q)) : "memory");
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pl[q]) : "r"(sg_map(smem_u32(block_l + i), q)) : "memory");
-          po[q] = sg_ld(sg_map(smem_u32(block_o + i * D + ch), q));
+        for (int k = 0; k < 8; k++) {
+          const int q = q0 + k;
+          pm[k] = -INFINITY;
+          pl[k] = 0.f;
+          if (q < p.parts) {
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pm[k]) : "r"(sg_map(smem_u32(block_m + i), q)) : "memory");
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pl[k]) : "r"(sg_map(smem_u32(block_l + i), q)) : "memory");
+            po[k] = sg_ld(sg_map(smem_u32(block_o + i * D + ch), q));
+          }
+          now = fmaxf(now, pm[k]);
         }
-        top = fmaxf(top, pm[q]);
-      }
+        if (q0 > 0 && top != -INFINITY) {
+          const float f = i4_exp2(top - now);
+          sum *= f;
+          acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+        }
+        top = now;
 #pragma unroll
-      for (int q = 0; q < I4_CLUSTER; q++) {
-        if (q >= p.parts || (pm[q] == -INFINITY && pl[q] == 0.f)) continue;     // saw no key
-        const float f = i4_exp2(pm[q] - top);
-        sum += pl[q] * f;
-        acc.x += po[q].x * f; acc.y += po[q].y * f; acc.z += po[q].z * f; acc.w += po[q].w * f;
+        for (int k = 0; k < 8; k++) {
+          if (q0 + k >= p.parts || (pm[k] == -INFINITY && pl[k] == 0.f)) continue;     // saw no key
+          const float f = i4_exp2(pm[k] - top);
+          sum += pl[k] * f;
+          acc.x += po[k].x * f; acc.y += po[k].y * f; acc.z += po[k].z * f; acc.w += po[k].w * f;
+        }
       }
       const float inv = sum == 0.f ? 0.f : KV4_UNDO / sum;
       const int tok = int4_div(row0 + i, p.G, p.g_inv), g = row0 + i - tok * p.G;
@@ -546,6 +558,10 @@ static int launch_int4(Int4Params p, int max_rows, cudaStream_t stream) {
   using Cfg = Int4Cfg<D, NT>;
   cudaError_t e = allow_smem<attn_int4_kernel<D, NT>>(Cfg::SMEM);
   if (e != cudaSuccess) return (int)e;
+  if (p.cluster && p.parts > 8) {                // more than every GPU of the architecture promises
+    e = cudaFuncSetAttribute(attn_int4_kernel<D, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return (int)e;
+  }
   p.row_blocks = (max_rows + Cfg::ROWS - 1) / Cfg::ROWS;
   const long x = (long)p.num_seqs * p.row_blocks;
   if (x > 0x7fffffffl || p.Hkv > 65535) return 9886;

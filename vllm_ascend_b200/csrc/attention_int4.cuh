@@ -4,7 +4,7 @@
 
 namespace b200 {
 
-constexpr int I4_CLUSTER = 8;      // blocks of a cluster at most
+constexpr int I4_CLUSTER = 16;     // blocks of a cluster at most
 constexpr int I4_PARTS = 64;       // parts at most
 
 struct Int4Params {

@@ -131,22 +131,26 @@ def read_kv_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tens
 
 
 #: parts whose blocks form a cluster and join in it
-CLUSTER = 8
+CLUSTER = 16
 #: us that a pair of query tiles takes to start and end, and a tile of 128 keys of one query tile (two: a quarter more), by head size
 PAIR_US = 7.5
 TILE_US = {128: 1.9, 64: 1.5}
 
 
 def _parts(blocks: int, max_len: int, at_once: int, known: bool) -> int:
-    """Parts that every sequence's keys are split into, by the blocks without a split and those that run at once.  More than a cluster's join in
-    a second kernel, 6 us more, which parts of few long sequences win back: 32 heads on 8, one sequence of 1337 tokens 6.2 us in 8 parts and 12 in
-    18, of 12000 13.4 and 15.9, of 40000 31 and 25.  In a graph ``max_len`` is what the table holds; a quarter of it counts there."""
+    """Parts that every sequence's keys are split into, by the blocks without a split and those that run at once.  Clusters of more than eight
+    find room where there are few, and pay for long sequences; more parts than a cluster's join in a second kernel, 6 us more.  32 heads on 8,
+    one sequence of 1337 tokens 6.2 us in 8 parts, 7.2 in 16, 12 in 18; of 12000 13.4, 11.8, 15.9; of 40000 31, 25, 24; four of 8000 15 in 8,
+    19.5 in 12.  64 on 8, three of 60000 76 in 8, 61 in 14, 58 in 18.  In a graph (lengths not ``known``) ``max_len`` is what the table holds;
+    a quarter of it counts."""
     if fixed_sums():
         return 1
-    most = min(at_once // max(1, blocks), -(-max_len // 128), 18)
-    if most > CLUSTER and (max_len if known else max_len / 4) * (1 / CLUSTER - 1 / most) < 1300:
-        most = CLUSTER
-    return max(1, most)
+    most, wide = min(at_once // max(1, blocks), -(-max_len // 128), 18), 16 if blocks <= 8 else 14
+    if most > CLUSTER and known and max_len > 40000:
+        return most
+    if most >= wide and blocks * 18 <= at_once and (max_len if known else max_len / 4) >= 8000:
+        return wide
+    return max(1, min(most, 8))
 
 
 def _parts_of_rounds(blocks: int, max_len: int, mean: float, at_once: int, D: int) -> int:
@@ -160,7 +164,7 @@ def _parts_of_rounds(blocks: int, max_len: int, mean: float, at_once: int, D: in
         if rounds <= 1:
             return 5 + max(0.72, 0.5 + 0.5 * rounds) * token * max_len / parts + 3 * (parts > 1)
         return (rounds + 0.5) * (5 + token * mean / parts) + 3 * (parts > 1)
-    return min(range(1, CLUSTER + 1), key=us)
+    return min(range(1, 9), key=us)
 
 
 def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta, scale: float,
