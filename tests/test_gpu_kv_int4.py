@@ -315,6 +315,27 @@ def test_modes_with_a_fixed_order_of_sums_over_mixed_batches(monkeypatch):
         assert torch.equal(ops.paged_attention_int4(q[cu[b]:cu[b + 1]], kc, vc, one, 0.1), out[cu[b]:cu[b + 1]])
 
 
+def test_sequences_without_new_tokens_in_front(kernel):
+    q, kc, vc, meta = _setup([0, 0, 200, 0], [60000, 5, 300, 9], 128, 8, 2, 128, 34)
+    _check(ops.paged_attention_int4(q, kc, vc, meta, 0.1), *_want(q, kc, vc, meta, 0.1))
+
+
+@pytest.mark.parametrize("most", [None, 1 << 20])
+@pytest.mark.parametrize("new,lens", [([1, 90, 3], [41000, 9000, 8]), ([300], [9000])])
+def test_memory_of_parts(new, lens, most, kernel, monkeypatch):
+    """Only of the rows that have parts, and no more than there may be."""
+    from vllm_ascend_b200.ops import kv_int4
+    if most:
+        monkeypatch.setattr(kv_int4, "MOST_BYTES", most)
+    asked, empty = [], torch.empty
+    q, kc, vc, meta = _setup(new, lens, 128, 8, 2, 128, 33)
+    monkeypatch.setattr(kv_int4.torch, "empty", lambda *a, **kw: asked.append(a[0]) or empty(*a, **kw))
+    out = ops.paged_attention_int4(q, kc, vc, meta, 0.1)
+    monkeypatch.undo()
+    assert all(4 * n <= (most or 256 << 20) for n in asked) and (most or asked or kernel == "few rows")
+    _check(out, *_want(q, kc, vc, meta, 0.1))
+
+
 @pytest.mark.parametrize("new,lens", [([1], [40000]), ([300], [9000])])
 def test_calls_on_two_streams_at_once(new, lens, kernel):
     """Sequences in parts that join through memory: every call, and every graph, has its own."""

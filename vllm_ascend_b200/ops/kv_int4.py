@@ -291,10 +291,13 @@ def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, 
         parts = _parts(blocks, longest, at_once, not capturing)
     else:
         parts = _parts_of_rounds(blocks, longest, min(float(meta.seq_lens_cpu[first:end].mean()), longest), at_once, D)
-    scratch = _results(q, parts) if parts > CLUSTER else None
+    ahead = T if end == meta.num_reqs else int(meta.query_start_loc_cpu[end])       # rows of these sequences and those in front of them
+    if parts > CLUSTER and parts > _most_parts(ahead, Hq, D):
+        parts = 8
+    scratch = _results(q, ahead, parts) if parts > CLUSTER else None
     cu, lens, table = _of(meta, first)
     rc = _native.lib().b200_attn_int4(
-        q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, cu.data_ptr(), lens.data_ptr(),
+        q.data_ptr(), q.stride(0), ahead, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, cu.data_ptr(), lens.data_ptr(),
         table.data_ptr(), table.stride(0), n, max_q, Hq, Hkv, D, scale, int(causal), int(window), parts,
         out.data_ptr(), out.stride(0), _native.ptr(scratch), _native.status_word(q.device).data_ptr(), _native.stream_ptr())
     _native.check(rc, "attn_int4")
@@ -307,10 +310,18 @@ def _of(meta, first: int):
     return (cu[first:], lens[first:], table[first:]) if first else (cu, lens, table)
 
 
-def _results(q, parts: int) -> torch.Tensor:
+#: bytes of the parts' results of a call at most
+MOST_BYTES = 256 << 20
+
+
+def _most_parts(rows: int, heads: int, D: int) -> int:
+    return MOST_BYTES // (max(rows, 1) * heads * (D + 1) * 4)
+
+
+def _results(q, rows: int, parts: int) -> torch.Tensor:
     """Memory for the results of parts.  Each call has its own: calls on two streams, or two graphs, may run at once."""
-    T, Hq, D = q.shape
-    return torch.empty(T * Hq * parts * (D + 1), dtype=torch.float32, device=q.device)
+    _, Hq, D = q.shape
+    return torch.empty(rows * Hq * parts * (D + 1), dtype=torch.float32, device=q.device)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -334,7 +345,9 @@ def _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, e
     NB, Hkv, _ = k_cache.shape
     longest = min(meta.max_seq_len, window + meta.max_query_len) if window else meta.max_seq_len
     parts = 1 if fixed_sums() else _prompt_parts(pairs * Hkv, longest, tokens, Hq, D, _native.sm_count(q.get_device()))
-    scratch = _results(q, parts) if parts > 1 else None
+    if parts > 1 and parts > _most_parts(T, Hq, D):
+        parts = 1
+    scratch = _results(q, T, parts) if parts > 1 else None
     cu, lens, table = _of(meta, first)
     rc = _native.lib().b200_attn_int4_prefill(
         q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, cu.data_ptr(), lens.data_ptr(), table.data_ptr(),
