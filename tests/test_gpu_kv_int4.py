@@ -83,7 +83,8 @@ def _check(got, want, tol):
 
 
 # ---------------------------------------------------------------- rows in and out
-@pytest.mark.parametrize("D,page,H,T", [(128, 128, 8, 1), (128, 128, 8, 700), (64, 16, 1, 333), (64, 48, 3, 17), (128, 256, 5, 129)])
+@pytest.mark.parametrize("D,page,H,T", [(128, 128, 8, 1), (128, 128, 8, 700), (64, 16, 1, 333), (64, 48, 3, 17), (128, 256, 5, 129), (128, 16, 40, 37),
+                                        (64, 16, 33, 1000), (128, 128, 2, 9000)])
 def test_bytes_of_stored_rows(D, page, H, T):
     g = torch.Generator().manual_seed(D + T)
     blocks = T // page + 3
