@@ -580,33 +580,31 @@ static int launch_int4(Int4Params p, int max_rows, cudaStream_t stream) {
   return e != cudaSuccess ? (int)e : B200_CHECK_LAUNCH();
 }
 
-int int4_params(Int4Params* p, const void* q, long q_stride, long q_rows, const void* k_cache, const void* v_cache, long num_blocks, int block_size,
-                const void* cu, const void* seq_lens, const void* block_table, int max_blocks, int num_seqs, int Hq, int Hkv, int D,
-                float scale, int causal, int window, int parts, void* out, long out_stride, void* scratch, int* status) {
-  const int G = Hkv > 0 ? Hq / Hkv : 0;
-  if (G < 1 || G * Hkv != Hq || (D != 64 && D != 128)) return 9883;
-  if (block_size < KV4_TOKENS || block_size % KV4_TOKENS) return 9884;
-  if ((q_stride & 7) || (out_stride & 7) || parts < 1 || parts > I4_PARTS) return 9885;
+int int4_params(Int4Params* p, const Int4Args& a) {
+  const int G = a.Hkv > 0 ? a.Hq / a.Hkv : 0;
+  if (G < 1 || G * a.Hkv != a.Hq || (a.D != 64 && a.D != 128)) return 9883;
+  if (a.block_size < KV4_TOKENS || a.block_size % KV4_TOKENS) return 9884;
+  if ((a.q_stride & 7) || (a.out_stride & 7) || a.parts < 1 || a.parts > I4_PARTS) return 9885;
   *p = Int4Params{};
-  p->q = (const __nv_bfloat16*)q;
-  p->k_cache = (const uint8_t*)k_cache;
-  p->v_cache = (const uint8_t*)v_cache;
-  p->cu = (const int*)cu;
-  p->seq_lens = (const int*)seq_lens;
-  p->block_table = (const int*)block_table;
-  p->out = (__nv_bfloat16*)out;
-  p->part_o = (float*)scratch;
-  p->part_lse = p->part_o + q_rows * Hq * parts * D;
-  p->q_stride = q_stride; p->out_stride = out_stride; p->num_blocks = num_blocks;
-  p->q_rows = q_rows;
-  p->num_seqs = num_seqs; p->max_blocks = max_blocks; p->block_size = block_size;
-  p->G = G; p->Hkv = Hkv; p->parts = parts; p->causal = causal; p->window = window;
-  const int upp = block_size / KV4_TOKENS;
-  if ((long)max_blocks * upp * upp > 0xffffffffl || (long)max_blocks * upp > 0xffffffffl / 65536) return 9888;      // 1M tokens a sequence and more
+  p->q = (const __nv_bfloat16*)a.q;
+  p->k_cache = (const uint8_t*)a.k_cache;
+  p->v_cache = (const uint8_t*)a.v_cache;
+  p->cu = a.cu;
+  p->seq_lens = a.seq_lens;
+  p->block_table = a.block_table;
+  p->out = (__nv_bfloat16*)a.out;
+  p->part_o = (float*)a.scratch;
+  p->part_lse = p->part_o + a.q_rows * a.Hq * a.parts * a.D;
+  p->q_stride = a.q_stride; p->out_stride = a.out_stride; p->num_blocks = a.num_blocks;
+  p->q_rows = a.q_rows;
+  p->num_seqs = a.num_seqs; p->max_blocks = a.max_blocks; p->block_size = a.block_size;
+  p->G = G; p->Hkv = a.Hkv; p->parts = a.parts; p->causal = a.causal; p->window = a.window;
+  const int upp = a.block_size / KV4_TOKENS;
+  if ((long)a.max_blocks * upp * upp > 0xffffffffl || (long)a.max_blocks * upp > 0xffffffffl / 65536) return 9888;      // 1M tokens a sequence and more
   p->g_inv = (uint32_t)((0x100000000ll + G - 1) / G);
   p->upp_inv = (uint32_t)((0x100000000ll + upp - 1) / upp);
-  p->scale_log2 = scale * 1.4426950408889634f * KV4_UNDO;
-  p->status = status;
+  p->scale_log2 = a.scale * 1.4426950408889634f * KV4_UNDO;
+  p->status = a.status;
   return 0;
 }
 
@@ -626,20 +624,16 @@ using namespace b200;
 
 // q [*, Hq, D] and out rows with token strides; cu [num_seqs + 1] their row numbers; max_q_len: no sequence has more new tokens.
 // parts > 1: joined in a cluster (up to I4_CLUSTER), or, where scratch of (rows of q) x Hq x parts x (D + 1) floats is given, there.
-B200_API int b200_attn_int4(const void* q, long q_stride, long q_rows, const void* k_cache, const void* v_cache, long num_blocks,
-                            int block_size, const void* cu, const void* seq_lens, const void* block_table, int max_blocks, int num_seqs,
-                            int max_q_len, int Hq, int Hkv, int D, float scale, int causal, int window, int parts, void* out,
-                            long out_stride, void* scratch, int* status, cudaStream_t stream) {
-  if (num_seqs <= 0 || q_rows <= 0 || max_q_len <= 0) return 0;
+B200_API int b200_attn_int4(const Int4Args* a) {
+  if (a->num_seqs <= 0 || a->q_rows <= 0 || a->max_q_len <= 0) return 0;
   Int4Params p;
-  int rc = int4_params(&p, q, q_stride, q_rows, k_cache, v_cache, num_blocks, block_size, cu, seq_lens, block_table, max_blocks, num_seqs,
-                       Hq, Hkv, D, scale, causal, window, parts, out, out_stride, scratch, status);
+  int rc = int4_params(&p, *a);
   if (rc) return rc;
-  const long rows = (long)max_q_len * p.G;
+  const long rows = (long)a->max_q_len * p.G;
   if (rows * p.G > 0x7fffffffl) return 9886;
-  p.cluster = parts > 1 && !scratch;
-  if (p.cluster && parts > I4_CLUSTER) return 9885;
-  if (D == 128) rc = rows <= 8 ? launch_int4<128, 1>(p, (int)rows, stream) : launch_int4<128, 2>(p, (int)rows, stream);
-  else rc = rows <= 8 ? launch_int4<64, 1>(p, (int)rows, stream) : launch_int4<64, 2>(p, (int)rows, stream);
-  return rc || parts == 1 || p.cluster ? rc : int4_join(p, D, q_rows, stream);
+  p.cluster = p.parts > 1 && !a->scratch;
+  if (p.cluster && p.parts > I4_CLUSTER) return 9885;
+  if (a->D == 128) rc = rows <= 8 ? launch_int4<128, 1>(p, (int)rows, a->stream) : launch_int4<128, 2>(p, (int)rows, a->stream);
+  else rc = rows <= 8 ? launch_int4<64, 1>(p, (int)rows, a->stream) : launch_int4<64, 2>(p, (int)rows, a->stream);
+  return rc || p.parts == 1 || p.cluster ? rc : int4_join(p, a->D, a->q_rows, a->stream);
 }

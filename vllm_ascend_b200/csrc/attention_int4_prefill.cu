@@ -517,17 +517,13 @@ static int launch_int4_prefill(const Int4Params& p, long tokens, cudaStream_t st
 using namespace b200;
 
 // The same for prompts: tokens bounds cu[num_seqs] - cu[0]; groups of up to 128 heads.
-B200_API int b200_attn_int4_prefill(const void* q, long q_stride, long q_rows, const void* k_cache, const void* v_cache, long num_blocks,
-                                    int block_size, const void* cu, const void* seq_lens, const void* block_table, int max_blocks,
-                                    int num_seqs, long tokens, int Hq, int Hkv, int D, float scale, int causal, int window, int parts,
-                                    void* out, long out_stride, void* scratch, int* status, cudaStream_t stream) {
-  if (num_seqs <= 0 || q_rows <= 0 || tokens <= 0) return 0;
+B200_API int b200_attn_int4_prefill(const Int4Args* a) {
+  if (a->num_seqs <= 0 || a->q_rows <= 0 || a->tokens <= 0) return 0;
   Int4Params p;
-  int rc = int4_params(&p, q, q_stride, q_rows, k_cache, v_cache, num_blocks, block_size, cu, seq_lens, block_table, max_blocks, num_seqs,
-                       Hq, Hkv, D, scale, causal, window, parts, out, out_stride, scratch, status);
+  int rc = int4_params(&p, *a);
   if (rc) return rc;
   if (p.G > 128) return 9883;
-  if (parts > 1 && !scratch) return 9885;
-  rc = D == 128 ? launch_int4_prefill<128>(p, tokens, stream) : launch_int4_prefill<64>(p, tokens, stream);
-  return rc || parts == 1 ? rc : int4_join(p, D, q_rows, stream);
+  if (p.parts > 1 && !a->scratch) return 9885;
+  rc = a->D == 128 ? launch_int4_prefill<128>(p, a->tokens, a->stream) : launch_int4_prefill<64>(p, a->tokens, a->stream);
+  return rc || p.parts == 1 ? rc : int4_join(p, a->D, a->q_rows, a->stream);
 }

@@ -219,19 +219,24 @@ static int kv4_rows(bool write, Kv4Rows p, cudaStream_t stream) {
 
 using namespace b200;
 
-// rows of k and v [rows, heads, D] (bf16, row strides given) into the slots of a 4-bit cache; slots below zero are skipped
-B200_API int b200_kv_int4_write(const void* k, long k_stride, const void* v, long v_stride, long rows, const void* slots, void* k_cache,
-                                void* v_cache, long num_slots, int heads, int D, int block_size, int* status, cudaStream_t stream) {
-  Kv4Rows p = {const_cast<void*>(k), const_cast<void*>(v), (uint8_t*)k_cache, (uint8_t*)v_cache, (const long long*)slots, k_stride, v_stride,
-               rows, num_slots, heads, D, block_size, 0, status};
-  return kv4_rows(true, p, stream);
+// by address, like attention's
+struct Kv4Args {
+  void *k, *v;
+  const long long* slots;
+  void *k_cache, *v_cache;
+  int* status;
+  cudaStream_t stream;
+  long k_stride, v_stride, rows, num_slots;
+  int heads, D, block_size;
+};
+static_assert(sizeof(Kv4Args) == 104, "pointers, longs and ints without gaps, as they are packed");
+static Kv4Rows kv4_args(const Kv4Args& a) {
+  return Kv4Rows{a.k, a.v, (uint8_t*)a.k_cache, (uint8_t*)a.v_cache, a.slots, a.k_stride, a.v_stride, a.rows, a.num_slots,
+                 a.heads, a.D, a.block_size, 0, a.status};
 }
 
+// rows of k and v [rows, heads, D] (bf16, row strides given) into the slots of a 4-bit cache; slots below zero are skipped
+B200_API int b200_kv_int4_write(const Kv4Args* a) { return kv4_rows(true, kv4_args(*a), a->stream); }
+
 // the rows of slots as dense bf16 [rows, heads, D]; slots below zero read as zeros
-B200_API int b200_kv_int4_read(void* k, void* v, long rows, const void* slots, const void* k_cache, const void* v_cache, long num_slots,
-                               int heads, int D, int block_size, int* status, cudaStream_t stream) {
-  const long stride = (long)heads * D;
-  Kv4Rows p = {k, v, (uint8_t*)const_cast<void*>(k_cache), (uint8_t*)const_cast<void*>(v_cache), (const long long*)slots, stride, stride,
-               rows, num_slots, heads, D, block_size, 0, status};
-  return kv4_rows(false, p, stream);
-}
+B200_API int b200_kv_int4_read(const Kv4Args* a) { return kv4_rows(false, kv4_args(*a), a->stream); }

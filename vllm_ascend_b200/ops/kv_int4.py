@@ -8,7 +8,8 @@ The reference quantises its cache to 8 bits with static scales (vllm_ascend/quan
 from __future__ import annotations
 
 import functools
-from ctypes import c_float, c_int, c_long, c_void_p
+import struct
+from ctypes import c_char_p
 from typing import Optional
 
 import numpy as np
@@ -18,13 +19,11 @@ from .. import _native
 from ..batch_invariant import fixed_sums
 from . import reference as ref
 
-_P, _I, _L, _F = c_void_p, c_int, c_long, c_float
-_native.register_signature("b200_kv_int4_write", [_P, _L, _P, _L, _L, _P, _P, _P, _L, _I, _I, _I, _P, _P])
-_native.register_signature("b200_kv_int4_read", [_P, _P, _L, _P, _P, _P, _L, _I, _I, _I, _P, _P])
-_native.register_signature("b200_attn_int4", [_P, _L, _L, _P, _P, _L, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P, _L, _P, _P, _P])
-
-_native.register_signature("b200_attn_int4_prefill",
-                           [_P, _L, _L, _P, _P, _L, _I, _P, _P, _P, _I, _I, _L, _I, _I, _I, _F, _I, _I, _I, _P, _L, _P, _P, _P])
+# arguments go by address, laid out as the sources' Kv4Args and Int4Args: packing them takes 0.3 us where ctypes takes 0.1 us for each
+_ROWS = struct.Struct("@7P4q3i")
+_ATTENTION = struct.Struct("@10P5qf10i")
+for _name in ("b200_kv_int4_write", "b200_kv_int4_read", "b200_attn_int4", "b200_attn_int4_prefill"):
+    _native.register_signature(_name, [c_char_p])
 
 HEAD_SIZES = (64, 128)
 #: rows (new tokens times heads of a group) of a sequence up to which the kernel for few rows always takes it
@@ -99,9 +98,9 @@ def write_kv_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     if device < 0 or k.dtype is not torch.bfloat16:
         return ref.write_kv_int4(k, v, k_cache, v_cache, slots)
     k, v = _dense_heads(k), _dense_heads(v)
-    rc = _native.lib().b200_kv_int4_write(
-        k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), T, slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        k_cache.shape[0] * bs, H, D, bs, _native.status_word(k.device).data_ptr(), _native.stream_ptr())
+    rc = _native.lib().b200_kv_int4_write(_ROWS.pack(
+        k.data_ptr(), v.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _native.status_word(k.device).data_ptr(),
+        _native.stream_ptr(), k.stride(0), v.stride(0), T, k_cache.shape[0] * bs, H, D, bs))
     _native.check(rc, "kv_int4_write")
     _native.count_launch()
 
@@ -119,12 +118,12 @@ def read_kv_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tens
     if device < 0:
         return ref.read_kv_int4(k_cache, v_cache, slots, dim)
     k = k_cache.new_empty((n, H, dim), dtype=torch.bfloat16)
-    v = k_cache.new_empty((n, H, dim), dtype=torch.bfloat16)
+    v = torch.empty_like(k)
     if n == 0:
         return k, v
-    rc = _native.lib().b200_kv_int4_read(
-        k.data_ptr(), v.data_ptr(), n, slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0] * bs, H, dim, bs,
-        _native.status_word(k.device).data_ptr(), _native.stream_ptr())
+    rc = _native.lib().b200_kv_int4_read(_ROWS.pack(
+        k.data_ptr(), v.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _native.status_word(k.device).data_ptr(),
+        _native.stream_ptr(), H * dim, H * dim, n, k_cache.shape[0] * bs, H, dim, bs))
     _native.check(rc, "kv_int4_read")
     _native.count_launch()
     return k, v
@@ -296,10 +295,10 @@ def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, 
         parts = 8
     scratch = _results(q, ahead, parts) if parts > CLUSTER else None
     cu, lens, table = _of(meta, first)
-    rc = _native.lib().b200_attn_int4(
-        q.data_ptr(), q.stride(0), ahead, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, cu.data_ptr(), lens.data_ptr(),
-        table.data_ptr(), table.stride(0), n, max_q, Hq, Hkv, D, scale, int(causal), int(window), parts,
-        out.data_ptr(), out.stride(0), _native.ptr(scratch), _native.status_word(q.device).data_ptr(), _native.stream_ptr())
+    rc = _native.lib().b200_attn_int4(_ATTENTION.pack(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cu.data_ptr(), lens.data_ptr(), table.data_ptr(), out.data_ptr(),
+        0 if scratch is None else scratch.data_ptr(), _native.status_word(q.device).data_ptr(), _native.stream_ptr(), q.stride(0), ahead, NB,
+        out.stride(0), 0, scale, bs, table.stride(0), n, max_q, Hq, Hkv, D, int(causal), window, parts))
     _native.check(rc, "attn_int4")
     _native.count_launch(1 + int(parts > CLUSTER))
 
@@ -349,9 +348,9 @@ def _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, e
         parts = 1
     scratch = _results(q, T, parts) if parts > 1 else None
     cu, lens, table = _of(meta, first)
-    rc = _native.lib().b200_attn_int4_prefill(
-        q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, cu.data_ptr(), lens.data_ptr(), table.data_ptr(),
-        table.stride(0), end - first, tokens, Hq, Hkv, D, scale, int(causal), int(window), parts, out.data_ptr(), out.stride(0),
-        _native.ptr(scratch), _native.status_word(q.device).data_ptr(), _native.stream_ptr())
+    rc = _native.lib().b200_attn_int4_prefill(_ATTENTION.pack(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cu.data_ptr(), lens.data_ptr(), table.data_ptr(), out.data_ptr(),
+        0 if scratch is None else scratch.data_ptr(), _native.status_word(q.device).data_ptr(), _native.stream_ptr(), q.stride(0), T, NB,
+        out.stride(0), tokens, scale, bs, table.stride(0), end - first, 0, Hq, Hkv, D, int(causal), window, parts))
     _native.check(rc, "attn_int4_prefill")
     _native.count_launch(1 + int(parts > 1))
