@@ -70,6 +70,7 @@ __global__ void __launch_bounds__(32 * D4_WARPS, Int4Cfg<D, NT>::BLOCKS) attn_in
   float* block_m = ls + D4_WARPS * ROWS;                                           // [rows] of the block, sums behind
   float* block_l = block_m + ROWS;
   volatile int* abort_word = (volatile int*)(block_l + ROWS);
+  volatile int* bad_page = abort_word + 1;       // apart from the word that ends waits: every warp still sees its own copies land
 
   const int seq = p.row_blocks == 1 ? blockIdx.x : blockIdx.x / p.row_blocks, row0 = (blockIdx.x - seq * p.row_blocks) * ROWS;
   const int h = blockIdx.y, part = blockIdx.z;
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(32 * D4_WARPS, Int4Cfg<D, NT>::BLOCKS) attn_in
   }
   if (lane == 0)
     for (int s = 0; s < Cfg::STAGES; s++) mbar_init(&bars[s], 1);
-  if (threadIdx.x == 0) *abort_word = 0;
+  if (threadIdx.x == 0) *abort_word = *bad_page = 0;
   mbar_fence_init();
   __syncthreads();
 
@@ -348,9 +349,11 @@ __global__ void __launch_bounds__(32 * D4_WARPS, Int4Cfg<D, NT>::BLOCKS) attn_in
 
   int stage = 0;
   uint32_t phase = 0;
+  bool late = false;
   for (int u0 = first; u0 < last; u0 += U) {
     if (bad && u0 >= next) break;                // tiles from a bad page on were not fetched
-    if (!__all_sync(0xffffffffu, mbar_wait(&bars[stage], phase, abort_word))) break;
+    late = !__all_sync(0xffffffffu, mbar_wait(&bars[stage], phase, abort_word));
+    if (late) break;
     const uint8_t* ks = ring + stage * Cfg::STAGE;
     const uint8_t* vs = ks + U * Cfg::UNIT;
     const int n = min(U, last - u0);
@@ -376,6 +379,10 @@ __global__ void __launch_bounds__(32 * D4_WARPS, Int4Cfg<D, NT>::BLOCKS) attn_in
     }
   }
 
+  if (late) {                                    // copies still in flight land before the ring gets results, or is released
+    const uint64_t t_start = globaltimer_ns();
+    while (globaltimer_ns() - t_start < 50000ull) __nanosleep(1000);
+  }
   // ---------------- join the warps: results into the rings' place
 #pragma unroll
   for (int nt = 0; nt < NT; nt++)
@@ -390,7 +397,7 @@ __global__ void __launch_bounds__(32 * D4_WARPS, Int4Cfg<D, NT>::BLOCKS) attn_in
         ls[warp * ROWS + nt * 8 + 2 * c + e] = x;
       }
     }
-  if (bad && lane == 0) *abort_word = B200_BAD_INDEX;
+  if (bad && lane == 0) *bad_page = 1;
   float* res = (float*)ring;                     // [rows][D]
 #pragma unroll
   for (int nt = 0; nt < NT; nt++)
@@ -405,14 +412,7 @@ __global__ void __launch_bounds__(32 * D4_WARPS, Int4Cfg<D, NT>::BLOCKS) attn_in
       }
     }
   __syncthreads();
-  if (*abort_word != 0) {
-    if (*abort_word == B200_TIMEOUT) {           // copies still in flight land before the block's shared memory is released
-      const uint64_t t_start = globaltimer_ns();
-      while (globaltimer_ns() - t_start < 50000ull) __nanosleep(1000);
-    }
-    if (threadIdx.x == 0 && p.status) atomicExch(p.status, *abort_word);
-    __syncthreads();
-  }
+  if (threadIdx.x == 0 && p.status && (*abort_word != 0 || *bad_page != 0)) atomicExch(p.status, *bad_page ? B200_BAD_INDEX : *abort_word);
   float* block_o = (float*)i4_smem + ROWS * D;
   for (int it = threadIdx.x; it < rows * (D / 8); it += 32 * D4_WARPS) {
     const int i = it / (D / 8), ch = (it - i * (D / 8)) * 8;
