@@ -1,0 +1,25 @@
+"""Calls of the 4-bit cache's operators that its other tests on the host do not make."""
+import pytest
+import torch
+
+from test_kv_int4_cpu import _meta
+from vllm_ascend_b200 import ops
+
+
+def test_caches_begin_on_16_bytes():
+    """The kernels' bulk copies and wide stores need it, wherever the cache was cut from."""
+    size = 2 * 2 * 16 * 64 * 9 // 16
+    pool = torch.zeros(size + 64, dtype=torch.uint8)
+    pool = pool[-pool.data_ptr() % 16:]
+    whole, rows, slots = pool[:size].view(2, 2, -1), torch.zeros(1, 2, 64), torch.zeros(1, dtype=torch.int64)
+    meta = _meta([1], [1], torch.zeros(1, 1, dtype=torch.int32), 4, 2, 64)
+    ops.write_kv_int4(rows, rows, whole, whole.clone(), slots)
+    for at in (1, 2, 4, 8):
+        odd = pool[at:at + size].view(2, 2, -1)
+        for pair in ((odd, whole), (whole, odd)):
+            with pytest.raises(ValueError, match="16 bytes"):
+                ops.write_kv_int4(rows, rows, *pair, slots)
+            with pytest.raises(ValueError, match="16 bytes"):
+                ops.read_kv_int4(*pair, slots, 64)
+            with pytest.raises(ValueError, match="16 bytes"):
+                ops.paged_attention_int4(torch.zeros(1, 4, 64), *pair, meta, 0.125)

@@ -3,7 +3,8 @@
 Groups of 32 adjacent channels of a token and head share a scale of five significant bits; a channel is a whole number in
 -7..7 times it, exact in bf16 (``reference.kv_int4_quantise``).  4.5 bits a channel: a GPU holds 3.5 times the tokens of a bf16
 cache, and decode reads 3.5 times fewer bytes.  A cache is one dense uint8 tensor [blocks, heads, bytes of
-a block] for the keys and one for the values (layout: csrc/kv_int4.cuh); head sizes 64 and 128, blocks of a multiple of 16 tokens.
+a block] for the keys and one for the values, each at an address that 16 divides (layout: csrc/kv_int4.cuh); head sizes 64 and 128, blocks of a
+multiple of 16 tokens.
 The reference quantises its cache to 8 bits with static scales (vllm_ascend/quantization/methods/kv_c8.py)."""
 from __future__ import annotations
 
@@ -46,18 +47,20 @@ def alloc_kv_cache_int4(num_blocks: int, block_size: int, heads: int, dim: int, 
 
 
 def _check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dim: int, device: int) -> int:
-    """Block size of a pair of caches that belong together, on the device of that index (-1: the host)."""
+    """Block size of a pair of caches that belong together, on the device of that index (-1: the host), where bulk copies can read them."""
     shape = k_cache.shape
     if dim in HEAD_SIZES and len(shape) == 3 and shape[2] and shape[2] % (9 * dim) == 0 and v_cache.shape == shape \
             and k_cache.dtype is v_cache.dtype is torch.uint8 and k_cache.is_contiguous() and v_cache.is_contiguous() \
-            and k_cache.get_device() == v_cache.get_device() == device:
+            and k_cache.get_device() == v_cache.get_device() == device and (k_cache.data_ptr() | v_cache.data_ptr()) & 15 == 0:
         return shape[2] // (9 * dim) * ref.KV_INT4_TOKENS
     if dim not in HEAD_SIZES:
         raise ValueError(f"a 4-bit cache takes heads of {HEAD_SIZES}, not {dim}")
     bs = ref.kv_int4_block_size(k_cache, dim)
     if v_cache.shape != shape or ref.kv_int4_block_size(v_cache, dim) != bs:
         raise ValueError(f"keys {tuple(shape)} and values {tuple(v_cache.shape)} are caches of different sizes")
-    raise ValueError(f"caches on {k_cache.device} and {v_cache.device}, rows on device {device}")
+    if not k_cache.get_device() == v_cache.get_device() == device:
+        raise ValueError(f"caches on {k_cache.device} and {v_cache.device}, rows on device {device}")
+    raise ValueError("a 4-bit cache begins on 16 bytes: bulk copies read it")
 
 
 def _check_slots(slots: torch.Tensor, rows: int, device: int) -> torch.Tensor:
