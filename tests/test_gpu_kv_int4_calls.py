@@ -28,3 +28,18 @@ def test_bad_pages_beside_good_ones(each):
     meta.block_table.copy_(table)
     assert torch.equal(ops.paged_attention_int4(q, kc, vc, meta, 0.1), good)
     _native.check_status(torch.device(DEV))
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [1, 90, 130]])
+def test_row_numbers_lengths_and_tables_that_are_views(new, kernel):
+    """Every second or third element of larger tensors, as slices of a batch's columns are."""
+    q, kc, vc, meta = _setup(new, [200, 333, 150], 32, 8, 2, 128, 41)
+    want = ops.paged_attention_int4(q, kc, vc, meta, 0.1)
+    _check(want, *_want(q, kc, vc, meta, 0.1))
+    for name, step in (("query_start_loc", 2), ("seq_lens", 3), ("block_table", 2)):
+        dense = getattr(meta, name)
+        wide = torch.full((*dense.shape, step), 1 << 20, dtype=torch.int32, device=DEV)
+        wide[..., 0] = dense
+        setattr(meta, name, wide[..., 0])
+        assert torch.equal(ops.paged_attention_int4(q, kc, vc, meta, 0.1), want), name
+    _native.check_status(torch.device(DEV))

@@ -1,4 +1,6 @@
 """Calls of the 4-bit cache's operators that its other tests on the host do not make."""
+import dataclasses
+
 import pytest
 import torch
 
@@ -23,3 +25,11 @@ def test_caches_begin_on_16_bytes():
                 ops.read_kv_int4(*pair, slots, 64)
             with pytest.raises(ValueError, match="16 bytes"):
                 ops.paged_attention_int4(torch.zeros(1, 4, 64), *pair, meta, 0.125)
+
+
+def test_metadata_of_other_shapes_is_refused():
+    kc, vc = (ops.alloc_kv_cache_int4(2, 16, 2, 64, "cpu") for _ in "kv")
+    meta = _meta([1, 1], [1, 1], torch.zeros(2, 1, dtype=torch.int32), 4, 2, 64)
+    for kw in (dict(block_table=meta.block_table[:, 0]), dict(seq_lens=meta.seq_lens.view(2, 1)), dict(query_start_loc=meta.query_start_loc.view(3, 1))):
+        with pytest.raises(ValueError, match="metadata of 2 sequences"):
+            ops.paged_attention_int4(torch.zeros(2, 4, 64), kc, vc, dataclasses.replace(meta, **kw), 0.125)

@@ -8,6 +8,7 @@ multiple of 16 tokens.
 The reference quantises its cache to 8 bits with static scales (vllm_ascend/quantization/methods/kv_c8.py)."""
 from __future__ import annotations
 
+import copy
 import functools
 import struct
 from ctypes import c_char_p
@@ -195,7 +196,7 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     n = meta.num_reqs
     cu, lens, table = meta.query_start_loc, meta.seq_lens, meta.block_table
     if not (cu.dtype is lens.dtype is table.dtype is torch.int32 and cu.get_device() == lens.get_device() == table.get_device() == device
-            and cu.numel() > n and lens.numel() >= n and table.shape[0] >= n and table.stride()[1] == 1):
+            and cu.dim() == lens.dim() == 1 and table.dim() == 2 and cu.shape[0] > n and lens.shape[0] >= n and table.shape[0] >= n):
         raise ValueError(f"metadata of {n} sequences: row numbers {cu.dtype} {tuple(cu.shape)}, lengths {lens.dtype} {tuple(lens.shape)}, "
                          f"pages {table.dtype} {tuple(table.shape)}, not int32 on device {device}")
     if device < 0 or q.dtype is not torch.bfloat16:
@@ -203,6 +204,9 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                                         causal, window, out=out)
     if n == 0 or T == 0:
         return out
+    if not (cu.is_contiguous() and lens.is_contiguous() and table.stride()[1] == 1):         # the kernels walk them as they lie
+        meta = copy.copy(meta)
+        meta.query_start_loc, meta.seq_lens, meta.block_table = cu.contiguous(), lens.contiguous(), table.contiguous()
     given, q = out, _dense_heads(q)
     row, head, channel = out.stride()
     if channel != 1 or head != D or row % 8 or out.data_ptr() % 16:
