@@ -43,3 +43,35 @@ def test_row_numbers_lengths_and_tables_that_are_views(new, kernel):
         setattr(meta, name, wide[..., 0])
         assert torch.equal(ops.paged_attention_int4(q, kc, vc, meta, 0.1), want), name
     _native.check_status(torch.device(DEV))
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [1, 90, 130]])
+def test_tables_that_rows_share_or_that_are_cut_from_wider_ones(new, kernel):
+    """One row of pages for all sequences (a row stride of zero); columns out of a table whose other entries are no pages, up to its very end."""
+    lens = [200, 333, 150]
+    q, kc, vc, meta = _setup(new, lens, 32, 8, 2, 128, 42)
+    table = meta.block_table
+    meta.block_table = table[1:2].expand(3, -1)
+    out = ops.paged_attention_int4(q, kc, vc, meta, 0.1)
+    _check(out, *_want(q, kc, vc, meta, 0.1))
+    meta.block_table = table[1:2].repeat(3, 1)
+    assert torch.equal(ops.paged_attention_int4(q, kc, vc, meta, 0.1), out)
+    wide = torch.full((3, 40), 1 << 20, dtype=torch.int32, device=DEV)
+    wide[:, 40 - table.shape[1]:] = table
+    meta.block_table = table
+    out = ops.paged_attention_int4(q, kc, vc, meta, 0.1)
+    meta.block_table = wide[:, 40 - table.shape[1]:]
+    assert torch.equal(ops.paged_attention_int4(q, kc, vc, meta, 0.1), out)
+    _native.check_status(torch.device(DEV))
+
+
+def test_lengths_beyond_the_columns_are_reported(kernel):
+    """A sequence with more keys than its row of the table has pages: what lies behind the row is not read."""
+    q, kc, vc, meta = _setup([1, 64], [333, 320], 32, 8, 2, 128, 43)
+    wide = torch.zeros((2, 40), dtype=torch.int32, device=DEV)
+    wide[:, :11] = meta.block_table
+    meta.block_table = wide[:, :10]
+    good = ops.paged_attention_int4(q, kc, vc, meta, 0.1)
+    with pytest.raises(_native.NativeError, match="BAD_INDEX"):
+        _native.check_status(torch.device(DEV))
+    _check(good[1:], *(t[1:] for t in _want(q, kc, vc, _meta([1, 64], [320, 320], meta.block_table, 8, 2, 128), 0.1)))

@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(32 * D4_WARPS, Int4Cfg<D, NT>::BLOCKS) attn_in
 
   // the next tile to copy: lanes below U know the page of a unit each, and the unit's place there, walked by additions
   const int upp = p.block_size / KV4_TOKENS;
-  const int* bt = p.block_table + (long)seq * p.max_blocks;
+  const int* bt = p.block_table + seq * p.table_stride;
   int next = first, col = int4_div(first + lane, upp, p.upp_inv), at = first + lane - col * upp, blk = 0;
   const int step = int4_div(U, upp, p.upp_inv), rest = U - step * upp;
   auto look_up = [&]() {
@@ -595,7 +595,7 @@ int int4_params(Int4Params* p, const Int4Args& a) {
   p->out = (__nv_bfloat16*)a.out;
   p->part_o = (float*)a.scratch;
   p->part_lse = p->part_o + a.q_rows * a.Hq * a.parts * a.D;
-  p->q_stride = a.q_stride; p->out_stride = a.out_stride; p->num_blocks = a.num_blocks;
+  p->q_stride = a.q_stride; p->out_stride = a.out_stride; p->table_stride = a.table_stride; p->num_blocks = a.num_blocks;
   p->q_rows = a.q_rows;
   p->num_seqs = a.num_seqs; p->max_blocks = a.max_blocks; p->block_size = a.block_size;
   p->G = G; p->Hkv = a.Hkv; p->parts = a.parts; p->causal = a.causal; p->window = a.window;

@@ -13,7 +13,7 @@ struct Int4Params {
   const int *cu, *seq_lens, *block_table;
   __nv_bfloat16* out;
   float *part_o, *part_lse;       // [tokens x heads][parts][D], [..][parts]: results of parts, normalised, with log2 of their sums
-  long q_stride, out_stride, num_blocks, q_rows;
+  long q_stride, out_stride, table_stride, num_blocks, q_rows;
   int num_seqs, max_blocks, block_size, G, Hkv, parts, cluster, row_blocks, causal, window;
   uint32_t g_inv, upp_inv;        // ceil(2^32 / .) of G and of the units of a page (int4_div)
   float scale_log2;               // of scores over unpacked keys, which carry 2^-40
@@ -41,11 +41,11 @@ struct Int4Args {
   void *out, *scratch;
   int* status;
   cudaStream_t stream;
-  long q_stride, q_rows, num_blocks, out_stride, tokens;
+  long q_stride, q_rows, num_blocks, out_stride, tokens, table_stride;
   float scale;
   int block_size, max_blocks, num_seqs, max_q_len, Hq, Hkv, D, causal, window, parts;
 };
-static_assert(sizeof(Int4Args) == 168, "pointers, longs and ints without gaps, as they are packed");
+static_assert(sizeof(Int4Args) == 176, "pointers, longs and ints without gaps, as they are packed");
 
 // Checks and fills what both kernels take; 0 or an error code.
 int int4_params(Int4Params* p, const Int4Args& a);

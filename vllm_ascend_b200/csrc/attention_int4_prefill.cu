@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
     if (warp == 12) {
       // ---------------------------------------------------------- packed tiles
       const int upp = p.block_size / KV4_TOKENS;
-      const int* bt = p.block_table + (long)seq * p.max_blocks;
+      const int* bt = p.block_table + seq * p.table_stride;
       const bool whole = upp % 8 == 0;           // a tile lies in one page
       for (int j = 0; j < n; j++) {
         const int u0 = (t_a + j) * 8, units = min(8, (key_hi + KV4_TOKENS - 1) / KV4_TOKENS - u0);

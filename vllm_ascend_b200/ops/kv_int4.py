@@ -23,7 +23,7 @@ from . import reference as ref
 
 # arguments go by address, laid out as the sources' Kv4Args and Int4Args: packing them takes 0.3 us where ctypes takes 0.1 us for each
 _ROWS = struct.Struct("@7P4q3i")
-_ATTENTION = struct.Struct("@10P5qf10i")
+_ATTENTION = struct.Struct("@10P6qf10i")
 for _name in ("b200_kv_int4_write", "b200_kv_int4_read", "b200_attn_int4", "b200_attn_int4_prefill"):
     _native.register_signature(_name, [c_char_p])
 
@@ -305,7 +305,7 @@ def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, 
     rc = _native.lib().b200_attn_int4(_ATTENTION.pack(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cu.data_ptr(), lens.data_ptr(), table.data_ptr(), out.data_ptr(),
         0 if scratch is None else scratch.data_ptr(), _native.status_word(q.device).data_ptr(), _native.stream_ptr(), q.stride(0), ahead, NB,
-        out.stride(0), 0, scale, bs, table.stride(0), n, max_q, Hq, Hkv, D, int(causal), window, parts))
+        out.stride(0), 0, table.stride(0), scale, bs, table.shape[1], n, max_q, Hq, Hkv, D, int(causal), window, parts))
     _native.check(rc, "attn_int4")
     _native.count_launch(1 + int(parts > CLUSTER))
 
@@ -358,6 +358,6 @@ def _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, e
     rc = _native.lib().b200_attn_int4_prefill(_ATTENTION.pack(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cu.data_ptr(), lens.data_ptr(), table.data_ptr(), out.data_ptr(),
         0 if scratch is None else scratch.data_ptr(), _native.status_word(q.device).data_ptr(), _native.stream_ptr(), q.stride(0), T, NB,
-        out.stride(0), tokens, scale, bs, table.stride(0), end - first, 0, Hq, Hkv, D, int(causal), window, parts))
+        out.stride(0), tokens, table.stride(0), scale, bs, table.shape[1], end - first, 0, Hq, Hkv, D, int(causal), window, parts))
     _native.check(rc, "attn_int4_prefill")
     _native.count_launch(1 + int(parts > 1))
