@@ -75,3 +75,15 @@ def test_lengths_beyond_the_columns_are_reported(kernel):
     with pytest.raises(_native.NativeError, match="BAD_INDEX"):
         _native.check_status(torch.device(DEV))
     _check(good[1:], *(t[1:] for t in _want(q, kc, vc, _meta([1, 64], [320, 320], meta.block_table, 8, 2, 128), 0.1)))
+
+
+@pytest.mark.parametrize("page,columns", [(128, 8192), (16, 70000), (256, 1 << 19)])
+def test_tables_of_a_million_tokens_and_more(page, columns, kernel):
+    """What a table could hold is no reason to refuse short sequences in it."""
+    q, kc, vc, meta = _setup([1, 70], [300, 170], page, 8, 2, 128, 44)
+    out = ops.paged_attention_int4(q, kc, vc, meta, 0.1)
+    wide = torch.full((2, columns), -1, dtype=torch.int32, device=DEV)
+    wide[:, :meta.block_table.shape[1]] = meta.block_table
+    meta.block_table = wide
+    assert torch.equal(ops.paged_attention_int4(q, kc, vc, meta, 0.1), out)
+    _native.check_status(torch.device(DEV))

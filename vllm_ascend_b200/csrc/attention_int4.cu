@@ -600,7 +600,8 @@ int int4_params(Int4Params* p, const Int4Args& a) {
   p->num_seqs = a.num_seqs; p->max_blocks = a.max_blocks; p->block_size = a.block_size;
   p->G = G; p->Hkv = a.Hkv; p->parts = a.parts; p->causal = a.causal; p->window = a.window;
   const int upp = a.block_size / KV4_TOKENS;
-  if ((long)a.max_blocks * upp * upp > 0xffffffffl || (long)a.max_blocks * upp > 0xffffffffl / 65536) return 9888;      // 1M tokens a sequence and more
+  // what int4_div takes, and units times parts in 32 bits: tables of nearly 2^30 tokens (a sequence of that many takes 72 GiB a head of 64)
+  if ((long)a.max_blocks * upp * upp > 0xffffffffl || (long)a.max_blocks * upp > 0xffffffffl / I4_PARTS) return 9888;
   p->g_inv = (uint32_t)((0x100000000ll + G - 1) / G);
   p->upp_inv = (uint32_t)((0x100000000ll + upp - 1) / upp);
   p->scale_log2 = a.scale * 1.4426950408889634f * KV4_UNDO;
