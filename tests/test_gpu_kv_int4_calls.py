@@ -87,3 +87,18 @@ def test_tables_of_a_million_tokens_and_more(page, columns, kernel):
     meta.block_table = wide
     assert torch.equal(ops.paged_attention_int4(q, kc, vc, meta, 0.1), out)
     _native.check_status(torch.device(DEV))
+
+
+@pytest.mark.parametrize("new,lens,Hq,Hkv,window", [
+    ([1, 1, 3], [1000, 3000, 700], 16, 2, 527), ([2, 3, 1], [900, 999, 40], 8, 2, 100), ([1, 4, 1, 1], [2049, 555, 2050, 2063], 8, 1, 1030)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_fixed_sums_in_windows_beside_longer_neighbours(new, lens, Hq, Hkv, window, D, monkeypatch):
+    """Eight rows of a sequence fill a tile alone; beside a neighbour of more rows, eight that do not exist join them in their block."""
+    q, kc, vc, meta = _setup(new, lens, 32, Hq, Hkv, D, 45)
+    monkeypatch.setattr("vllm_ascend_b200.ops.kv_int4.fixed_sums", lambda: True)
+    out = ops.paged_attention_int4(q, kc, vc, meta, 0.1, window=window)
+    _check(out, *_want(q, kc, vc, meta, 0.1, window))
+    cu = meta.query_start_loc_cpu
+    for b in range(len(new)):
+        one = _meta(new[b:b + 1], lens[b:b + 1], meta.block_table[b:b + 1], Hq, Hkv, D)
+        assert torch.equal(ops.paged_attention_int4(q[cu[b]:cu[b + 1]], kc, vc, one, 0.1, window=window), out[cu[b]:cu[b + 1]]), b

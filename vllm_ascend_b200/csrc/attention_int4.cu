@@ -179,7 +179,10 @@ __global__ void __launch_bounds__(32 * D4_WARPS, Int4Cfg<D, NT>::BLOCKS) attn_in
   float o[NT][MT][4], m[NT][2], l[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
-    m[nt][0] = m[nt][1] = -INFINITY;
+    // rows that do not exist score 0, or -inf at an edge: a maximum of 0 never moves, so no row's rounding follows from how many
+    // rows its block has room for
+#pragma unroll
+    for (int e = 0; e < 2; e++) m[nt][e] = nt * 8 + 2 * c + e < rows ? -INFINITY : 0.f;
     l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < MT; i++)
