@@ -102,3 +102,12 @@ def test_fixed_sums_in_windows_beside_longer_neighbours(new, lens, Hq, Hkv, wind
     for b in range(len(new)):
         one = _meta(new[b:b + 1], lens[b:b + 1], meta.block_table[b:b + 1], Hq, Hkv, D)
         assert torch.equal(ops.paged_attention_int4(q[cu[b]:cu[b + 1]], kc, vc, one, 0.1, window=window), out[cu[b]:cu[b + 1]]), b
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 2, 2 ** 31 - 1, 1 << 40])
+def test_windows_wider_than_any_sequence(window, kernel):
+    """The same as none, in front of the first key too, where positions are below zero."""
+    q, kc, vc, meta = _setup([300, 3, 64, 1], [20, 1, 64, 500], 16, 8, 2, 128, 46)
+    out = ops.paged_attention_int4(q, kc, vc, meta, 0.1, window=window)
+    _check(out, *_want(q, kc, vc, meta, 0.1, window))
+    assert torch.equal(ops.paged_attention_int4(q, kc, vc, meta, 0.1), out)

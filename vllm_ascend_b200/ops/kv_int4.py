@@ -213,7 +213,7 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         out = q.new_empty((T, Hq, D))
         out.copy_(given)
     max_q, G = meta.max_query_len, Hq // Hkv
-    window = min(window, 2 ** 31 - 1)
+    window = min(window, 2 ** 31 - 1 - T)            # the first key of a window in 32 bits: positions are -T at least
     args = (q, k_cache, v_cache, meta, scale, out, causal, window, bs)
     if max_q * G <= FEW_ROWS or G > 128:
         _few_rows(*args, 0, n, max_q)
