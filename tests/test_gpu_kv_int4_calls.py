@@ -111,3 +111,25 @@ def test_windows_wider_than_any_sequence(window, kernel):
     out = ops.paged_attention_int4(q, kc, vc, meta, 0.1, window=window)
     _check(out, *_want(q, kc, vc, meta, 0.1, window))
     assert torch.equal(ops.paged_attention_int4(q, kc, vc, meta, 0.1), out)
+
+
+@pytest.mark.parametrize("pinned", [True, False])
+def test_blocks_swapped_to_the_host_and_back(pinned):
+    """A cache's blocks are on the host when the call returns, behind whatever work the device still had."""
+    from vllm_ascend_b200.attention.backend import B200AttentionBackend
+    g = torch.Generator().manual_seed(47)
+    data = torch.randint(1, 255, (64, 8, 128 * 128 * 9 // 16), generator=g, dtype=torch.uint8)
+    src, host = torch.zeros_like(data, device=DEV), torch.zeros(16, *data.shape[1:], dtype=torch.uint8, pin_memory=pinned)
+    pairs = torch.tensor([[i * 5 % 64, i] for i in range(16)])
+    big = torch.randn(8192, 8192, device=DEV, dtype=torch.bfloat16)
+    for _ in range(3):
+        for _ in range(20):
+            big @ big
+        src.copy_(data.to(DEV))
+        B200AttentionBackend.swap_blocks(src, host, pairs)
+        assert torch.equal(host, data[pairs[:, 0]])
+        back = torch.zeros_like(src)
+        B200AttentionBackend.swap_blocks(host, back, pairs.flip(1))
+        assert torch.equal(back[pairs[:, 0].to(DEV)], src[pairs[:, 0].to(DEV)])
+        host.zero_()
+        src.zero_()

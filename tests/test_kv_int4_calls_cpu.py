@@ -33,3 +33,30 @@ def test_metadata_of_other_shapes_is_refused():
     for kw in (dict(block_table=meta.block_table[:, 0]), dict(seq_lens=meta.seq_lens.view(2, 1)), dict(query_start_loc=meta.query_start_loc.view(3, 1))):
         with pytest.raises(ValueError, match="metadata of 2 sequences"):
             ops.paged_attention_int4(torch.zeros(2, 4, 64), kc, vc, dataclasses.replace(meta, **kw), 0.125)
+
+
+class _OnADevice:
+    """A cache on a device whose copies to the host arrive when it is waited for: a copy that does not block holds zeros until then."""
+    is_cuda, device = True, torch.device("cuda", 0)
+
+    def __init__(self, data):
+        self.data, self.dtype, self.shape = data, data.dtype, data.shape
+
+    def dim(self):
+        return self.data.dim()
+
+    def __getitem__(self, at):
+        return _OnADevice(self.data[at])
+
+    def to(self, device, non_blocking=False):
+        assert torch.device(device).type == "cpu"
+        return torch.zeros_like(self.data) if non_blocking else self.data.clone()
+
+
+def test_swapped_blocks_have_arrived_on_the_host(monkeypatch):
+    from vllm_ascend_b200.attention.backend import B200AttentionBackend
+    host, pairs, to = ops.alloc_kv_cache_int4(3, 16, 2, 64, "cpu"), torch.tensor([[0, 2], [3, 1]]), torch.Tensor.to
+    src = torch.randint(1, 255, (4, *host.shape[1:]), dtype=torch.uint8)
+    monkeypatch.setattr(torch.Tensor, "to", lambda t, d, *a, **kw: t if torch.device(d).type == "cuda" else to(t, d, *a, **kw))     # the pairs
+    B200AttentionBackend.swap_blocks(_OnADevice(src), host, pairs)
+    assert torch.equal(host[2], src[0]) and torch.equal(host[1], src[3]) and not host[0].any()

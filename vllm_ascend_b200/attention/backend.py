@@ -110,7 +110,8 @@ def _swap_blocks(src: torch.Tensor, dst: torch.Tensor, src_to_dst: torch.Tensor)
     if not ok:
         s = src_to_dst[:, 0].long()
         d = src_to_dst[:, 1].long()
-        dst[d.to(dst.device)] = src[s.to(src.device)].to(dst.device, non_blocking=True)
+        # the host writes into its cache at once, so what comes from a device has to be there by then
+        dst[d.to(dst.device)] = src[s.to(src.device)].to(dst.device, non_blocking=dst.is_cuda)
         return
     import vllm_ascend_b200.distributed.kv_transfer.nvlink_connector  # noqa: F401  (signatures)
     e = src.element_size()
