@@ -133,3 +133,36 @@ def test_blocks_swapped_to_the_host_and_back(pinned):
         assert torch.equal(back[pairs[:, 0].to(DEV)], src[pairs[:, 0].to(DEV)])
         host.zero_()
         src.zero_()
+
+
+def test_slots_and_pages_out_of_range_with_other_types():
+    """fp32 rows go through the operators' definition; what is out of range is reported as the kernels report it, the rest is done."""
+    q, kc, vc, meta = _setup([1, 3], [50, 90], 16, 8, 2, 64, 48)
+    want, tol = _want(q, kc, vc, meta, 0.2)
+    k4, v4 = kc.clone(), vc.clone()
+    rows = torch.ones(4, 2, 64, device=DEV)
+    ops.write_kv_int4(rows, rows, k4, v4, torch.tensor([3, kc.shape[0] * 16, -1, 1 << 40], device=DEV))
+    with pytest.raises(_native.NativeError, match="BAD_INDEX"):
+        _native.check_status(torch.device(DEV))
+    ops.write_kv_int4(rows[:1], rows[:1], kc, vc, torch.tensor([3], device=DEV))
+    assert torch.equal(k4, kc) and torch.equal(v4, vc)
+    want, tol = _want(q, kc, vc, meta, 0.2)
+    for bad in (kc.shape[0], 1 << 30, -1, -(1 << 30)):
+        page = int(meta.block_table[0, 2])
+        meta.block_table[0, 2] = bad
+        out = ops.paged_attention_int4(q.float(), kc, vc, meta, 0.2)
+        with pytest.raises(_native.NativeError, match="BAD_INDEX"):
+            _native.check_status(torch.device(DEV))
+        assert float((out[1:].double() - want[1:]).abs().max()) < 1e-4
+        meta.block_table[0, 2] = page
+    # in front of a window, and behind a sequence's end, a table may hold anything
+    for window in (1, 20):
+        want, tol = _want(q, kc, vc, meta, 0.2, window)
+        table = meta.block_table.clone()
+        for b, n, a in ((0, 50, 1), (1, 90, 3)):
+            meta.block_table[b, :max(0, n - a - window + 1) // 16] = -(1 << 30)
+        out = ops.paged_attention_int4(q.float(), kc, vc, meta, 0.2, window=window)
+        assert float((out.double() - want).abs().max()) < 1e-4
+        _check(ops.paged_attention_int4(q, kc, vc, meta, 0.2, window=window), want, tol)
+        meta.block_table.copy_(table)
+    _native.check_status(torch.device(DEV))

@@ -178,7 +178,8 @@ def status_word(device: torch.device) -> torch.Tensor:
     return t
 
 
-STATUS_NAMES = {0: "OK", 1: "TIMEOUT", 2: "BAD_INDEX", 3: "OVERFLOW"}
+BAD_INDEX = 2
+STATUS_NAMES = {0: "OK", 1: "TIMEOUT", BAD_INDEX: "BAD_INDEX", 3: "OVERFLOW"}
 
 
 def check_status(device: torch.device) -> None:

@@ -78,6 +78,12 @@ def _dense_heads(x: torch.Tensor) -> torch.Tensor:
     return x.clone(memory_format=torch.contiguous_format)
 
 
+def _report(wrong: torch.Tensor, device: torch.device) -> None:
+    """Sets the device's status word where an index is out of range, as the kernels do.  An indexing operator would end the process's
+    work on that GPU."""
+    _native.status_word(device).masked_fill_(wrong.any(), _native.BAD_INDEX)
+
+
 def _elsewhere(device: int) -> bool:
     """Whether tensors of that device index are on a GPU that is not the current one."""
     return device >= 0 and device != torch.cuda.current_device()
@@ -100,6 +106,10 @@ def write_kv_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     if T == 0:
         return
     if device < 0 or k.dtype is not torch.bfloat16:
+        if device >= 0:
+            beyond = slots >= k_cache.shape[0] * bs
+            _report(beyond, k.device)
+            slots = slots.masked_fill(beyond, -1)
         return ref.write_kv_int4(k, v, k_cache, v_cache, slots)
     k, v = _dense_heads(k), _dense_heads(v)
     rc = _native.lib().b200_kv_int4_write(_ROWS.pack(
@@ -200,8 +210,9 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError(f"metadata of {n} sequences: row numbers {cu.dtype} {tuple(cu.shape)}, lengths {lens.dtype} {tuple(lens.shape)}, "
                          f"pages {table.dtype} {tuple(table.shape)}, not int32 on device {device}")
     if device < 0 or q.dtype is not torch.bfloat16:
-        return ref.paged_attention_int4(q, k_cache, v_cache, meta.query_start_loc_cpu, meta.seq_lens_cpu, meta.block_table, scale,
-                                        causal, window, out=out)
+        if device >= 0:
+            table = _pages_in_range(cu, lens, table[:n], k_cache.shape[0], bs, window)
+        return ref.paged_attention_int4(q, k_cache, v_cache, meta.query_start_loc_cpu, meta.seq_lens_cpu, table, scale, causal, window, out=out)
     if n == 0 or T == 0:
         return out
     if not (cu.is_contiguous() and lens.is_contiguous() and table.stride()[1] == 1):         # the kernels walk them as they lie
@@ -226,6 +237,19 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
             else:
                 _prompts(*args, first, end, *what)
     return out if out is given else given.copy_(out)
+
+
+def _pages_in_range(cu, lens, table, blocks: int, bs: int, window: int) -> torch.Tensor:
+    """The table with page 0 in place of what is no page; reported where a new token sees such a page."""
+    n, columns = table.shape
+    new, lens = (cu[1:n + 1] - cu[:n]).unsqueeze(1), lens[:n].unsqueeze(1)
+    col = torch.arange(columns, device=table.device)
+    seen = (new > 0) & (col * bs < lens)
+    if window:
+        seen &= (col + 1) * bs > lens.long() - new - window + 1
+    wrong = (table < 0) | (table >= blocks)
+    _report(wrong & seen, table.device)
+    return table.masked_fill(wrong, 0)
 
 
 def _few_us(new, keys, G: int, Hkv: int, D: int, sms: int) -> float:
