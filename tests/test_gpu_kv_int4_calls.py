@@ -166,3 +166,19 @@ def test_slots_and_pages_out_of_range_with_other_types():
         _check(ops.paged_attention_int4(q, kc, vc, meta, 0.2, window=window), want, tol)
         meta.block_table.copy_(table)
     _native.check_status(torch.device(DEV))
+
+
+def test_what_is_no_number_with_other_types():
+    """fp32 queries over a cache in which other sequences, later tokens and freed slots hold NaN: the rows that see none are as the kernels'."""
+    q, kc, vc, meta = _setup([0, 3, 64], [5000, 70, 90], 16, 8, 2, 128, 49)
+    want, tol = _want(q, kc, vc, meta, 0.1)
+    nan = torch.full((1, 2, 128), float("nan"), device=DEV, dtype=torch.bfloat16)
+    for b, t in ((0, 3), (1, 69), (1, 71), (2, 80)):
+        ops.write_kv_int4(nan, nan, kc, vc, (meta.block_table[b, t // 16].long() * 16 + t % 16).view(1))
+    rows = [0, 1, *range(3, 3 + 54)]                              # token 69 is the second sequence's last, 80 the third's 55th new one
+    f32, own = ops.paged_attention_int4(q.float(), kc, vc, meta, 0.1), ops.paged_attention_int4(q, kc, vc, meta, 0.1)
+    for out in (f32, own):
+        _check(out[rows], want[rows], tol[rows])
+        rest = torch.ones(len(q), dtype=torch.bool)
+        rest[rows] = False
+        assert out[rest].isnan().all()

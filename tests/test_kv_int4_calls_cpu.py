@@ -60,3 +60,30 @@ def test_swapped_blocks_have_arrived_on_the_host(monkeypatch):
     monkeypatch.setattr(torch.Tensor, "to", lambda t, d, *a, **kw: t if torch.device(d).type == "cuda" else to(t, d, *a, **kw))     # the pairs
     B200AttentionBackend.swap_blocks(_OnADevice(src), host, pairs)
     assert torch.equal(host[2], src[0]) and torch.equal(host[1], src[3]) and not host[0].any()
+
+
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 9), (False, 0)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_what_is_no_number_reaches_the_rows_that_see_it(causal, window, dtype):
+    """A group of keys takes a row's heads of the group whole, one of values its 32 channels; other rows have the bits they have without it."""
+    g = torch.Generator().manual_seed(window)
+    Hq, Hkv, D, page, new, lens = 6, 2, 64, 16, [1, 6, 3], [30, 21, 48]
+    table = torch.tensor([[5, 1, 0], [2, 7, 0], [3, 4, 6]], dtype=torch.int32)
+    kc, vc = (ops.alloc_kv_cache_int4(8, page, Hkv, D, "cpu") for _ in "kv")
+    k, v = (torch.randn(8 * page, Hkv, D, generator=g).to(dtype) for _ in "kv")
+    ops.write_kv_int4(k, v, kc, vc, torch.arange(8 * page))
+    q, meta = torch.randn(sum(new), Hq, D, generator=g).to(dtype), _meta(new, lens, table, Hq, Hkv, D)
+    spots = [(0, 28, "v"), (0, 31, "v"), (1, 17, "k"), (1, 19, "v"), (1, 25, "k"), (2, 2, "k"), (2, 46, "v"), (2, 47, "k")]
+    slots = torch.stack([table[b, t // page].long() * page + t % page for b, t, _ in spots])
+    want = ops.paged_attention_int4(q, kc, vc, meta, 0.125, causal=causal, window=window)
+    assert torch.isfinite(want).all()
+    hit = torch.zeros_like(want, dtype=torch.bool)
+    for i, (b, t, what) in enumerate(spots):
+        (k if what == "k" else v)[slots[i], 1 if what == "k" else 0, 40] = float("inf" if i % 2 else "nan")
+        for row, pos in enumerate(range(lens[b] - new[b], lens[b]), sum(new[:b])):
+            if t >= lens[b] or causal and t > pos or window and t <= pos - window:
+                continue
+            hit[row, slice(3, 6) if what == "k" else slice(0, 3), 0 if what == "k" else 32:] = True
+    ops.write_kv_int4(k, v, kc, vc, torch.arange(8 * page))
+    out = ops.paged_attention_int4(q, kc, vc, meta, 0.125, causal=causal, window=window)
+    assert out.isnan().equal(hit) and torch.equal(out[~hit], want[~hit])

@@ -350,9 +350,29 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                          block_table: torch.Tensor, scale: float, causal: bool = True, window: int = 0, out: Optional[torch.Tensor] = None):
     dim = q.shape[-1]
     B, bs = k_cache.shape[0], kv_int4_block_size(k_cache, dim)
-    dense = read_kv_int4(k_cache, v_cache, torch.arange(B * bs, device=q.device), dim, torch.float32)
-    return paged_attention(q, *(t.view(B, bs, -1, dim) for t in dense), query_start_loc, seq_lens, block_table, scale, causal,
-                           window, out=out)
+    k, v = read_kv_int4(k_cache, v_cache, torch.arange(B * bs, device=q.device), dim, torch.float32)
+    odd_k, odd_v = k.isnan().any(-1), v.unflatten(-1, (-1, KV_INT4_GROUP)).isnan().any(-1)              # [slots, heads], with groups
+    no_numbers = bool(odd_k.any() or odd_v.any())
+    if no_numbers:
+        k, v = k.nan_to_num(0.0), v.nan_to_num(0.0)
+    out = paged_attention(q, *(t.view(B, bs, -1, dim) for t in (k, v)), query_start_loc, seq_lens, block_table, scale, causal, window, out=out)
+    # groups that are no numbers reach the rows that see them, and no others
+    for b in range(len(seq_lens) if no_numbers else 0):
+        first, end, n = int(query_start_loc[b]), int(query_start_loc[b + 1]), int(seq_lens[b])
+        if end <= first:
+            continue
+        pos = torch.arange(n, device=q.device)
+        own, at = torch.arange(n - (end - first), n, device=q.device).unsqueeze(1), block_table[b].long()[pos // bs] * bs + pos % bs
+        sees = torch.ones((end - first, n), dtype=torch.bool, device=q.device)
+        if causal:
+            sees &= pos <= own
+        if window > 0:
+            sees &= pos > own - window
+        hit = (torch.einsum("qk,kh->qh", sees.float(), odd_k[at].float()) > 0).unsqueeze(-1) \
+            | (torch.einsum("qk,khg->qhg", sees.float(), odd_v[at].float()) > 0)
+        hit = hit.repeat_interleave(q.shape[1] // odd_k.shape[1], 1).repeat_interleave(KV_INT4_GROUP, 2)
+        out[first:end] = torch.where(hit, float("nan"), out[first:end])
+    return out
 
 
 def merge_attn_states(o1, lse1, o2, lse2):
