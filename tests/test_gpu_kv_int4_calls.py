@@ -182,3 +182,30 @@ def test_what_is_no_number_with_other_types():
         rest = torch.ones(len(q), dtype=torch.bool)
         rest[rows] = False
         assert out[rest].isnan().all()
+
+
+@pytest.mark.parametrize("method", ["eagle", "draft_model", "ngram"])
+def test_engine_drafts_over_a_4_bit_cache(method):
+    """Drafts keep their own pages beside the model's; blocks counted by what memory holds; repeated prompts come from the prefix cache (not with a
+    draft model, whose catching up over whole prompts does not fit into a step)."""
+    import numpy as np
+    from vllm_ascend_b200.config import ModelConfig
+    from vllm_ascend_b200.engine.llm import LLM
+    from vllm_ascend_b200.engine.request import SamplingParams
+    cfg = ModelConfig(name="t", architecture="Qwen3ForCausalLM", vocab_size=2048, hidden_size=512, intermediate_size=1024,
+                      num_hidden_layers=3, num_attention_heads=8, num_key_value_heads=2, head_dim=128, qk_norm=True, rope_theta=1e6,
+                      dtype="bfloat16", init_std=0.05)
+    prompts = [np.tile(np.random.default_rng(i).integers(0, 2048, size=40), 8)[:n].tolist() for i, n in enumerate((300, 40, 133))]
+    spec = {"method": method, "num_speculative_tokens": 3, **({"model": cfg} if method == "draft_model" else {})}
+    llm = LLM(cfg, device="cuda", max_model_len=512, max_num_seqs=8, max_num_batched_tokens=256, kv_cache_dtype="int4",
+              enable_prefix_caching=method != "draft_model", cudagraph_capture_sizes=[2, 4, 8], speculative_config=spec)
+    runner = llm.engine.runner
+    for _ in range(2):
+        outs = llm.generate(prompts, SamplingParams(temperature=0.0, max_tokens=20, ignore_eos=True))
+        assert all(len(o.outputs[0].token_ids) == 20 for o in outs)
+    assert runner.spec_stats["draft_tokens"] > 0
+    if method == "draft_model":                # the model itself drafts, over bf16 pages
+        assert runner.spec_stats["accepted_tokens"] > 0 and runner.draft_bytes_per_block() * 9 == runner.kv_bytes_per_block() * 32
+        assert all(t.dtype == torch.bfloat16 and t.shape[0] == runner.num_blocks for c in runner.proposer.kv_caches for t in c)
+    assert all(t.dtype == torch.uint8 for c in runner.kv_caches for t in c)
+    _native.check_status(torch.device(DEV))

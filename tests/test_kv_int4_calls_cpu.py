@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from test_kv_int4_cpu import _meta
+from test_kv_int4_engine_cpu import _cfg
 from vllm_ascend_b200 import ops
 
 
@@ -87,3 +88,32 @@ def test_what_is_no_number_reaches_the_rows_that_see_it(causal, window, dtype):
     ops.write_kv_int4(k, v, kc, vc, torch.arange(8 * page))
     out = ops.paged_attention_int4(q, kc, vc, meta, 0.125, causal=causal, window=window)
     assert out.isnan().equal(hit) and torch.equal(out[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("method,layers", [("eagle", 1), ("eagle3", 1), ("draft_model", 3), ("ngram", 0)])
+@pytest.mark.parametrize("kv", ["int4", "auto"])
+def test_draft_caches_count_against_the_memory_of_blocks(method, layers, kv, monkeypatch):
+    """Drafts keep keys and values of every block in the model's type, whatever the model's own cache is."""
+    from vllm_ascend_b200.engine.llm import LLM
+    from vllm_ascend_b200.engine.model_runner import ModelRunner
+    from vllm_ascend_b200.engine.request import SamplingParams
+    made, whole = [], ModelRunner.determine_num_blocks
+    monkeypatch.setattr(ModelRunner, "determine_num_blocks", lambda r: made.append(r.proposer) or whole(r))
+    spec = {"method": method, "num_speculative_tokens": 2, "model": _cfg(name="d", num_hidden_layers=3, num_key_value_heads=4, dtype="bfloat16")}
+    llm = LLM(_cfg(dtype="bfloat16"), device="cpu", max_model_len=1 << 16, max_num_seqs=2, block_size=16, max_num_batched_tokens=64, kv_cache_dtype=kv,
+              num_gpu_blocks_override=64, speculative_config={k: v for k, v in spec.items() if k != "model" or method == "draft_model"})
+    r = llm.engine.runner
+    assert made == [r.proposer]                                    # its weights are there when the rest is measured
+    heads = 4 if method == "draft_model" else 2
+    draft = layers * 2 * 16 * heads * 64 * 2
+    assert r.draft_bytes_per_block() == draft
+    llm.generate([[3, 4, 5] * 9], SamplingParams(temperature=0.0, max_tokens=6, ignore_eos=True))
+    if layers:
+        assert sum(t[0].numel() * t.element_size() for c in r.proposer.kv_caches for t in c) == draft
+    room = 100 * (r.kv_bytes_per_block() + draft) + 5
+    r.is_cuda, r.cfg.cache.num_gpu_blocks = True, None
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    monkeypatch.setattr(r, "activation_bytes_estimate", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *a: (room, room))
+    r.cfg.cache.gpu_memory_utilization = 1.0
+    assert r.determine_num_blocks() == 100

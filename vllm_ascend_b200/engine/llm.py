@@ -42,6 +42,9 @@ class LLMEngine:
         self.sleep_level = 0
         self.worker.load_model()
         self.moe_runtime = self.worker.moe_runtime
+        if cfg.speculative_config:               # in front of the cache, whose blocks share the memory with drafts' weights and pages
+            from ..spec_decode import get_spec_decode_method
+            self.runner.proposer = get_spec_decode_method(cfg.speculative_config, self.runner)
         num_blocks = self.worker.determine_num_blocks()
         self.worker.initialize_cache(num_blocks)
         self.worker.compile_or_warm_up_model()
@@ -64,8 +67,6 @@ class LLMEngine:
         if cfg.enable_lora:
             self.scheduler.max_loras = cfg.max_loras
         if cfg.speculative_config:
-            from ..spec_decode import get_spec_decode_method
-            self.runner.proposer = get_spec_decode_method(cfg.speculative_config, self.runner)
             self.scheduler.spec_slack = int(cfg.speculative_config.get("num_speculative_tokens", 3))
             dsc = get_b200_config().dynamic_spec_config
             if dsc.method:

@@ -259,6 +259,10 @@ class ModelRunner:
             per_tok = self._num_kv_layers() * sum(self._cache_widths())
         return self.block_size * per_tok * itemsize
 
+    def draft_bytes_per_block(self) -> int:
+        """What a proposer's own layers store for every block of this cache."""
+        return self.proposer.bytes_per_block() if hasattr(self.proposer, "bytes_per_block") else 0
+
     @property
     def kv_dtype(self) -> torch.dtype:
         return self.mcfg.torch_dtype
@@ -301,7 +305,7 @@ class ModelRunner:
         free, total = torch.cuda.mem_get_info(self.device)
         budget = total * cc.gpu_memory_utilization - (total - free) - self.activation_bytes_estimate() \
             - self.state_bytes()
-        n = int(budget // max(self.kv_bytes_per_block(), 1))      # a purely recurrent model pages nothing
+        n = int(budget // max(self.kv_bytes_per_block() + self.draft_bytes_per_block(), 1))      # a purely recurrent model pages nothing
         if n < 8:
             raise RuntimeError(f"not enough memory for the KV cache ({budget / 2**30:.1f} GiB left)")
         # a block beyond what max_num_seqs full-length sequences can use is wasted

@@ -275,21 +275,25 @@ class DraftModelProposer:
         self.computed: dict[str, int] = {}        # request id -> draft positions with valid KV
         self.stats = {"draft_forwards": 0}
 
+    def _cache_widths(self, attn) -> list[tuple[int, int]]:
+        """(heads, width) of the tensors that a draft layer keeps in pages."""
+        if hasattr(attn, "dc"):                   # MLA draft layer: latent, rope key (and index keys)
+            return [(1, w) for w in [attn.dc, attn.dr] + ([attn.idx_dim] if getattr(attn, "index_topk", 0) else [])]
+        return [(attn.Hkv, attn.D)] * 2
+
+    def bytes_per_block(self) -> int:
+        """What the draft layers keep for a block of the target's cache, whose numbers they share; in the model's type always."""
+        itemsize = torch.empty(0, dtype=self.runner.kv_dtype).element_size()
+        return self.runner.block_size * itemsize * sum(h * w for L in self.model.layers for h, w in self._cache_widths(L.self_attn))
+
     def _ensure_cache(self) -> None:
         if self.kv_caches is not None:
             return
         r = self.runner
         layout = r.cfg.cache.kv_layout if r.is_cuda else "NHD"
-        self.kv_caches = []
-        for layer in self.model.layers:
-            a = layer.self_attn
-            if hasattr(a, "dc"):                  # MLA draft layer: latent, rope key (and index keys)
-                widths = [a.dc, a.dr] + ([a.idx_dim] if getattr(a, "index_topk", 0) else [])
-                self.kv_caches.append(tuple(ops.alloc_kv_cache(r.num_blocks, r.block_size, 1, w, r.kv_dtype,
-                                                               r.device, "NHD") for w in widths))
-                continue
-            self.kv_caches.append(tuple(ops.alloc_kv_cache(r.num_blocks, r.block_size, a.Hkv, a.D, r.kv_dtype,
-                                                           r.device, layout) for _ in range(2)))
+        self.kv_caches = [tuple(ops.alloc_kv_cache(r.num_blocks, r.block_size, h, w, r.kv_dtype, r.device,
+                                                   "NHD" if hasattr(L.self_attn, "dc") else layout)
+                                for h, w in self._cache_widths(L.self_attn)) for L in self.model.layers]
 
     # ------------------------------------------------------------------
     def _forward(self, items: list, shift: int, hidden_rows: Optional[torch.Tensor]):
