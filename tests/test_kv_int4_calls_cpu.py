@@ -117,3 +117,25 @@ def test_draft_caches_count_against_the_memory_of_blocks(method, layers, kv, mon
     monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *a: (room, room))
     r.cfg.cache.gpu_memory_utilization = 1.0
     assert r.determine_num_blocks() == 100
+
+
+def test_names_of_cache_types(caplog):
+    """Text that names no type is refused; types that there is no cache of are stored in the model's, with a word."""
+    import logging
+    from vllm_ascend_b200.config import CacheConfig
+    from vllm_ascend_b200.engine.llm import LLM
+    small = dict(device="cpu", max_model_len=64, max_num_seqs=2, block_size=16)
+    for text in ("INT4", "int4 ", "int-4", "", "4"):
+        with pytest.raises(ValueError, match="kv_cache_dtype"):
+            LLM(_cfg(), kv_cache_dtype=text, **small)
+    assert CacheConfig(kv_cache_dtype=None).kv_cache_dtype == "auto"
+    logger = logging.getLogger("vllm_ascend_b200")
+    logger.addHandler(caplog.handler)
+    try:
+        for text, said in (("auto", False), ("float32", False), ("int4", False), ("fp8", True), ("bfloat16", True)):
+            caplog.clear()
+            caches = LLM(_cfg(), kv_cache_dtype=text, **small).engine.runner.kv_caches
+            assert caches[0][0].dtype is (torch.uint8 if text == "int4" else torch.float32)
+            assert any("kv_cache_dtype" in r.getMessage() for r in caplog.records) is said
+    finally:
+        logger.removeHandler(caplog.handler)

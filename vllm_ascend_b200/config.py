@@ -595,6 +595,12 @@ def get_model_config(name_or_path: str, **over) -> ModelConfig:
     raise ValueError(f"unknown model {name_or_path!r}: not a preset {sorted(PRESETS)} nor a directory")
 
 
+#: names that vLLM takes, and int4
+KV_CACHE_DTYPES = ("auto", "int4", "bfloat16", "float16", "half", "float32", "float", "fp8", "fp8_e4m3", "fp8_e5m2", "fp8_inc", "fp8_ds_mla",
+                   "fp8_per_token_head", "int8_per_token_head", "nvfp4", "turboquant_k8v4", "turboquant_4bit_nc", "turboquant_k3v4_nc",
+                   "turboquant_3bit_nc")
+
+
 @dataclass
 class CacheConfig:
     block_size: int = 128              # reference default (vllm_ascend/utils.py:1162-1212)
@@ -603,6 +609,11 @@ class CacheConfig:
     enable_prefix_caching: bool = False
     kv_cache_dtype: str = "auto"       # int4: ops/kv_int4.py; others: the model's type
     kv_layout: str = "HND"             # physical order inside a block: HND (per-head pages) | NHD
+
+    def __post_init__(self):
+        self.kv_cache_dtype = "auto" if self.kv_cache_dtype is None else self.kv_cache_dtype
+        if self.kv_cache_dtype not in KV_CACHE_DTYPES:
+            raise ValueError(f"kv_cache_dtype {self.kv_cache_dtype!r} is none of {', '.join(KV_CACHE_DTYPES)}")
 
 
 @dataclass

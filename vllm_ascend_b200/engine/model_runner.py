@@ -21,6 +21,7 @@ from .. import _native, envs, ops
 from ..attention.metadata import (AttentionMetadata, AttentionState, build_tile_worklist,
                                   split_decodes_and_prefills)
 from ..config import EngineConfig
+from ..logger import logger
 from ..parallel import state as pstate
 from ..sample.sampler import Sampler, SamplingMetadata
 from .request import Request
@@ -338,6 +339,9 @@ class ModelRunner:
             per_layer.append(shapes)
         layout = self.cfg.cache.kv_layout if self.is_cuda else "NHD"
         int4 = self._kv_int4()
+        asked = self.cfg.cache.kv_cache_dtype
+        if not int4 and asked != "auto" and {"half": "float16", "float": "float32"}.get(asked, asked) != str(self.kv_dtype).split(".")[-1]:
+            logger.warning("kv_cache_dtype %r: keys and values are stored in the model's type, %s", asked, self.kv_dtype)
         self.kv_arena = None
         if self.cfg.kv_transfer_config and any(self._extra_states(L.self_attn) for L in self.model.layers):
             raise NotImplementedError("KV transfer of layers that keep a state beside their pages")
