@@ -209,3 +209,40 @@ def test_engine_drafts_over_a_4_bit_cache(method):
         assert all(t.dtype == torch.bfloat16 and t.shape[0] == runner.num_blocks for c in runner.proposer.kv_caches for t in c)
     assert all(t.dtype == torch.uint8 for c in runner.kv_caches for t in c)
     _native.check_status(torch.device(DEV))
+
+
+@pytest.mark.parametrize("new,lens,Hq,Hkv", [([1], [45000], 8, 2), ([1, 1], [41001, 60000], 16, 8), ([300], [9000], 8, 2)])
+def test_calls_at_once_whose_parts_join_through_memory(new, lens, Hq, Hkv, monkeypatch):
+    """Every call has memory of its own for its parts' results: two streams, and a captured prompt replayed beside them.  Decodes that a graph
+    holds join in clusters."""
+    from vllm_ascend_b200.ops import kv_int4
+    asked, results = [], kv_int4._results
+    monkeypatch.setattr(kv_int4, "_results", lambda *a: asked.append(results(*a)) or asked[-1])
+    sets = [_setup(new, lens, 128, Hq, Hkv, 128, seed) for seed in (50, 51)]
+    want = [ops.paged_attention_int4(*s, 0.09) for s in sets]
+    assert len(asked) == 2 and asked[0].data_ptr() != asked[1].data_ptr()
+    for s, w in zip(sets, want):
+        _check(w, *_want(*s, 0.09))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        replayed = ops.paged_attention_int4(*sets[0], 0.09)
+    assert len(asked) == (2 if max(new) == 1 else 3)
+    replayed.zero_()
+    asked.clear()
+    torch.cuda.synchronize()
+    sides, got = [torch.cuda.Stream() for _ in range(3)], [[], []]
+    for _ in range(20):
+        for i, s in enumerate(sets):
+            with torch.cuda.stream(sides[i]):
+                got[i].append(ops.paged_attention_int4(*s, 0.09))
+        with torch.cuda.stream(sides[2]):
+            graph.replay()
+    torch.cuda.synchronize()
+    assert len(asked) == 40
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+    if max(new) > 1:
+        assert torch.equal(replayed, want[0])
+    else:
+        _check(replayed, *_want(*sets[0], 0.09))
+    _native.check_status(torch.device(DEV))
