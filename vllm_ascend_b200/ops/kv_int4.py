@@ -47,13 +47,14 @@ def alloc_kv_cache_int4(num_blocks: int, block_size: int, heads: int, dim: int, 
     return arena.take(shape, torch.uint8) if arena is not None else torch.zeros(shape, dtype=torch.uint8, device=device)
 
 
-def _check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dim: int, device: int) -> int:
-    """Block size of a pair of caches that belong together, on the device of that index (-1: the host), where bulk copies can read them."""
-    shape = k_cache.shape
+def _check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dim: int, device: int) -> tuple[int, int, int, int, int]:
+    """Blocks, heads, block size and addresses of a pair of caches that belong together, on the device of that index (-1: the host), where bulk
+    copies can read them."""
+    shape, k_at, v_at = k_cache.shape, k_cache.data_ptr(), v_cache.data_ptr()
     if dim in HEAD_SIZES and len(shape) == 3 and shape[2] and shape[2] % (9 * dim) == 0 and v_cache.shape == shape \
             and k_cache.dtype is v_cache.dtype is torch.uint8 and k_cache.is_contiguous() and v_cache.is_contiguous() \
-            and k_cache.get_device() == v_cache.get_device() == device and (k_cache.data_ptr() | v_cache.data_ptr()) & 15 == 0:
-        return shape[2] // (9 * dim) * ref.KV_INT4_TOKENS
+            and k_cache.get_device() == v_cache.get_device() == device and (k_at | v_at) & 15 == 0:
+        return shape[0], shape[1], shape[2] // (9 * dim) * ref.KV_INT4_TOKENS, k_at, v_at
     if dim not in HEAD_SIZES:
         raise ValueError(f"a 4-bit cache takes heads of {HEAD_SIZES}, not {dim}")
     bs = ref.kv_int4_block_size(k_cache, dim)
@@ -99,22 +100,22 @@ def write_kv_int4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     if _elsewhere(device):
         with torch.cuda.device(device):
             return write_kv_int4(k, v, k_cache, v_cache, slot_mapping)
-    bs = _check_caches(k_cache, v_cache, D, device)
-    if H != k_cache.shape[1]:
-        raise ValueError(f"rows of {H} heads, a cache of {k_cache.shape[1]}")
+    NB, heads, bs, k_at, v_at = _check_caches(k_cache, v_cache, D, device)
+    if H != heads:
+        raise ValueError(f"rows of {H} heads, a cache of {heads}")
     slots = _check_slots(slot_mapping, T, device)
     if T == 0:
         return
     if device < 0 or k.dtype is not torch.bfloat16:
         if device >= 0:
-            beyond = slots >= k_cache.shape[0] * bs
+            beyond = slots >= NB * bs
             _report(beyond, k.device)
             slots = slots.masked_fill(beyond, -1)
         return ref.write_kv_int4(k, v, k_cache, v_cache, slots)
     k, v = _dense_heads(k), _dense_heads(v)
     rc = _native.lib().b200_kv_int4_write(_ROWS.pack(
-        k.data_ptr(), v.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _native.status_word(k.device).data_ptr(),
-        _native.stream_ptr(), k.stride(0), v.stride(0), T, k_cache.shape[0] * bs, H, D, bs))
+        k.data_ptr(), v.data_ptr(), slots.data_ptr(), k_at, v_at, _native.status_word(k.device).data_ptr(),
+        _native.stream_ptr(), k.stride(0), v.stride(0), T, NB * bs, H, D, bs))
     _native.check(rc, "kv_int4_write")
     _native.count_launch()
 
@@ -126,8 +127,8 @@ def read_kv_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tens
     if _elsewhere(device):
         with torch.cuda.device(device):
             return read_kv_int4(k_cache, v_cache, slots, dim)
-    bs = _check_caches(k_cache, v_cache, dim, device)
-    n, H = slots.shape[0] if slots.dim() else 0, k_cache.shape[1]
+    NB, H, bs, k_at, v_at = _check_caches(k_cache, v_cache, dim, device)
+    n = slots.shape[0] if slots.dim() else 0
     slots = _check_slots(slots, n, device)
     if device < 0:
         return ref.read_kv_int4(k_cache, v_cache, slots, dim)
@@ -136,8 +137,8 @@ def read_kv_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tens
     if n == 0:
         return k, v
     rc = _native.lib().b200_kv_int4_read(_ROWS.pack(
-        k.data_ptr(), v.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _native.status_word(k.device).data_ptr(),
-        _native.stream_ptr(), H * dim, H * dim, n, k_cache.shape[0] * bs, H, dim, bs))
+        k.data_ptr(), v.data_ptr(), slots.data_ptr(), k_at, v_at, _native.status_word(k.device).data_ptr(),
+        _native.stream_ptr(), H * dim, H * dim, n, NB * bs, H, dim, bs))
     _native.check(rc, "kv_int4_read")
     _native.count_launch()
     return k, v
@@ -191,8 +192,7 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     if _elsewhere(device):
         with torch.cuda.device(device):
             return paged_attention_int4(q, k_cache, v_cache, meta, scale, out, causal, window)
-    bs = _check_caches(k_cache, v_cache, D, device)
-    Hkv = k_cache.shape[1]
+    NB, Hkv, bs, k_at, v_at = _check_caches(k_cache, v_cache, D, device)
     if Hkv == 0 or Hq % Hkv or Hq == 0:
         raise ValueError(f"{Hq} query heads do not share {Hkv} heads of a cache evenly")
     if not scale > 0:
@@ -205,19 +205,19 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError(f"out: {q.dtype} {tuple(q.shape)} on {q.device}, not {out.dtype} {tuple(out.shape)} on {out.device}")
     n = meta.num_reqs
     cu, lens, table = meta.query_start_loc, meta.seq_lens, meta.block_table
+    pages, strides = table.shape, table.stride()
     if not (cu.dtype is lens.dtype is table.dtype is torch.int32 and cu.get_device() == lens.get_device() == table.get_device() == device
-            and cu.dim() == lens.dim() == 1 and table.dim() == 2 and cu.shape[0] > n and lens.shape[0] >= n and table.shape[0] >= n):
-        raise ValueError(f"metadata of {n} sequences: row numbers {cu.dtype} {tuple(cu.shape)}, lengths {lens.dtype} {tuple(lens.shape)}, "
-                         f"pages {table.dtype} {tuple(table.shape)}, not int32 on device {device}")
+            and cu.stride() == lens.stride() == (1,) and len(strides) == 2 and strides[1] == 1 and cu.numel() > n and lens.numel() >= n
+            and pages[0] >= n):
+        meta = _dense(meta, device)
+        cu, lens, table = meta.query_start_loc, meta.seq_lens, meta.block_table
+        pages, strides = table.shape, table.stride()
     if device < 0 or q.dtype is not torch.bfloat16:
         if device >= 0:
-            table = _pages_in_range(cu, lens, table[:n], k_cache.shape[0], bs, window)
+            table = _pages_in_range(cu, lens, table[:n], NB, bs, window)
         return ref.paged_attention_int4(q, k_cache, v_cache, meta.query_start_loc_cpu, meta.seq_lens_cpu, table, scale, causal, window, out=out)
     if n == 0 or T == 0:
         return out
-    if not (cu.is_contiguous() and lens.is_contiguous() and table.stride()[1] == 1):         # the kernels walk them as they lie
-        meta = copy.copy(meta)
-        meta.query_start_loc, meta.seq_lens, meta.block_table = cu.contiguous(), lens.contiguous(), table.contiguous()
     given, q = out, _dense_heads(q)
     row, head, channel = out.stride()
     if channel != 1 or head != D or row % 8 or out.data_ptr() % 16:
@@ -225,7 +225,7 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         out.copy_(given)
     max_q, G = meta.max_query_len, Hq // Hkv
     window = min(window, 2 ** 31 - 1 - T)            # the first key of a window in 32 bits: positions are -T at least
-    args = (q, k_cache, v_cache, meta, scale, out, causal, window, bs)
+    args = (q, k_at, v_at, NB, Hkv, meta, pages[1], strides[0], scale, out, causal, window, bs)
     if max_q * G <= FEW_ROWS or G > 128:
         _few_rows(*args, 0, n, max_q)
     else:
@@ -237,6 +237,18 @@ def paged_attention_int4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
             else:
                 _prompts(*args, first, end, *what)
     return out if out is given else given.copy_(out)
+
+
+def _dense(meta, device: int):
+    """Metadata as the kernels walk it: row numbers and lengths without gaps, tables whose rows have none."""
+    n, cu, lens, table = meta.num_reqs, meta.query_start_loc, meta.seq_lens, meta.block_table
+    if not (cu.dtype is lens.dtype is table.dtype is torch.int32 and cu.get_device() == lens.get_device() == table.get_device() == device
+            and cu.dim() == lens.dim() == 1 and table.dim() == 2 and cu.shape[0] > n and lens.shape[0] >= n and table.shape[0] >= n):
+        raise ValueError(f"metadata of {n} sequences: row numbers {cu.dtype} {tuple(cu.shape)}, lengths {lens.dtype} {tuple(lens.shape)}, "
+                         f"pages {table.dtype} {tuple(table.shape)}, not int32 on device {device}")
+    meta = copy.copy(meta)
+    meta.query_start_loc, meta.seq_lens, meta.block_table = cu.contiguous(), lens.contiguous(), table.contiguous()
+    return meta
 
 
 def _pages_in_range(cu, lens, table, blocks: int, bs: int, window: int) -> torch.Tensor:
@@ -305,16 +317,15 @@ def _plan(cu: bytes, cu_type: str, lens: bytes, lens_type: str, n: int, window: 
     return tuple(plan)
 
 
-def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, end, max_q) -> None:
+def _few_rows(q, k_at, v_at, NB, Hkv, meta, columns, pitch, scale, out, causal, window, bs, first, end, max_q) -> None:
     """Sequences ``first`` to ``end``, none with more than ``max_q`` new tokens."""
     T, Hq, D = q.shape
     n = end - first
-    NB, Hkv, _ = k_cache.shape
     rows = max_q * (Hq // Hkv)
     blocks = n * Hkv * (1 if rows <= 8 else -(-rows // 16))
     # a captured graph is replayed with other lengths, up to what the table holds
     capturing = torch.cuda.is_current_stream_capturing()
-    longest, at_once = meta.block_table.shape[1] * bs if capturing else meta.max_seq_len, (3 if rows <= 8 else 2) * _native.sm_count(q.get_device())
+    longest, at_once = columns * bs if capturing else meta.max_seq_len, (3 if rows <= 8 else 2) * _native.sm_count(q.get_device())
     if window:
         longest = min(longest, window + max_q)
     if 2 * blocks <= at_once or longest < 2048 or capturing or fixed_sums():
@@ -327,9 +338,9 @@ def _few_rows(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, 
     scratch = _results(q, ahead, parts) if parts > CLUSTER else None
     cu, lens, table = _of(meta, first)
     rc = _native.lib().b200_attn_int4(_ATTENTION.pack(
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cu.data_ptr(), lens.data_ptr(), table.data_ptr(), out.data_ptr(),
+        q.data_ptr(), k_at, v_at, cu.data_ptr(), lens.data_ptr(), table.data_ptr(), out.data_ptr(),
         0 if scratch is None else scratch.data_ptr(), _native.status_word(q.device).data_ptr(), _native.stream_ptr(), q.stride(0), ahead, NB,
-        out.stride(0), 0, table.stride(0), scale, bs, table.shape[1], n, max_q, Hq, Hkv, D, int(causal), window, parts))
+        out.stride(0), 0, pitch, scale, bs, columns, n, max_q, Hq, Hkv, D, int(causal), window, parts))
     _native.check(rc, "attn_int4")
     _native.count_launch(1 + int(parts > CLUSTER))
 
@@ -369,10 +380,9 @@ def _prompt_parts(blocks: int, max_len: int, tokens: int, heads: int, D: int, sm
     return min(range(1, max(1, min(max_len // 512, 16)) + 1), key=us)
 
 
-def _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, end, tokens, pairs) -> None:
+def _prompts(q, k_at, v_at, NB, Hkv, meta, columns, pitch, scale, out, causal, window, bs, first, end, tokens, pairs) -> None:
     """Sequences ``first`` to ``end`` with so many new tokens and pairs of query tiles."""
     T, Hq, D = q.shape
-    NB, Hkv, _ = k_cache.shape
     longest = min(meta.max_seq_len, window + meta.max_query_len) if window else meta.max_seq_len
     parts = 1 if fixed_sums() else _prompt_parts(pairs * Hkv, longest, tokens, Hq, D, _native.sm_count(q.get_device()))
     if parts > 1 and parts > _most_parts(T, Hq, D):
@@ -380,8 +390,8 @@ def _prompts(q, k_cache, v_cache, meta, scale, out, causal, window, bs, first, e
     scratch = _results(q, T, parts) if parts > 1 else None
     cu, lens, table = _of(meta, first)
     rc = _native.lib().b200_attn_int4_prefill(_ATTENTION.pack(
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cu.data_ptr(), lens.data_ptr(), table.data_ptr(), out.data_ptr(),
+        q.data_ptr(), k_at, v_at, cu.data_ptr(), lens.data_ptr(), table.data_ptr(), out.data_ptr(),
         0 if scratch is None else scratch.data_ptr(), _native.status_word(q.device).data_ptr(), _native.stream_ptr(), q.stride(0), T, NB,
-        out.stride(0), tokens, table.stride(0), scale, bs, table.shape[1], end - first, 0, Hq, Hkv, D, int(causal), window, parts))
+        out.stride(0), tokens, pitch, scale, bs, columns, end - first, 0, Hq, Hkv, D, int(causal), window, parts))
     _native.check(rc, "attn_int4_prefill")
     _native.count_launch(1 + int(parts > 1))
