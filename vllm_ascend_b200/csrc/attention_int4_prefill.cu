@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) attn_int4_prefill_kernel(const 
               mx[q] = fmaxf(mx[q], fmaxf(__uint_as_float(sr[i + 2 * q]), __uint_as_float(sr[i + 2 * q + 1])));
         }
         const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        // O is rescaled only when the running maximum moved by more than 2^8 (powers of two: exact)
+        // O is rescaled only where a score outgrew the maximum by more than a factor of 2^8: no probability then overflows bf16
         float alpha = 1.f;
         bool need = false;
         if (mt > m && (m == -INFINITY || (mt - m) * sl2 > 8.f)) {

@@ -282,7 +282,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           for (int q = 0; q < 4; q++)
             mx[q] = fmaxf(mx[q], fmaxf(__uint_as_float(sreg[i + 2 * q]), __uint_as_float(sreg[i + 2 * q + 1])));
         const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        // O is rescaled only when the running maximum moved by more than a threshold (powers of two: exact)
+        // O is rescaled only when the running maximum moved by more than a threshold
         float alpha = 1.f;
         bool need = false;
         if (mt > m && (m == -INFINITY || (mt - m) * sl2 > p.rescale_threshold)) {
