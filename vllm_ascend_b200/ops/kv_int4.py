@@ -155,8 +155,8 @@ def _parts(blocks: int, max_len: int, at_once: int, known: bool) -> int:
     """Parts that every sequence's keys are split into, by the blocks without a split and those that run at once.  Clusters of more than eight
     find room where there are few, and pay for long sequences; more parts than a cluster's join in a second kernel, 6 us more.  32 heads on 8,
     one sequence of 1337 tokens 6.2 us in 8 parts, 7.2 in 16, 12 in 18; of 12000 13.4, 11.8, 15.9; of 40000 31, 25, 24; four of 8000 15 in 8,
-    19.5 in 12.  64 on 8, three of 60000 76 in 8, 61 in 14, 58 in 18, the most that was tried; all with heads of 128.  In a graph (lengths not ``known``) ``max_len`` is what the table holds;
-    a quarter of it counts."""
+    19.5 in 12.  64 on 8, three of 60000 76 in 8, 61 in 14, 58 in 18, the most that was tried; all with heads of 128.  In a graph (lengths not
+    ``known``) ``max_len`` is what the table holds; a quarter of it counts."""
     if fixed_sums():
         return 1
     most, wide = min(at_once // max(1, blocks), -(-max_len // 128), 18), 16 if blocks <= 8 else 14
