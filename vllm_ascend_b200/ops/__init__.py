@@ -983,3 +983,6 @@ def rms_norm_gated(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, eps: 
 
 # ---------------------------------------------------------------- 4-bit cache
 from .kv_int4 import alloc_kv_cache_int4, paged_attention_int4, read_kv_int4, write_kv_int4  # noqa: E402,F401
+
+# ---------------------------------------------------------------- beam search
+from .beam import BeamStates, beam_select, beam_states, reorder_beams  # noqa: E402,F401

@@ -533,3 +533,40 @@ def rms_norm_gated(x: torch.Tensor, z: torch.Tensor, w: torch.Tensor, eps: float
     if norm_before_gate:
         y = y * gate
     return y.reshape(x.shape).to(x.dtype)
+
+
+# ---------------------------------------------------------------- beam search
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """logits [groups * beams, vocab], scores [groups, beams] -> the k best totals of each group, their beams and tokens."""
+    (groups, width), vocab = scores.shape, logits.shape[1]
+    x = logits.double()
+    x = x - torch.logsumexp(x, -1, keepdim=True)                # NaN where a row has no distribution
+    total = torch.nan_to_num(scores.double().reshape(-1, 1) + x, nan=-torch.inf, posinf=-torch.inf, neginf=-torch.inf)
+    best, at = torch.sort(total.reshape(groups, width * vocab), dim=-1, descending=True, stable=True)
+    best, at = best[:, :k], at[:, :k]
+    return best.float(), (at // vocab).to(torch.int32), at % vocab
+
+
+def reorder_beams(tensors, rows: torch.Tensor, parents: torch.Tensor, lengths: Optional[torch.Tensor] = None, int4_dim: int = 0) -> None:
+    """Rows (or the first ``lengths`` tokens of pages) of every tensor, in place; rows and parents out of range raise."""
+    source, dest, tokens = [], [], []
+    for g, (mine, follows) in enumerate(zip(rows.tolist(), parents.tolist())):
+        for w, p in enumerate(follows):
+            if not -1 <= p < len(mine) or mine[w] < -1 or p >= 0 and mine[w] >= 0 and mine[p] < 0:
+                raise IndexError(f"group {g}: beam {w} in row {mine[w]} follows beam {p} of {len(mine)}")
+            if p >= 0 and mine[w] >= 0 and p != w:
+                source.append(mine[p])
+                dest.append(mine[w])
+                tokens.append(-1 if lengths is None else max(0, int(lengths[g])))
+    for t in tensors:
+        if any(r >= t.shape[0] for r in source + dest):
+            raise IndexError(f"a row above {t.shape[0]}")
+        old = t[torch.tensor(source, dtype=torch.int64)] if source else None
+        for i, (r, n) in enumerate(zip(dest, tokens)):
+            if n < 0:
+                t[r] = old[i]
+            elif t.dtype == torch.uint8:
+                n = (n + KV_INT4_TOKENS - 1) // KV_INT4_TOKENS * 9 * int4_dim
+                t[r, :, :n] = old[i, :, :n]
+            else:
+                t[r, :n] = old[i, :n]
