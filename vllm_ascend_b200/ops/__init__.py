@@ -986,3 +986,4 @@ from .kv_int4 import alloc_kv_cache_int4, paged_attention_int4, read_kv_int4, wr
 
 # ---------------------------------------------------------------- beam search
 from .beam import BeamStates, beam_select, beam_states, reorder_beams  # noqa: E402,F401
+from .shared_prefix import SharedPrefixPlan, paged_attention_shared, plan_shared_prefix  # noqa: E402,F401

@@ -570,3 +570,31 @@ def reorder_beams(tensors, rows: torch.Tensor, parents: torch.Tensor, lengths: O
                 t[r, :, :n] = old[i, :, :n]
             else:
                 t[r, :n] = old[i, :n]
+
+
+def paged_attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, query_start_loc, seq_lens, block_table: torch.Tensor,
+                           group_starts, prefix_lens, scale: float, out: torch.Tensor) -> torch.Tensor:
+    """Causal attention where the first ``prefix_lens[g]`` keys of the sequences of group g are read through its first sequence's pages."""
+    cu, lens = [int(x) for x in query_start_loc], [int(x) for x in seq_lens]
+    n, bs = len(lens), k_cache.shape[1]
+    if any(not 0 <= a <= b <= n for a, b in zip(group_starts, group_starts[1:])):
+        raise IndexError(f"group starts {group_starts} of {n} sequences")
+    first, prefix = list(range(n)), [0] * n
+    for a, b, p in zip(group_starts, group_starts[1:], prefix_lens):
+        p = max(0, min([p] + [max(0, lens[s] - (cu[s + 1] - cu[s])) for s in range(a, b) if cu[s + 1] > cu[s]]))
+        for s in range(a, b):
+            first[s], prefix[s] = a, p
+    G = q.shape[1] // k_cache.shape[2]
+    for s in range(n):
+        new = cu[s + 1] - cu[s]
+        if new <= 0:
+            continue
+        pos = torch.arange(max(lens[s], 0), device=q.device)
+        page = torch.where(pos < prefix[s], block_table[first[s]][pos // bs], block_table[s][pos // bs]).long()
+        k, v = (t[page, pos % bs].float().repeat_interleave(G, 1) for t in (k_cache, v_cache))
+        score = torch.einsum("qhd,khd->hqk", q[cu[s]:cu[s + 1]].float(), k) * scale
+        hidden = pos[None] > torch.arange(lens[s] - new, lens[s], device=q.device)[:, None]
+        score = score.masked_fill(hidden, -torch.inf)
+        p = torch.where(hidden.all(-1)[None, :, None], 0.0, torch.softmax(score, -1))
+        out[cu[s]:cu[s + 1]] = torch.einsum("hqk,khd->qhd", p, v).to(out.dtype)
+    return out
