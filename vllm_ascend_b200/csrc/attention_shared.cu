@@ -13,9 +13,9 @@
 // of the base tells pieces apart.  A last kernel joins them.
 //
 //   warps 0..3, 4..7   softmax, one thread a query row; step s of a block belongs to group s mod 2
-//   warp 8             TMA producer;  warp 9  MMA issuer
+//   warps 8, 10        TMA producers of queries and keys, of values;  warp 9  MMA issuer
 // Up to 128 rows (a group's beams, a sequence's own keys): the groups of warps take tiles of 128 keys in turn, each with scores and an
-// output of its own (S0, S1, O0, O1 fill tensor memory), joined at the end of the piece.  128 x 128 scores take a group
+// output of its own (S0, S1, O0, O1 fill tensor memory) and results of its own.  128 x 128 scores take a group
 // about 1.5 us, 64 KB of keys and values an SM's share of HBM 1.47: two groups keep the stream going.  Above 128 rows both groups work on
 // every tile, each with 128 rows of its own.  Probabilities replace scores in tensor memory; warps whose 32 rows are empty skip them.
 // Rows of V that no key of the range stands for are zeroed in shared memory where a product would read them (their
@@ -29,7 +29,7 @@
 
 namespace b200 {
 
-constexpr int SH_THREADS = 320;
+constexpr int SH_THREADS = 352;
 constexpr int SH_HALF = 128 * 128;           // 128 rows x 64 bf16
 constexpr int SH_ROWS = 256;                 // query rows of a base at most
 
@@ -39,14 +39,20 @@ struct SharedBase {
   int key_lo, key_hi;          // keys of the range
   int q_pos0;                  // position of token tok0 among them (behind key_hi: all see all)
   int tiles;                   // tiles of 128 keys, tile 0 at key_lo rounded down
+  int weight;                  // units of a tile
   int cum;                     // units of cost in front of it
   int part_row;                // first row of its partial results
   int seg0;                    // block of its first tile
-  int pad[2];
+  int pad;
 };
 
-// plan: [0] units of cost, [1] bases, then block_first[blocks], tok_prefix[tokens], tok_own[tokens] (base of a token, -1 no keys, -2 no
-// sequence), group_ctx[groups], bases
+// What a tile of 128 keys and the begin and end of a piece cost, in units of half a tile.  A tile for two query tiles takes the softmax of twice the
+// rows on the same schedulers.
+constexpr int COST_TILE = 2, COST_PAIR = 3, COST_PIECE = 2;
+
+// plan: [0] units of cost, [1] bases, [2] blocks with work, then block_first[blocks] and block_unit[blocks + 1] (base and unit that a block begins
+// with), tok_prefix[tokens], tok_own[tokens] (base of a token, -1 no keys, -2 no sequence), group_ctx[groups], bases, and for every base and
+// head the first row and the number of its partial results
 struct PlanArgs {
   const int* cu;               // [seqs + 1] first query row of each sequence
   const int* seq_lens;
@@ -58,7 +64,11 @@ struct PlanArgs {
   int seqs, groups, tokens, G, Hkv, blocks, max_bases, bases_at;       // bases_at: ints in front of the bases
 };
 
-__device__ __forceinline__ int plan_group_ctx(const PlanArgs& a) { return 2 + a.blocks + 2 * a.tokens; }
+constexpr int PLAN_HEAD = 3;
+__host__ __device__ __forceinline__ int plan_tokens_at(int blocks) { return PLAN_HEAD + 2 * blocks + 1; }
+__host__ __device__ __forceinline__ int plan_heads_at(int bases_at, int max_bases) {
+  return bases_at + max_bases * (int)(sizeof(SharedBase) / 4);
+}
 
 // block that unit y of n falls to, and the first unit of block b
 __device__ __forceinline__ int block_of(long y, long n, long blocks) { return (int)(((y + 1) * blocks + n - 1) / n - 1); }
@@ -92,11 +102,13 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   __shared__ int bad;
   const int tid = threadIdx.x;
   int* head = a.plan;
-  int* block_first = head + 2;
-  int* tok_prefix = block_first + a.blocks;
+  int* block_first = head + PLAN_HEAD;
+  int* block_unit = block_first + a.blocks;
+  int* tok_prefix = head + plan_tokens_at(a.blocks);
   int* tok_own = tok_prefix + a.tokens;
-  int* group_ctx = head + plan_group_ctx(a);
+  int* group_ctx = tok_own + a.tokens;
   SharedBase* bases = reinterpret_cast<SharedBase*>(head + a.bases_at);
+  int2* heads = reinterpret_cast<int2*>(head + plan_heads_at(a.bases_at, a.max_bases));
   if (tid == 0) bad = 0;
   __syncthreads();
   for (int t = tid; t < a.tokens; t += 1024) tok_prefix[t] = -1, tok_own[t] = -2;
@@ -110,7 +122,7 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   __syncthreads();
   if (bad) {
     if (tid == 0) {
-      head[0] = head[1] = 0;
+      head[0] = head[1] = head[2] = 0;
       if (a.status) atomicExch(a.status, B200_BAD_INDEX);
     }
     return;
@@ -166,7 +178,8 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
       b.q_pos0 = group ? ctx : ctx + i * per;
       b.key_hi = group ? hi : min(hi, b.q_pos0 + b.ntok);
       b.tiles = b.key_hi > lo ? ((b.key_hi + 127) >> 7) - (lo >> 7) : 0;
-      b.cum = b.part_row = b.seg0 = b.pad[0] = b.pad[1] = 0;
+      b.weight = b.ntok > per / 2 ? COST_PAIR : COST_TILE;
+      b.cum = b.part_row = b.seg0 = b.pad = 0;
       bases[at] = b;
       int* to = group ? tok_prefix : tok_own;
       for (int t = 0; t < b.ntok; t++) to[b.tok0 + t] = b.tiles > 0 ? at : -1;
@@ -179,29 +192,44 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
     const int i = i0 + tid;
     const int tiles = i < count ? bases[i].tiles : 0;
     int all;
-    const int before = units + block_scan(tiles > 0 ? a.Hkv * (tiles + 1) : 0, part, all);
+    const int before = units + block_scan(tiles > 0 ? a.Hkv * (tiles * bases[i].weight + COST_PIECE) : 0, part, all);
     if (i < count) bases[i].cum = before;
     units += all;
   }
-  // blocks and partial rows of every base; every block has a unit, so the blocks that share a head's tiles leave rows without a gap
-  const int blocks = min(a.blocks, units);
+  // Blocks and partial rows of every base.  A block has as many units as a tile at least, so those from the one of a head's first tile to the one
+  // of its last all have tiles of it, and their rows leave no gap.
+  const int blocks = min(a.blocks, units / COST_PAIR);
   int rows = 0;
   for (int i0 = 0; i0 < count; i0 += 1024) {
     const int i = i0 + tid;
     int need = 0, first = 0, tiles = 0;
     if (i < count && (tiles = bases[i].tiles) > 0) {
-      const long cum = bases[i].cum, cost = (long)a.Hkv * (tiles + 1);
-      first = block_of(cum + 1, units, blocks);
-      const int last = block_of(cum + cost - 1, units, blocks);
-      need = bases[i].ntok * a.G * (a.Hkv + last - first);
-      for (int b = cum > 0 ? block_of(cum - 1, units, blocks) + 1 : 0; b <= last; b++) block_first[b] = i;
+      const SharedBase b = bases[i];
+      const long cum = b.cum, head_cost = (long)tiles * b.weight + COST_PIECE, cost = a.Hkv * head_cost;
+      first = block_of(cum + COST_PIECE, units, blocks);
+      const int last = block_of(cum + cost - b.weight, units, blocks);
+      // up to 128 rows, each group of warps leaves results of its own
+      need = b.ntok * a.G * (a.Hkv + last - first) * (b.weight == COST_PAIR ? 1 : 2);
+      const int end = block_of(cum + cost - 1, units, blocks);
+      for (int c = cum > 0 ? block_of(cum - 1, units, blocks) + 1 : 0; c <= end; c++) block_first[c] = i;
     }
     int all;
     const int before = rows + block_scan(need, part, all);
     if (i < count) bases[i].part_row = before, bases[i].seg0 = first;
     rows += all;
   }
-  if (tid == 0) head[0] = units, head[1] = count;
+  for (int c = tid; c <= blocks; c += 1024) block_unit[c] = blocks > 0 ? first_unit(c, units, blocks) : 0;
+  __syncthreads();
+  for (int j = tid; j < count * a.Hkv; j += 1024) {
+    const int i = j / a.Hkv, h = j - i * a.Hkv;
+    const SharedBase b = bases[i];
+    if (b.tiles <= 0) continue;
+    const long at = b.cum + (long)h * (b.tiles * b.weight + COST_PIECE) + COST_PIECE;       // unit of the first tile
+    const int b0 = block_of(at, units, blocks), b1 = block_of(at + (b.tiles - 1) * b.weight, units, blocks);
+    const int slots = b.weight == COST_PAIR ? 1 : 2;
+    heads[j] = make_int2(b.part_row + (h + b0 - b.seg0) * slots * b.ntok * a.G, (b1 - b0 + 1) * slots);
+  }
+  if (tid == 0) head[0] = units, head[1] = count, head[2] = blocks;
 }
 
 // ---------------------------------------------------------------- attention
@@ -209,9 +237,9 @@ struct SharedParams {
   const int* plan;
   const int* block_table;
   long pitch;                  // ints between rows of the table
-  int max_blocks, block_size, rows_per_load, piece;
+  int max_blocks, block_size, page_shift, rows_per_load, piece;        // page_shift: log2 of the block size, -1: no power of two
   int G, Hkv, Hq, tpt;         // tpt: tokens of a tile of 128 rows
-  int blocks, tokens, bases_at;
+  int blocks, tokens, bases_at, heads_at;
   float scale_log2;
   float* part_o;               // [partial rows, D]
   float2* part_ml;             // [partial rows] maximum (log2, scaled) and sum
@@ -227,7 +255,7 @@ struct SharedCfg {
   static constexpr int TILE = NH * SH_HALF;              // bytes of 128 rows
   static constexpr int NK = D == 128 ? 2 : 3;
   static constexpr int NV = D == 128 ? 3 : 5;
-  static constexpr int SMEM = (2 + NK + NV) * TILE + 1024 + 1024 + 512;
+  static constexpr int SMEM = (2 + NK + NV) * TILE + 1024 + 512;
 };
 
 __device__ __forceinline__ float sh_exp2(float x) {
@@ -246,31 +274,31 @@ struct Pieces {
     const int4* p = reinterpret_cast<const int4*>(bases + i);
     const int4 u = __ldg(p), v = __ldg(p + 1), w = __ldg(p + 2);
     b.tok0 = u.x; b.ntok = u.y; b.table_row = u.z; b.key_lo = u.w;
-    b.key_hi = v.x; b.q_pos0 = v.y; b.tiles = v.z; b.cum = v.w;
-    b.part_row = w.x; b.seg0 = w.y;
+    b.key_hi = v.x; b.q_pos0 = v.y; b.tiles = v.z; b.weight = v.w;
+    b.cum = w.x; b.part_row = w.y; b.seg0 = w.z;
   }
   __device__ __forceinline__ bool start(const SharedParams& p) {
-    const int units = __ldg(p.plan);
+    const int* at = p.plan + PLAN_HEAD + blockIdx.x;
+    const int blocks = __ldg(p.plan + 2);
+    i = __ldg(at);
+    x0 = __ldg(at + p.blocks);
+    x1 = __ldg(at + p.blocks + 1);
     count = __ldg(p.plan + 1);
     bases = reinterpret_cast<const SharedBase*>(p.plan + p.bases_at);
     Hkv = p.Hkv;
-    const int blocks = min(p.blocks, units);
     if ((int)blockIdx.x >= blocks) return false;
-    x0 = first_unit(blockIdx.x, units, blocks);
-    x1 = first_unit(blockIdx.x + 1, units, blocks);
-    i = __ldg(p.plan + 2 + blockIdx.x);
     load();
-    h = (x0 - b.cum) / (b.tiles + 1);
+    h = (x0 - b.cum) / (b.tiles * b.weight + COST_PIECE);
     return settle();
   }
-  // to the first piece from (i, h) on that has tiles in this block
+  // to the first piece from (i, h) on that has tiles in this block: a tile belongs to the block of its first unit
   __device__ __forceinline__ bool settle() {
     while (true) {
-      const int at = b.cum + h * (b.tiles + 1) + 1;       // unit of tile 0
       if (b.tiles > 0) {
+        const int at = b.cum + h * (b.tiles * b.weight + COST_PIECE) + COST_PIECE;       // unit of tile 0
         if (at >= x1) return false;
-        t0 = max(0, x0 - at);
-        t1 = min(b.tiles, x1 - at);
+        t0 = x0 > at ? (x0 - at + b.weight - 1) / b.weight : 0;
+        t1 = min(b.tiles, (x1 - at + b.weight - 1) / b.weight);
         if (t1 > t0) return true;
       }
       if (!step()) return false;
@@ -318,8 +346,8 @@ struct Tiles {
 
 template <int D>
 __global__ void __launch_bounds__(SH_THREADS, 1)
-attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_q4,
-                   const __grid_constant__ CUtensorMap tmap_q1, const __grid_constant__ CUtensorMap tmap_k,
+attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_q64,
+                   const __grid_constant__ CUtensorMap tmap_q4, const __grid_constant__ CUtensorMap tmap_q1, const __grid_constant__ CUtensorMap tmap_k,
                    const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_kp,
                    const __grid_constant__ CUtensorMap tmap_vp, const SharedParams p) {
   using Cfg = SharedCfg<D>;
@@ -331,8 +359,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   uint8_t* Qs = smem;
   uint8_t* Ks = Qs + 2 * TILE;
   uint8_t* Vs = Ks + NK * TILE;
-  float2* ml = (float2*)(Vs + NV * TILE);          // [128] of the group of warps that does not finish a piece
-  uint64_t* q_full = (uint64_t*)(ml + 128);        // 2
+  uint64_t* q_full = (uint64_t*)(Vs + NV * TILE);  // 2
   uint64_t* q_empty = q_full + 2;                  // 2
   uint64_t* k_full = q_empty + 2;                  // NK
   uint64_t* k_empty = k_full + NK;
@@ -342,9 +369,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   uint64_t* p_full = s_full + 2;                   // 2: its probabilities
   uint64_t* o_full = p_full + 2;                   // 2: its last product of a piece
   uint64_t* o_free = o_full + 2;                   // 2: its output has been read
-  uint64_t* ml_full = o_free + 2;
-  uint64_t* ml_empty = ml_full + 1;
-  uint32_t* tmem_ptr = (uint32_t*)(ml_empty + 1);
+  int* pages = (int*)(o_free + 2);                 // 16 of each producer
+  uint32_t* tmem_ptr = (uint32_t*)(pages + 32);
   volatile int* abort_word = (volatile int*)(tmem_ptr + 1);
   if (threadIdx.x == 0) {
     for (int b = 0; b < 2; b++) {
@@ -363,8 +389,6 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       mbar_init(&v_full[b], 1);
       mbar_init(&v_empty[b], 1);
     }
-    mbar_init(ml_full, 4);
-    mbar_init(ml_empty, 4);
     *abort_word = 0;
     mbar_fence_init();
   }
@@ -382,76 +406,77 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   tc_fence_after();
   const uint32_t tmem_base = warp_uniform(*tmem_ptr);
 
-  if (warp == 8) {
-    // ------------------------------------------------------------ producer: K0 K1 V0 K2 V1 K3 ..., queries in front of a piece's first keys
-    const int rpl = p.rows_per_load, parts = 128 / rpl, piece = p.piece;
-    Tiles ck, cv;
-    ck.start(p);
-    cv.start(p);
-    // lane i: page of part i of a tile; parts outside of the range take the nearest page inside
-    auto load_blk = [&](const Tiles& c) -> int {
-      if (!c.more || lane >= parts) return 0;
-      const int key = min(max(c.base() + lane * rpl, c.p.b.key_lo), c.p.b.key_hi - 1), col = key / p.block_size;
-      return col < p.max_blocks ? __ldg(p.block_table + (long)c.p.b.table_row * p.pitch + col) : -1;
-    };
-    auto load_tile = [&](const Tiles& c, int blk_mine, uint8_t* dst, uint64_t* fullb, const CUtensorMap* whole, const CUtensorMap* pieces) -> bool {
-      const bool bad = __any_sync(0xffffffffu, lane < parts && (blk_mine < 0 || blk_mine >= p.num_blocks_total));
-      if (bad) {
-        *abort_word = B200_BAD_INDEX;
-        return false;
-      }
-      const int base = c.base(), lo = c.c_lo(), hi = c.c_hi();
-      const bool full = lo == 0 && hi == 128;
-      const int rows = full ? rpl : piece, first = full ? 0 : lo / rows, end = full ? parts : (hi + rows - 1) / rows;
-      if (elect_one()) mbar_expect_tx(fullb, (uint32_t)((end - first) * rows * 128 * NH));
-      __syncwarp();
-      for (int i = first; i < end; i++) {
-        const int blk = __shfl_sync(0xffffffffu, blk_mine, i * rows / rpl);
-        const int off = (base + i * rows) % p.block_size;
-        if (elect_one())
-#pragma unroll
-          for (int hf = 0; hf < NH; hf++)
-            tma_load_4d(dst + hf * SH_HALF + i * rows * 128, full ? whole : pieces, fullb, hf * 64, c.p.h, off, blk);
-        __syncwarp();
-      }
-      return true;
-    };
-    auto load_k = [&](int blk) -> bool {
-      const uint32_t st = ck.gt % NK;
-      if (ck.t == ck.p.t0) {
-        for (int s = 0; s < ck.nsel; s++) {
-          const uint32_t q = ck.qc + s, b = q & 1;
-          if (!mbar_wait(&q_empty[b], ((q >> 1) & 1u) ^ 1u, abort_word)) return false;
-          const int tok = ck.p.b.tok0 + s * p.tpt, n = min(p.tpt, ck.p.b.ntok - s * p.tpt);
-          const int box = n <= 1 ? 1 : (n <= 4 && p.tpt > 4 ? 4 : p.tpt);
-          const CUtensorMap* tm = box == p.tpt ? &tmap_q : (box == 1 ? &tmap_q1 : &tmap_q4);
-          if (elect_one()) {
-            mbar_expect_tx(&q_full[b], (uint32_t)(box * p.G * 128 * NH));
-#pragma unroll
-            for (int hf = 0; hf < NH; hf++) tma_load_4d(Qs + b * TILE + hf * SH_HALF, tm, &q_full[b], hf * 64, 0, ck.p.h, tok);
-          }
-          __syncwarp();
+  if (warp == 8 || warp == 10) {
+    // ------------------------------------------------------------ producers: warp 8 queries and keys, warp 10 values; one thread of each walks the
+    // loop (see warp_uniform).  One for both took 1.3 us a tile, about what the bytes take.
+    if (elect_one()) {
+      const bool values = warp == 10;
+      const int rpl = p.rows_per_load, parts = 128 / rpl, depth = values ? NV : NK;
+      const CUtensorMap* whole = values ? &tmap_v : &tmap_k;
+      const CUtensorMap* pieces = values ? &tmap_vp : &tmap_kp;
+      uint8_t* stages = values ? Vs : Ks;
+      uint64_t* full_bars = values ? v_full : k_full;
+      uint64_t* empty_bars = values ? v_empty : k_empty;
+      Tiles c;
+      c.start(p);
+      // Pages of a tile's parts go to shared memory while the tile in front is waited for; parts outside of the range take the nearest page inside.
+      // Loops stay rolled: what all roles execute a tile has to stay in the instruction caches (60000 keys: 54 us a block unrolled, 45 rolled).
+      int* my_pages = pages + (values ? 16 : 0);
+      auto fetch_pages = [&]() {
+        const int* row = p.block_table + (long)c.p.b.table_row * p.pitch;
+        int key = c.base();
+#pragma unroll 1
+        for (int i = 0; i < parts; i++, key += rpl) {
+          const int near = min(max(key, c.p.b.key_lo), c.p.b.key_hi - 1);
+          const int col = p.page_shift >= 0 ? near >> p.page_shift : near / p.block_size;
+          if (col < p.max_blocks) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(my_pages + i)), "l"(row + col) : "memory");
+          else my_pages[i] = -1;
         }
-      }
-      if (!mbar_wait(&k_empty[st], ((ck.gt / NK) & 1u) ^ 1u, abort_word)) return false;
-      return load_tile(ck, blk, Ks + st * TILE, &k_full[st], &tmap_k, &tmap_kp);
-    };
-    int blk = load_blk(ck);
-    for (int i = 0; i < 2 && ck.more; i++) {
-      if (!load_k(blk)) goto done;
-      ck.next(p);
-      blk = load_blk(ck);
-    }
-    while (cv.more) {
-      const uint32_t st = cv.gt % NV;
-      const int blk_v = load_blk(cv);
-      if (!mbar_wait(&v_empty[st], ((cv.gt / NV) & 1u) ^ 1u, abort_word)) goto done;
-      if (!load_tile(cv, blk_v, Vs + st * TILE, &v_full[st], &tmap_v, &tmap_vp)) goto done;
-      cv.next(p);
-      if (ck.more) {
-        if (!load_k(blk)) goto done;
-        ck.next(p);
-        blk = load_blk(ck);
+      };
+      if (c.more) fetch_pages();
+      uint32_t st = 0, ph = 1;
+      while (c.more) {
+        if (!values && c.t == c.p.t0) {
+          const bool twice = c.p.b.ntok * p.G <= 64;       // the second group of warps finds the rows 64 further on
+#pragma unroll 1
+          for (int s = 0; s < c.nsel; s++) {
+            const uint32_t q = c.qc + s, b = q & 1;
+            if (!mbar_wait(&q_empty[b], ((q >> 1) & 1u) ^ 1u, abort_word)) goto done;
+            const int tok = c.p.b.tok0 + s * p.tpt, n = min(p.tpt, c.p.b.ntok - s * p.tpt);
+            int box = p.tpt;                     // tokens of the copy
+            const CUtensorMap* tm = &tmap_q;
+            if (n == 1) box = 1, tm = &tmap_q1;
+            else if (n <= 4 && p.G <= 16) box = 4, tm = &tmap_q4;
+            else if (twice) box = 64 / p.G, tm = &tmap_q64;
+            mbar_expect_tx(&q_full[b], (uint32_t)(box * p.G * 128 * NH * (twice ? 2 : 1)));
+#pragma unroll 1
+            for (int i = 0; i < (twice ? 2 : 1); i++)
+#pragma unroll
+              for (int hf = 0; hf < NH; hf++)
+                tma_load_4d(Qs + b * TILE + hf * SH_HALF + i * 64 * 128, tm, &q_full[b], hf * 64, 0, c.p.h, tok);
+          }
+        }
+        if (!mbar_wait(&empty_bars[st], ph, abort_word)) goto done;
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        const int base = c.base(), lo = c.c_lo(), hi = c.c_hi();
+        const bool full = lo == 0 && hi == 128;
+        const int rows = full ? rpl : p.piece, end = (hi + rows - 1) / rows;
+        const CUtensorMap* tm = full ? whole : pieces;
+        uint8_t* dst = stages + st * TILE;
+        mbar_expect_tx(&full_bars[st], (uint32_t)((end - lo / rows) * rows * 128 * NH));
+#pragma unroll 1
+        for (int i = lo / rows; i < end; i++) {
+          const int page = my_pages[i * rows / rpl], off = p.page_shift >= 0 ? (base + i * rows) & (p.block_size - 1) : (base + i * rows) % p.block_size;
+          if (page < 0 || page >= p.num_blocks_total) {
+            *abort_word = B200_BAD_INDEX;
+            goto done;
+          }
+#pragma unroll
+          for (int hf = 0; hf < NH; hf++) tma_load_4d(dst + hf * SH_HALF + i * rows * 128, tm, &full_bars[st], hf * 64, c.p.h, off, page);
+        }
+        if (++st == (uint32_t)depth) st = 0, ph ^= 1u;
+        c.next(p);
+        if (c.more) fetch_pages();
       }
     }
   } else if (warp == 9) {
@@ -518,23 +543,24 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   } else {
     // ------------------------------------------------------------ softmax and results, group of warps w
     const uint32_t w = warp >> 2;
-    const int row = (warp & 3) * 32 + lane, G = p.G;
-    const int tok = row / G;
+    const int lane_row = (warp & 3) * 32 + lane, G = p.G;
     const uint32_t t_lane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t t_s = t_lane + w * 128, t_o = t_lane + O_COL;
     const float sl2 = p.scale_log2;
     constexpr float kRescale = 8.f;              // log2 by which the reference maximum may lag behind
     Pieces c;
     bool more = c.start(p);
-    uint32_t s0 = 0, gt0 = 0, oc[2] = {0, 0}, mc = 0;
+    uint32_t s0 = 0, gt0 = 0, oc = 0;            // steps, tiles and pieces of mine in front
     while (more) {
       const int n = c.t1 - c.t0, nsel = c.b.ntok > p.tpt ? 2 : 1;
       const uint32_t off = (w ^ s0) & 1u;        // my first step of the piece
       const int first = nsel == 2 ? 0 : (int)off, turn = nsel == 2 ? 1 : 2;
       const int tok_first = nsel == 2 && off ? p.tpt : 0;
-      const int nt = min(p.tpt, c.b.ntok - tok_first);
-      const bool row_valid = tok < nt && tok < p.tpt;
-      const bool warp_valid = (warp & 3) * 32 < nt * G;
+      const int nt = min(p.tpt, c.b.ntok - tok_first), rows = nt * G;
+      // up to 64 rows: the second group's are 64 lanes further on, so that all four schedulers have a warp with rows
+      const int shift = nsel == 1 && rows <= 64 && w == 1 ? 64 : 0, row = lane_row - shift, tok = row / G;
+      const bool row_valid = row >= 0 && row < rows;
+      const bool warp_valid = (warp & 3) * 32 >= shift && (warp & 3) * 32 - shift < rows;
       const int q_pos = c.b.q_pos0 + tok_first + tok;
       const int k_hi = min(c.b.key_hi, q_pos + 1), all_hi = min(c.b.key_hi, c.b.q_pos0 + tok_first + 1);
       float m = -INFINITY, l = 0.f;
@@ -545,26 +571,29 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         if (!mbar_wait(&s_full[w], (step >> 1) & 1u, abort_word)) goto done;
         tc_fence_after();
         if (warp_valid) {
-          uint32_t sreg[128];
+          // Scores are read twice, for the maximum and for the exponentials, 32 columns at a time: held, the 128 of a row spilled (three warps
+          // of a scheduler have 168 registers a thread) and a tile took 4.6 us.
+          const bool masked = c_lo > 0 || key0 + 128 > all_hi;
+          const int ch0 = c_lo >> 5, ch1 = (c_hi + 31) >> 5;
+          auto scores = [&](int ch, uint32_t* x) {
+            tmem_ld_32x32b_x32(t_s + ch * 32, x);
+            tmem_ld_wait();
+            if (masked) {                        // columns of 32 that the row sees
+              const int lo = c_lo - ch * 32, hi = k_hi - key0 - ch * 32;
+              const uint32_t bits = (hi >= 32 ? ~0u : (hi <= 0 ? 0u : (1u << hi) - 1)) & (lo <= 0 ? ~0u : (lo >= 32 ? 0u : ~((1u << lo) - 1)));
 #pragma unroll
-          for (int ch = 0; ch < 4; ch++)
-            if (ch * 32 < c_hi && ch * 32 + 32 > c_lo) tmem_ld_32x32b_x32(t_s + ch * 32, sreg + ch * 32);
-          tmem_ld_wait();
-          if (c_lo > 0 || key0 + 128 > all_hi) {
-#pragma unroll
-            for (int j = 0; j < 128; j++)
-              if (j < c_lo || key0 + j >= k_hi) sreg[j] = 0xff800000u;   // -inf
-          }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int ch = 0; ch < 4; ch++)
-            if (ch * 32 < c_hi && ch * 32 + 32 > c_lo) {
-#pragma unroll
-              for (int j = 0; j < 32; j += 8)
-#pragma unroll
-                for (int q = 0; q < 4; q++)
-                  mx[q] = fmaxf(mx[q], fmaxf(__uint_as_float(sreg[ch * 32 + j + 2 * q]), __uint_as_float(sreg[ch * 32 + j + 2 * q + 1])));
+              for (int j = 0; j < 32; j++) x[j] = bits >> j & 1 ? x[j] : 0xff800000u;      // -inf
             }
+          };
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int ch = ch0; ch < ch1; ch++) {
+            uint32_t x[32];
+            scores(ch, x);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2)
+              mx[(j >> 1) & 3] = fmaxf(mx[(j >> 1) & 3], fmaxf(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
+          }
           const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           float alpha = 1.f;
           bool need = false;
@@ -588,20 +617,20 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           }
           const float nmb = m == -INFINITY ? 0.f : -m * sl2;
           float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+          for (int ch = ch0; ch < ch1; ch++) {
+            uint32_t x[32], pk[16];
+            scores(ch, x);
 #pragma unroll
-          for (int ch = 0; ch < 4; ch++)
-            if (ch * 32 < c_hi && ch * 32 + 32 > c_lo) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int j = 0; j < 16; j++) {
-                const float p0 = sh_exp2(fmaf(__uint_as_float(sreg[ch * 32 + 2 * j]), sl2, nmb));
-                const float p1 = sh_exp2(fmaf(__uint_as_float(sreg[ch * 32 + 2 * j + 1]), sl2, nmb));
-                rs[(j & 1) * 2] += p0;
-                rs[(j & 1) * 2 + 1] += p1;
-                pk[j] = pack_bf16x2(p0, p1);     // the product takes bf16; the sum keeps 32 bits
-              }
-              tmem_st_32x32b_x16(t_s + ch * 16, pk);
+            for (int j = 0; j < 16; j++) {
+              const float p0 = sh_exp2(fmaf(__uint_as_float(x[2 * j]), sl2, nmb));
+              const float p1 = sh_exp2(fmaf(__uint_as_float(x[2 * j + 1]), sl2, nmb));
+              rs[(j & 1) * 2] += p0;
+              rs[(j & 1) * 2 + 1] += p1;
+              pk[j] = pack_bf16x2(p0, p1);       // the product takes bf16; the sum keeps 32 bits
             }
+            tmem_st_32x32b_x16(t_s + ch * 16, pk);       // over columns that have been read
+          }
           l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
           tmem_st_wait();
         }
@@ -609,8 +638,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           if (nsel == 1 || off == 0) {
             const uint32_t st = gt % NV;
             if (!mbar_wait(&v_full[st], (gt / NV) & 1u, abort_word)) goto done;
-            const int lo0 = c_lo & ~15, hi1 = (c_hi + 15) & ~15, nlo = c_lo - lo0, rows = nlo + hi1 - c_hi;
-            for (int j = row; j < rows * 8 * NH; j += 128) {
+            const int lo0 = c_lo & ~15, hi1 = (c_hi + 15) & ~15, nlo = c_lo - lo0, beside = nlo + hi1 - c_hi;
+            for (int j = lane_row; j < beside * 8 * NH; j += 128) {
               const int r = j / (8 * NH), x = j - r * 8 * NH, at = r < nlo ? lo0 + r : c_hi + r - nlo;
               *reinterpret_cast<uint4*>(Vs + st * TILE + (x >> 3) * SH_HALF + at * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
@@ -621,46 +650,21 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[w]);
       }
-      // ---- the piece's rows
-      const bool both = nsel == 1 && n > 1;
-      const uint32_t finisher = both ? (s0 + n - 1) & 1u : w;
-      if (both && finisher != w) {
-        if (!mbar_wait(ml_empty, (mc & 1u) ^ 1u, abort_word)) goto done;
-        ml[row] = make_float2(m, l);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(ml_full);
-      } else if (nsel == 2 || both || off == 0) {
-        if (!mbar_wait(&o_full[w], oc[w] & 1u, abort_word)) goto done;
-        float a_own = 1.f, a_other = 0.f;
-        if (both) {
-          if (!mbar_wait(&o_full[w ^ 1], oc[w ^ 1] & 1u, abort_word)) goto done;
-          if (!mbar_wait(ml_full, mc & 1u, abort_word)) goto done;
-          const float2 o = ml[row];
-          __syncwarp();
-          if (lane == 0) mbar_arrive(ml_empty);
-          const float top = fmaxf(m, o.x);
-          if (top > -INFINITY) {
-            a_own = sh_exp2((m - top) * sl2);
-            a_other = sh_exp2((o.x - top) * sl2);
-          }
-          l = l * a_own + o.y * a_other;
-          m = top;
-        }
+      // ---- the piece's rows: two slots up to 128 rows, one for each group of warps
+      const long slot = (long)c.b.part_row + (long)(c.h + (int)blockIdx.x - c.b.seg0) * (nsel == 2 ? 1 : 2) * (c.b.ntok * G);
+      const long at = slot + (nsel == 2 ? tok_first * G : (int)off * rows) + row;
+      if (first < n) {
+        if (row_valid) p.part_ml[at] = make_float2(l != l && m == -INFINITY ? 0.f : m * sl2, l);      // scores without a number count
+        if (!mbar_wait(&o_full[w], oc & 1u, abort_word)) goto done;
+        oc++;
         tc_fence_after();
         if (warp_valid) {
-          const long at = (long)c.b.part_row + (long)(c.h + (int)blockIdx.x - c.b.seg0) * (c.b.ntok * G) + tok_first * G + row;
-          if (row_valid) p.part_ml[at] = make_float2(l != l && m == -INFINITY ? 0.f : m * sl2, l);      // scores without a number count
           float* dst = p.part_o + at * D;
 #pragma unroll 1
           for (int ch = 0; ch < D / 32; ch++) {
-            uint32_t r[32], x[32];
+            uint32_t r[32];
             tmem_ld_32x32b_x32(t_o + w * 128 + ch * 32, r);
-            if (both) tmem_ld_32x32b_x32(t_o + (w ^ 1) * 128 + ch * 32, x);
             tmem_ld_wait();
-            if (both) {
-#pragma unroll
-              for (int j = 0; j < 32; j++) r[j] = __float_as_uint(__uint_as_float(r[j]) * a_own + __uint_as_float(x[j]) * a_other);
-            }
             if (row_valid) {
 #pragma unroll
               for (int j = 0; j < 8; j++)
@@ -670,18 +674,10 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&o_free[w]);
-          if (both) mbar_arrive(&o_free[w ^ 1]);
-        }
+        if (lane == 0) mbar_arrive(&o_free[w]);
+      } else if (row_valid) {
+        p.part_ml[at] = make_float2(-INFINITY, 0.f);     // a piece of one tile is the other group's: no rows of mine
       }
-      if (nsel == 2 || both) {
-        oc[0]++;
-        oc[1]++;
-      } else {
-        oc[s0 & 1u]++;
-      }
-      mc += both;
       s0 += n * nsel;
       gt0 += n;
       more = c.next();
@@ -704,57 +700,59 @@ done:
   }
 }
 
-// One warp a (token, head): pieces of the prefix and of the sequence's own keys, by their maxima and sums.
+// One warp a (token, head): partial results of the prefix and of the sequence's own keys, by their maxima and sums.
 template <int D>
-__global__ void __launch_bounds__(256) shared_join_kernel(const SharedParams p) {
+__global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) {
   const int lane = threadIdx.x & 31;
-  const long id = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int t = (int)(id / p.Hq), hq = (int)(id - (long)t * p.Hq);
   if (t >= p.tokens) return;
-  const int units = __ldg(p.plan), blocks = min(p.blocks, units);
-  const int* tok_base = p.plan + 2 + p.blocks;
+  const int* tok_base = p.plan + plan_tokens_at(p.blocks);
   const int which[2] = {__ldg(tok_base + t), __ldg(tok_base + p.tokens + t)};
   if (which[1] == -2) return;                    // behind the last sequence: left as it is
-  const SharedBase* bases = reinterpret_cast<const SharedBase*>(p.plan + p.bases_at);
   const int h = hq / p.G, g = hq - h * p.G;
   long at[2];
-  int n[2], rows[2];
+  int n[2], pitch[2];
 #pragma unroll
   for (int k = 0; k < 2; k++) {
-    n[k] = 0;
+    at[k] = n[k] = pitch[k] = 0;
     if (which[k] < 0) continue;
-    const int4* q = reinterpret_cast<const int4*>(bases + which[k]);
-    const int4 u = __ldg(q), v = __ldg(q + 1), x = __ldg(q + 2);
-    const int first = v.w + h * (v.z + 1) + 1;   // unit of its first tile
-    const int b0 = block_of(first, units, blocks), b1 = block_of(first + v.z - 1, units, blocks);
-    rows[k] = u.y * p.G;
-    at[k] = (long)x.x + (long)(h + b0 - x.y) * rows[k] + (t - u.x) * p.G + g;
-    n[k] = b1 - b0 + 1;
+    const int2 head = __ldg(reinterpret_cast<const int2*>(p.plan + p.heads_at) + (long)which[k] * p.Hkv + h);
+    const int2 tok = __ldg(reinterpret_cast<const int2*>(reinterpret_cast<const SharedBase*>(p.plan + p.bases_at) + which[k]));
+    pitch[k] = tok.y * p.G;
+    at[k] = (long)head.x + (t - tok.x) * p.G + g;
+    n[k] = head.y;
   }
-  float top = -INFINITY;
-  for (int k = 0; k < 2; k++)
-    for (int i = lane; i < n[k]; i += 32) top = fmaxf(top, p.part_ml[at[k] + (long)i * rows[k]].x);
-  top = warp_reduce_max(top);
   constexpr int V = D / 32;
-  float acc[V], sum = 0.f;
+  float acc[V], sum = 0.f, top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < V; j++) acc[j] = 0.f;
-  if (top > -INFINITY) {
-    for (int k = 0; k < 2; k++)
-#pragma unroll 4
-      for (int i = 0; i < n[k]; i++) {
-        const long r = at[k] + (long)i * rows[k];
-        const float2 e = p.part_ml[r];
-        const float f = sh_exp2(e.x - top);
-        sum += f * e.y;
-        if constexpr (V == 4) {
-          const float4 o = reinterpret_cast<const float4*>(p.part_o + r * D)[lane];
-          acc[0] += f * o.x; acc[1] += f * o.y; acc[2] += f * o.z; acc[3] += f * o.w;
-        } else {
-          const float2 o = reinterpret_cast<const float2*>(p.part_o + r * D)[lane];
-          acc[0] += f * o.x; acc[1] += f * o.y;
-        }
+  const int all = n[0] + n[1];
+  auto row_of = [&](int i) -> long { return i < n[0] ? at[0] + (long)i * pitch[0] : at[1] + (long)(i - n[0]) * pitch[1]; };
+  for (int i0 = 0; i0 < all; i0 += 32) {         // a lane a partial result: maximum and sum
+    const int m = min(32, all - i0);
+    const float2 e = lane < m ? p.part_ml[row_of(i0 + lane)] : make_float2(-INFINITY, 0.f);
+    const float now = fmaxf(top, warp_reduce_max(e.x));
+    if (now == -INFINITY) continue;
+    const float old = sh_exp2(top - now);        // 0 in front of the first
+    top = now;
+    const float f = lane < m && e.x > -INFINITY ? sh_exp2(e.x - now) : 0.f;
+    sum = sum * old + warp_reduce_sum(e.x > -INFINITY ? f * e.y : 0.f);
+#pragma unroll
+    for (int j = 0; j < V; j++) acc[j] *= old;
+#pragma unroll 8
+    for (int i = 0; i < m; i++) {
+      const float w = __shfl_sync(0xffffffffu, f, i);
+      if (w == 0.f) continue;                    // no rows there
+      const float* o = p.part_o + row_of(i0 + i) * D + lane * V;
+      if constexpr (V == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(o);
+        acc[0] += w * x.x; acc[1] += w * x.y; acc[2] += w * x.z; acc[3] += w * x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(o);
+        acc[0] += w * x.x; acc[1] += w * x.y;
       }
+    }
   }
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   __nv_bfloat16* dst = p.out + (long)t * p.out_stride + (long)hq * D + lane * V;
@@ -778,7 +776,7 @@ struct SharedArgs {
   long q_stride, T, num_blocks, pitch, out_stride, part_rows;
   long block_stride, token_stride, head_stride;      // of the caches, in elements
   float scale;
-  int block_size, max_blocks, Hq, Hkv, D, blocks, tokens, bases_at;
+  int block_size, max_blocks, Hq, Hkv, D, blocks, tokens, bases_at, max_bases;
 };
 
 static int shared_tmap(CUtensorMap* out, const void* base, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
@@ -807,11 +805,11 @@ template <int D>
 static int launch_shared(const CUtensorMap* tm, const SharedParams& p, cudaStream_t stream) {
   const cudaError_t e = allow_smem<&attn_shared_kernel<D>>(SharedCfg<D>::SMEM);
   if (e != cudaSuccess) return (int)e;
-  attn_shared_kernel<D><<<p.blocks, SH_THREADS, SharedCfg<D>::SMEM, stream>>>(tm[0], tm[1], tm[2], tm[3], tm[4], tm[5], tm[6], p);
+  attn_shared_kernel<D><<<p.blocks, SH_THREADS, SharedCfg<D>::SMEM, stream>>>(tm[0], tm[1], tm[2], tm[3], tm[4], tm[5], tm[6], tm[7], p);
   const int rc = B200_CHECK_LAUNCH();
   if (rc) return rc;
   const long warps = (long)p.tokens * p.Hq;
-  shared_join_kernel<D><<<(unsigned)((warps + 7) / 8), 256, 0, stream>>>(p);
+  shared_join_kernel<D><<<(unsigned)((warps + 3) / 4), 128, 0, stream>>>(p);
   return B200_CHECK_LAUNCH();
 }
 
@@ -823,7 +821,7 @@ B200_API int b200_shared_plan(const b200::PlanArgs* args) {
   if (a.seqs < 0 || a.groups < 0 || a.tokens < 0 || a.G < 1 || a.G > 128 || a.Hkv < 1 || a.blocks < 1) return 9950;
   const int per = 2 * (128 / a.G);
   if ((long)a.max_bases < (long)a.groups + a.seqs + 2 * ((long)a.tokens / per) || (a.bases_at & 3) ||
-      a.bases_at < 2 + a.blocks + 2 * a.tokens + a.groups || ((uintptr_t)a.plan & 15))
+      a.bases_at < plan_tokens_at(a.blocks) + 2 * a.tokens + a.groups || ((uintptr_t)a.plan & 15))
     return 9951;
   shared_plan_kernel<<<1, 1024, 0, a.stream>>>(a);
   return B200_CHECK_LAUNCH();
@@ -841,13 +839,13 @@ B200_API int b200_attn_shared(const b200::SharedArgs* args) {
     return 9957;
   const int G = a.Hq / a.Hkv, tpt = 128 / G;
   // what the pieces of a plan of these sizes have room for
-  if (a.part_rows < 2L * a.tokens * a.Hq + (long)a.blocks * SH_ROWS) return 9958;
-  CUtensorMap tm[7];
+  if (a.part_rows < 4L * a.tokens * a.Hq + (long)a.blocks * SH_ROWS) return 9958;
+  CUtensorMap tm[8];
   {
     const uint64_t dims[4] = {(uint64_t)a.D, (uint64_t)G, (uint64_t)a.Hkv, (uint64_t)a.T};
     const uint64_t str[3] = {(uint64_t)a.D * 2, (uint64_t)G * a.D * 2, (uint64_t)a.q_stride * 2};
-    const uint32_t n[3] = {(uint32_t)tpt, (uint32_t)(tpt < 4 ? tpt : 4), 1};
-    for (int i = 0; i < 3; i++) {
+    const uint32_t n[4] = {(uint32_t)tpt, (uint32_t)(G <= 64 ? 64 / G : 1), (uint32_t)(tpt < 4 ? tpt : 4), 1};
+    for (int i = 0; i < 4; i++) {
       const uint32_t box[4] = {64, (uint32_t)G, 1, n[i]};
       const int rc = shared_tmap(&tm[i], a.q, dims, str, box);
       if (rc) return rc;
@@ -858,7 +856,7 @@ B200_API int b200_attn_shared(const b200::SharedArgs* args) {
     const uint64_t dims[4] = {(uint64_t)a.D, (uint64_t)a.Hkv, (uint64_t)bs, (uint64_t)a.num_blocks};
     const uint64_t str[3] = {(uint64_t)a.head_stride * 2, (uint64_t)a.token_stride * 2, (uint64_t)a.block_stride * 2};
     const uint32_t box[4] = {64, 1, (uint32_t)(i < 2 ? rpl : piece), 1};
-    const int rc = shared_tmap(&tm[3 + i], i & 1 ? a.v_cache : a.k_cache, dims, str, box);
+    const int rc = shared_tmap(&tm[4 + i], i & 1 ? a.v_cache : a.k_cache, dims, str, box);
     if (rc) return rc;
   }
   SharedParams p;
@@ -867,12 +865,14 @@ B200_API int b200_attn_shared(const b200::SharedArgs* args) {
   p.pitch = a.pitch;
   p.max_blocks = a.max_blocks;
   p.block_size = bs;
+  p.page_shift = bs & (bs - 1) ? -1 : 31 - __builtin_clz(bs);
   p.rows_per_load = rpl;
   p.piece = piece;
   p.G = G; p.Hkv = a.Hkv; p.Hq = a.Hq; p.tpt = tpt;
   p.blocks = a.blocks;
   p.tokens = a.tokens;
   p.bases_at = a.bases_at;
+  p.heads_at = plan_heads_at(a.bases_at, a.max_bases);
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.part_o = a.parts;
   p.part_ml = (float2*)(a.parts + a.part_rows * a.D);

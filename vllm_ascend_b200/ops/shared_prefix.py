@@ -18,7 +18,7 @@ from .kv_int4 import _dense, _dense_heads, _elsewhere, _report
 
 # laid out as the source's PlanArgs and SharedArgs
 _PLAN = struct.Struct("@7P8i")
-_ATTENTION = struct.Struct("@9P9qf8i")
+_ATTENTION = struct.Struct("@9P9qf9i")
 for _name in ("b200_shared_plan", "b200_attn_shared"):
     _native.register_signature(_name, [c_char_p])
 
@@ -38,6 +38,7 @@ class SharedPrefixPlan:
     seqs: int
     blocks: int = 0
     bases_at: int = 0
+    bases: int = 0
     table: Optional[torch.Tensor] = None
 
 
@@ -67,10 +68,10 @@ def plan_shared_prefix(meta, group_starts, prefix_lens, heads: int, kv_heads: in
     if device < 0:
         return plan
     G, groups, n = heads // kv_heads, prefixes.shape[0], meta.num_reqs
-    bases = groups + n + 2 * (plan.tokens // (2 * (128 // G)))
     plan.blocks = _native.sm_count(device)
-    plan.bases_at = -(-(2 + plan.blocks + 2 * plan.tokens + groups) // 4) * 4
-    plan.table = torch.empty(plan.bases_at + bases * _BASE, dtype=torch.int32, device=where)
+    plan.bases = bases = groups + n + 2 * (plan.tokens // (2 * (128 // G)))
+    plan.bases_at = -(-(4 + 2 * plan.blocks + 2 * plan.tokens + groups) // 4) * 4
+    plan.table = torch.empty(plan.bases_at + bases * (_BASE + 2 * kv_heads), dtype=torch.int32, device=where)
     rc = _native.lib().b200_shared_plan(_PLAN.pack(
         meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(), starts.data_ptr(), prefixes.data_ptr(), plan.table.data_ptr(),
         _native.status_word(where).data_ptr(), _native.stream_ptr(), n, groups, plan.tokens, G, kv_heads, plan.blocks, bases, plan.bases_at))
@@ -124,7 +125,7 @@ def paged_attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     if channel != 1 or head != D or row % 8 or out.data_ptr() % 16:
         out = q.new_empty((T, Hq, D))
         out.copy_(given)
-    part_rows = 2 * plan.tokens * Hq + plan.blocks * _ROWS
+    part_rows = 4 * plan.tokens * Hq + plan.blocks * _ROWS
     # every call has its own: calls on two streams, or two graphs, may run at once
     parts = torch.empty(part_rows * (D + 2), dtype=torch.float32, device=q.device)
     block, token, khead, _ = k_cache.stride()
@@ -132,7 +133,7 @@ def paged_attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     rc = _native.lib().b200_attn_shared(_ATTENTION.pack(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), plan.table.data_ptr(), table.data_ptr(), parts.data_ptr(), out.data_ptr(),
         _native.status_word(q.device).data_ptr(), _native.stream_ptr(), q.stride(0), T, NB, table.stride(0), out.stride(0), part_rows, block, token,
-        khead, scale, bs, table.shape[1], Hq, Hkv, D, plan.blocks, plan.tokens, plan.bases_at))
+        khead, scale, bs, table.shape[1], Hq, Hkv, D, plan.blocks, plan.tokens, plan.bases_at, plan.bases))
     _native.check(rc, "attn_shared")
     _native.count_launch(2)
     return out if out is given else given.copy_(out)
