@@ -46,9 +46,8 @@ struct SharedBase {
   int pad;
 };
 
-// What a tile of 128 keys and the begin and end of a piece cost, in units of half a tile.  A tile for two query tiles takes the softmax of twice the
-// rows on the same schedulers.
-constexpr int COST_TILE = 2, COST_PAIR = 3, COST_PIECE = 2;
+// What a tile of 128 keys, one for two query tiles (the softmax of twice the rows on the same schedulers) and the begin and end of a piece cost
+constexpr int COST_TILE = 4, COST_PAIR = 9, COST_PIECE = 4;
 
 // plan: [0] units of cost, [1] bases, [2] blocks with work, then block_first[blocks] and block_unit[blocks + 1] (base and unit that a block begins
 // with), tok_prefix[tokens], tok_own[tokens] (base of a token, -1 no keys, -2 no sequence), group_ctx[groups], bases, and for every base and
@@ -198,7 +197,9 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   }
   // Blocks and partial rows of every base.  A block has as many units as a tile at least, so those from the one of a head's first tile to the one
   // of its last all have tiles of it, and their rows leave no gap.
-  const int blocks = min(a.blocks, units / COST_PAIR);
+  bool pairs = false;
+  for (int i = tid; i < count; i += 1024) pairs |= bases[i].tiles > 0 && bases[i].weight == COST_PAIR;
+  const int blocks = min(a.blocks, units / (__syncthreads_or(pairs) ? COST_PAIR : COST_TILE));
   int rows = 0;
   for (int i0 = 0; i0 < count; i0 += 1024) {
     const int i = i0 + tid;
@@ -575,9 +576,7 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           // of a scheduler have 168 registers a thread) and a tile took 4.6 us.
           const bool masked = c_lo > 0 || key0 + 128 > all_hi;
           const int ch0 = c_lo >> 5, ch1 = (c_hi + 31) >> 5;
-          auto scores = [&](int ch, uint32_t* x) {
-            tmem_ld_32x32b_x32(t_s + ch * 32, x);
-            tmem_ld_wait();
+          auto hide = [&](int ch, uint32_t* x) {
             if (masked) {                        // columns of 32 that the row sees
               const int lo = c_lo - ch * 32, hi = k_hi - key0 - ch * 32;
               const uint32_t bits = (hi >= 32 ? ~0u : (hi <= 0 ? 0u : (1u << hi) - 1)) & (lo <= 0 ? ~0u : (lo >= 32 ? 0u : ~((1u << lo) - 1)));
@@ -586,13 +585,18 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
           };
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-          for (int ch = ch0; ch < ch1; ch++) {
-            uint32_t x[32];
-            scores(ch, x);
+          auto maxima = [&](int ch, uint32_t* x) {
+            hide(ch, x);
 #pragma unroll
             for (int j = 0; j < 32; j += 2)
               mx[(j >> 1) & 3] = fmaxf(mx[(j >> 1) & 3], fmaxf(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
+          };
+#pragma unroll 1
+          for (int ch = ch0; ch < ch1; ch++) {
+            uint32_t x[32];
+            tmem_ld_32x32b_x32(t_s + ch * 32, x);
+            tmem_ld_wait();
+            maxima(ch, x);
           }
           const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           float alpha = 1.f;
@@ -617,10 +621,9 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           }
           const float nmb = m == -INFINITY ? 0.f : -m * sl2;
           float rs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-          for (int ch = ch0; ch < ch1; ch++) {
-            uint32_t x[32], pk[16];
-            scores(ch, x);
+          auto exps = [&](int ch, uint32_t* x) {
+            hide(ch, x);
+            uint32_t pk[16];
 #pragma unroll
             for (int j = 0; j < 16; j++) {
               const float p0 = sh_exp2(fmaf(__uint_as_float(x[2 * j]), sl2, nmb));
@@ -630,6 +633,13 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               pk[j] = pack_bf16x2(p0, p1);       // the product takes bf16; the sum keeps 32 bits
             }
             tmem_st_32x32b_x16(t_s + ch * 16, pk);       // over columns that have been read
+          };
+#pragma unroll 1
+          for (int ch = ch0; ch < ch1; ch++) {
+            uint32_t x[32];
+            tmem_ld_32x32b_x32(t_s + ch * 32, x);
+            tmem_ld_wait();
+            exps(ch, x);
           }
           l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
           tmem_st_wait();
@@ -700,16 +710,16 @@ done:
   }
 }
 
-// One warp a (token, head): partial results of the prefix and of the sequence's own keys, by their maxima and sums.
-template <int D>
+// Partial results of the prefix and of the sequence's own keys by their maxima and sums; WARPS warps a (token, head).
+template <int D, int WARPS>
 __global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) {
-  const int lane = threadIdx.x & 31;
-  const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  constexpr int V = D / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WARPS;
+  const long id = (long)blockIdx.x * (4 / WARPS) + warp / WARPS;
   const int t = (int)(id / p.Hq), hq = (int)(id - (long)t * p.Hq);
-  if (t >= p.tokens) return;
   const int* tok_base = p.plan + plan_tokens_at(p.blocks);
-  const int which[2] = {__ldg(tok_base + t), __ldg(tok_base + p.tokens + t)};
-  if (which[1] == -2) return;                    // behind the last sequence: left as it is
+  int which[2] = {-1, -2};
+  if (t < p.tokens) which[0] = __ldg(tok_base + t), which[1] = __ldg(tok_base + p.tokens + t);
   const int h = hq / p.G, g = hq - h * p.G;
   long at[2];
   int n[2], pitch[2];
@@ -723,37 +733,58 @@ __global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) 
     at[k] = (long)head.x + (t - tok.x) * p.G + g;
     n[k] = head.y;
   }
-  constexpr int V = D / 32;
   float acc[V], sum = 0.f, top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < V; j++) acc[j] = 0.f;
   const int all = n[0] + n[1];
   auto row_of = [&](int i) -> long { return i < n[0] ? at[0] + (long)i * pitch[0] : at[1] + (long)(i - n[0]) * pitch[1]; };
-  for (int i0 = 0; i0 < all; i0 += 32) {         // a lane a partial result: maximum and sum
-    const int m = min(32, all - i0);
-    const float2 e = lane < m ? p.part_ml[row_of(i0 + lane)] : make_float2(-INFINITY, 0.f);
+  for (int i0 = sub; i0 < all; i0 += 32 * WARPS) {         // a lane a partial result: maximum and sum
+    const int mine = i0 + lane * WARPS, m = min(32, (all - i0 + WARPS - 1) / WARPS);
+    const float2 e = lane < m ? p.part_ml[row_of(mine)] : make_float2(-INFINITY, 0.f);
     const float now = fmaxf(top, warp_reduce_max(e.x));
     if (now == -INFINITY) continue;
     const float old = sh_exp2(top - now);        // 0 in front of the first
     top = now;
-    const float f = lane < m && e.x > -INFINITY ? sh_exp2(e.x - now) : 0.f;
+    const float f = e.x > -INFINITY ? sh_exp2(e.x - now) : 0.f;
     sum = sum * old + warp_reduce_sum(e.x > -INFINITY ? f * e.y : 0.f);
 #pragma unroll
     for (int j = 0; j < V; j++) acc[j] *= old;
-#pragma unroll 8
+#pragma unroll 4
     for (int i = 0; i < m; i++) {
       const float w = __shfl_sync(0xffffffffu, f, i);
-      if (w == 0.f) continue;                    // no rows there
-      const float* o = p.part_o + row_of(i0 + i) * D + lane * V;
-      if constexpr (V == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(o);
-        acc[0] += w * x.x; acc[1] += w * x.y; acc[2] += w * x.z; acc[3] += w * x.w;
-      } else {
-        const float2 x = *reinterpret_cast<const float2*>(o);
-        acc[0] += w * x.x; acc[1] += w * x.y;
-      }
+      const float* o = p.part_o + row_of(i0 + i * WARPS) * D + lane * V;
+      float x[V];
+      if constexpr (V == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(o);
+      else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(o);
+#pragma unroll
+      for (int j = 0; j < V; j++) acc[j] += w == 0.f ? 0.f : w * x[j];       // where a group of warps had no tile, nothing was left
     }
   }
+  if constexpr (WARPS > 1) {
+    __shared__ float4 parts[4][33];
+    float4* mine = parts[warp];
+    mine[lane] = make_float4(acc[0], acc[1], V == 4 ? acc[V - 2] : 0.f, V == 4 ? acc[V - 1] : 0.f);
+    if (lane == 0) mine[32] = make_float4(top, sum, 0.f, 0.f);
+    __syncthreads();
+    if (sub != 0) return;
+    float tops[WARPS];
+#pragma unroll
+    for (int k = 0; k < WARPS; k++) tops[k] = parts[warp + k][32].x, top = fmaxf(top, tops[k]);
+    sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; j++) acc[j] = 0.f;
+#pragma unroll
+    for (int k = 0; k < WARPS; k++) {
+      if (tops[k] == -INFINITY) continue;
+      const float f = sh_exp2(tops[k] - top);
+      const float4 x = parts[warp + k][lane];
+      sum += f * parts[warp + k][32].y;
+      acc[0] += f * x.x;
+      acc[1] += f * x.y;
+      if constexpr (V == 4) acc[2] += f * x.z, acc[3] += f * x.w;
+    }
+  }
+  if (which[1] == -2) return;                    // behind the last sequence: left as it is
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   __nv_bfloat16* dst = p.out + (long)t * p.out_stride + (long)hq * D + lane * V;
   if constexpr (V == 4)
@@ -808,8 +839,10 @@ static int launch_shared(const CUtensorMap* tm, const SharedParams& p, cudaStrea
   attn_shared_kernel<D><<<p.blocks, SH_THREADS, SharedCfg<D>::SMEM, stream>>>(tm[0], tm[1], tm[2], tm[3], tm[4], tm[5], tm[6], tm[7], p);
   const int rc = B200_CHECK_LAUNCH();
   if (rc) return rc;
-  const long warps = (long)p.tokens * p.Hq;
-  shared_join_kernel<D><<<(unsigned)((warps + 3) / 4), 128, 0, stream>>>(p);
+  // few rows may have many partial results: up to 2 a block; there are warps to spare
+  const long rows = (long)p.tokens * p.Hq;
+  if (rows <= 4096) shared_join_kernel<D, 4><<<(unsigned)rows, 128, 0, stream>>>(p);
+  else shared_join_kernel<D, 1><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(p);
   return B200_CHECK_LAUNCH();
 }
 
