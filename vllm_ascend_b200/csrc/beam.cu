@@ -4,10 +4,12 @@
 //   total[g, w, v] = score[g, w] + logits[w, v] - log sum_v' exp(logits[w, v'])          the k best of each group, best first
 //
 // Selection reads the logits once.  A block walks a part of a row: every thread keeps a running maximum and the sum of exponentials
-// under it, and puts elements above the part's k-th best so far into a list in shared memory; within a row totals are ordered as
-// logits are, so the list needs no sum.  A list that grows is cut back to its k best: the k-th largest of the maxima of at least 2 k
-// slices of it is a bound that k elements or more reach, and what reaches it (about k for values in no order) is ranked by
-// counting.  Keys carry the value and, below it, the place: no two are equal, ties go to the lowest place by themselves.
+// under it; elements that reach the bound of the k-th best so far go to their warp's list in shared memory.  Within a row totals are
+// ordered as logits are, so the lists need no sum.  The bound begins with the first 4096 elements: the k-th largest of the maxima of
+// at least 2 k slices of them, which k elements or more reach, and about k for values in no order.  A warp whose list is full cuts it back to its
+// k best, whose last raises the bound for all.  Keys carry the value and, below it, the place: no two are equal, ties go to the
+// lowest place by themselves, and rows of equal values (masked ones) put nothing behind their first into a list.
+// Bound by HBM for many rows: about six instructions and an exponential an element are 0.6 of what an SM issues at its share of the bytes.
 // A second kernel, a block a group, adds up the sums of the parts, turns its beams' keys into totals and cuts them back in the same way.
 // Parts' sums are added in 64 bits and totals compared in 64: with thousands of candidates, sums of 32 bits would order near ones
 // by their rounding.
@@ -19,9 +21,9 @@ namespace b200 {
 constexpr int BEAM_THREADS = 512;
 constexpr int BEAM_VEC = 8;                               // elements a thread takes of a tile
 constexpr int BEAM_TILE = BEAM_THREADS * BEAM_VEC;
-constexpr int BEAM_SLACK = 1024;                          // the list is cut back when it holds more than this
-constexpr int BEAM_ROOM = BEAM_TILE + BEAM_SLACK;         // a tile more always fits
+constexpr int BEAM_WARPS = BEAM_THREADS / 32;
 constexpr int BEAM_MOST = 256;                            // k at most
+constexpr int BEAM_ROOM = 4096, BEAM_SLACK = 1024;        // candidates of a group that are looked at together, and that are kept until then
 constexpr float kBeamLog2e = 1.4426950408889634f;
 
 struct SelectArgs {
@@ -73,76 +75,78 @@ struct GroupKey {
   }
 };
 
-template <typename Key>
-struct BeamList {
-  Key keys[BEAM_ROOM];
-  Key slices[BEAM_THREADS];
-  Key bound;
-  int count;
-};
-
-// Cuts the list back to its k best, best first.  All threads of the block; the list has been written before a barrier.
-template <typename Key>
-__device__ void cut_back(BeamList<Key>& list, int k) {
-  constexpr int PER = (BEAM_ROOM + BEAM_THREADS - 1) / BEAM_THREADS;
-  const int tid = threadIdx.x;
-  int n = list.count;
-  int lanes = 32;                                         // lanes of a slice
+// ---------------------------------------------------------------- the k best of a list
+__device__ __forceinline__ int slice_lanes(int k) {       // lanes that share a slice: 2 k slices of 512 threads at least
+  int lanes = 32;
   while (BEAM_THREADS / lanes < 2 * k && lanes > 1) lanes >>= 1;
-  const int slices = BEAM_THREADS / lanes;
+  return lanes;
+}
+
+// The k-th largest of the maxima of the block's slices, `top` a thread's; none where fewer than k slices have elements.  Ends with a barrier.
+template <typename Key>
+__device__ __forceinline__ Key slice_bound(Key top, int k, Key* slices, Key* bound) {
+  const int tid = threadIdx.x, lanes = slice_lanes(k), count = BEAM_THREADS / lanes;
+  for (int o = 1; o < lanes; o <<= 1) {
+    const Key other = top.other_lane(o);
+    if (other.above(top)) top = other;
+  }
+  if (tid % lanes == 0) slices[tid / lanes] = top;
+  if (tid == 0) *bound = Key::none();
+  __syncthreads();
+  int rank = 0;                                           // all lanes of a slice count
+  for (int j = tid % lanes; j < count; j += lanes) rank += slices[j].above(top);
+  for (int o = 1; o < lanes; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+  if (tid % lanes == 0 && rank == k - 1) *bound = top;    // one slice, but for those without an element, all of them none
+  __syncthreads();
+  return *bound;
+}
+
+// The k best of n keys, best first, into out[0..k); returns how many.  All threads of the block, the keys written before a barrier; `keys` is
+// worked in, out may be part of it.  Ends with a barrier.
+template <typename Key, int PER>
+__device__ int select_best(Key* keys, int n, int k, Key* out, Key* slices, Key* bound, int* count) {
+  const int tid = threadIdx.x;
   // Only k slices reach the bound, and 2 k slices share the threads: a pass leaves 256 elements at most for every element that a thread
   // holds, 2560, 1280, 768, 512, 256 in turn; values in no order take one pass.
-  while (n > max(3 * k, 256)) {
+  for (bool more = n > max(2 * k, 64); more; more = n > max(3 * k, 256)) {
     Key mine[PER], top = Key::none();
 #pragma unroll
     for (int i = 0; i < PER; i++) {
       const int at = tid + i * BEAM_THREADS;
-      mine[i] = at < n ? list.keys[at] : Key::none();
+      mine[i] = at < n ? keys[at] : Key::none();
       if (mine[i].above(top)) top = mine[i];
     }
-    for (int o = 1; o < lanes; o <<= 1) {
-      const Key other = top.other_lane(o);
-      if (other.above(top)) top = other;
-    }
-    if (tid % lanes == 0) list.slices[tid / lanes] = top;
-    if (tid == 0) list.bound = Key::none();
-    __syncthreads();
-    if (tid < slices) {
-      const Key own = list.slices[tid];
-      int rank = 0;
-      for (int j = 0; j < slices; j++) rank += list.slices[j].above(own);
-      if (rank == k - 1) list.bound = own;                // one thread, but for slices without an element: all of them none
-    }
-    if (tid == 0) list.count = 0;
-    __syncthreads();
-    const Key bound = list.bound;
+    if (tid == 0) *count = 0;
+    const Key least = slice_bound(top, k, slices, bound);
 #pragma unroll
     for (int i = 0; i < PER; i++)
-      if (mine[i].above(Key::none()) && !bound.above(mine[i])) list.keys[atomicAdd(&list.count, 1)] = mine[i];
+      if (mine[i].above(Key::none()) && !least.above(mine[i])) keys[atomicAdd(count, 1)] = mine[i];
     __syncthreads();
-    n = list.count;
+    n = *count;
     __syncthreads();
   }
-  // rank by counting: 3 k elements at most
+  // ranked by counting: 3 k elements at most, the block's threads shared between them
   static_assert(3 * BEAM_MOST <= 2 * BEAM_THREADS, "two elements a thread");
+  int each = 1;
+  while (each < 32 && n * each * 2 <= BEAM_THREADS) each <<= 1;
   Key own[2];
   int rank[2];
 #pragma unroll
   for (int i = 0; i < 2; i++) {
-    const int at = tid + i * BEAM_THREADS;
-    rank[i] = k;
-    if (at < n) {
-      own[i] = list.keys[at];
-      rank[i] = 0;
-      for (int j = 0; j < n; j++) rank[i] += list.keys[j].above(own[i]);
-    }
+    const int at = i * BEAM_THREADS + tid / each;         // a second one only where each is 1
+    own[i] = at < n && (i == 0 || each == 1) ? keys[at] : Key::none();
+    rank[i] = 0;
+    if (own[i].above(Key::none()))
+      for (int j = tid % each; j < n; j += each) rank[i] += keys[j].above(own[i]);
+    if (i == 0)
+      for (int o = 1; o < each; o <<= 1) rank[i] += __shfl_xor_sync(0xffffffffu, rank[i], o);
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; i++)
-    if (rank[i] < k) list.keys[rank[i]] = own[i];
-  if (tid == 0) list.count = min(n, k);
+    if (tid % each == 0 && own[i].above(Key::none()) && rank[i] < k) out[rank[i]] = own[i];
   __syncthreads();
+  return min(n, k);
 }
 
 // ---------------------------------------------------------------- parts of rows
@@ -152,149 +156,255 @@ __device__ __forceinline__ float beam_exp2(float x) {
   return y;
 }
 
+// eight elements as they lie in memory
 template <typename T>
-__device__ __forceinline__ void load8(const T* at, float* x) {
-  if constexpr (sizeof(T) == 2) {
-    const uint4 r = __ldg(reinterpret_cast<const uint4*>(at));
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+struct Vec {
+  uint4 r[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* row, int at, int end) {        // those in [0, end), -inf beside
+    if (at >= 0 && at + BEAM_VEC <= end) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      for (int i = 0; i < (int)sizeof(T) / 2; i++) r[i] = __ldg(reinterpret_cast<const uint4*>(row + at) + i);
+    } else {
+      uint32_t w[4 * (sizeof(T) / 2)];
+#pragma unroll
+      for (int i = 0; i < 4 * ((int)sizeof(T) / 2); i++) {
+        if constexpr (sizeof(T) == 2) {
+          const unsigned short* e = reinterpret_cast<const unsigned short*>(row);
+          const int j = at + 2 * i;
+          w[i] = (j >= 0 && j < end ? e[j] : 0xff80u) | (uint32_t)(j + 1 >= 0 && j + 1 < end ? e[j + 1] : 0xff80u) << 16;
+        } else {
+          w[i] = at + i >= 0 && at + i < end ? __float_as_uint(row[at + i]) : 0xff800000u;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; i++) r[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     }
-  } else {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(at)), b = __ldg(reinterpret_cast<const float4*>(at) + 1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
   }
-}
+  __device__ __forceinline__ void get(float* x) const {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t w[4] = {r[0].x, r[0].y, r[0].z, r[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    } else {
+      const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = __uint_as_float(w[i]);
+    }
+  }
+};
 
 __device__ __forceinline__ bool is_score(float s) { return s > -INFINITY && s < INFINITY; }
+
+// A warp's list: room for k keys and two more steps of 32.
+__host__ __device__ constexpr int list_room(int k) { return (k + 31) / 32 * 32 + 64; }
+constexpr int LIST_MOST = list_room(BEAM_MOST) / 32;
+
+// A warp's n keys cut back to their k best, best first; returns the last of them.
+__device__ __noinline__ uint64_t cut_back(RowKey* list, int n, int k) {
+  const int lane = threadIdx.x & 31;
+  RowKey own[LIST_MOST];
+  int rank[LIST_MOST];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < LIST_MOST; i++) {
+    const int at = i * 32 + lane;
+    own[i].v = at < n ? list[at].v : 0;
+    rank[i] = at < n ? 0 : k;
+  }
+  for (int j = 0; j < n; j++) {
+    const uint64_t v = list[j].v;
+#pragma unroll
+    for (int i = 0; i < LIST_MOST; i++) rank[i] += v > own[i].v;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < LIST_MOST; i++)
+    if (rank[i] < k) list[rank[i]] = own[i];
+  __syncwarp();
+  return list[k - 1].v;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const SelectArgs a) {
   extern __shared__ __align__(16) uint8_t beam_smem[];
-  BeamList<RowKey>& list = *reinterpret_cast<BeamList<RowKey>*>(beam_smem);
-  __shared__ float warp_max[BEAM_THREADS / 32];
-  __shared__ double warp_sum[BEAM_THREADS / 32];
-  const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts, tid = threadIdx.x;
-  if (!is_score(a.scores[row])) return;                  // the beam has ended: the second kernel asks its score first
+  __shared__ RowKey slices[BEAM_THREADS], first_bound;
+  __shared__ unsigned long long bound;             // what a key has to reach, the k-th best of some that were seen
+  __shared__ int count;
+  __shared__ float warp_max[BEAM_WARPS];
+  __shared__ double warp_sum[BEAM_WARPS];
+  const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (!is_score(a.scores[row])) return;            // the beam has ended: the second kernel asks its score first
   const T* x0 = (const T*)a.logits + (long)row * a.row_stride;
   // vectors lie on 16-byte boundaries of memory, whatever the row's first element does; a vector holds elements [at, at + 8)
   const int shift = (int)(((uintptr_t)x0 & 15) / sizeof(T));
   const int from = part * a.per_part - shift, to = min(from + a.per_part, a.vocab);
-  float m = -INFINITY, s = 0.f, least = -INFINITY;
-  if (tid == 0) list.count = 0;
-  __syncthreads();
-  auto fetch = [&](int at, float* x) {
-    if (at >= 0 && at + BEAM_VEC <= a.vocab) {
-      load8(x0 + at, x);
-    } else {
+  const int room = list_room(a.k);
+  RowKey* list = reinterpret_cast<RowKey*>(beam_smem) + warp * room;
+  int held = 0;                                    // keys in the warp's list
+  auto key_of = [&](float x, int at) -> uint64_t { return at >= 0 && at < to ? ((uint64_t)order32(x) << 32) | (uint32_t)~at : 0; };
+  float m = -INFINITY, s = 0.f;
+  auto add = [&](const float* x, float top) {
+    if (top > m) {
+      s *= beam_exp2((m - top) * kBeamLog2e);      // nothing before the first element that is above -inf
+      m = top;
+    }
+    // differences from the maximum are taken before the factor: a product of the maximum would carry its rounding into every term
+    const float under = m == -INFINITY ? 0.f : m;
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < BEAM_VEC; j++) x[j] = at + j >= 0 && at + j < a.vocab ? (float)x0[at + j] : -INFINITY;
+    for (int j = 0; j < BEAM_VEC; j++) t[j & 3] += beam_exp2((x[j] - under) * kBeamLog2e);         // a NaN or +inf: NaN
+    s += (t[0] + t[1]) + (t[2] + t[3]);
+  };
+  auto top_of = [&](const float* x) -> float {
+    float t = x[0];
+#pragma unroll
+    for (int j = 1; j < BEAM_VEC; j++) t = fmaxf(t, x[j]);
+    return t;
+  };
+  // keys of a vector that reach the bound; all lanes of the warp
+  auto keep = [&](const float* x, int at) {
+#pragma unroll 1
+    for (int j = 0; j < BEAM_VEC; j++) {
+      float v = x[0];                              // x[j] without an index into registers
+#pragma unroll
+      for (int i = 1; i < BEAM_VEC; i++) v = j == i ? x[i] : v;
+      const uint64_t key = key_of(v, at + j);
+      const bool in = key != 0 && key >= *(volatile unsigned long long*)&bound;
+      const uint32_t who = __ballot_sync(0xffffffffu, in);
+      if (who == 0) continue;
+      if (held + 32 > room) {
+        const uint64_t last = cut_back(list, held, a.k);
+        held = a.k;
+        if (lane == 0) atomicMax(&bound, (unsigned long long)last);
+        __syncwarp();
+      }
+      if (in) list[held + __popc(who & ((1u << lane) - 1))].v = key;
+      held += __popc(who);
     }
   };
-  float next[BEAM_VEC];
+  // ---- the first 4096 elements and the bound that they give
+  constexpr int AHEAD = 16 / sizeof(T) / 2;        // vectors on their way, 64 bytes a thread: 4 of bf16, 2 of fp32
+  Vec<T> ahead[AHEAD];
   int at = from + tid * BEAM_VEC;
-  if (at < to) fetch(at, next);
-  bool first = true;
-  for (int base = from; base < to; base += BEAM_TILE, at += BEAM_TILE) {
-    float x[BEAM_VEC];
 #pragma unroll
-    for (int j = 0; j < BEAM_VEC; j++) x[j] = next[j];
-    const bool mine = at < to;
-    if (at + BEAM_TILE < to) fetch(at + BEAM_TILE, next);
-    bool over = false;
-    if (mine) {
-      float top = x[0];
+  for (int i = 0; i < AHEAD; i++) ahead[i].load(x0, at + i * BEAM_TILE < to ? at + i * BEAM_TILE : a.vocab, a.vocab);
+  float x[BEAM_VEC];
+  ahead[0].get(x);
+  RowKey top = RowKey::none();
 #pragma unroll
-      for (int j = 1; j < BEAM_VEC; j++) top = fmaxf(top, x[j]);
-      if (top > m) {
-        s *= beam_exp2((m - top) * kBeamLog2e);          // nothing before the first element that is above -inf
-        m = top;
-      }
-      // differences from the maximum are taken before the factor: a product of the maximum would carry its rounding into every term
-      const float under = m == -INFINITY ? 0.f : m;
-      float t[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < BEAM_VEC; j++) t[j & 3] += beam_exp2((x[j] - under) * kBeamLog2e);       // a NaN or +inf: NaN
-      s += (t[0] + t[1]) + (t[2] + t[3]);
-      if (first) {
-#pragma unroll
-        for (int j = 0; j < BEAM_VEC; j++)
-          if (at + j >= 0 && at + j < a.vocab)
-            list.keys[atomicAdd(&list.count, 1)].v = ((uint64_t)order32(x[j]) << 32) | (uint32_t)~(at + j);
-      } else if (top > least) {
-#pragma unroll
-        for (int j = 0; j < BEAM_VEC; j++)
-          if (x[j] > least && at + j < a.vocab) {
-            const int place = atomicAdd(&list.count, 1);
-            list.keys[place].v = ((uint64_t)order32(x[j]) << 32) | (uint32_t)~(at + j);
-            over |= place >= BEAM_SLACK;
-          }
-      }
-    }
-    if (__syncthreads_or(over) || first) {
-      cut_back(list, a.k);
-      if (list.count == a.k) least = unorder32((uint32_t)(list.keys[a.k - 1].v >> 32));
-      __syncthreads();
-    }
-    first = false;
+  for (int j = 0; j < BEAM_VEC; j++) {
+    const RowKey key = {key_of(x[j], at + j)};
+    if (key.above(top)) top = key;
   }
-  if (list.count > a.k) cut_back(list, a.k);
-  const long slot = (long)row * a.parts + part;
-  for (int i = tid; i < list.count; i += BEAM_THREADS) a.keys[slot * a.k + i] = list.keys[i].v;
-  // the part's maximum and its sum under it
-  float top = m;
+  top = slice_bound(top, a.k, slices, &first_bound);
+  if (tid == 0) bound = top.v;
+  __syncthreads();
+  bool first = true;
+  // ---- all of the part, a warp by itself
+  for (int base = from; base < to; base += AHEAD * BEAM_TILE) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((tid & 31) == 0) warp_max[tid >> 5] = top;
+    for (int i = 0; i < AHEAD; i++) {
+      const int here = base + i * BEAM_TILE;
+      if (here >= to) break;
+      const int mine = here + tid * BEAM_VEC;
+      ahead[i].get(x);
+      const int next = mine + AHEAD * BEAM_TILE;
+      if (here + AHEAD * BEAM_TILE < to) ahead[i].load(x0, next < to ? next : a.vocab, a.vocab);
+      const float t = top_of(x);
+      if (mine < to) add(x, t);
+      const float reach = unorder32((uint32_t)(*(volatile unsigned long long*)&bound >> 32));
+      if (__any_sync(0xffffffffu, mine < to && (first || !(t < reach)))) keep(x, mine);
+      first = false;
+    }
+  }
+  // ---- the block's k best
+  for (int i = held + lane; i < room; i += 32) list[i] = RowKey::none();
+  if (tid == 0) count = 0;
+  __syncthreads();
+  RowKey* all = reinterpret_cast<RowKey*>(beam_smem);
+  const uint64_t least = bound;
+  uint64_t mine[LIST_MOST];
+#pragma unroll
+  for (int i = 0; i < LIST_MOST; i++) {
+    const int j = tid + i * BEAM_THREADS;
+    mine[i] = j < BEAM_WARPS * room ? all[j].v : 0;
+  }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < BEAM_THREADS / 32; i++) top = fmaxf(top, warp_max[i]);
-  double sum = m == -INFINITY ? (double)s : (double)s * (double)beam_exp2((m - top) * kBeamLog2e);
+  for (int i = 0; i < LIST_MOST; i++)
+    if (mine[i] != 0 && mine[i] >= least) all[atomicAdd(&count, 1)].v = mine[i];
+  __syncthreads();
+  const int n = count;
+  __syncthreads();
+  const int got = select_best<RowKey, LIST_MOST>(all, n, a.k, all, slices, &first_bound, &count);
+  const long slot = (long)row * a.parts + part;
+  for (int i = tid; i < got; i += BEAM_THREADS) a.keys[slot * a.k + i] = all[i].v;
+  // ---- the part's maximum and its sum under it
+  float high = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+  if (lane == 0) warp_max[warp] = high;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < BEAM_WARPS; i++) high = fmaxf(high, warp_max[i]);
+  double sum = m == -INFINITY ? (double)s : (double)s * (double)beam_exp2((m - high) * kBeamLog2e);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if ((tid & 31) == 0) warp_sum[tid >> 5] = sum;
+  if (lane == 0) warp_sum[warp] = sum;
   __syncthreads();
   if (tid == 0) {
     sum = 0.0;
-    for (int i = 0; i < BEAM_THREADS / 32; i++) sum += warp_sum[i];
-    a.maxima[slot] = top;
+    for (int i = 0; i < BEAM_WARPS; i++) sum += warp_sum[i];
+    a.maxima[slot] = high;
     a.sums[slot] = sum;
-    a.counts[slot] = list.count;
+    a.counts[slot] = got;
   }
 }
 
 // ---------------------------------------------------------------- groups
+struct GroupList {
+  GroupKey keys[BEAM_ROOM + BEAM_SLACK];
+  GroupKey slices[BEAM_THREADS];
+  GroupKey bound;
+  int count;
+};
+
 __global__ void __launch_bounds__(BEAM_THREADS, 1) select_groups_kernel(const SelectArgs a) {
   extern __shared__ __align__(16) uint8_t beam_smem[];
-  BeamList<GroupKey>& list = *reinterpret_cast<BeamList<GroupKey>*>(beam_smem);
-  double* norm = reinterpret_cast<double*>(beam_smem + sizeof(BeamList<GroupKey>));      // log of a beam's sum; NaN: it has no candidates
-  const int g = blockIdx.x, tid = threadIdx.x;
-  for (int w = tid; w < a.width; w += BEAM_THREADS) {
+  GroupList& list = *reinterpret_cast<GroupList*>(beam_smem);
+  double* norm = reinterpret_cast<double*>(beam_smem + sizeof(GroupList));      // log of a beam's sum; NaN: it has no candidates
+  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+  for (int w = tid >> 5; w < a.width; w += BEAM_WARPS) {          // a warp a beam, a lane a part
     const long row = (long)g * a.width + w;
     double l = __longlong_as_double(0x7ff8000000000000ll);
     if (is_score(a.scores[row])) {
       float top = -INFINITY;
-      for (int p = 0; p < a.parts; p++) top = fmaxf(top, a.maxima[row * a.parts + p]);
+      for (int p = lane; p < a.parts; p += 32) top = fmaxf(top, a.maxima[row * a.parts + p]);
+      top = warp_reduce_max(top);
       double sum = 0.0;
-      for (int p = 0; p < a.parts; p++) {
+      for (int p = lane; p < a.parts; p += 32) {
         const float mp = a.maxima[row * a.parts + p];
         const double sp = a.sums[row * a.parts + p];
         sum += mp == -INFINITY ? sp : sp * exp((double)mp - (double)top);
       }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (top > -INFINITY && top < INFINITY && sum > 0.0 && sum < 1e300) l = (double)top + log(sum);      // NaN fails both
     }
-    norm[w] = l;
+    if (lane == 0) norm[w] = l;
   }
-  if (tid == 0) list.count = 0;
   __syncthreads();
   // candidates [beam, part, place in its list]; a beam without a distribution offers its first tokens at -inf
   const int per_beam = a.parts * a.k, all = a.width * per_beam;
   GroupKey least = GroupKey::none();
-  for (int base = 0; base < all; base += BEAM_TILE) {
-    for (int i = base + tid; i < min(base + BEAM_TILE, all); i += BEAM_THREADS) {
+  int n = 0;
+  for (int base = 0; base < all; base += BEAM_ROOM) {
+    if (tid == 0) list.count = n;
+    __syncthreads();
+    for (int i = base + tid; i < min(base + BEAM_ROOM, all); i += BEAM_THREADS) {
       const int w = i / per_beam, j = i - w * per_beam, p = j / a.k, c = j - p * a.k;
       const long row = (long)g * a.width + w, slot = row * a.parts + p;
       const double l = norm[w];
@@ -309,11 +419,13 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1) select_groups_kernel(const Se
       if (key.above(least)) list.keys[atomicAdd(&list.count, 1)] = key;
     }
     __syncthreads();
-    if (list.count > BEAM_SLACK || base + BEAM_TILE >= all) {
-      cut_back(list, a.k);
-      if (list.count == a.k) least = list.keys[a.k - 1];
-    }
+    n = list.count;
     __syncthreads();
+    if (n > BEAM_SLACK || base + BEAM_ROOM >= all) {
+      n = select_best<GroupKey, (BEAM_ROOM + BEAM_SLACK) / BEAM_THREADS>(list.keys, n, a.k, list.keys, list.slices, &list.bound, &list.count);
+      if (n == a.k) least = list.keys[a.k - 1];
+      __syncthreads();
+    }
   }
   for (int i = tid; i < a.k; i += BEAM_THREADS) {
     const GroupKey key = list.keys[i];
@@ -341,7 +453,7 @@ struct ReorderArgs {
   const int* lengths;            // [groups] filled tokens of the beams' pages, or null
   int* status;
   cudaStream_t stream;
-  int num_tensors, groups, beams, chunks;
+  int num_tensors, groups, beams, wide, sms;     // wide: the first so many tensors move 16 bytes at once
 };
 
 template <int BYTES>
@@ -354,55 +466,11 @@ template <> struct Bits<1> { using type = uint8_t; };
 
 constexpr int REORDER_BEAMS = 1024;        // beams of a group at most
 
-// Elements [first, first + blockDim) of every row that moves: all loads, then all stores.  Up to MOST beams stay in registers; with
-// MOST = 0 a thread's loads go to its column of shared memory (cp.async where 16 bytes move at once).
-template <int BYTES, int MOST>
-__device__ __forceinline__ void move_rows(const BeamTensor& t, const int* from, const int* to, int beams, long offset, uint8_t* stage) {
-  using V = typename Bits<BYTES>::type;
-  uint8_t* at = t.base + offset;
-  if constexpr (MOST > 0) {
-    V v[MOST];
-#pragma unroll
-    for (int w = 0; w < MOST; w++)
-      if (w < beams && from[w] >= 0) v[w] = *reinterpret_cast<const V*>(at + (long)from[w] * t.row_stride);
-#pragma unroll
-    for (int w = 0; w < MOST; w++)
-      if (w < beams && from[w] >= 0) *reinterpret_cast<V*>(at + (long)to[w] * t.row_stride) = v[w];
-  } else {
-    V* mine = reinterpret_cast<V*>(stage) + threadIdx.x;
-    const int pitch = blockDim.x;
-    for (int w = 0; w < beams; w++) {
-      if (from[w] < 0) continue;
-      const uint8_t* src = at + (long)from[w] * t.row_stride;
-      if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(mine + w * pitch)), "l"(src) : "memory");
-      else
-        mine[w * pitch] = *reinterpret_cast<const V*>(src);
-    }
-    if constexpr (BYTES == 16) asm volatile("cp.async.wait_all;" ::: "memory");
-    for (int w = 0; w < beams; w++)
-      if (from[w] >= 0) *reinterpret_cast<V*>(at + (long)to[w] * t.row_stride) = mine[w * pitch];
-  }
-}
-
-template <int MOST>
-__global__ void __launch_bounds__(256, MOST == 16 ? 1 : (MOST == 8 ? 2 : 4)) reorder_kernel(const ReorderArgs a) {
-  extern __shared__ __align__(16) uint8_t beam_smem[];
-  int* from = reinterpret_cast<int*>(beam_smem);         // row that a beam's row becomes; -1: it stays as it is
-  int* to = from + a.beams;
-  uint8_t* stage = beam_smem + ((2 * a.beams * sizeof(int) + 15) & ~(size_t)15);
-  const int g = blockIdx.z;
-  const BeamTensor t = a.tensors[blockIdx.y];
-  int units = t.units;
-  if (t.unit_tokens > 0 && a.lengths) {
-    const int len = max(0, a.lengths[g]);
-    units = min(units, (len + t.unit_tokens - 1) / t.unit_tokens);
-  }
-  const long run = (long)units * t.unit_bytes / t.width, all = run * t.outer;       // elements of a run, of a row
-  if ((long)blockIdx.x * blockDim.x >= all) return;
+// What rows become: from[w] for beam w's, -1: it stays; all blocks of a group find the same.  False where nothing moves.
+__device__ __forceinline__ bool find_sources(const ReorderArgs& a, const BeamTensor& t, int* from, int* to) {
   bool any = false;
   for (int w = threadIdx.x; w < a.beams; w += blockDim.x) {
-    const long b = (long)g * a.beams;
+    const long b = (long)blockIdx.z * a.beams;
     const int row = a.rows[b + w], p = a.parents[b + w];
     int source = -1;
     bool bad = row < -1 || row >= t.rows || p < -1 || p >= a.beams;
@@ -419,17 +487,84 @@ __global__ void __launch_bounds__(256, MOST == 16 ? 1 : (MOST == 8 ? 2 : 4)) reo
     to[w] = row;
     any |= source >= 0;
   }
-  if (!__syncthreads_or(any)) return;
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (long)gridDim.x * blockDim.x) {
-    const long o = i / run, offset = o * t.outer_stride + (i - o * run) * t.width;
-    switch (t.width) {
-      case 16: move_rows<16, MOST>(t, from, to, a.beams, offset, stage); break;
-      case 8: move_rows<8, MOST>(t, from, to, a.beams, offset, stage); break;
-      case 4: move_rows<4, MOST>(t, from, to, a.beams, offset, stage); break;
-      case 2: move_rows<2, MOST>(t, from, to, a.beams, offset, stage); break;
-      default: move_rows<1, MOST>(t, from, to, a.beams, offset, stage); break;
-    }
+  return __syncthreads_or(any);
+}
+
+// bytes of a run that move
+__device__ __forceinline__ long run_bytes(const ReorderArgs& a, const BeamTensor& t) {
+  int units = t.units;
+  if (t.unit_tokens > 0 && a.lengths) units = min((long)units, ((long)max(0, a.lengths[blockIdx.z]) + t.unit_tokens - 1) / t.unit_tokens);
+  return (long)units * t.unit_bytes;
+}
+
+// A block's share of the positions in a row, `width` bytes each: `move` is called with the offset of each.
+template <typename Move>
+__device__ __forceinline__ void walk_row(const BeamTensor& t, long run, int width, Move move) {
+  const long all = run * t.outer, step = (long)gridDim.x * blockDim.x * width;
+  for (long at = ((long)blockIdx.x * blockDim.x + threadIdx.x) * width; at < all; at += step) {
+    const long o = t.outer == 1 ? 0 : (all <= 0xffffffffl ? (long)((uint32_t)at / (uint32_t)run) : at / run);
+    move(at + o * (t.outer_stride - run));
   }
+}
+
+// Up to MOST beams: what a thread's 16 bytes of all rows become is loaded before the first is stored.  Blocks walk several positions, so that what it
+// takes to find the sources (three loads one behind the other) shows once: 64 rows of 2.1 MB in 4 layers 174 us with one position a thread.
+template <int MOST>
+__global__ void __launch_bounds__(256, MOST == 16 ? 2 : 4) reorder_kernel(const ReorderArgs a) {
+  __shared__ int from[MOST], to[MOST];
+  const BeamTensor t = a.tensors[blockIdx.y];
+  const long run = run_bytes(a, t);
+  if (!find_sources(a, t, from, to) || run == 0) return;
+  walk_row(t, run, 16, [&](long offset) {
+    uint8_t* at = t.base + offset;
+    uint4 v[MOST];
+#pragma unroll
+    for (int w = 0; w < MOST; w++)
+      if (w < a.beams && from[w] >= 0) v[w] = *reinterpret_cast<const uint4*>(at + (long)from[w] * t.row_stride);
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int w = 0; w < MOST; w++)
+      if (w < a.beams && from[w] >= 0) *reinterpret_cast<uint4*>(at + (long)to[w] * t.row_stride) = v[w];
+  });
+}
+
+// Any number of beams and any alignment: a thread's loads go to its column of shared memory (asynchronously where 16 bytes move at once).
+template <int BYTES>
+__device__ __forceinline__ void move_staged(const BeamTensor& t, const int* from, const int* to, int beams, long offset, uint8_t* stage) {
+  using V = typename Bits<BYTES>::type;
+  uint8_t* at = t.base + offset;
+  V* mine = reinterpret_cast<V*>(stage) + threadIdx.x;
+  const int pitch = blockDim.x;
+  for (int w = 0; w < beams; w++) {
+    if (from[w] < 0) continue;
+    const uint8_t* src = at + (long)from[w] * t.row_stride;
+    if constexpr (BYTES == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(mine + w * pitch)), "l"(src) : "memory");
+    else
+      mine[w * pitch] = *reinterpret_cast<const V*>(src);
+  }
+  if constexpr (BYTES == 16) asm volatile("cp.async.wait_all;" ::: "memory");
+  for (int w = 0; w < beams; w++)
+    if (from[w] >= 0) *reinterpret_cast<V*>(at + (long)to[w] * t.row_stride) = mine[w * pitch];
+}
+
+__global__ void __launch_bounds__(256) reorder_staged_kernel(const ReorderArgs a) {
+  extern __shared__ __align__(16) uint8_t beam_smem[];
+  int* from = reinterpret_cast<int*>(beam_smem);
+  int* to = from + a.beams;
+  uint8_t* stage = beam_smem + ((2 * a.beams * sizeof(int) + 15) & ~(size_t)15);
+  const BeamTensor t = a.tensors[blockIdx.y];
+  const long run = run_bytes(a, t);
+  if (!find_sources(a, t, from, to) || run == 0) return;
+  walk_row(t, run, t.width, [&](long offset) {
+    switch (t.width) {
+      case 16: move_staged<16>(t, from, to, a.beams, offset, stage); break;
+      case 8: move_staged<8>(t, from, to, a.beams, offset, stage); break;
+      case 4: move_staged<4>(t, from, to, a.beams, offset, stage); break;
+      case 2: move_staged<2>(t, from, to, a.beams, offset, stage); break;
+      default: move_staged<1>(t, from, to, a.beams, offset, stage); break;
+    }
+  });
 }
 
 }  // namespace b200
@@ -445,10 +580,10 @@ B200_API int b200_beam_select(const b200::SelectArgs* args) {
   if (a.parts < 1 || a.per_part < BEAM_VEC || a.per_part % BEAM_VEC || (long)a.parts * a.per_part > 0x7fffffffL - BEAM_TILE ||
       (long)a.parts * a.per_part < (long)a.vocab + BEAM_VEC - 1)
     return 9932;
-  const int row_smem = (int)sizeof(BeamList<RowKey>), group_smem = (int)sizeof(BeamList<GroupKey>) + a.width * 8;
+  const int row_smem = BEAM_WARPS * list_room(a.k) * (int)sizeof(RowKey), group_smem = (int)sizeof(GroupList) + a.width * 8;
   if (group_smem > 200 * 1024) return 9933;
   const unsigned grid = (unsigned)(rows * a.parts);
-  cudaError_t e = a.fp32 ? allow_smem<&select_rows_kernel<float>>(row_smem) : allow_smem<&select_rows_kernel<__nv_bfloat16>>(row_smem);
+  cudaError_t e = a.fp32 ? allow_smem<&select_rows_kernel<float>>(64 * 1024) : allow_smem<&select_rows_kernel<__nv_bfloat16>>(64 * 1024);
   if (e == cudaSuccess) e = allow_smem<&select_groups_kernel>(200 * 1024);
   if (e != cudaSuccess) return (int)e;
   if (a.fp32) select_rows_kernel<float><<<grid, BEAM_THREADS, row_smem, a.stream>>>(a);
@@ -461,21 +596,31 @@ B200_API int b200_beam_select(const b200::SelectArgs* args) {
 
 B200_API int b200_beam_reorder(const b200::ReorderArgs* args) {
   using namespace b200;
-  const ReorderArgs& a = *args;
-  if (a.groups <= 0 || a.beams <= 0 || a.num_tensors <= 0 || a.chunks <= 0) return 0;
-  if (a.beams > REORDER_BEAMS || a.groups > 65535 || a.num_tensors > 65535) return 9940;
-  const dim3 grid((unsigned)a.chunks, (unsigned)a.num_tensors, (unsigned)a.groups);
-  const int lists = (2 * a.beams * 4 + 15) & ~15;
-  if (a.beams <= 4) reorder_kernel<4><<<grid, 256, lists, a.stream>>>(a);
-  else if (a.beams <= 8) reorder_kernel<8><<<grid, 256, lists, a.stream>>>(a);
-  else if (a.beams <= 16) reorder_kernel<16><<<grid, 256, lists, a.stream>>>(a);
-  else {
-    // 32 threads of up to 128 beams, fewer of more: a block's columns stay within 64 KB
-    const int threads = a.beams <= 128 ? 32 : (a.beams <= 256 ? 16 : (a.beams <= 512 ? 8 : 4));
-    const int smem = lists + a.beams * threads * 16;
-    const cudaError_t e = allow_smem<&reorder_kernel<0>>(80 * 1024);
+  ReorderArgs a = *args;
+  if (a.groups <= 0 || a.beams <= 0 || a.num_tensors <= 0) return 0;
+  if (a.beams > REORDER_BEAMS || a.groups > 65535 || a.num_tensors > 65535 || a.wide < 0 || a.wide > a.num_tensors) return 9940;
+  const int wide = a.beams <= 16 ? a.wide : 0, rest = a.num_tensors - wide;
+  // blocks enough to fill the GPU a few times over, whatever the tensors' and the groups' number
+  if (wide > 0) {
+    const long pairs = (long)wide * a.groups;
+    const dim3 grid((unsigned)((32L * a.sms + pairs - 1) / pairs), (unsigned)wide, (unsigned)a.groups);
+    if (a.beams <= 4) reorder_kernel<4><<<grid, 256, 0, a.stream>>>(a);
+    else if (a.beams <= 8) reorder_kernel<8><<<grid, 256, 0, a.stream>>>(a);
+    else reorder_kernel<16><<<grid, 256, 0, a.stream>>>(a);
+    const int rc = B200_CHECK_LAUNCH();
+    if (rc) return rc;
+  }
+  if (rest > 0) {
+    // a block's columns stay within 64 KB
+    int threads = 256;
+    while (threads * a.beams > 4096 && threads > 4) threads >>= 1;
+    const int smem = ((2 * a.beams * 4 + 15) & ~15) + a.beams * threads * 16;
+    const cudaError_t e = allow_smem<&reorder_staged_kernel>(80 * 1024);
     if (e != cudaSuccess) return (int)e;
-    reorder_kernel<0><<<grid, threads, smem, a.stream>>>(a);
+    a.tensors += wide;
+    const long pairs = (long)rest * a.groups, blocks = 32L * a.sms * (256 / threads);
+    const dim3 grid((unsigned)((blocks + pairs - 1) / pairs), (unsigned)rest, (unsigned)a.groups);
+    reorder_staged_kernel<<<grid, threads, smem, a.stream>>>(a);
   }
   return B200_CHECK_LAUNCH();
 }

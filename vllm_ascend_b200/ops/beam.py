@@ -18,7 +18,7 @@ from . import reference as ref
 # laid out as the source's SelectArgs, BeamTensor and ReorderArgs
 _SELECT = struct.Struct("@11Pq7i")
 _TENSOR = struct.Struct("@P4q4i")
-_REORDER = struct.Struct("@6P4i")
+_REORDER = struct.Struct("@6P5i")
 for _name in ("b200_beam_select", "b200_beam_reorder"):
     _native.register_signature(_name, [c_char_p])
 
@@ -95,12 +95,12 @@ class BeamStates:
     def __init__(self, tensors: list, paged: bool, int4_dim: int):
         self.tensors, self.paged, self.int4_dim = tensors, paged, int4_dim
         self.device = tensors[0].device
-        self._table, self._most = None, 0
-        rows = [_layout(t, paged, int4_dim) for t in tensors]
+        self._table, self._wide = None, 0
+        rows = sorted((_layout(t, paged, int4_dim) for t in tensors), key=lambda r: -r[-1])
         if self.device.type == "cuda":
             packed = b"".join(_TENSOR.pack(*r) for r in rows)
             self._table = torch.frombuffer(bytearray(packed), dtype=torch.uint8).to(self.device)
-            self._most = max(outer * units * unit // width for _, _, _, unit, _, outer, units, _, width in rows)
+            self._wide = sum(r[-1] == 16 for r in rows)
 
 
 def _layout(t: torch.Tensor, paged: bool, int4_dim: int) -> tuple:
@@ -165,7 +165,7 @@ def reorder_beams(states: BeamStates, rows: torch.Tensor, parents: torch.Tensor,
         raise ValueError(f"{groups} groups of {beams} beams: up to 65535 of {MOST_BEAMS}")
     if lengths is not None and (not states.paged or lengths.shape != (groups,) or lengths.dtype != torch.int32 or lengths.get_device() != device):
         raise ValueError(f"lengths int32 [{groups}] on {states.device} for pages, not {lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
-    if groups == 0 or beams == 0 or states._most == 0 and device >= 0:
+    if groups == 0 or beams == 0:
         return
     if device < 0:
         return ref.reorder_beams(states.tensors, rows, parents, lengths, states.int4_dim)
@@ -174,10 +174,10 @@ def reorder_beams(states: BeamStates, rows: torch.Tensor, parents: torch.Tensor,
             return reorder_beams(states, rows, parents, lengths)
     rows, parents = rows.contiguous(), parents.contiguous()
     lengths = None if lengths is None else lengths.contiguous()
-    threads = 256 if beams <= 16 else max(4, min(32, 4096 // beams))
     rc = _native.lib().b200_beam_reorder(_REORDER.pack(
         states._table.data_ptr(), rows.data_ptr(), parents.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
-        _native.status_word(rows.device).data_ptr(), _native.stream_ptr(), len(states.tensors), groups, beams,
-        min(-(-states._most // threads), 1 << 20)))
+        _native.status_word(rows.device).data_ptr(), _native.stream_ptr(), len(states.tensors), groups, beams, states._wide,
+        _native.sm_count(device)))
     _native.check(rc, "beam_reorder")
-    _native.count_launch()
+    wide = states._wide if beams <= 16 else 0
+    _native.count_launch((wide > 0) + (wide < len(states.tensors)))
