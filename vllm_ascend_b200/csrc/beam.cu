@@ -23,6 +23,7 @@ constexpr int BEAM_VEC = 8;                               // elements a thread t
 constexpr int BEAM_TILE = BEAM_THREADS * BEAM_VEC;
 constexpr int BEAM_WARPS = BEAM_THREADS / 32;
 constexpr int BEAM_MOST = 256;                            // k at most
+constexpr int STAGE_BYTES = 64;                           // of a row on their way, a thread
 constexpr int BEAM_ROOM = 4096, BEAM_SLACK = 1024;        // candidates of a group that are looked at together, and that are kept until then
 constexpr float kBeamLog2e = 1.4426950408889634f;
 
@@ -156,75 +157,79 @@ __device__ __forceinline__ float beam_exp2(float x) {
   return y;
 }
 
-// eight elements as they lie in memory
+// Eight elements on their way to a place in shared memory that belongs to the thread: those of the row in [0, end), -inf beside.
 template <typename T>
-struct Vec {
-  uint4 r[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* row, int at, int end) {        // those in [0, end), -inf beside
-    if (at >= 0 && at + BEAM_VEC <= end) {
+__device__ __forceinline__ void bring(T* to, const T* row, int at, int end) {
+  if (at >= 0 && at + BEAM_VEC <= end) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; i++) r[i] = __ldg(reinterpret_cast<const uint4*>(row + at) + i);
-    } else {
-      uint32_t w[4 * (sizeof(T) / 2)];
-#pragma unroll
-      for (int i = 0; i < 4 * ((int)sizeof(T) / 2); i++) {
-        if constexpr (sizeof(T) == 2) {
-          const unsigned short* e = reinterpret_cast<const unsigned short*>(row);
-          const int j = at + 2 * i;
-          w[i] = (j >= 0 && j < end ? e[j] : 0xff80u) | (uint32_t)(j + 1 >= 0 && j + 1 < end ? e[j + 1] : 0xff80u) << 16;
-        } else {
-          w[i] = at + i >= 0 && at + i < end ? __float_as_uint(row[at + i]) : 0xff800000u;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; i++) r[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    }
+    for (int i = 0; i < (int)sizeof(T) / 2; i++)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to) + 16 * i), "l"(reinterpret_cast<const uint4*>(row + at) + i)
+                   : "memory");
+  } else {
+#pragma unroll 1
+    for (int j = 0; j < BEAM_VEC; j++) to[j] = at + j >= 0 && at + j < end ? row[at + j] : T(-INFINITY);
   }
-  __device__ __forceinline__ void get(float* x) const {
-    if constexpr (sizeof(T) == 2) {
-      const uint32_t w[4] = {r[0].x, r[0].y, r[0].z, r[0].w};
+}
+template <typename T>
+__device__ __forceinline__ void take(const T* from, float* x) {
+  const uint4 a = *reinterpret_cast<const uint4*>(from);
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
-    } else {
-      const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
-#pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = __uint_as_float(w[i]);
+    for (int i = 0; i < 4; i++) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
+  } else {
+    const uint4 b = *(reinterpret_cast<const uint4*>(from) + 1);
+    const uint32_t v[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = __uint_as_float(w[i]), x[4 + i] = __uint_as_float(v[i]);
   }
-};
+}
 
 __device__ __forceinline__ bool is_score(float s) { return s > -INFINITY && s < INFINITY; }
 
-// A warp's list: room for k keys and two more steps of 32.
-__host__ __device__ constexpr int list_room(int k) { return (k + 31) / 32 * 32 + 64; }
+// A warp's list: room for k keys and more, and for what a vector of its lanes may add.
+__host__ __device__ constexpr int list_room(int k) { return (k + 31) / 32 * 32 + 64 + 32 * BEAM_VEC; }
 constexpr int LIST_MOST = list_room(BEAM_MOST) / 32;
+// keys that are looked at together in the end: the warps' k best at least
+__host__ __device__ constexpr int list_all(int k) { return BEAM_WARPS * k > 1024 ? BEAM_WARPS * k : 1024; }
 
-// A warp's n keys cut back to their k best, best first; returns the last of them.
-__device__ __noinline__ uint64_t cut_back(RowKey* list, int n, int k) {
+// A warp's n > k different keys cut back to its k best, in no order; returns the last of them, found bit by bit.
+__device__ __noinline__ uint64_t cut_back(uint64_t* list, int n, int k) {
   const int lane = threadIdx.x & 31;
-  RowKey own[LIST_MOST];
-  int rank[LIST_MOST];
+  uint64_t own[LIST_MOST];
   __syncwarp();
+#pragma unroll
+  for (int i = 0; i < LIST_MOST; i++) own[i] = i * 32 + lane < n ? list[i * 32 + lane] : 0;
+  // bits above the highest in which two keys differ are those of all
+  const uint64_t some = __shfl_sync(0xffffffffu, own[0], 0);
+  uint64_t differ = 0;
+#pragma unroll
+  for (int i = 0; i < LIST_MOST; i++) differ |= own[i] ? own[i] ^ some : 0;
+  const uint32_t high = __reduce_or_sync(0xffffffffu, (uint32_t)(differ >> 32)), low = __reduce_or_sync(0xffffffffu, (uint32_t)differ);
+  const int first = high ? 63 - __clz(high) : 31 - __clz(low | 1);
+  uint64_t last = some & ~((2ull << first) - 1);
+  for (int bit = first; bit >= 0; bit--) {
+    const uint64_t next = last | 1ull << bit;
+    int reach = 0;
+#pragma unroll
+    for (int i = 0; i < LIST_MOST; i++) reach += own[i] >= next;
+    reach = __reduce_add_sync(0xffffffffu, reach);
+    if (reach >= k) last = next;
+    if (reach == k) break;
+  }
+  __syncwarp();
+  int at = 0;
 #pragma unroll
   for (int i = 0; i < LIST_MOST; i++) {
-    const int at = i * 32 + lane;
-    own[i].v = at < n ? list[at].v : 0;
-    rank[i] = at < n ? 0 : k;
-  }
-  for (int j = 0; j < n; j++) {
-    const uint64_t v = list[j].v;
-#pragma unroll
-    for (int i = 0; i < LIST_MOST; i++) rank[i] += v > own[i].v;
+    const uint32_t who = __ballot_sync(0xffffffffu, own[i] >= last);
+    if (own[i] >= last) list[at + __popc(who & ((1u << lane) - 1))] = own[i];
+    at += __popc(who);
   }
   __syncwarp();
-#pragma unroll
-  for (int i = 0; i < LIST_MOST; i++)
-    if (rank[i] < k) list[rank[i]] = own[i];
-  __syncwarp();
-  return list[k - 1].v;
+  return last;
 }
 
 template <typename T>
@@ -232,7 +237,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
   extern __shared__ __align__(16) uint8_t beam_smem[];
   __shared__ RowKey slices[BEAM_THREADS], first_bound;
   __shared__ unsigned long long bound;             // what a key has to reach, the k-th best of some that were seen
-  __shared__ int count;
+  __shared__ int held[BEAM_WARPS], count;          // keys in the warps' lists
   __shared__ float warp_max[BEAM_WARPS];
   __shared__ double warp_sum[BEAM_WARPS];
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -242,106 +247,123 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
   const int shift = (int)(((uintptr_t)x0 & 15) / sizeof(T));
   const int from = part * a.per_part - shift, to = min(from + a.per_part, a.vocab);
   const int room = list_room(a.k);
-  RowKey* list = reinterpret_cast<RowKey*>(beam_smem) + warp * room;
-  int held = 0;                                    // keys in the warp's list
-  auto key_of = [&](float x, int at) -> uint64_t { return at >= 0 && at < to ? ((uint64_t)order32(x) << 32) | (uint32_t)~at : 0; };
-  float m = -INFINITY, s = 0.f;
-  auto add = [&](const float* x, float top) {
-    if (top > m) {
-      s *= beam_exp2((m - top) * kBeamLog2e);      // nothing before the first element that is above -inf
-      m = top;
-    }
-    // differences from the maximum are taken before the factor: a product of the maximum would carry its rounding into every term
-    const float under = m == -INFINITY ? 0.f : m;
-    float t[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < BEAM_VEC; j++) t[j & 3] += beam_exp2((x[j] - under) * kBeamLog2e);         // a NaN or +inf: NaN
-    s += (t[0] + t[1]) + (t[2] + t[3]);
+  constexpr int STAGES = STAGE_BYTES / (BEAM_VEC * (int)sizeof(T));
+  T* stage = reinterpret_cast<T*>(beam_smem) + tid * BEAM_VEC;       // [stages][threads][8], a thread's own
+  uint64_t* all = reinterpret_cast<uint64_t*>(beam_smem + BEAM_THREADS * STAGE_BYTES);       // then the lists
+  uint64_t* list = all + list_all(a.k) + warp * room;
+  // Of the elements at -inf only the row's first ones can be wanted: where fewer than k others are, k of them lie in the first 2 k places.
+  auto key_of = [&](float x, int at) -> uint64_t {
+    return at >= 0 && at < to && (x > -INFINITY || at < 2 * a.k) ? ((uint64_t)order32(x) << 32) | (uint32_t)~at : 0;
   };
-  auto top_of = [&](const float* x) -> float {
-    float t = x[0];
-#pragma unroll
-    for (int j = 1; j < BEAM_VEC; j++) t = fmaxf(t, x[j]);
-    return t;
-  };
-  // keys of a vector that reach the bound; all lanes of the warp
-  auto keep = [&](const float* x, int at) {
+  // ---- the bound that the first elements give, 32 a thread (16 of fp32)
+  const int at0 = from + tid * BEAM_VEC;
 #pragma unroll 1
-    for (int j = 0; j < BEAM_VEC; j++) {
-      float v = x[0];                              // x[j] without an index into registers
-#pragma unroll
-      for (int i = 1; i < BEAM_VEC; i++) v = j == i ? x[i] : v;
-      const uint64_t key = key_of(v, at + j);
-      const bool in = key != 0 && key >= *(volatile unsigned long long*)&bound;
-      const uint32_t who = __ballot_sync(0xffffffffu, in);
-      if (who == 0) continue;
-      if (held + 32 > room) {
-        const uint64_t last = cut_back(list, held, a.k);
-        held = a.k;
-        if (lane == 0) atomicMax(&bound, (unsigned long long)last);
-        __syncwarp();
-      }
-      if (in) list[held + __popc(who & ((1u << lane) - 1))].v = key;
-      held += __popc(who);
-    }
-  };
-  // ---- the first 4096 elements and the bound that they give
-  constexpr int AHEAD = 16 / sizeof(T) / 2;        // vectors on their way, 64 bytes a thread: 4 of bf16, 2 of fp32
-  Vec<T> ahead[AHEAD];
-  int at = from + tid * BEAM_VEC;
-#pragma unroll
-  for (int i = 0; i < AHEAD; i++) ahead[i].load(x0, at + i * BEAM_TILE < to ? at + i * BEAM_TILE : a.vocab, a.vocab);
-  float x[BEAM_VEC];
-  ahead[0].get(x);
+  for (int i = 0; i < STAGES; i++) {
+    bring(stage + i * BEAM_TILE, x0, at0 + i * BEAM_TILE < to ? at0 + i * BEAM_TILE : a.vocab, a.vocab);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   RowKey top = RowKey::none();
+#pragma unroll 1
+  for (int i = 0; i < STAGES; i++) {
+    float x[BEAM_VEC], t = -INFINITY;
+    take(stage + i * BEAM_TILE, x);
+    int first = -1;                                // of its largest elements, inside the part
 #pragma unroll
-  for (int j = 0; j < BEAM_VEC; j++) {
-    const RowKey key = {key_of(x[j], at + j)};
+    for (int j = 0; j < BEAM_VEC; j++) {
+      const int e = at0 + i * BEAM_TILE + j;
+      if (e >= 0 && e < to && (first < 0 || x[j] > t)) t = x[j], first = e;       // a NaN stays where it comes first: the row has no candidates
+    }
+    const RowKey key = {first >= 0 ? key_of(t, first) : 0ull};
     if (key.above(top)) top = key;
   }
   top = slice_bound(top, a.k, slices, &first_bound);
   if (tid == 0) bound = top.v;
+  if (lane == 0) held[warp] = 0;
   __syncthreads();
-  bool first = true;
   // ---- all of the part, a warp by itself
-  for (int base = from; base < to; base += AHEAD * BEAM_TILE) {
-#pragma unroll
-    for (int i = 0; i < AHEAD; i++) {
-      const int here = base + i * BEAM_TILE;
-      if (here >= to) break;
-      const int mine = here + tid * BEAM_VEC;
-      ahead[i].get(x);
-      const int next = mine + AHEAD * BEAM_TILE;
-      if (here + AHEAD * BEAM_TILE < to) ahead[i].load(x0, next < to ? next : a.vocab, a.vocab);
-      const float t = top_of(x);
-      if (mine < to) add(x, t);
-      const float reach = unorder32((uint32_t)(*(volatile unsigned long long*)&bound >> 32));
-      if (__any_sync(0xffffffffu, mine < to && (first || !(t < reach)))) keep(x, mine);
-      first = false;
+  float m = -INFINITY, s = 0.f, reach = 0.f;
+  uint64_t least = 0;
+  int place = 0, st = 0;
+#pragma unroll 1
+  for (int mine = at0; mine - tid * BEAM_VEC < to; mine += BEAM_TILE) {
+    if (st == 0) {                                 // the bound, as others have raised it
+      least = *(volatile unsigned long long*)&bound;
+      reach = least ? unorder32((uint32_t)(least >> 32)) : -INFINITY;
+      place = least ? (int)~(uint32_t)least : a.vocab;       // equal values count up to there
     }
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    float x[BEAM_VEC];
+    take(stage + st * BEAM_TILE, x);
+    float t = x[0];
+#pragma unroll
+    for (int j = 1; j < BEAM_VEC; j++) t = fmaxf(t, x[j]);
+    if (mine < to) {
+      if (t > m) {
+        s *= beam_exp2((m - t) * kBeamLog2e);      // nothing before the first element that is above -inf
+        m = t;
+      }
+      // differences from the maximum are taken before the factor: a product of the maximum would carry its rounding into every term
+      const float under = m == -INFINITY ? 0.f : m;
+      float u[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < BEAM_VEC; j++) u[j & 3] += beam_exp2((x[j] - under) * kBeamLog2e);       // a NaN or +inf: NaN
+      s += (u[0] + u[1]) + (u[2] + u[3]);
+    }
+    const bool hit = mine < to && (t > reach || (reach > -INFINITY ? t == reach && mine <= place : mine < 2 * a.k));
+    if (__any_sync(0xffffffffu, hit)) {
+      if (hit) {
+        uint32_t which = 0;
+#pragma unroll
+        for (int j = 0; j < BEAM_VEC; j++) which |= x[j] >= reach ? 1u << j : 0u;
+        while (which) {
+          const int j = __ffs(which) - 1;
+          which &= which - 1;
+          const uint64_t key = key_of((float)stage[st * BEAM_TILE + j], mine + j);
+          if (key != 0 && key >= least) list[atomicAdd(&held[warp], 1)] = key;
+        }
+      }
+      __syncwarp();
+      const int n = *(volatile int*)&held[warp];
+      if (n > room - 32 * BEAM_VEC) {              // the next vector has room
+        const uint64_t last = cut_back(list, n, a.k);
+        if (lane == 0) {
+          held[warp] = a.k;
+          atomicMax(&bound, (unsigned long long)last);
+        }
+      }
+      __syncwarp();
+    }
+    const int next = mine + STAGES * BEAM_TILE;
+    if (next < to) bring(stage + st * BEAM_TILE, x0, next, a.vocab);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (++st == STAGES) st = 0;
   }
   // ---- the block's k best
-  for (int i = held + lane; i < room; i += 32) list[i] = RowKey::none();
-  if (tid == 0) count = 0;
-  __syncthreads();
-  RowKey* all = reinterpret_cast<RowKey*>(beam_smem);
-  const uint64_t least = bound;
-  uint64_t mine[LIST_MOST];
-#pragma unroll
-  for (int i = 0; i < LIST_MOST; i++) {
-    const int j = tid + i * BEAM_THREADS;
-    mine[i] = j < BEAM_WARPS * room ? all[j].v : 0;
+  {
+    __syncthreads();
+    int n = 0;
+    for (int i = 0; i < BEAM_WARPS; i++) n += held[i];
+    const bool many = n > list_all(a.k);           // values in an order against the bound
+    n = held[warp];
+    if (many && n > a.k) {
+      const uint64_t last = cut_back(list, n, a.k);
+      if (lane == 0) atomicMax(&bound, (unsigned long long)last);
+      n = a.k;
+    }
+    if (tid == 0) count = 0;
+    __syncthreads();
+    const uint64_t least = bound;
+    for (int i = lane; i < n; i += 32)
+      if (list[i] >= least) all[atomicAdd(&count, 1)] = list[i];
+    __syncthreads();
   }
+  const int found = count;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < LIST_MOST; i++)
-    if (mine[i] != 0 && mine[i] >= least) all[atomicAdd(&count, 1)].v = mine[i];
-  __syncthreads();
-  const int n = count;
-  __syncthreads();
-  const int got = select_best<RowKey, LIST_MOST>(all, n, a.k, all, slices, &first_bound, &count);
+  RowKey* best = reinterpret_cast<RowKey*>(all);
+  const int got = select_best<RowKey, BEAM_MOST * BEAM_WARPS / BEAM_THREADS>(best, found, a.k, best, slices, &first_bound, &count);
   const long slot = (long)row * a.parts + part;
-  for (int i = tid; i < got; i += BEAM_THREADS) a.keys[slot * a.k + i] = all[i].v;
+  for (int i = tid; i < got; i += BEAM_THREADS) a.keys[slot * a.k + i] = all[i];
   // ---- the part's maximum and its sum under it
   float high = m;
 #pragma unroll
@@ -580,10 +602,10 @@ B200_API int b200_beam_select(const b200::SelectArgs* args) {
   if (a.parts < 1 || a.per_part < BEAM_VEC || a.per_part % BEAM_VEC || (long)a.parts * a.per_part > 0x7fffffffL - BEAM_TILE ||
       (long)a.parts * a.per_part < (long)a.vocab + BEAM_VEC - 1)
     return 9932;
-  const int row_smem = BEAM_WARPS * list_room(a.k) * (int)sizeof(RowKey), group_smem = (int)sizeof(GroupList) + a.width * 8;
+  const int row_smem = BEAM_THREADS * STAGE_BYTES + (BEAM_WARPS * list_room(a.k) + list_all(a.k)) * 8, group_smem = (int)sizeof(GroupList) + a.width * 8;
   if (group_smem > 200 * 1024) return 9933;
   const unsigned grid = (unsigned)(rows * a.parts);
-  cudaError_t e = a.fp32 ? allow_smem<&select_rows_kernel<float>>(64 * 1024) : allow_smem<&select_rows_kernel<__nv_bfloat16>>(64 * 1024);
+  cudaError_t e = a.fp32 ? allow_smem<&select_rows_kernel<float>>(144 * 1024) : allow_smem<&select_rows_kernel<__nv_bfloat16>>(144 * 1024);
   if (e == cudaSuccess) e = allow_smem<&select_groups_kernel>(200 * 1024);
   if (e != cudaSuccess) return (int)e;
   if (a.fp32) select_rows_kernel<float><<<grid, BEAM_THREADS, row_smem, a.stream>>>(a);
