@@ -6,7 +6,7 @@
 // Selection reads the logits once.  A block walks a part of a row: every thread keeps a running maximum and the sum of exponentials
 // under it; elements that reach the bound of the k-th best so far go to their warp's list in shared memory.  Within a row totals are
 // ordered as logits are, so the lists need no sum.  The bound begins with the first 4096 elements: the k-th largest of the maxima of
-// at least 2 k slices of them, which k elements or more reach, and about k for values in no order.  A warp whose list is full cuts it back to its
+// slices of them, which k elements or more reach, and not many more where values are in no order.  A warp whose list is full cuts it back to its
 // k best, whose last raises the bound for all.  Keys carry the value and, below it, the place: no two are equal, ties go to the
 // lowest place by themselves, and rows of equal values (masked ones) put nothing behind their first into a list.
 // Bound by HBM for many rows: about six instructions and an exponential an element are 0.6 of what an SM issues at its share of the bytes.
@@ -77,16 +77,14 @@ struct GroupKey {
 };
 
 // ---------------------------------------------------------------- the k best of a list
-__device__ __forceinline__ int slice_lanes(int k) {       // lanes that share a slice: 2 k slices of 512 threads at least
-  int lanes = 32;
-  while (BEAM_THREADS / lanes < 2 * k && lanes > 1) lanes >>= 1;
-  return lanes;
-}
-
-// The k-th largest of the maxima of the block's slices, `top` a thread's; none where fewer than k slices have elements.  Ends with a barrier.
+// The k-th largest of the maxima of slices of n elements, `top` that of a thread's (element i belongs to thread i mod 512); none where fewer than k
+// slices have elements.  A slice is the lanes that leave 4 k of them, one at least.  Ends with a barrier.
 template <typename Key>
-__device__ __forceinline__ Key slice_bound(Key top, int k, Key* slices, Key* bound) {
-  const int tid = threadIdx.x, lanes = slice_lanes(k), count = BEAM_THREADS / lanes;
+__device__ __forceinline__ Key slice_bound(Key top, int n, int k, Key* slices, Key* bound) {
+  const int tid = threadIdx.x;
+  int lanes = 32;
+  while (min(n, BEAM_THREADS) < 4 * k * lanes && lanes > 1) lanes >>= 1;
+  const int count = (min(n, BEAM_THREADS) + lanes - 1) / lanes;
   for (int o = 1; o < lanes; o <<= 1) {
     const Key other = top.other_lane(o);
     if (other.above(top)) top = other;
@@ -95,6 +93,7 @@ __device__ __forceinline__ Key slice_bound(Key top, int k, Key* slices, Key* bou
   if (tid == 0) *bound = Key::none();
   __syncthreads();
   int rank = 0;                                           // all lanes of a slice count
+#pragma unroll 4
   for (int j = tid % lanes; j < count; j += lanes) rank += slices[j].above(top);
   for (int o = 1; o < lanes; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
   if (tid % lanes == 0 && rank == k - 1) *bound = top;    // one slice, but for those without an element, all of them none
@@ -102,28 +101,32 @@ __device__ __forceinline__ Key slice_bound(Key top, int k, Key* slices, Key* bou
   return *bound;
 }
 
-// The k best of n keys, best first, into out[0..k); returns how many.  All threads of the block, the keys written before a barrier; `keys` is
-// worked in, out may be part of it.  Ends with a barrier.
-template <typename Key, int PER>
-__device__ int select_best(Key* keys, int n, int k, Key* out, Key* slices, Key* bound, int* count) {
+// The k best of n keys, best first, into keys[0..k); returns how many.  All threads of the block, the keys written before a barrier; `other` has
+// room for half of the keys, 256 at least.  Ends with a barrier.  Loops stay rolled here and in the group's kernel: code that runs once takes as long as it
+// is fetched from memory.
+template <typename Key>
+__device__ int select_best(Key* keys, Key* other, int n, int k, Key* slices, Key* bound, int* count) {
   const int tid = threadIdx.x;
-  // Only k slices reach the bound, and 2 k slices share the threads: a pass leaves 256 elements at most for every element that a thread
-  // holds, 2560, 1280, 768, 512, 256 in turn; values in no order take one pass.
+  Key* from = keys;
+  // Only k slices reach the bound: a quarter of the elements at most, or where a slice is a thread, its k elements for every 512; values in no order
+  // take one pass.
   for (bool more = n > max(2 * k, 64); more; more = n > max(3 * k, 256)) {
-    Key mine[PER], top = Key::none();
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const int at = tid + i * BEAM_THREADS;
-      mine[i] = at < n ? keys[at] : Key::none();
-      if (mine[i].above(top)) top = mine[i];
-    }
+    Key top = Key::none();
+#pragma unroll 1
+    for (int i = tid; i < n; i += BEAM_THREADS)
+      if (from[i].above(top)) top = from[i];
     if (tid == 0) *count = 0;
-    const Key least = slice_bound(top, k, slices, bound);
-#pragma unroll
-    for (int i = 0; i < PER; i++)
-      if (mine[i].above(Key::none()) && !least.above(mine[i])) keys[atomicAdd(count, 1)] = mine[i];
+    const Key least = slice_bound(top, n, k, slices, bound);
+#pragma unroll 1
+    for (int i = tid; i < n; i += BEAM_THREADS) {
+      const Key key = from[i];
+      if (!least.above(key)) other[atomicAdd(count, 1)] = key;
+    }
     __syncthreads();
     n = *count;
+    Key* swap = from;
+    from = other;
+    other = swap;
     __syncthreads();
   }
   // ranked by counting: 3 k elements at most, the block's threads shared between them
@@ -135,17 +138,19 @@ __device__ int select_best(Key* keys, int n, int k, Key* out, Key* slices, Key* 
 #pragma unroll
   for (int i = 0; i < 2; i++) {
     const int at = i * BEAM_THREADS + tid / each;         // a second one only where each is 1
-    own[i] = at < n && (i == 0 || each == 1) ? keys[at] : Key::none();
+    own[i] = at < n && (i == 0 || each == 1) ? from[at] : Key::none();
     rank[i] = 0;
-    if (own[i].above(Key::none()))
-      for (int j = tid % each; j < n; j += each) rank[i] += keys[j].above(own[i]);
+    if (own[i].above(Key::none())) {
+#pragma unroll 4
+      for (int j = tid % each; j < n; j += each) rank[i] += from[j].above(own[i]);
+    }
     if (i == 0)
       for (int o = 1; o < each; o <<= 1) rank[i] += __shfl_xor_sync(0xffffffffu, rank[i], o);
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; i++)
-    if (tid % each == 0 && own[i].above(Key::none()) && rank[i] < k) out[rank[i]] = own[i];
+    if (tid % each == 0 && own[i].above(Key::none()) && rank[i] < k) keys[rank[i]] = own[i];
   __syncthreads();
   return min(n, k);
 }
@@ -191,8 +196,10 @@ __device__ __forceinline__ void take(const T* from, float* x) {
 __device__ __forceinline__ bool is_score(float s) { return s > -INFINITY && s < INFINITY; }
 
 // A warp's list: room for k keys and more, and for what a vector of its lanes may add.
-__host__ __device__ constexpr int list_room(int k) { return (k + 31) / 32 * 32 + 64 + 32 * BEAM_VEC; }
+__host__ __device__ constexpr int list_room(int k) { return (k + 31) / 32 * 32 + 32 + 32 * BEAM_VEC; }
 constexpr int LIST_MOST = list_room(BEAM_MOST) / 32;
+static_assert(BEAM_MOST * BEAM_WARPS * 8 <= BEAM_THREADS * STAGE_BYTES, "the warps' best lie in the place of the elements");
+static_assert(BEAM_WARPS * list_room(1) >= BEAM_THREADS + BEAM_MOST * BEAM_WARPS / 2, "slices and half of the keys lie in the place of the lists");
 // keys that are looked at together in the end: the warps' k best at least
 __host__ __device__ constexpr int list_all(int k) { return BEAM_WARPS * k > 1024 ? BEAM_WARPS * k : 1024; }
 
@@ -235,7 +242,7 @@ __device__ __noinline__ uint64_t cut_back(uint64_t* list, int n, int k) {
 template <typename T>
 __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const SelectArgs a) {
   extern __shared__ __align__(16) uint8_t beam_smem[];
-  __shared__ RowKey slices[BEAM_THREADS], first_bound;
+  __shared__ RowKey first_bound;
   __shared__ unsigned long long bound;             // what a key has to reach, the k-th best of some that were seen
   __shared__ int held[BEAM_WARPS], count;          // keys in the warps' lists
   __shared__ float warp_max[BEAM_WARPS];
@@ -249,8 +256,9 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
   const int room = list_room(a.k);
   constexpr int STAGES = STAGE_BYTES / (BEAM_VEC * (int)sizeof(T));
   T* stage = reinterpret_cast<T*>(beam_smem) + tid * BEAM_VEC;       // [stages][threads][8], a thread's own
-  uint64_t* all = reinterpret_cast<uint64_t*>(beam_smem + BEAM_THREADS * STAGE_BYTES);       // then the lists
-  uint64_t* list = all + list_all(a.k) + warp * room;
+  uint64_t* lists = reinterpret_cast<uint64_t*>(beam_smem + BEAM_THREADS * STAGE_BYTES);
+  uint64_t* list = lists + warp * room;
+  RowKey* slices = reinterpret_cast<RowKey*>(lists);       // while there are no lists, and when they have been read
   // Of the elements at -inf only the row's first ones can be wanted: where fewer than k others are, k of them lie in the first 2 k places.
   auto key_of = [&](float x, int at) -> uint64_t {
     return at >= 0 && at < to && (x > -INFINITY || at < 2 * a.k) ? ((uint64_t)order32(x) << 32) | (uint32_t)~at : 0;
@@ -263,22 +271,19 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
-  RowKey top = RowKey::none();
-#pragma unroll 1
-  for (int i = 0; i < STAGES; i++) {
-    float x[BEAM_VEC], t = -INFINITY;
-    take(stage + i * BEAM_TILE, x);
-    int first = -1;                                // of its largest elements, inside the part
+  float high = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < BEAM_VEC; j++) {
-      const int e = at0 + i * BEAM_TILE + j;
-      if (e >= 0 && e < to && (first < 0 || x[j] > t)) t = x[j], first = e;       // a NaN stays where it comes first: the row has no candidates
+  for (int i = 0; i < STAGES; i++) {
+    float x[BEAM_VEC];
+    take(stage + i * BEAM_TILE, x);
+    if (at0 + i * BEAM_TILE < to) {
+#pragma unroll
+      for (int j = 0; j < BEAM_VEC; j++) high = fmaxf(high, x[j]);
     }
-    const RowKey key = {first >= 0 ? key_of(t, first) : 0ull};
-    if (key.above(top)) top = key;
   }
-  top = slice_bound(top, a.k, slices, &first_bound);
-  if (tid == 0) bound = top.v;
+  // told apart by their threads; of the bound the value counts, all that equal it reach it
+  const RowKey top = slice_bound(RowKey{high > -INFINITY ? ((uint64_t)order32(high) << 32) | (uint32_t)~tid : 0ull}, BEAM_THREADS, a.k, slices, &first_bound);
+  if (tid == 0) bound = top.v >> 32 << 32;
   if (lane == 0) held[warp] = 0;
   __syncthreads();
   // ---- all of the part, a warp by itself
@@ -290,7 +295,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
     if (st == 0) {                                 // the bound, as others have raised it
       least = *(volatile unsigned long long*)&bound;
       reach = least ? unorder32((uint32_t)(least >> 32)) : -INFINITY;
-      place = least ? (int)~(uint32_t)least : a.vocab;       // equal values count up to there
+      place = (uint32_t)least ? (int)~(uint32_t)least : a.vocab;       // equal values count up to there
     }
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
     float x[BEAM_VEC];
@@ -339,7 +344,9 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
     asm volatile("cp.async.commit_group;" ::: "memory");
     if (++st == STAGES) st = 0;
   }
-  // ---- the block's k best
+  // ---- the block's k best, in the place of the elements
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  uint64_t* all = reinterpret_cast<uint64_t*>(beam_smem);
   {
     __syncthreads();
     int n = 0;
@@ -354,6 +361,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
     if (tid == 0) count = 0;
     __syncthreads();
     const uint64_t least = bound;
+#pragma unroll 1
     for (int i = lane; i < n; i += 32)
       if (list[i] >= least) all[atomicAdd(&count, 1)] = list[i];
     __syncthreads();
@@ -361,11 +369,11 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
   const int found = count;
   __syncthreads();
   RowKey* best = reinterpret_cast<RowKey*>(all);
-  const int got = select_best<RowKey, BEAM_MOST * BEAM_WARPS / BEAM_THREADS>(best, found, a.k, best, slices, &first_bound, &count);
+  const int got = select_best<RowKey>(best, slices + BEAM_THREADS, found, a.k, slices, &first_bound, &count);
   const long slot = (long)row * a.parts + part;
   for (int i = tid; i < got; i += BEAM_THREADS) a.keys[slot * a.k + i] = all[i];
   // ---- the part's maximum and its sum under it
-  float high = m;
+  high = m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
   if (lane == 0) warp_max[warp] = high;
@@ -377,9 +385,12 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) warp_sum[warp] = sum;
   __syncthreads();
+  if (tid < 32) {
+    sum = lane < BEAM_WARPS ? warp_sum[lane] : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
   if (tid == 0) {
-    sum = 0.0;
-    for (int i = 0; i < BEAM_WARPS; i++) sum += warp_sum[i];
     a.maxima[slot] = high;
     a.sums[slot] = sum;
     a.counts[slot] = got;
@@ -388,11 +399,40 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
 
 // ---------------------------------------------------------------- groups
 struct GroupList {
-  GroupKey keys[BEAM_ROOM + BEAM_SLACK];
+  GroupKey keys[BEAM_ROOM + BEAM_SLACK], other[(BEAM_ROOM + BEAM_SLACK) / 2];
   GroupKey slices[BEAM_THREADS];
   GroupKey bound;
   int count;
 };
+
+// e^x for x <= 0 and log x for x >= 1 in 64 bits, by their series: short loops where the library's functions are a few hundred instructions that a
+// kernel of this length waits for.
+__constant__ double kInverseOdd[16] = {1., 1. / 3, 1. / 5, 1. / 7, 1. / 9, 1. / 11, 1. / 13, 1. / 15, 1. / 17, 1. / 19, 1. / 21, 1. / 23,
+                                           1. / 25, 1. / 27, 1. / 29, 1. / 31};
+__constant__ double kInverse[14] = {1., 1., 1. / 2, 1. / 3, 1. / 4, 1. / 5, 1. / 6, 1. / 7, 1. / 8, 1. / 9, 1. / 10, 1. / 11, 1. / 12, 1. / 13};
+__device__ __forceinline__ double series_exp(double x) {       // e^x = 2^n e^r, |r| <= log(2) / 2
+  if (x < -700.) return 0.;
+  const double n = rint(x * 1.4426950408889634), r = x - n * 0.69314718055994531;
+  double e = 1.;
+#pragma unroll 1
+  for (int i = 13; i > 0; i--) e = 1. + e * r * kInverse[i];
+  return e * __longlong_as_double((long long)(1023 + (int)n) << 52);
+}
+__device__ __forceinline__ double series_log(double x) {       // log 2^n m = n log 2 + 2 atanh((m - 1) / (m + 1)), m in [0.75, 1.5)
+  const uint64_t b = (uint64_t)__double_as_longlong(x);
+  int n = (int)(b >> 52) - 1023;
+  double m = __longlong_as_double((long long)((b & 0xfffffffffffffull) | 0x3ff0000000000000ull));
+  if (m >= 1.5) m *= 0.5, n++;
+  const double d = m + 1.;
+  double inv = (double)(1.f / (float)d);
+  inv = inv * (2. - d * inv);
+  inv = inv * (2. - d * inv);
+  const double z = (m - 1.) * inv, q = z * z;                  // |z| <= 0.2: sixteen terms are 3e-24
+  double t = 0.;
+#pragma unroll 1
+  for (int i = 15; i >= 0; i--) t = t * q + kInverseOdd[i];
+  return n * 0.69314718055994531 + 2. * z * t;
+}
 
 __global__ void __launch_bounds__(BEAM_THREADS, 1) select_groups_kernel(const SelectArgs a) {
   extern __shared__ __align__(16) uint8_t beam_smem[];
@@ -410,11 +450,11 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1) select_groups_kernel(const Se
       for (int p = lane; p < a.parts; p += 32) {
         const float mp = a.maxima[row * a.parts + p];
         const double sp = a.sums[row * a.parts + p];
-        sum += mp == -INFINITY ? sp : sp * exp((double)mp - (double)top);
+        sum += mp == -INFINITY ? sp : sp * series_exp((double)mp - (double)top);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (top > -INFINITY && top < INFINITY && sum > 0.0 && sum < 1e300) l = (double)top + log(sum);      // NaN fails both
+      if (top > -INFINITY && top < INFINITY && sum >= 1.0 && sum < 1e300) l = (double)top + series_log(sum);      // the largest adds 1; NaN fails all
     }
     if (lane == 0) norm[w] = l;
   }
@@ -426,6 +466,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1) select_groups_kernel(const Se
   for (int base = 0; base < all; base += BEAM_ROOM) {
     if (tid == 0) list.count = n;
     __syncthreads();
+#pragma unroll 1
     for (int i = base + tid; i < min(base + BEAM_ROOM, all); i += BEAM_THREADS) {
       const int w = i / per_beam, j = i - w * per_beam, p = j / a.k, c = j - p * a.k;
       const long row = (long)g * a.width + w, slot = row * a.parts + p;
@@ -444,7 +485,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1) select_groups_kernel(const Se
     n = list.count;
     __syncthreads();
     if (n > BEAM_SLACK || base + BEAM_ROOM >= all) {
-      n = select_best<GroupKey, (BEAM_ROOM + BEAM_SLACK) / BEAM_THREADS>(list.keys, n, a.k, list.keys, list.slices, &list.bound, &list.count);
+      n = select_best<GroupKey>(list.keys, list.other, n, a.k, list.slices, &list.bound, &list.count);
       if (n == a.k) least = list.keys[a.k - 1];
       __syncthreads();
     }
@@ -602,10 +643,10 @@ B200_API int b200_beam_select(const b200::SelectArgs* args) {
   if (a.parts < 1 || a.per_part < BEAM_VEC || a.per_part % BEAM_VEC || (long)a.parts * a.per_part > 0x7fffffffL - BEAM_TILE ||
       (long)a.parts * a.per_part < (long)a.vocab + BEAM_VEC - 1)
     return 9932;
-  const int row_smem = BEAM_THREADS * STAGE_BYTES + (BEAM_WARPS * list_room(a.k) + list_all(a.k)) * 8, group_smem = (int)sizeof(GroupList) + a.width * 8;
+  const int row_smem = BEAM_THREADS * STAGE_BYTES + BEAM_WARPS * list_room(a.k) * 8, group_smem = (int)sizeof(GroupList) + a.width * 8;
   if (group_smem > 200 * 1024) return 9933;
   const unsigned grid = (unsigned)(rows * a.parts);
-  cudaError_t e = a.fp32 ? allow_smem<&select_rows_kernel<float>>(144 * 1024) : allow_smem<&select_rows_kernel<__nv_bfloat16>>(144 * 1024);
+  cudaError_t e = a.fp32 ? allow_smem<&select_rows_kernel<float>>(112 * 1024) : allow_smem<&select_rows_kernel<__nv_bfloat16>>(112 * 1024);
   if (e == cudaSuccess) e = allow_smem<&select_groups_kernel>(200 * 1024);
   if (e != cudaSuccess) return (int)e;
   if (a.fp32) select_rows_kernel<float><<<grid, BEAM_THREADS, row_smem, a.stream>>>(a);
