@@ -55,6 +55,9 @@ class AttentionMetadata:
     mrope_positions: Optional[torch.Tensor] = None
     pcp: object = None                      # attention.pcp.PCPMeta on split prefill steps
     deepstack: object = None                # (rows [n], features [L, n, H]) added after the first L layers
+    # sequences that share prefixes: (int32 [groups + 1] first sequences, int32 [groups] prefix lengths), and the step's plan
+    shared_groups: Optional[tuple] = None
+    shared: object = None                   # ops.SharedPrefixPlan
     # decode-context-parallel / extras
     dcp_world_size: int = 1
     dcp_rank: int = 0

@@ -42,6 +42,7 @@ class BatchDescriptor:
     uniform_decode: bool = True
     query_len: int = 1            # tokens per sequence (1 + speculative tokens)
     has_lora: bool = False
+    shared_prefixes: bool = False      # attention by a plan for prefixes that sequences share
 
 
 @dataclass

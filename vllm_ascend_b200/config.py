@@ -672,3 +672,4 @@ class EngineConfig:
     enable_lora: bool = False
     max_loras: int = 4
     max_lora_rank: int = 64
+    disable_cascade_attn: bool = True       # False: decode batches with a common prefix read it once (beam search always may)

@@ -390,7 +390,8 @@ class LLM:
                  decode_context_parallel_size: int = 1, prefill_context_parallel_size: int = 1,
                  enable_lora: bool = False, max_loras: int = 4,
                  max_lora_rank: int = 64, async_scheduling: Optional[bool] = None, load_format: str = "auto",
-                 model_loader_extra_config: Optional[dict] = None, kv_cache_dtype: str = "auto", **unused):
+                 model_loader_extra_config: Optional[dict] = None, kv_cache_dtype: str = "auto",
+                 disable_cascade_attn: bool = True, **unused):
         mcfg = model if isinstance(model, ModelConfig) else get_model_config(model)
         if dtype:
             mcfg.dtype = dtype
@@ -428,7 +429,7 @@ class LLM:
             speculative_config=speculative_config,
             enable_sleep_mode=enable_sleep_mode, enable_lora=enable_lora, max_loras=max_loras,
             max_lora_rank=max_lora_rank, async_scheduling=async_scheduling, load_format=load_format,
-            model_loader_extra_config=model_loader_extra_config)
+            model_loader_extra_config=model_loader_extra_config, disable_cascade_attn=disable_cascade_attn)
         if device == "cuda":
             cfg.scheduler.decode_batch_alignment = 256
         from ..platform_config import check_and_update_config
@@ -470,16 +471,19 @@ class LLM:
 
     def beam_search(self, prompts, beam_width: int = 4, max_tokens: int = 16, length_penalty: float = 1.0,
                     ignore_eos: bool = False, temperature: float = 0.0) -> list[list[dict]]:
-        """Beam search over the engine: every round extends all live beams of all prompts by one
-        token in ONE batch (``logprobs = 2 * beam_width`` candidates each; automatic prefix caching
-        makes a round cost one decode step per beam), keeps the ``beam_width`` best continuations
-        per prompt by cumulative log-probability and retires beams that emit the end token.
+        """Beam search over the engine: every round extends all live beams of all prompts by one token in ONE batch, keeps the ``beam_width`` best
+        continuations per prompt by cumulative log-probability and retires beams that emit the end token.  Single-GPU engines without drafts,
+        connectors or other requests at work select on the device (``engine/beam.py``): a round is one decode step, beams share their prompt's pages.
+        Others ask for ``2 * beam_width`` log-probabilities of every beam as a request of its own each round (with prefix caching, one decode step too).
         Returns, per prompt, the ``beam_width`` best sequences as dicts ``{"tokens",
         "cum_logprob", "score"}`` with score = cum_logprob / len ** length_penalty."""
         del temperature
-        eos = self.engine.eos_token_id
+        from . import beam
         width = int(beam_width)
         plist = [list(p["prompt_token_ids"]) if isinstance(p, dict) else list(p) for p in prompts]
+        if width >= 1 and max_tokens >= 1 and beam.on_device(self.engine, plist, width, max_tokens):
+            return beam.BeamSearch(self.engine, width, max_tokens, length_penalty, ignore_eos).run(plist)
+        eos = self.engine.eos_token_id
         live = [[(p, 0.0)] for p in plist]              # per prompt: (tokens, cum_logprob)
         done: list[list[tuple]] = [[] for _ in plist]
         sp = SamplingParams(temperature=0.0, max_tokens=1, logprobs=2 * width, ignore_eos=True)

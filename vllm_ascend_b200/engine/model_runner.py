@@ -125,6 +125,9 @@ class ModelRunner:
         self.state_meta = torch.zeros((2, B), dtype=i32, device=device)     # [slot; has_initial_state]
         self._h_sampled2 = [torch.zeros(B, dtype=i64, pin_memory=pin) for _ in range(2)]   # async steps
         self._async_flip = 0
+        self.share_prefixes = not cfg.disable_cascade_attn      # look for common prefixes in decode batches
+        self._shared_meta = torch.zeros((2, B + 1), dtype=i32, device=device)      # [first sequences; prefix lengths] of groups
+        self._shared_asked: dict[int, int] = {}                 # capture size -> steps that shared prefixes and had no graph
         # ---- CUDA graphs
         self.graphs: dict[tuple, object] = {}     # (capture size, has_lora) -> BatchDescriptor
         self.graph_wrapper = None
@@ -550,6 +553,15 @@ class ModelRunner:
             positions=self.positions[:Tp], query_start_loc_cpu=qsl_cpu, seq_lens_cpu=sl_cpu,
             attn_state=state, num_decodes=nd, num_decode_tokens=ndt, num_prefills=npf,
             num_input_tokens=Tp)
+        if so.shared_groups:
+            firsts = np.full(Bp + 1, B, dtype=np.int32)          # groups behind the last are empty
+            prefixes = np.zeros(Bp, dtype=np.int32)
+            np.cumsum([n for n, _ in so.shared_groups], out=firsts[1:len(so.shared_groups) + 1])
+            firsts[0] = 0
+            prefixes[:len(so.shared_groups)] = [p for _, p in so.shared_groups]
+            self._shared_meta[0, :Bp + 1].copy_(self._to_dev(torch.from_numpy(firsts)))
+            self._shared_meta[1, :Bp].copy_(self._to_dev(torch.from_numpy(prefixes)))
+            meta.shared_groups = (self._shared_meta[0, :Bp + 1], self._shared_meta[1, :Bp])
         meta.dcp_interleave = self.dcp_interleave
         if self.dcp_size > 1:
             from ..attention.dcp import local_seq_lens
@@ -680,6 +692,71 @@ class ModelRunner:
         compile-time constant of the captured graph."""
         return ops.choose_num_splits(batch, Hkv, self.max_model_len, self.sm_count)
 
+    # ------------------------------------------------------------------ beams
+    def beam_states(self) -> tuple:
+        """(handle of all caches of pages, handle of all states of batch rows) for ``ops.reorder_beams``, None where a model has none."""
+        pages, rows, seen = [], [], set()
+        for layer, cache in zip(self.model.layers, self.kv_caches):
+            linear = getattr(layer.self_attn, "is_linear_attention", False)
+            own = len(cache) if linear else len(self._extra_states(layer.self_attn))
+            for i, t in enumerate(cache):
+                if t.data_ptr() not in seen:                   # a layer may read another one's cache
+                    seen.add(t.data_ptr())
+                    (rows if i >= len(cache) - own else pages).append(t)
+        int4 = self._attn_layer().D if self._kv_int4() else 0
+        return (ops.beam_states(pages, paged=True, int4_dim=int4) if pages else None, ops.beam_states(rows) if rows else None)
+
+    # ------------------------------------------------------------------ shared prefixes
+    def can_share_prefixes(self) -> bool:
+        """Whether decode steps can read prefixes that their sequences share once a group: grouped-query attention over pages of the model's type, in a
+        mode that leaves the order of sums open, with nothing beside pages that a graph's warm-up would touch."""
+        c = self.mcfg
+        from ..batch_invariant import fixed_sums
+        return not (c.use_mla or c.layer_plan or c.sliding_window or c.keeps_sequence_state or self._kv_int4() or self.dcp_size > 1
+                    or self.pp.world_size > 1 or self.pcp.world_size > 1 or self.sparse_offload is not None or self.lora_manager is not None
+                    or self.moe_runtime is not None or fixed_sums())
+
+    def _sharing_pays(self, groups: list) -> bool:
+        """Whether a layer's attention takes less time with prefixes read once: what is not read again, at 6 TB/s, against 6 us for results that
+        two kernels join (32 heads on 8 of 128, eight beams over 2048 tokens: 14 us shared, 19 plain; four over 1500: 13 and 11)."""
+        if not self.is_cuda:
+            return True
+        a = self._attn_layer()
+        return sum((n - 1) * prefix for n, prefix in groups) * a.Hkv * a.D * 2 * self._kv_itemsize() / 6e6 > 6
+
+    def _kv_itemsize(self) -> int:
+        return torch.empty(0, dtype=self.kv_dtype).element_size()
+
+    def _find_shared(self, so: SchedulerOutput) -> None:
+        """Groups of a decode step: those that the caller knows, or all of its sequences where they begin with the same blocks."""
+        if so.shared_groups is None and self.share_prefixes and len(so.scheduled) > 1 and self.can_share_prefixes():
+            reqs = [r for r, _ in so.scheduled]
+            whole = min(r.num_computed_tokens for r in reqs) // self.block_size
+            table = self.block_table_cpu[[r.row for r in reqs], :whole]
+            differ = np.flatnonzero((table != table[0]).any(0))
+            same = int(differ[0]) if differ.size else whole
+            so.shared_groups = [(len(reqs), same * self.block_size)]
+        if so.shared_groups is not None and not (self.can_share_prefixes() and self._sharing_pays(so.shared_groups)):
+            so.shared_groups = None
+
+    def _shared_graph(self, gsize: Optional[int]):
+        """Descriptor of the graph for a decode step that shares prefixes; None: it runs eagerly.  A size is captured when it is asked for a third time."""
+        if gsize is None:
+            return None
+        key = (gsize, "shared")
+        if key not in self.graphs:
+            self._shared_asked[gsize] = self._shared_asked.get(gsize, 0) + 1
+            if self._shared_asked[gsize] < 3:
+                return None
+            from ..compilation.cuda_graph import BatchDescriptor
+            torch.cuda.synchronize()
+            meta, T, Tp, _, _ = self._dummy_meta(gsize, 1, shared_groups=[(gsize, 0)])
+            meta.slot_mapping.fill_(-1)
+            desc = BatchDescriptor(num_tokens=gsize, shared_prefixes=True)
+            self.graph_wrapper.capture(desc, Tp, meta)
+            self.graphs[key] = desc
+        return self.graphs[key]
+
     # ------------------------------------------------------------------ execution
     def _forward(self, T: int, meta: AttentionMetadata) -> torch.Tensor:
         from ..profiler import nvtx_range
@@ -688,6 +765,9 @@ class ModelRunner:
 
     def _forward_impl(self, T: int, meta: AttentionMetadata) -> torch.Tensor:
         pp = self.pp
+        if meta.shared_groups is not None:
+            a = self._attn_layer()
+            meta.shared = ops.plan_shared_prefix(meta, *meta.shared_groups, a.Hq, a.Hkv)
         emb = self.mm.inputs_embeds(self.input_ids[:T]) if self.mm is not None else None
         if emb is not None:
             meta.deepstack = self.mm.deepstack
@@ -743,10 +823,16 @@ class ModelRunner:
         gsize = self._graph_size_for(B) if decode_only else None
         if gsize is not None and self._lora_step_needs_eager(so):
             gsize = None
+        shared = None
+        if decode_only:
+            self._find_shared(so)
+            if so.shared_groups:
+                shared = self._shared_graph(gsize)
+                gsize = gsize if shared is not None else None
         meta, T, Tp, sel, sample_reqs = self._prepare_inputs(so, pad_to=gsize)
         t_prep = time.perf_counter()
         if gsize is not None:
-            desc = self.graphs[(gsize, self.lora_manager is not None and self.lora_manager.punica.any_active)]
+            desc = shared or self.graphs[(gsize, self.lora_manager is not None and self.lora_manager.punica.any_active)]
             hidden_out = self.graph_wrapper.replay(desc)
             self.stats["graph_replays"] += 1
             self.stats["graph_kernel_launches"] += self.graph_wrapper.entries[desc].num_launches
@@ -814,20 +900,31 @@ class ModelRunner:
         at = req.num_computed_tokens
         self.token_ids_cpu[req.row, at:at + len(tokens)] = tokens
 
-    @torch.inference_mode()
-    def execute_logits(self, so: SchedulerOutput, rows: list) -> Optional[torch.Tensor]:
-        """One step that samples nothing: the logits (fp32, on the host) at the given token rows of the
-        batch (``so.scheduled`` order).  Decode-only batches replay their graph, as in ``execute``."""
+    def _execute_hidden(self, so: SchedulerOutput) -> torch.Tensor:
+        """Hidden states of a step that samples nothing; decode-only batches replay their graph, as in ``execute``."""
         self.stats["steps"] += 1
         self._sync_rows(so)
-        gsize = self._graph_size_for(len(so.scheduled)) if all(n == 1 for _, n in so.scheduled) else None
+        decode_only = all(n == 1 for _, n in so.scheduled)
+        gsize, shared = (self._graph_size_for(len(so.scheduled)), None) if decode_only else (None, None)
+        if so.shared_groups:
+            self._find_shared(so)
+            if so.shared_groups:
+                shared = self._shared_graph(gsize)
+                gsize = gsize if shared is not None else None
         meta, T, Tp, _, _ = self._prepare_inputs(so, pad_to=gsize)
         if gsize is not None:
-            hidden = self.graph_wrapper.replay(self.graphs[(gsize, False)])
+            hidden = self.graph_wrapper.replay(shared or self.graphs[(gsize, False)])
             self.stats["graph_replays"] += 1
         else:
             hidden = self._forward(Tp, meta)
             self.stats["eager_steps"] += 1
+        return hidden
+
+    @torch.inference_mode()
+    def execute_logits(self, so: SchedulerOutput, rows: list) -> Optional[torch.Tensor]:
+        """One step that samples nothing: the logits (fp32, on the host) at the given token rows of the
+        batch (``so.scheduled`` order)."""
+        hidden = self._execute_hidden(so)
         out = []
         for a in range(0, len(rows), 1024):            # bounded logits footprint
             idx = torch.tensor(rows[a:a + 1024], dtype=torch.int64, device=self.device)
@@ -836,6 +933,14 @@ class ModelRunner:
             torch.cuda.current_stream().synchronize()
             _native.check_status(self.device)
         return torch.cat(out) if out else None
+
+    @torch.inference_mode()
+    def device_logits(self, so: SchedulerOutput, rows: Optional[list] = None) -> torch.Tensor:
+        """The same on the device, as the model computes them; ``rows`` None: every token's."""
+        hidden = self._execute_hidden(so)
+        if rows is None:
+            return self.model.compute_logits(hidden[:so.num_scheduled_tokens])
+        return self.model.compute_logits(hidden[self._to_dev(torch.tensor(rows, dtype=torch.int64))])
 
     def _sample_pcp(self, hidden: torch.Tensor, sel: list, sample_reqs: list) -> dict:
         """Split prefill step: PCP rank 0 holds the last token of every chunk, samples, and sends
@@ -886,6 +991,12 @@ class ModelRunner:
         gsize = self._graph_size_for(B) if decode_only else None
         if gsize is not None and self._lora_step_needs_eager(so):
             gsize = None
+        shared = None
+        if decode_only:
+            self._find_shared(so)
+            if so.shared_groups:
+                shared = self._shared_graph(gsize)
+                gsize = gsize if shared is not None else None
         ev_start = None
         if self._step_timing:
             # device-side account of the step: time between the first and the last GPU operation of
@@ -908,7 +1019,7 @@ class ModelRunner:
                 self.input_ids.index_copy_(0, idx[1], prev.tokens.index_select(0, idx[0]))
         t_prep = time.perf_counter()
         if gsize is not None:
-            desc = self.graphs[(gsize, self.lora_manager is not None and self.lora_manager.punica.any_active)]
+            desc = shared or self.graphs[(gsize, self.lora_manager is not None and self.lora_manager.punica.any_active)]
             hidden_out = self.graph_wrapper.replay(desc)
             self.stats["graph_replays"] += 1
             self.stats["graph_kernel_launches"] += self.graph_wrapper.entries[desc].num_launches
@@ -1203,7 +1314,7 @@ class ModelRunner:
         return g
 
     # ------------------------------------------------------------------ warm-up / capture
-    def _dummy_meta(self, B: int, q_len: int, pad_to: Optional[int] = None):
+    def _dummy_meta(self, B: int, q_len: int, pad_to: Optional[int] = None, shared_groups: Optional[list] = None):
         """Synthetic batch of B sequences of q_len tokens over block 0."""
         class _R:  # minimal request stand-in
             pass
@@ -1213,7 +1324,7 @@ class ModelRunner:
             r.row, r.num_computed_tokens, r.num_tokens = i, 0, q_len + 1
             r.request_id = f"_dummy{i}"
             sched.append((r, q_len))
-        so = SchedulerOutput(scheduled=sched)
+        so = SchedulerOutput(scheduled=sched, shared_groups=shared_groups)
         saved = self.block_table_cpu[:B].copy()
         self.block_table_cpu[:B] = 0
         try:

@@ -31,6 +31,8 @@ class SchedulerOutput:
     new_block_rows: list = field(default_factory=list)   # requests whose block list grew
     kv_connector_metadata: Optional[object] = None
     step_id: int = 0
+    # neighbours in ``scheduled`` whose sequences share leading tokens: [(number of requests, shared tokens)], all requests in order
+    shared_groups: Optional[list] = None
 
     @property
     def is_empty(self) -> bool:
@@ -345,6 +347,39 @@ class Scheduler:
         out.scheduled = decodes + prefills
         out.num_scheduled_tokens = sum(n for _, n in out.scheduled)
         return out
+
+    def fork(self, parent: Request, request_id: str) -> Request:
+        """A request that goes on from ``parent``'s computed tokens: a batch row of its own, the full blocks shared, a block of its own for a
+        partly filled last one (the caller copies its content, and what the layers keep beside pages)."""
+        if not self._free_rows:
+            raise RuntimeError(f"no free batch row for request {request_id}")
+        full = parent.num_computed_tokens // self.block_size
+        tail = self.pool.allocate(1) if parent.num_computed_tokens % self.block_size else []
+        req = Request(request_id, parent.prompt_token_ids, parent.sampling_params)
+        req.num_computed_tokens, req.status, req.row = parent.num_computed_tokens, RequestStatus.RUNNING, self._free_rows.pop()
+        req.block_ids = parent.block_ids[:full] + tail
+        self.pool.touch(parent.block_ids[:full])
+        self.requests[request_id] = req
+        self.running.append(req)
+        return req
+
+    def follow(self, reqs: list, parents: list) -> None:
+        """Request i goes on from the computed tokens of ``reqs[parents[i]]`` (all have as many): it shares that one's full blocks and keeps its own
+        partly filled block."""
+        full = reqs[0].num_computed_tokens // self.block_size
+        old = [r.block_ids for r in reqs]
+        new = [old[p][:full] + r.block_ids[full:] for r, p in zip(reqs, parents)]
+        for p in parents:
+            self.pool.touch(old[p][:full])
+        for blocks in old:
+            self.pool.free(blocks[:full])
+        for r, blocks in zip(reqs, new):
+            r.block_ids = blocks
+
+    def drop(self, req: Request) -> None:
+        """Forget a request that ``schedule_portions`` or ``fork`` made."""
+        self.abort_request(req.request_id)
+        self.requests.pop(req.request_id, None)
 
     # ------------------------------------------------------------------ results
     def advance(self, out: SchedulerOutput) -> None:
