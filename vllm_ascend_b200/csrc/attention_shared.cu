@@ -24,7 +24,7 @@
 #include "common.cuh"
 
 #include <mutex>
-#include <string>
+#include <string.h>
 #include <unordered_map>
 
 namespace b200 {
@@ -241,6 +241,7 @@ struct SharedParams {
   int max_blocks, block_size, page_shift, rows_per_load, piece;        // page_shift: log2 of the block size, -1: no power of two
   int G, Hkv, Hq, tpt;         // tpt: tokens of a tile of 128 rows
   int blocks, tokens, bases_at, heads_at;
+  int rows;                    // of q and out
   float scale_log2;
   float* part_o;               // [partial rows, D]
   float2* part_ml;             // [partial rows] maximum (log2, scaled) and sum
@@ -406,6 +407,8 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = warp_uniform(*tmem_ptr);
+  // the join may take its place beside these blocks, all of them running by then, and find its rows; it waits for their end before it reads results
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp == 8 || warp == 10) {
     // ------------------------------------------------------------ producers: warp 8 queries and keys, warp 10 values; one thread of each walks the
@@ -425,9 +428,16 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       int* my_pages = pages + (values ? 16 : 0);
       auto fetch_pages = [&]() {
         const int* row = p.block_table + (long)c.p.b.table_row * p.pitch;
-        int key = c.base();
+        const int base = c.base();
+        if (p.page_shift >= 0 && c.c_lo() == 0 && c.c_hi() == 128 && (base + 127) >> p.page_shift < p.max_blocks) {
+          row += base >> p.page_shift;
+#pragma unroll 2
+          for (int i = 0; i < parts; i++)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(my_pages + i)), "l"(row + i) : "memory");
+          return;
+        }
 #pragma unroll 1
-        for (int i = 0; i < parts; i++, key += rpl) {
+        for (int i = 0, key = base; i < parts; i++, key += rpl) {
           const int near = min(max(key, c.p.b.key_lo), c.p.b.key_hi - 1);
           const int col = p.page_shift >= 0 ? near >> p.page_shift : near / p.block_size;
           if (col < p.max_blocks) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(my_pages + i)), "l"(row + col) : "memory");
@@ -460,20 +470,34 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         if (!mbar_wait(&empty_bars[st], ph, abort_word)) goto done;
         asm volatile("cp.async.wait_all;" ::: "memory");
         const int base = c.base(), lo = c.c_lo(), hi = c.c_hi();
-        const bool full = lo == 0 && hi == 128;
-        const int rows = full ? rpl : p.piece, end = (hi + rows - 1) / rows;
-        const CUtensorMap* tm = full ? whole : pieces;
         uint8_t* dst = stages + st * TILE;
-        mbar_expect_tx(&full_bars[st], (uint32_t)((end - lo / rows) * rows * 128 * NH));
-#pragma unroll 1
-        for (int i = lo / rows; i < end; i++) {
-          const int page = my_pages[i * rows / rpl], off = p.page_shift >= 0 ? (base + i * rows) & (p.block_size - 1) : (base + i * rows) % p.block_size;
-          if (page < 0 || page >= p.num_blocks_total) {
-            *abort_word = B200_BAD_INDEX;
-            goto done;
-          }
+        bool bad = false;                        // copies of pages out of range read zeros
+        if (lo == 0 && hi == 128) {
+          mbar_expect_tx(&full_bars[st], TILE);
+          const int off = parts > 1 ? 0 : (p.page_shift >= 0 ? base & (p.block_size - 1) : base % p.block_size);
+#pragma unroll 2
+          for (int i = 0; i < parts; i++, dst += rpl * 128) {
+            const int page = my_pages[i];
+            bad |= (uint32_t)page >= (uint32_t)p.num_blocks_total;
 #pragma unroll
-          for (int hf = 0; hf < NH; hf++) tma_load_4d(dst + hf * SH_HALF + i * rows * 128, tm, &full_bars[st], hf * 64, c.p.h, off, page);
+            for (int hf = 0; hf < NH; hf++) tma_load_4d(dst + hf * SH_HALF, whole, &full_bars[st], hf * 64, c.p.h, off, page);
+          }
+        } else {
+          const int rows = p.piece, end = (hi + rows - 1) / rows;
+          mbar_expect_tx(&full_bars[st], (uint32_t)((end - lo / rows) * rows * 128 * NH));
+#pragma unroll 1
+          for (int i = lo / rows; i < end; i++) {
+            const int page = my_pages[i * rows / rpl];
+            const int off = p.page_shift >= 0 ? (base + i * rows) & (p.block_size - 1) : (base + i * rows) % p.block_size;
+            bad |= (uint32_t)page >= (uint32_t)p.num_blocks_total;
+#pragma unroll
+            for (int hf = 0; hf < NH; hf++)
+              tma_load_4d(dst + hf * SH_HALF + i * rows * 128, pieces, &full_bars[st], hf * 64, c.p.h, off, page);
+          }
+        }
+        if (bad) {
+          *abort_word = B200_BAD_INDEX;
+          goto done;
         }
         if (++st == (uint32_t)depth) st = 0, ph ^= 1u;
         c.next(p);
@@ -719,7 +743,7 @@ __global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) 
   const int t = (int)(id / p.Hq), hq = (int)(id - (long)t * p.Hq);
   const int* tok_base = p.plan + plan_tokens_at(p.blocks);
   int which[2] = {-1, -2};
-  if (t < p.tokens) which[0] = __ldg(tok_base + t), which[1] = __ldg(tok_base + p.tokens + t);
+  if (t < p.rows) which[0] = __ldg(tok_base + t), which[1] = __ldg(tok_base + p.tokens + t);
   const int h = hq / p.G, g = hq - h * p.G;
   long at[2];
   int n[2], pitch[2];
@@ -733,6 +757,7 @@ __global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) 
     at[k] = (long)head.x + (t - tok.x) * p.G + g;
     n[k] = head.y;
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");       // by every thread: what follows this kernel counts on those in front of it
   float acc[V], sum = 0.f, top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < V; j++) acc[j] = 0.f;
@@ -810,40 +835,66 @@ struct SharedArgs {
   int block_size, max_blocks, Hq, Hkv, D, blocks, tokens, bases_at, max_bases;
 };
 
-static int shared_tmap(CUtensorMap* out, const void* base, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
-  static std::unordered_map<std::string, CUtensorMap> map;
-  static std::mutex mu;
-  char key[80];
-  memcpy(key, &base, 8);
-  memcpy(key + 8, dims, 32);
-  memcpy(key + 40, strides, 24);
-  memcpy(key + 64, box, 16);
-  std::string k(key, 80);
-  std::lock_guard<std::mutex> g(mu);
-  auto it = map.find(k);
-  if (it != map.end()) {
-    *out = it->second;
-    return 0;
+// Maps of the queries (four boxes) or of a pair of caches (whole tiles and pieces), kept by what they encode.
+struct SharedMapKey {
+  const void* base[2];
+  uint64_t dims[4], strides[3];
+  uint32_t boxes[4];
+  bool operator==(const SharedMapKey& o) const { return memcmp(this, &o, sizeof(*this)) == 0; }
+};
+struct SharedMapHash {
+  size_t operator()(const SharedMapKey& k) const {
+    const uint64_t* w = reinterpret_cast<const uint64_t*>(&k);
+    uint64_t h = 0;
+    for (size_t i = 0; i < sizeof(k) / 8; i++) h = (h ^ w[i]) * 0x9e3779b97f4a7c15ull, h ^= h >> 29;
+    return (size_t)h;
   }
-  const int rc = make_tmap(out, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc) return rc;
-  if (map.size() > 4096) map.clear();
-  map.emplace(std::move(k), *out);
+};
+struct SharedMaps {
+  CUtensorMap map[4];
+};
+
+// box i: 64 columns of all heads of a group by boxes[i] tokens, or of boxes[i] tokens of a page (keys and values in turn)
+static int shared_maps(SharedMaps* out, const SharedMapKey& key, bool queries) {
+  static std::unordered_map<SharedMapKey, SharedMaps, SharedMapHash> maps;
+  static std::mutex mu;
+  std::lock_guard<std::mutex> g(mu);
+  auto it = maps.find(key);
+  if (it == maps.end()) {
+    SharedMaps m;
+    for (int i = 0; i < 4; i++) {
+      const uint32_t box[4] = {64, queries ? (uint32_t)key.dims[1] : 1u, queries ? 1u : key.boxes[i], queries ? key.boxes[i] : 1u};
+      const int rc = make_tmap(&m.map[i], key.base[queries ? 0 : i & 1], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, key.dims, key.strides, box,
+                               CU_TENSOR_MAP_SWIZZLE_128B);
+      if (rc) return rc;
+    }
+    if (maps.size() > 2048) maps.clear();
+    it = maps.emplace(key, m).first;
+  }
+  *out = it->second;
   return 0;
 }
 
 template <int D>
-static int launch_shared(const CUtensorMap* tm, const SharedParams& p, cudaStream_t stream) {
+static int launch_shared(const SharedMaps& q, const SharedMaps& kv, const SharedParams& p, cudaStream_t stream) {
   const cudaError_t e = allow_smem<&attn_shared_kernel<D>>(SharedCfg<D>::SMEM);
   if (e != cudaSuccess) return (int)e;
-  attn_shared_kernel<D><<<p.blocks, SH_THREADS, SharedCfg<D>::SMEM, stream>>>(tm[0], tm[1], tm[2], tm[3], tm[4], tm[5], tm[6], tm[7], p);
+  attn_shared_kernel<D><<<p.blocks, SH_THREADS, SharedCfg<D>::SMEM, stream>>>(q.map[0], q.map[1], q.map[2], q.map[3], kv.map[0],
+                                                                                  kv.map[1], kv.map[2], kv.map[3], p);
   const int rc = B200_CHECK_LAUNCH();
   if (rc) return rc;
   // few rows may have many partial results: up to 2 a block; there are warps to spare
-  const long rows = (long)p.tokens * p.Hq;
-  if (rows <= 4096) shared_join_kernel<D, 4><<<(unsigned)rows, 128, 0, stream>>>(p);
-  else shared_join_kernel<D, 1><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(p);
-  return B200_CHECK_LAUNCH();
+  const long rows = (long)p.rows * p.Hq;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows <= 4096 ? rows : (rows + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return (int)(rows <= 4096 ? cudaLaunchKernelEx(&cfg, shared_join_kernel<D, 4>, p) : cudaLaunchKernelEx(&cfg, shared_join_kernel<D, 1>, p));
 }
 
 }  // namespace b200
@@ -865,7 +916,7 @@ B200_API int b200_attn_shared(const b200::SharedArgs* args) {
   const SharedArgs& a = *args;
   if (a.T <= 0 || a.tokens <= 0) return 0;
   const int bs = a.block_size;
-  if (a.Hkv < 1 || a.Hq % a.Hkv || a.Hq / a.Hkv > 128 || (a.D != 64 && a.D != 128) || a.tokens > a.T) return 9955;
+  if (a.Hkv < 1 || a.Hq % a.Hkv || a.Hq / a.Hkv > 128 || (a.D != 64 && a.D != 128)) return 9955;
   if (bs < 8 || (bs < 128 && 128 % bs) || (bs > 128 && bs % 128)) return 9956;
   if ((a.q_stride & 7) || (a.out_stride & 7) || ((uintptr_t)a.q & 15) || ((uintptr_t)a.out & 15) || ((uintptr_t)a.k_cache & 15) ||
       ((uintptr_t)a.v_cache & 15) || (a.block_stride & 7) || (a.token_stride & 7) || (a.head_stride & 7))
@@ -873,25 +924,22 @@ B200_API int b200_attn_shared(const b200::SharedArgs* args) {
   const int G = a.Hq / a.Hkv, tpt = 128 / G;
   // what the pieces of a plan of these sizes have room for
   if (a.part_rows < 4L * a.tokens * a.Hq + (long)a.blocks * SH_ROWS) return 9958;
-  CUtensorMap tm[8];
-  {
-    const uint64_t dims[4] = {(uint64_t)a.D, (uint64_t)G, (uint64_t)a.Hkv, (uint64_t)a.T};
-    const uint64_t str[3] = {(uint64_t)a.D * 2, (uint64_t)G * a.D * 2, (uint64_t)a.q_stride * 2};
-    const uint32_t n[4] = {(uint32_t)tpt, (uint32_t)(G <= 64 ? 64 / G : 1), (uint32_t)(tpt < 4 ? tpt : 4), 1};
-    for (int i = 0; i < 4; i++) {
-      const uint32_t box[4] = {64, (uint32_t)G, 1, n[i]};
-      const int rc = shared_tmap(&tm[i], a.q, dims, str, box);
-      if (rc) return rc;
-    }
-  }
   const int rpl = bs < 128 ? bs : 128, piece = rpl < 32 ? rpl : 32;
-  for (int i = 0; i < 4; i++) {
-    const uint64_t dims[4] = {(uint64_t)a.D, (uint64_t)a.Hkv, (uint64_t)bs, (uint64_t)a.num_blocks};
-    const uint64_t str[3] = {(uint64_t)a.head_stride * 2, (uint64_t)a.token_stride * 2, (uint64_t)a.block_stride * 2};
-    const uint32_t box[4] = {64, 1, (uint32_t)(i < 2 ? rpl : piece), 1};
-    const int rc = shared_tmap(&tm[4 + i], i & 1 ? a.v_cache : a.k_cache, dims, str, box);
-    if (rc) return rc;
-  }
+  SharedMaps q, kv;
+  SharedMapKey key;
+  memset(&key, 0, sizeof(key));                // padding, if there is any, is compared
+  key.base[0] = a.q;
+  key.dims[0] = a.D, key.dims[1] = G, key.dims[2] = a.Hkv, key.dims[3] = a.T;
+  key.strides[0] = a.D * 2, key.strides[1] = (uint64_t)G * a.D * 2, key.strides[2] = (uint64_t)a.q_stride * 2;
+  key.boxes[0] = tpt, key.boxes[1] = G <= 64 ? 64 / G : 1, key.boxes[2] = tpt < 4 ? tpt : 4, key.boxes[3] = 1;
+  int rc = shared_maps(&q, key, true);
+  if (rc) return rc;
+  key.base[0] = a.k_cache, key.base[1] = a.v_cache;
+  key.dims[1] = a.Hkv, key.dims[2] = bs, key.dims[3] = a.num_blocks;
+  key.strides[0] = (uint64_t)a.head_stride * 2, key.strides[1] = (uint64_t)a.token_stride * 2, key.strides[2] = (uint64_t)a.block_stride * 2;
+  key.boxes[0] = key.boxes[1] = rpl, key.boxes[2] = key.boxes[3] = piece;
+  rc = shared_maps(&kv, key, false);
+  if (rc) return rc;
   SharedParams p;
   p.plan = a.plan;
   p.block_table = a.block_table;
@@ -904,6 +952,7 @@ B200_API int b200_attn_shared(const b200::SharedArgs* args) {
   p.G = G; p.Hkv = a.Hkv; p.Hq = a.Hq; p.tpt = tpt;
   p.blocks = a.blocks;
   p.tokens = a.tokens;
+  p.rows = (int)(a.T < a.tokens ? a.T : a.tokens);
   p.bases_at = a.bases_at;
   p.heads_at = plan_heads_at(a.bases_at, a.max_bases);
   p.scale_log2 = a.scale * 1.4426950408889634f;
@@ -913,5 +962,5 @@ B200_API int b200_attn_shared(const b200::SharedArgs* args) {
   p.status = a.status;
   p.out = (__nv_bfloat16*)a.out;
   p.out_stride = a.out_stride;
-  return a.D == 64 ? launch_shared<64>(tm, p, a.stream) : launch_shared<128>(tm, p, a.stream);
+  return a.D == 64 ? launch_shared<64>(q, kv, p, a.stream) : launch_shared<128>(q, kv, p, a.stream);
 }

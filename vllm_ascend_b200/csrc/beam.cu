@@ -248,6 +248,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
   __shared__ float warp_max[BEAM_WARPS];
   __shared__ double warp_sum[BEAM_WARPS];
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // once all blocks run, groups' may take their places and wait
   if (!is_score(a.scores[row])) return;            // the beam has ended: the second kernel asks its score first
   const T* x0 = (const T*)a.logits + (long)row * a.row_stride;
   // vectors lie on 16-byte boundaries of memory, whatever the row's first element does; a vector holds elements [at, at + 8)
@@ -439,6 +440,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1) select_groups_kernel(const Se
   GroupList& list = *reinterpret_cast<GroupList*>(beam_smem);
   double* norm = reinterpret_cast<double*>(beam_smem + sizeof(GroupList));      // log of a beam's sum; NaN: it has no candidates
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");       // the blocks of rows have ended, and what came in front of them
   for (int w = tid >> 5; w < a.width; w += BEAM_WARPS) {          // a warp a beam, a lane a part
     const long row = (long)g * a.width + w;
     double l = __longlong_as_double(0x7ff8000000000000ll);
@@ -653,8 +655,17 @@ B200_API int b200_beam_select(const b200::SelectArgs* args) {
   else select_rows_kernel<__nv_bfloat16><<<grid, BEAM_THREADS, row_smem, a.stream>>>(a);
   int rc = B200_CHECK_LAUNCH();
   if (rc) return rc;
-  select_groups_kernel<<<a.groups, BEAM_THREADS, group_smem, a.stream>>>(a);
-  return B200_CHECK_LAUNCH();
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.groups);
+  cfg.blockDim = dim3(BEAM_THREADS);
+  cfg.dynamicSmemBytes = group_smem;
+  cfg.stream = a.stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, select_groups_kernel, a);
 }
 
 B200_API int b200_beam_reorder(const b200::ReorderArgs* args) {

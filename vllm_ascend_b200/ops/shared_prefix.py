@@ -86,57 +86,58 @@ def paged_attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     new tokens a sequence.  Rows of ``out`` behind the last sequence are left as they are; a token without keys gets zeros.  bf16 with heads of
     64 and 128 runs the kernel; other types and sizes the definition.  Keys and values of pages that lie outside of a sequence may hold anything,
     those of its own new tokens are numbers."""
-    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[3] != q.shape[2]:
-        raise ValueError(f"queries [T, heads, D] and caches [blocks, tokens, heads, D], not {tuple(q.shape)}, {tuple(k_cache.shape)} and "
-                         f"{tuple(v_cache.shape)}")
-    T, Hq, D = q.shape
-    device = q.get_device()
+    shape, pages, device = q.shape, k_cache.shape, q.get_device()
+    if len(shape) != 3 or len(pages) != 4 or v_cache.shape != pages or pages[3] != shape[2]:
+        raise ValueError(f"queries [T, heads, D] and caches [blocks, tokens, heads, D], not {tuple(shape)}, {tuple(pages)} and {tuple(v_cache.shape)}")
     if _elsewhere(device):
         with torch.cuda.device(device):
             return paged_attention_shared(q, k_cache, v_cache, meta, plan, scale, out)
-    NB, bs, Hkv, _ = k_cache.shape
-    if (Hq, Hkv) != (plan.heads, plan.kv_heads):
+    (T, Hq, D), (NB, bs, Hkv, _) = shape, pages
+    if Hq != plan.heads or Hkv != plan.kv_heads:
         raise ValueError(f"{Hq} heads on {Hkv}, a plan for {plan.heads} on {plan.kv_heads}")
-    if not q.dtype == k_cache.dtype == v_cache.dtype:
-        raise ValueError(f"queries {q.dtype}, keys {k_cache.dtype} and values {v_cache.dtype} are not of one type")
+    dtype = q.dtype
+    if not dtype == k_cache.dtype == v_cache.dtype:
+        raise ValueError(f"queries {dtype}, keys {k_cache.dtype} and values {v_cache.dtype} are not of one type")
     if not k_cache.get_device() == v_cache.get_device() == plan.prefix_lens.get_device() == device:
         raise ValueError(f"queries on {q.device}, caches on {k_cache.device} and {v_cache.device}, the plan on {plan.prefix_lens.device}")
     if not scale > 0:
         raise ValueError(f"scale {scale} is not above zero")
-    if meta.num_reqs != plan.seqs:
-        raise ValueError(f"{meta.num_reqs} sequences, a plan for {plan.seqs}")
-    if out is None:
-        out = q.new_empty((T, Hq, D))
-    elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device:
-        raise ValueError(f"out: {q.dtype} {tuple(q.shape)} on {q.device}, not {out.dtype} {tuple(out.shape)} on {out.device}")
-    if T < plan.tokens and T < int(meta.query_start_loc_cpu[meta.num_reqs]):
+    n = meta.num_reqs
+    if n != plan.seqs:
+        raise ValueError(f"{n} sequences, a plan for {plan.seqs}")
+    if T < plan.tokens and T < int(meta.query_start_loc_cpu[n]):
         raise ValueError(f"{T} query rows, a plan for {plan.tokens}")
-    meta = _dense(meta, device)
-    if device < 0 or q.dtype is not torch.bfloat16 or D not in HEAD_SIZES or bs < 8 or (128 % bs if bs < 128 else bs % 128):
-        return _definition(q, k_cache, v_cache, meta, plan, scale, out)
-    tokens = min(T, plan.tokens)
-    if tokens == 0 or meta.num_reqs == 0:
+    given = out
+    if out is None:
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype != dtype or out.get_device() != device:
+        raise ValueError(f"out: {dtype} {tuple(shape)} on {q.device}, not {out.dtype} {tuple(out.shape)} on {out.device}")
+    if device < 0 or dtype is not torch.bfloat16 or D not in HEAD_SIZES or bs < 8 or (128 % bs if bs < 128 else bs % 128):
+        return _definition(q, k_cache, v_cache, _dense(meta, device), plan, scale, out)
+    if T == 0 or plan.tokens == 0 or n == 0:
         return out
-    given, q = out, _dense_heads(q)
-    k_cache, v_cache = _as_pages(k_cache), _as_pages(v_cache)
-    if k_cache.stride() != v_cache.stride():
-        v_cache = torch.empty_strided(k_cache.shape, k_cache.stride(), dtype=v_cache.dtype, device=v_cache.device).copy_(v_cache)
-    row, head, channel = out.stride()
-    if channel != 1 or head != D or row % 8 or out.data_ptr() % 16:
-        out = q.new_empty((T, Hq, D))
-        out.copy_(given)
-    part_rows = 4 * plan.tokens * Hq + plan.blocks * _ROWS
-    # every call has its own: calls on two streams, or two graphs, may run at once
-    parts = torch.empty(part_rows * (D + 2), dtype=torch.float32, device=q.device)
-    block, token, khead, _ = k_cache.stride()
     table = meta.block_table
+    if not (table.dtype is torch.int32 and table.dim() == 2 and table.stride(1) == 1 and table.shape[0] >= n and table.get_device() == device):
+        table = _dense(meta, device).block_table
+    q, k_cache, v_cache = _dense_heads(q), _as_pages(k_cache), _as_pages(v_cache)
+    strides = k_cache.stride()
+    if strides != v_cache.stride():
+        v_cache = torch.empty_strided(pages, strides, dtype=dtype, device=v_cache.device).copy_(v_cache)
+    if given is not None:
+        row, head, channel = out.stride()
+        if channel != 1 or head != D or row % 8 or out.data_ptr() % 16:
+            out = q.new_empty(shape)
+            out.copy_(given)
+    # every call has its own results of pieces: calls on two streams, or two graphs, may run at once
+    part_rows = 4 * plan.tokens * Hq + plan.blocks * _ROWS
+    parts = plan.prefix_lens.new_empty(part_rows * (D + 2))          # of 32 bits each
     rc = _native.lib().b200_attn_shared(_ATTENTION.pack(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), plan.table.data_ptr(), table.data_ptr(), parts.data_ptr(), out.data_ptr(),
-        _native.status_word(q.device).data_ptr(), _native.stream_ptr(), q.stride(0), T, NB, table.stride(0), out.stride(0), part_rows, block, token,
-        khead, scale, bs, table.shape[1], Hq, Hkv, D, plan.blocks, plan.tokens, plan.bases_at, plan.bases))
+        _native.status_word(plan.prefix_lens.device).data_ptr(), _native.stream_ptr(), q.stride(0), T, NB, table.stride(0), out.stride(0), part_rows,
+        strides[0], strides[1], strides[2], scale, bs, table.shape[1], Hq, Hkv, D, plan.blocks, plan.tokens, plan.bases_at, plan.bases))
     _native.check(rc, "attn_shared")
     _native.count_launch(2)
-    return out if out is given else given.copy_(out)
+    return out if given is None or out is given else given.copy_(out)
 
 
 def _as_pages(cache: torch.Tensor) -> torch.Tensor:
