@@ -257,7 +257,7 @@ struct SharedCfg {
   static constexpr int TILE = NH * SH_HALF;              // bytes of 128 rows
   static constexpr int NK = D == 128 ? 2 : 3;
   static constexpr int NV = D == 128 ? 3 : 5;
-  static constexpr int SMEM = (2 + NK + NV) * TILE + 1024 + 512;
+  static constexpr int SMEM = (2 + NK + NV) * TILE + 512;        // with 1 KB of the system's, what a join's block needs stays free
 };
 
 __device__ __forceinline__ float sh_exp2(float x) {
@@ -356,8 +356,11 @@ attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   constexpr int NH = Cfg::NH, NK = Cfg::NK, NV = Cfg::NV, TILE = Cfg::TILE;
   constexpr int O_COL = 256;
   const int warp = warp_index(), lane = threadIdx.x & 31;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];          // there is no other shared memory: it begins where the system's first KB ends
+  if (smem_u32(smem) & 1023) {
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, B200_OVERFLOW);
+    return;
+  }
   uint8_t* Qs = smem;
   uint8_t* Ks = Qs + 2 * TILE;
   uint8_t* Vs = Ks + NK * TILE;
@@ -785,28 +788,23 @@ __global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) 
       for (int j = 0; j < V; j++) acc[j] += w == 0.f ? 0.f : w * x[j];       // where a group of warps had no tile, nothing was left
     }
   }
-  if constexpr (WARPS > 1) {
-    __shared__ float4 parts[4][33];
-    float4* mine = parts[warp];
-    mine[lane] = make_float4(acc[0], acc[1], V == 4 ? acc[V - 2] : 0.f, V == 4 ? acc[V - 1] : 0.f);
-    if (lane == 0) mine[32] = make_float4(top, sum, 0.f, 0.f);
+  if constexpr (WARPS == 2) {
+    __shared__ float4 parts[2][33];
+    float4* other = parts[warp >> 1];
+    if (sub == 1) {
+      other[lane] = make_float4(acc[0], acc[1], V == 4 ? acc[V - 2] : 0.f, V == 4 ? acc[V - 1] : 0.f);
+      if (lane == 0) other[32] = make_float4(top, sum, 0.f, 0.f);
+    }
     __syncthreads();
-    if (sub != 0) return;
-    float tops[WARPS];
-#pragma unroll
-    for (int k = 0; k < WARPS; k++) tops[k] = parts[warp + k][32].x, top = fmaxf(top, tops[k]);
-    sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < V; j++) acc[j] = 0.f;
-#pragma unroll
-    for (int k = 0; k < WARPS; k++) {
-      if (tops[k] == -INFINITY) continue;
-      const float f = sh_exp2(tops[k] - top);
-      const float4 x = parts[warp + k][lane];
-      sum += f * parts[warp + k][32].y;
-      acc[0] += f * x.x;
-      acc[1] += f * x.y;
-      if constexpr (V == 4) acc[2] += f * x.z, acc[3] += f * x.w;
+    if (sub == 1) return;
+    const float4 e = other[32], x = other[lane];
+    const float now = fmaxf(top, e.x);
+    if (now > -INFINITY) {
+      const float f = sh_exp2(top - now), fo = sh_exp2(e.x - now);
+      sum = f * sum + fo * e.y;
+      acc[0] = f * acc[0] + fo * x.x;
+      acc[1] = f * acc[1] + fo * x.y;
+      if constexpr (V == 4) acc[2] = f * acc[2] + fo * x.z, acc[3] = f * acc[3] + fo * x.w;
     }
   }
   if (which[1] == -2) return;                    // behind the last sequence: left as it is
@@ -883,18 +881,18 @@ static int launch_shared(const SharedMaps& q, const SharedMaps& kv, const Shared
                                                                                   kv.map[1], kv.map[2], kv.map[3], p);
   const int rc = B200_CHECK_LAUNCH();
   if (rc) return rc;
-  // few rows may have many partial results: up to 2 a block; there are warps to spare
+  // few rows may have many partial results, up to two of each block: two warps a row
   const long rows = (long)p.rows * p.Hq;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows <= 4096 ? rows : (rows + 3) / 4));
+  cfg.gridDim = dim3((unsigned)(rows <= 4096 ? (rows + 1) / 2 : (rows + 3) / 4));
   cfg.blockDim = dim3(128);
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return (int)(rows <= 4096 ? cudaLaunchKernelEx(&cfg, shared_join_kernel<D, 4>, p) : cudaLaunchKernelEx(&cfg, shared_join_kernel<D, 1>, p));
+  return (int)(rows <= 4096 ? cudaLaunchKernelEx(&cfg, shared_join_kernel<D, 2>, p) : cudaLaunchKernelEx(&cfg, shared_join_kernel<D, 1>, p));
 }
 
 }  // namespace b200

@@ -24,7 +24,7 @@ constexpr int BEAM_TILE = BEAM_THREADS * BEAM_VEC;
 constexpr int BEAM_WARPS = BEAM_THREADS / 32;
 constexpr int BEAM_MOST = 256;                            // k at most
 constexpr int STAGE_BYTES = 64;                           // of a row on their way, a thread
-constexpr int BEAM_ROOM = 4096, BEAM_SLACK = 1024;        // candidates of a group that are looked at together, and that are kept until then
+constexpr int BEAM_ROOM = 1024;                           // candidates of a group that are looked at together
 constexpr float kBeamLog2e = 1.4426950408889634f;
 
 struct SelectArgs {
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
 
 // ---------------------------------------------------------------- groups
 struct GroupList {
-  GroupKey keys[BEAM_ROOM + BEAM_SLACK], other[(BEAM_ROOM + BEAM_SLACK) / 2];
+  GroupKey keys[BEAM_ROOM + BEAM_MOST], other[(BEAM_ROOM + BEAM_MOST) / 2 + 128];
   GroupKey slices[BEAM_THREADS];
   GroupKey bound;
   int count;
@@ -461,16 +461,18 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1) select_groups_kernel(const Se
     if (lane == 0) norm[w] = l;
   }
   __syncthreads();
-  // candidates [beam, part, place in its list]; a beam without a distribution offers its first tokens at -inf
-  const int per_beam = a.parts * a.k, all = a.width * per_beam;
+  // Candidates by their places in the lists, which are sorted: the best of all lists come first, few behind them reach what those leave, and where no
+  // list has one that does, none comes behind it.  A beam without a distribution offers its first tokens at -inf.
+  const int lists = a.width * a.parts, levels = max(1, BEAM_ROOM / lists);
   GroupKey least = GroupKey::none();
   int n = 0;
-  for (int base = 0; base < all; base += BEAM_ROOM) {
+  for (int c0 = 0; c0 < a.k; c0 += levels) {
     if (tid == 0) list.count = n;
     __syncthreads();
+    bool any = false;
 #pragma unroll 1
-    for (int i = base + tid; i < min(base + BEAM_ROOM, all); i += BEAM_THREADS) {
-      const int w = i / per_beam, j = i - w * per_beam, p = j / a.k, c = j - p * a.k;
+    for (int i = tid; i < min(levels, a.k - c0) * lists; i += BEAM_THREADS) {
+      const int c = c0 + i / lists, j = i % lists, w = j / a.parts, p = j - w * a.parts;
       const long row = (long)g * a.width + w, slot = row * a.parts + p;
       const double l = norm[w];
       GroupKey key = GroupKey::none();
@@ -481,16 +483,18 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1) select_groups_kernel(const Se
         const float x = unorder32((uint32_t)(r >> 32));
         key = {order64((double)a.scores[row] + ((double)x - l)), ~((uint32_t)(w * a.vocab) + ~(uint32_t)r)};
       }
-      if (key.above(least)) list.keys[atomicAdd(&list.count, 1)] = key;
+      if (key.above(least)) {
+        list.keys[atomicAdd(&list.count, 1)] = key;
+        any = true;
+      }
     }
-    __syncthreads();
+    any = __syncthreads_or(any);
     n = list.count;
     __syncthreads();
-    if (n > BEAM_SLACK || base + BEAM_ROOM >= all) {
-      n = select_best<GroupKey>(list.keys, list.other, n, a.k, list.slices, &list.bound, &list.count);
-      if (n == a.k) least = list.keys[a.k - 1];
-      __syncthreads();
-    }
+    if (!any) break;
+    n = select_best<GroupKey>(list.keys, list.other, n, a.k, list.slices, &list.bound, &list.count);
+    if (n == a.k) least = list.keys[a.k - 1];
+    __syncthreads();
   }
   for (int i = tid; i < a.k; i += BEAM_THREADS) {
     const GroupKey key = list.keys[i];
@@ -646,10 +650,10 @@ B200_API int b200_beam_select(const b200::SelectArgs* args) {
       (long)a.parts * a.per_part < (long)a.vocab + BEAM_VEC - 1)
     return 9932;
   const int row_smem = BEAM_THREADS * STAGE_BYTES + BEAM_WARPS * list_room(a.k) * 8, group_smem = (int)sizeof(GroupList) + a.width * 8;
-  if (group_smem > 200 * 1024) return 9933;
+  if ((long)a.width * a.parts > BEAM_ROOM) return 9933;      // a level of all lists is looked at together
   const unsigned grid = (unsigned)(rows * a.parts);
   cudaError_t e = a.fp32 ? allow_smem<&select_rows_kernel<float>>(112 * 1024) : allow_smem<&select_rows_kernel<__nv_bfloat16>>(112 * 1024);
-  if (e == cudaSuccess) e = allow_smem<&select_groups_kernel>(200 * 1024);
+  if (e == cudaSuccess) e = allow_smem<&select_groups_kernel>(64 * 1024);
   if (e != cudaSuccess) return (int)e;
   if (a.fp32) select_rows_kernel<float><<<grid, BEAM_THREADS, row_smem, a.stream>>>(a);
   else select_rows_kernel<__nv_bfloat16><<<grid, BEAM_THREADS, row_smem, a.stream>>>(a);
