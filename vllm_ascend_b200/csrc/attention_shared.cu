@@ -257,7 +257,7 @@ struct SharedCfg {
   static constexpr int TILE = NH * SH_HALF;              // bytes of 128 rows
   static constexpr int NK = D == 128 ? 2 : 3;
   static constexpr int NV = D == 128 ? 3 : 5;
-  static constexpr int SMEM = (2 + NK + NV) * TILE + 512;        // with 1 KB of the system's, what a join's block needs stays free
+  static constexpr int SMEM = (2 + NK + NV) * TILE + 384;        // of 228 KB, what a join's block needs stays free (each takes 1 KB more)
 };
 
 __device__ __forceinline__ float sh_exp2(float x) {
@@ -788,19 +788,21 @@ __global__ void __launch_bounds__(128) shared_join_kernel(const SharedParams p) 
       for (int j = 0; j < V; j++) acc[j] += w == 0.f ? 0.f : w * x[j];       // where a group of warps had no tile, nothing was left
     }
   }
-  if constexpr (WARPS == 2) {
-    __shared__ float4 parts[2][33];
-    float4* other = parts[warp >> 1];
-    if (sub == 1) {
-      other[lane] = make_float4(acc[0], acc[1], V == 4 ? acc[V - 2] : 0.f, V == 4 ? acc[V - 1] : 0.f);
-      if (lane == 0) other[32] = make_float4(top, sum, 0.f, 0.f);
+  if constexpr (WARPS == 4) {
+    __shared__ float4 parts[3][33];
+    if (sub > 0) {
+      parts[sub - 1][lane] = make_float4(acc[0], acc[1], V == 4 ? acc[V - 2] : 0.f, V == 4 ? acc[V - 1] : 0.f);
+      if (lane == 0) parts[sub - 1][32] = make_float4(top, sum, 0.f, 0.f);
     }
     __syncthreads();
-    if (sub == 1) return;
-    const float4 e = other[32], x = other[lane];
-    const float now = fmaxf(top, e.x);
-    if (now > -INFINITY) {
+    if (sub > 0) return;
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+      const float4 e = parts[k][32], x = parts[k][lane];
+      const float now = fmaxf(top, e.x);
+      if (now == -INFINITY) continue;
       const float f = sh_exp2(top - now), fo = sh_exp2(e.x - now);
+      top = now;
       sum = f * sum + fo * e.y;
       acc[0] = f * acc[0] + fo * x.x;
       acc[1] = f * acc[1] + fo * x.y;
@@ -881,18 +883,19 @@ static int launch_shared(const SharedMaps& q, const SharedMaps& kv, const Shared
                                                                                   kv.map[1], kv.map[2], kv.map[3], p);
   const int rc = B200_CHECK_LAUNCH();
   if (rc) return rc;
-  // few rows may have many partial results, up to two of each block: two warps a row
+  // Few rows may have many partial results, up to two of each block: four warps a row.  They exchange theirs in shared memory that is not free beside
+  // the attention's blocks, so they start behind those; blocks without begin early (192 sequences behind 2048 tokens 134 -> 131 us).
   const long rows = (long)p.rows * p.Hq;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows <= 4096 ? (rows + 1) / 2 : (rows + 3) / 4));
+  cfg.gridDim = dim3((unsigned)(rows <= 4096 ? rows : (rows + 3) / 4));
   cfg.blockDim = dim3(128);
   cfg.stream = stream;
   cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return (int)(rows <= 4096 ? cudaLaunchKernelEx(&cfg, shared_join_kernel<D, 2>, p) : cudaLaunchKernelEx(&cfg, shared_join_kernel<D, 1>, p));
+  cfg.numAttrs = rows <= 4096 ? 0 : 1;
+  return (int)(rows <= 4096 ? cudaLaunchKernelEx(&cfg, shared_join_kernel<D, 4>, p) : cudaLaunchKernelEx(&cfg, shared_join_kernel<D, 1>, p));
 }
 
 }  // namespace b200

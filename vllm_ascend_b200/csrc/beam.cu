@@ -77,14 +77,46 @@ struct GroupKey {
 };
 
 // ---------------------------------------------------------------- the k best of a list
+// The k-th largest of one key a thread, found bit by bit (a barrier counts); all threads of the block.  Ranks by counting take as many steps as there are
+// keys: 512 of them 20000 clocks, 64 bits 3000.
+template <int LOW = 0>                                    // bits below LOW stay 0: a bound that more than k may reach
+__device__ __forceinline__ RowKey kth_largest(RowKey mine, int k) {
+  uint64_t last = 0;
+#pragma unroll 1
+  for (int bit = 63; bit >= LOW; bit--) {
+    const uint64_t next = last | 1ull << bit;
+    if (__syncthreads_count(mine.v >= next) >= k) last = next;
+  }
+  return {last};
+}
+template <int LOW = 0>
+__device__ __forceinline__ GroupKey kth_largest(GroupKey mine, int k) {
+  const uint64_t v = kth_largest<LOW>(RowKey{mine.v}, k).v;
+  k -= __syncthreads_count(mine.v > v);                   // places decide among equal totals
+  uint32_t last = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; bit--) {
+    const uint32_t next = last | 1u << bit;
+    if (__syncthreads_count(mine.v == v && mine.place >= next) >= k) last = next;
+  }
+  return {v, last};
+}
+
 // The k-th largest of the maxima of slices of n elements, `top` that of a thread's (element i belongs to thread i mod 512); none where fewer than k
 // slices have elements.  A slice is the lanes that leave 4 k of them, one at least.  Ends with a barrier.
-template <typename Key>
+template <typename Key, int... LOW>
 __device__ __forceinline__ Key slice_bound(Key top, int n, int k, Key* slices, Key* bound) {
   const int tid = threadIdx.x;
   int lanes = 32;
   while (min(n, BEAM_THREADS) < 4 * k * lanes && lanes > 1) lanes >>= 1;
   const int count = (min(n, BEAM_THREADS) + lanes - 1) / lanes;
+  if (count > 128) {
+    for (int o = 1; o < lanes; o <<= 1) {
+      const Key other = top.other_lane(o);
+      if (other.above(top)) top = other;
+    }
+    return kth_largest<LOW...>(tid % lanes == 0 ? top : Key::none(), k);
+  }
   for (int o = 1; o < lanes; o <<= 1) {
     const Key other = top.other_lane(o);
     if (other.above(top)) top = other;
@@ -127,6 +159,16 @@ __device__ int select_best(Key* keys, Key* other, int n, int k, Key* slices, Key
     Key* swap = from;
     from = other;
     other = swap;
+    __syncthreads();
+  }
+  if (n > k && n > 128 && n <= BEAM_THREADS) {            // down to k, which are ranked sooner
+    const Key own = tid < n ? from[tid] : Key::none();
+    const Key least = kth_largest(own, k);
+    if (tid == 0) *count = 0;
+    __syncthreads();
+    if (tid < n && !least.above(own)) from[atomicAdd(count, 1)] = own;
+    __syncthreads();
+    n = *count;
     __syncthreads();
   }
   // ranked by counting: 3 k elements at most, the block's threads shared between them
@@ -283,7 +325,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
     }
   }
   // told apart by their threads; of the bound the value counts, all that equal it reach it
-  const RowKey top = slice_bound(RowKey{high > -INFINITY ? ((uint64_t)order32(high) << 32) | (uint32_t)~tid : 0ull}, BEAM_THREADS, a.k, slices, &first_bound);
+  const RowKey top = slice_bound<RowKey, 32>(RowKey{high > -INFINITY ? ((uint64_t)order32(high) << 32) | (uint32_t)~tid : 0ull}, BEAM_THREADS, a.k, slices, &first_bound);
   if (tid == 0) bound = top.v >> 32 << 32;
   if (lane == 0) held[warp] = 0;
   __syncthreads();
