@@ -47,7 +47,8 @@ struct SharedBase {
 };
 
 // What a tile of 128 keys, one for two query tiles (the softmax of twice the rows on the same schedulers) and the begin and end of a piece cost
-constexpr int COST_TILE = 4, COST_PAIR = 9, COST_PIECE = 4;
+constexpr int COST_TILE = 4, COST_PAIR = 9;
+__host__ __device__ __forceinline__ constexpr int cost_piece(int weight) { return weight == COST_PAIR ? 13 : 4; }
 
 // plan: [0] units of cost, [1] bases, [2] blocks with work, then block_first[blocks] and block_unit[blocks + 1] (base and unit that a block begins
 // with), tok_prefix[tokens], tok_own[tokens] (base of a token, -1 no keys, -2 no sequence), group_ctx[groups], bases, and for every base and
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
     const int i = i0 + tid;
     const int tiles = i < count ? bases[i].tiles : 0;
     int all;
-    const int before = units + block_scan(tiles > 0 ? a.Hkv * (tiles * bases[i].weight + COST_PIECE) : 0, part, all);
+    const int before = units + block_scan(tiles > 0 ? a.Hkv * (tiles * bases[i].weight + cost_piece(bases[i].weight)) : 0, part, all);
     if (i < count) bases[i].cum = before;
     units += all;
   }
@@ -206,8 +207,8 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
     int need = 0, first = 0, tiles = 0;
     if (i < count && (tiles = bases[i].tiles) > 0) {
       const SharedBase b = bases[i];
-      const long cum = b.cum, head_cost = (long)tiles * b.weight + COST_PIECE, cost = a.Hkv * head_cost;
-      first = block_of(cum + COST_PIECE, units, blocks);
+      const long cum = b.cum, head_cost = (long)tiles * b.weight + cost_piece(b.weight), cost = a.Hkv * head_cost;
+      first = block_of(cum + cost_piece(b.weight), units, blocks);
       const int last = block_of(cum + cost - b.weight, units, blocks);
       // up to 128 rows, each group of warps leaves results of its own
       need = b.ntok * a.G * (a.Hkv + last - first) * (b.weight == COST_PAIR ? 1 : 2);
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
     const int i = j / a.Hkv, h = j - i * a.Hkv;
     const SharedBase b = bases[i];
     if (b.tiles <= 0) continue;
-    const long at = b.cum + (long)h * (b.tiles * b.weight + COST_PIECE) + COST_PIECE;       // unit of the first tile
+    const long at = b.cum + (long)h * (b.tiles * b.weight + cost_piece(b.weight)) + cost_piece(b.weight);       // unit of the first tile
     const int b0 = block_of(at, units, blocks), b1 = block_of(at + (b.tiles - 1) * b.weight, units, blocks);
     const int slots = b.weight == COST_PAIR ? 1 : 2;
     heads[j] = make_int2(b.part_row + (h + b0 - b.seg0) * slots * b.ntok * a.G, (b1 - b0 + 1) * slots);
@@ -290,14 +291,14 @@ struct Pieces {
     Hkv = p.Hkv;
     if ((int)blockIdx.x >= blocks) return false;
     load();
-    h = (x0 - b.cum) / (b.tiles * b.weight + COST_PIECE);
+    h = (x0 - b.cum) / (b.tiles * b.weight + cost_piece(b.weight));
     return settle();
   }
   // to the first piece from (i, h) on that has tiles in this block: a tile belongs to the block of its first unit
   __device__ __forceinline__ bool settle() {
     while (true) {
       if (b.tiles > 0) {
-        const int at = b.cum + h * (b.tiles * b.weight + COST_PIECE) + COST_PIECE;       // unit of tile 0
+        const int at = b.cum + h * (b.tiles * b.weight + cost_piece(b.weight)) + cost_piece(b.weight);       // unit of tile 0
         if (at >= x1) return false;
         t0 = x0 > at ? (x0 - at + b.weight - 1) / b.weight : 0;
         t1 = min(b.tiles, (x1 - at + b.weight - 1) / b.weight);
