@@ -1,6 +1,6 @@
 """Beam search on the engine's own batch: a round is one decode step of all live beams, selection and reordering run on the device.
 
-A prompt is computed once.  Its beams are requests that share its full blocks and own a batch row and their partly filled block; the choice of
+A prompt is computed once, behind what the prefix cache holds of it.  Its beams are requests that share its full blocks and own a batch row and their partly filled block; the choice of
 a round moves what is in those (``ops.reorder_beams``: pages as far as they are filled, recurrent states by batch row), full blocks change hands by
 reference.  Attention may read the prompt's keys and values once for all beams (``ops.paged_attention_shared``)."""
 from __future__ import annotations
@@ -134,6 +134,7 @@ class BeamSearch:
         for i, g in enumerate(groups):
             req = Request(f"beam-{next(_ids)}", np.asarray(g.prompt, dtype=np.int32), SamplingParams(max_tokens=1, temperature=0.0))
             g.slots, g.live = [req], [(list(g.prompt), 0.0)]
+            self.scheduler.reuse(req)
             left.append((i, req))
         while left:
             portions, room = [], budget
@@ -152,6 +153,8 @@ class BeamSearch:
             for j, i in enumerate(ends):
                 kept[i] = logits[j]
             self._computed(so)
+            for req, _ in so.scheduled:
+                self.scheduler.keep(req)
             left = [(i, req) for i, req in left if i not in ends]
         return torch.stack(kept)
 

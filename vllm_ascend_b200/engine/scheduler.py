@@ -348,6 +348,20 @@ class Scheduler:
         out.num_scheduled_tokens = sum(n for _, n in out.scheduled)
         return out
 
+    def reuse(self, req: Request) -> None:
+        """A request that ``schedule_portions`` has not seen yet begins behind those blocks of its prompt that the prefix cache holds."""
+        if self.pool.enable_prefix_caching:
+            hashes = self._hashes[req.request_id] = self.pool.block_hashes(req.prompt_token_ids)
+            req.block_ids = self.pool.find_cached_prefix(hashes[:(req.num_prompt_tokens - 1) // self.block_size])
+            self.pool.touch(req.block_ids)
+            req.num_cached_tokens = req.num_computed_tokens = len(req.block_ids) * self.block_size
+
+    def keep(self, req: Request) -> None:
+        """What is computed of its prompt goes into the prefix cache."""
+        if self.pool.enable_prefix_caching:
+            full = min(req.num_computed_tokens, req.num_prompt_tokens) // self.block_size
+            self.pool.cache_full_blocks(req.block_ids, self._hashes[req.request_id], full)
+
     def fork(self, parent: Request, request_id: str) -> Request:
         """A request that goes on from ``parent``'s computed tokens: a batch row of its own, the full blocks shared, a block of its own for a
         partly filled last one (the caller copies its content, and what the layers keep beside pages)."""
