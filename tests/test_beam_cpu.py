@@ -62,3 +62,21 @@ def test_reorderings_that_are_refused():
     for r, p in (([[0, 1, 6]], [[0, 0, 0]]), ([[0, 1, 2]], [[0, 3, 0]]), ([[0, -1, 2]], [[1, 0, 0]])):
         with pytest.raises(IndexError):
             ops.reorder_beams(plain, torch.tensor(r, dtype=torch.int32), torch.tensor(p, dtype=torch.int32))
+
+
+def test_tensors_that_share_memory_are_refused():
+    x, slices = torch.zeros(6, 16, 2, 4), torch.arange(6 * 12.).view(6, 12)
+    for tensors, paged in (([x, x], False), ([x, x[2:]], False), ([x.view(6, -1)[:, :100], x.view(6, -1)[:, 96:]], False), ([x, x], True),
+                           ([slices, slices.view(12, 6)], False), ([slices[:, :4], slices[:, 8:], slices[2:, 2:6]], False)):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.beam_states(tensors, paged=paged)
+    both = torch.zeros(5, 2, 3, 16, 4)                   # keys and values of a page side by side
+    ops.beam_states([both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)], paged=True)
+    each = torch.zeros(5, 3, 2, 16, 4)                   # of a head
+    ops.beam_states([each[:, :, 0].transpose(1, 2), each[:, :, 1].transpose(1, 2)], paged=True)
+    ops.beam_states([slices[:3], slices[3:]])
+    parts = [slices[:, :4], slices[:, 4:]]
+    rows, parents = torch.tensor([[0, 5]], dtype=torch.int32), torch.tensor([[1, 0]], dtype=torch.int32)
+    want = slices[[5, 1, 2, 3, 4, 0]]
+    ops.reorder_beams(ops.beam_states(parts), rows, parents)
+    assert torch.equal(slices, want)

@@ -95,12 +95,16 @@ class BeamStates:
     def __init__(self, tensors: list, paged: bool, int4_dim: int):
         self.tensors, self.paged, self.int4_dim = tensors, paged, int4_dim
         self.device = tensors[0].device
-        self._table, self._wide = None, 0
-        rows = sorted((_layout(t, paged, int4_dim) for t in tensors), key=lambda r: -r[-1])
+        self._table, self._wide, self._stream = None, 0, 0
+        rows = [_layout(t, paged, int4_dim) for t in tensors]
+        _check_apart(rows)
+        rows.sort(key=lambda r: -r[-1])
         if self.device.type == "cuda":
             packed = b"".join(_TENSOR.pack(*r) for r in rows)
             self._table = torch.frombuffer(bytearray(packed), dtype=torch.uint8).to(self.device)
             self._wide = sum(r[-1] == 16 for r in rows)
+            with torch.cuda.device(self.device):
+                self._stream = _native.stream_ptr()
 
 
 def _layout(t: torch.Tensor, paged: bool, int4_dim: int) -> tuple:
@@ -137,10 +141,26 @@ def _layout(t: torch.Tensor, paged: bool, int4_dim: int) -> tuple:
     return t.data_ptr(), row, run, unit, t.shape[0], outer, units, tokens, width
 
 
+def _check_apart(rows: list) -> None:
+    """Refuses memory that two tensors would move: rows that lie between each other's, as in slices of one buffer, do not overlap."""
+    ordered = sorted(r for r in rows if r[4] and r[6] * r[3])
+    for i, (at, row, run, unit, n, outer, units, _, _) in enumerate(ordered):
+        end = at + (n - 1) * row + (outer - 1) * run + units * unit
+        for at2, row2, run2, unit2, _, outer2, units2, _, _ in ordered[i + 1:]:
+            if at2 >= end:
+                break
+            one, two = units * unit, units2 * unit2           # bytes in one piece
+            off = (at2 - at) % row if row else 0
+            apart = row == row2 and (outer - 1) * run + one <= off and off + (outer2 - 1) * run2 + two <= row
+            off %= run or 1
+            if not (apart or row == row2 and outer > 1 and (outer, run) == (outer2, run2) and one <= off and off + two <= run):
+                raise ValueError("two of the tensors share memory")
+
+
 def beam_states(tensors: Sequence[torch.Tensor], paged: bool = False, int4_dim: int = 0) -> BeamStates:
     """Handle for ``reorder_beams``: tensors of any types and sizes on one device whose first dimension is a row (recurrent states) or, with
-    ``paged``, a page (caches [pages, tokens, heads, channels] in either physical order, or 4-bit ones of heads of ``int4_dim``).  It holds addresses:
-    keep it as long as the tensors, make another when they are replaced."""
+    ``paged``, a page (caches [pages, tokens, heads, channels] in either physical order, or 4-bit ones of heads of ``int4_dim``).  No two of them share
+    memory.  It holds addresses: keep it as long as the tensors, make another when they are replaced."""
     tensors = list(tensors)
     if not tensors:
         raise ValueError("no tensors")
@@ -172,11 +192,14 @@ def reorder_beams(states: BeamStates, rows: torch.Tensor, parents: torch.Tensor,
     if device != torch.cuda.current_device():
         with torch.cuda.device(device):
             return reorder_beams(states, rows, parents, lengths)
+    stream = _native.stream_ptr()
+    if stream != states._stream:
+        states._table.record_stream(torch.cuda.current_stream())
     rows, parents = rows.contiguous(), parents.contiguous()
     lengths = None if lengths is None else lengths.contiguous()
     rc = _native.lib().b200_beam_reorder(_REORDER.pack(
         states._table.data_ptr(), rows.data_ptr(), parents.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
-        _native.status_word(rows.device).data_ptr(), _native.stream_ptr(), len(states.tensors), groups, beams, states._wide,
+        _native.status_word(rows.device).data_ptr(), stream, len(states.tensors), groups, beams, states._wide,
         _native.sm_count(device)))
     _native.check(rc, "beam_reorder")
     wide = states._wide if beams <= 16 else 0
