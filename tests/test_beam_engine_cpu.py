@@ -137,3 +137,36 @@ def test_engines_that_search_by_requests(monkeypatch):
     llm.engine.runner.lora_manager = None
     assert beam.on_device(llm.engine, [[1] * 10], 2, 4)
     assert llm.beam_search([], beam_width=2, max_tokens=3) == []
+
+
+def test_prompts_begin_behind_what_the_prefix_cache_holds(monkeypatch):
+    llm = LLM("tiny-qwen", device="cpu", seed=1, block_size=16, max_model_len=128, max_num_seqs=16, enable_prefix_caching=True)
+    free = llm.engine.scheduler.pool.num_free_blocks
+    steps = []
+    runner = llm.engine.runner
+    logits = runner.device_logits
+    monkeypatch.setattr(runner, "device_logits", lambda so, rows=None: steps.append(so.num_scheduled_tokens) or logits(so, rows))
+    prompts = _prompts(33, 64, 40)
+    first = llm.beam_search(prompts, beam_width=3, max_tokens=20, ignore_eos=True)
+    assert steps[0] == 33 + 64 + 40
+    _idle(llm, free)
+    steps.clear()
+    _same(llm.beam_search(prompts, beam_width=3, max_tokens=20, ignore_eos=True), first)
+    assert steps[0] == 1 + 16 + 8                        # a last token is always computed
+    steps.clear()
+    _same(llm.beam_search([p + [7] for p in prompts], beam_width=2, max_tokens=3, ignore_eos=True),
+          LLM("tiny-qwen", device="cpu", seed=1, block_size=16, max_model_len=128, max_num_seqs=16).beam_search(
+              [p + [7] for p in prompts], beam_width=2, max_tokens=3, ignore_eos=True))
+    assert steps[0] == 2 + 1 + 9
+    _idle(llm, free)
+
+
+def test_engines_that_read_every_prefix_for_itself():
+    assert LLM("tiny-qwen", device="cpu", max_model_len=64, max_num_seqs=2).engine.runner.can_share_prefixes()
+    for model, kw in (("tiny-qwen", {"speculative_config": {"method": "ngram", "num_speculative_tokens": 2}}), ("tiny-qwen", {"kv_cache_dtype": "int4"}),
+                      ("tiny-gdn", {})):
+        from vllm_ascend_b200.config import get_model_config
+        cfg = get_model_config(model)
+        if kw.get("kv_cache_dtype"):
+            cfg.head_dim = 64
+        assert not LLM(cfg, device="cpu", max_model_len=64, max_num_seqs=2, disable_cascade_attn=False, **kw).engine.runner.can_share_prefixes()

@@ -91,3 +91,8 @@ def test_decode_batches_with_a_common_prefix(monkeypatch):
         lp = [[lps[t] for lps, t in zip(o.logprobs, o.token_ids)] for o in (a, b)]
         np.testing.assert_allclose(lp[0][:n], lp[1][:n], atol=0.06)
     assert sum(a.token_ids[:3] == b.token_ids[:3] for a, b in zip(*outs)) >= 4
+
+
+def test_engines_without_the_kernel_read_every_prefix_for_itself():
+    assert _llm().engine.runner.can_share_prefixes()
+    assert not _llm("float32", enforce_eager=True, disable_cascade_attn=False).engine.runner.can_share_prefixes()

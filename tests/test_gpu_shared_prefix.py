@@ -181,3 +181,40 @@ def test_bad_pages_and_starts_are_reported():
         with pytest.raises(_native.NativeError, match="BAD_INDEX"):
             _native.check_status(b.q.device)
         assert out.eq(3).all()
+
+
+@pytest.mark.parametrize("prefix,seqs", [(128, 64), (100, 33), (16, 70)])
+def test_short_prefixes_of_many_sequences(prefix, seqs):
+    b = Batch([(prefix, [(1 + 37 * i % 150, 1) for i in range(seqs)])], 32, 8, 128, 16, device="cuda", seed=3)
+    b.check(b.run(_ops()))
+
+
+def test_lengths_that_no_cache_holds_are_reported():
+    from vllm_ascend_b200 import _native
+    b = Batch(GROUPS["one prompt, four beams"], 8, 8, 128, 128, device="cuda")
+    b.meta.seq_lens.fill_(2 ** 31 - 200)
+    b.prefixes = torch.zeros_like(b.prefixes)
+    out = torch.full((b.rows, 8, 128), 3.0, dtype=torch.bfloat16, device="cuda")
+    b.run(_ops(), out)
+    torch.cuda.synchronize()
+    with pytest.raises(_native.NativeError, match="BAD_INDEX"):
+        _native.check_status(b.q.device)
+    assert out.eq(3).all()
+
+
+def test_a_plan_outlives_its_owner_on_another_stream():
+    ops = _ops()
+    b = Batch(GROUPS["one prompt, four beams"], 32, 8, 128, 128, device="cuda")
+    want = b.run(ops)
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        plan = b.plan(ops)
+        size = plan.table.numel()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = [ops.paged_attention_shared(b.q, b.k_cache, b.v_cache, b.meta, plan, b.scale) for _ in range(8)]
+        del plan
+        junk = [torch.full((size,), -1, dtype=torch.int32, device="cuda") for _ in range(4)]      # would take its place
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, want) for x in got)
+        del junk

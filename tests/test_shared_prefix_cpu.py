@@ -54,3 +54,19 @@ def test_refusals():
     with pytest.raises(IndexError):
         bad = ops.plan_shared_prefix(b.meta, torch.tensor([1, 0], dtype=torch.int32), b.prefixes, 4, 2)
         ops.paged_attention_shared(q, k, v, b.meta, bad, 1.0)
+
+
+def test_a_plan_is_not_used_for_another_batch():
+    import copy
+    b = Batch([(16, [(5, 1), (9, 1)])], 4, 2, 8, 8, dtype=torch.float32)
+    meta = b.meta
+    meta.block_table[1, :2] = meta.block_table[0, :2]
+    meta.shared = b.plan(ops)
+    want = b.run(ops)
+    assert torch.equal(ops.paged_attention(b.q.contiguous(), b.k_cache, b.v_cache, meta, b.scale), want)
+    other = copy.copy(meta)                              # what a drafter does with a step's metadata
+    other.seq_lens, other.seq_lens_cpu = meta.seq_lens - 1, meta.seq_lens_cpu - 1
+    got = ops.paged_attention(b.q.contiguous(), b.k_cache, b.v_cache, other, b.scale)
+    other.shared = None
+    assert torch.equal(got, ops.paged_attention(b.q.contiguous(), b.k_cache, b.v_cache, other, b.scale))
+    assert not torch.allclose(got, want)

@@ -48,6 +48,7 @@ struct SharedBase {
 
 // What a tile of 128 keys, one for two query tiles (the softmax of twice the rows on the same schedulers) and the begin and end of a piece cost
 constexpr int COST_TILE = 4, COST_PAIR = 9;
+constexpr unsigned long long MOST_UNITS = 1ull << 30;
 __host__ __device__ __forceinline__ constexpr int cost_piece(int weight) { return weight == COST_PAIR ? 13 : 4; }
 
 // plan: [0] units of cost, [1] bases, [2] blocks with work, then block_first[blocks] and block_unit[blocks + 1] (base and unit that a block begins
@@ -100,6 +101,7 @@ __device__ __forceinline__ int block_scan(int v, int* part, int& all) {
 __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   __shared__ int part[32];
   __shared__ int bad;
+  __shared__ unsigned long long all_units;
   const int tid = threadIdx.x;
   int* head = a.plan;
   int* block_first = head + PLAN_HEAD;
@@ -109,7 +111,7 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
   int* group_ctx = tok_own + a.tokens;
   SharedBase* bases = reinterpret_cast<SharedBase*>(head + a.bases_at);
   int2* heads = reinterpret_cast<int2*>(head + plan_heads_at(a.bases_at, a.max_bases));
-  if (tid == 0) bad = 0;
+  if (tid == 0) bad = 0, all_units = 0;
   __syncthreads();
   for (int t = tid; t < a.tokens; t += 1024) tok_prefix[t] = -1, tok_own[t] = -2;
   for (int g = tid; g < a.groups; g += 1024) group_ctx[g] = 0x7fffffff;
@@ -186,7 +188,20 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
     }
   }
   __syncthreads();
-  // cost
+  // Cost: units are counted in 32 bits.  What a cache can hold stays far below (180 GB are 50 million units); lengths that are none do not.
+  unsigned long long mine = 0;
+  for (int i = tid; i < count; i += 1024)
+    if (bases[i].tiles > 0) mine += (unsigned long long)a.Hkv * ((long)bases[i].tiles * bases[i].weight + cost_piece(bases[i].weight));
+  atomicAdd(&all_units, mine);
+  __syncthreads();
+  if (all_units > MOST_UNITS) {
+    for (int t = tid; t < a.tokens; t += 1024) tok_prefix[t] = -1, tok_own[t] = -2;
+    if (tid == 0) {
+      head[0] = head[1] = head[2] = 0;
+      if (a.status) atomicExch(a.status, B200_BAD_INDEX);
+    }
+    return;
+  }
   int units = 0;
   for (int i0 = 0; i0 < count; i0 += 1024) {
     const int i = i0 + tid;

@@ -709,23 +709,23 @@ class ModelRunner:
     # ------------------------------------------------------------------ shared prefixes
     def can_share_prefixes(self) -> bool:
         """Whether decode steps can read prefixes that their sequences share once a group: grouped-query attention over pages of the model's type, in a
-        mode that leaves the order of sums open, with nothing beside pages that a graph's warm-up would touch."""
+        mode that leaves the order of sums open, with nothing beside pages that a graph's warm-up would touch, on one GPU and without drafts (a
+        drafter goes on with the step's lengths)."""
         c = self.mcfg
         from ..batch_invariant import fixed_sums
-        return not (c.use_mla or c.layer_plan or c.sliding_window or c.keeps_sequence_state or self._kv_int4() or self.dcp_size > 1
-                    or self.pp.world_size > 1 or self.pcp.world_size > 1 or self.sparse_offload is not None or self.lora_manager is not None
-                    or self.moe_runtime is not None or fixed_sums())
+        from ..ops.shared_prefix import has_kernel
+        if c.use_mla or c.layer_plan or c.sliding_window or c.keeps_sequence_state or self._kv_int4() or self.dcp_size > 1 \
+                or self.pp.world_size > 1 or self.pcp.world_size > 1 or self.cfg.parallel.tensor_parallel_size > 1 \
+                or self.sparse_offload is not None or self.lora_manager is not None or self.moe_runtime is not None \
+                or self.proposer is not None or fixed_sums():
+            return False
+        return not self.is_cuda or has_kernel(self.kv_dtype, self._attn_layer().D, self.block_size)
 
     def _sharing_pays(self, groups: list) -> bool:
-        """Whether a layer's attention takes less time with prefixes read once: what is not read again, at 6 TB/s, against 6 us for results that
-        two kernels join (32 heads on 8 of 128, eight beams over 2048 tokens: 14 us shared, 19 plain; four over 1500: 13 and 11)."""
-        if not self.is_cuda:
-            return True
-        a = self._attn_layer()
-        return sum((n - 1) * prefix for n, prefix in groups) * a.Hkv * a.D * 2 * self._kv_itemsize() / 6e6 > 6
-
-    def _kv_itemsize(self) -> int:
-        return torch.empty(0, dtype=self.kv_dtype).element_size()
+        """Whether a layer's attention takes less time with prefixes read once: where 256 keys a sequence are not read again.  Behind them every sequence
+        costs a piece of work of its own, which plain decoding splits and feeds better.  32 heads on 8 of 128, us shared (plain): 4 beams over 512 keys
+        12 (13.5), over 4096 16 (21); 64 requests over 128 32 (27), over 256 32 (30), over 512 34 (38); 192 over 128 127 (122), over 512 128 (153)."""
+        return not self.is_cuda or sum((n - 1) * prefix for n, prefix in groups) >= 256 * sum(n for n, _ in groups)
 
     def _find_shared(self, so: SchedulerOutput) -> None:
         """Groups of a decode step: those that the caller knows, or all of its sequences where they begin with the same blocks."""

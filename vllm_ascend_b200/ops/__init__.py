@@ -665,11 +665,11 @@ def paged_attention_consistent(q: torch.Tensor, k_cache: torch.Tensor, v_cache: 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta,
                     scale: float, out: Optional[torch.Tensor] = None, causal: bool = True,
                     window: int = 0) -> torch.Tensor:
-    """Attention of every scheduled token over its sequence's paged KV.  With a plan for shared prefixes in ``meta.shared`` they are read once a
-    group, where the cache is not quantised and there is no window."""
-    plan = meta.shared
-    if plan is not None and causal and not window and k_cache.dtype != torch.uint8 and not fixed_sums() and v_cache.shape == k_cache.shape \
-            and (q.shape[1], k_cache.shape[2]) == (plan.heads, plan.kv_heads):
+    """Attention of every scheduled token over its sequence's paged KV.  With a plan for shared prefixes of these very sequences in ``meta.shared``
+    they are read once a group, where the cache is of the queries' type and there is no window."""
+    plan = getattr(meta, "shared", None)
+    if plan is not None and plan.of(meta) and causal and not window and q.dtype == k_cache.dtype == v_cache.dtype and not fixed_sums() \
+            and v_cache.shape == k_cache.shape and (q.shape[1], k_cache.shape[2]) == (plan.heads, plan.kv_heads):
         return paged_attention_shared(q, k_cache, v_cache, meta, plan, scale, out)
     if k_cache.dtype == torch.uint8:
         return paged_attention_int4(q, k_cache, v_cache, meta, scale, out, causal, window)

@@ -27,6 +27,11 @@ HEAD_SIZES = (64, 128)
 _BASE, _ROWS = 12, 256
 
 
+def has_kernel(dtype: torch.dtype, head_size: int, block_size: int) -> bool:
+    """Whether queries and caches of that type, heads and pages of that size run the kernel on a GPU."""
+    return dtype is torch.bfloat16 and head_size in HEAD_SIZES and block_size >= 8 and not (128 % block_size if block_size < 128 else block_size % 128)
+
+
 @dataclass
 class SharedPrefixPlan:
     """Which sequences share which prefix, and how the work is dealt out; made once a step for all layers of one head layout."""
@@ -40,6 +45,13 @@ class SharedPrefixPlan:
     bases_at: int = 0
     bases: int = 0
     table: Optional[torch.Tensor] = None
+    stream: int = 0                                  # it was made on
+    starts: Optional[torch.Tensor] = None            # the batch's own tensors: first query rows, lengths
+    lens: Optional[torch.Tensor] = None
+
+    def of(self, meta) -> bool:
+        """Whether it was made for this batch, not for one that a copy of its metadata stands for."""
+        return meta.query_start_loc is self.starts and meta.seq_lens is self.lens and meta.num_reqs == self.seqs
 
 
 def plan_shared_prefix(meta, group_starts, prefix_lens, heads: int, kv_heads: int) -> SharedPrefixPlan:
@@ -49,7 +61,8 @@ def plan_shared_prefix(meta, group_starts, prefix_lens, heads: int, kv_heads: in
     tokens counts up to where they begin.
 
     Lengths are read on the device: a captured plan follows what replays find there, as long as sequences, groups and query rows are no more than
-    at capture.  Starts that are out of order or out of range are reported through the status word, and nothing is computed."""
+    at capture.  Starts that are out of order or out of range, and lengths beyond what any cache holds, are reported through the status word, and nothing is
+    computed.  A plan belongs to the stream that it is made on; calls on others wait for that one first."""
     device = meta.query_start_loc.get_device()
     if _elsewhere(device):
         with torch.cuda.device(device):
@@ -62,9 +75,10 @@ def plan_shared_prefix(meta, group_starts, prefix_lens, heads: int, kv_heads: in
             and starts.get_device() == prefixes.get_device() == device):
         raise ValueError(f"group starts int32 [groups + 1] and prefix lengths int32 [groups] on {where}, not {starts.dtype} {tuple(starts.shape)} on "
                          f"{starts.device} and {prefixes.dtype} {tuple(prefixes.shape)} on {prefixes.device}")
-    meta = _dense(meta, device)
+    given, meta = meta, _dense(meta, device)
     starts, prefixes = starts.contiguous(), prefixes.contiguous()
-    plan = SharedPrefixPlan(starts, prefixes, heads, kv_heads, max(int(meta.num_actual_tokens), int(meta.num_input_tokens)), meta.num_reqs)
+    plan = SharedPrefixPlan(starts, prefixes, heads, kv_heads, max(int(meta.num_actual_tokens), int(meta.num_input_tokens)), meta.num_reqs,
+                            starts=given.query_start_loc, lens=given.seq_lens)
     if device < 0:
         return plan
     G, groups, n = heads // kv_heads, prefixes.shape[0], meta.num_reqs
@@ -72,9 +86,10 @@ def plan_shared_prefix(meta, group_starts, prefix_lens, heads: int, kv_heads: in
     plan.bases = bases = groups + n + 2 * (plan.tokens // (2 * (128 // G)))
     plan.bases_at = -(-(4 + 2 * plan.blocks + 2 * plan.tokens + groups) // 4) * 4
     plan.table = torch.empty(plan.bases_at + bases * (_BASE + 2 * kv_heads), dtype=torch.int32, device=where)
+    plan.stream = _native.stream_ptr()
     rc = _native.lib().b200_shared_plan(_PLAN.pack(
         meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(), starts.data_ptr(), prefixes.data_ptr(), plan.table.data_ptr(),
-        _native.status_word(where).data_ptr(), _native.stream_ptr(), n, groups, plan.tokens, G, kv_heads, plan.blocks, bases, plan.bases_at))
+        _native.status_word(where).data_ptr(), plan.stream, n, groups, plan.tokens, G, kv_heads, plan.blocks, bases, plan.bases_at))
     _native.check(rc, "shared_plan")
     _native.count_launch()
     return plan
@@ -84,7 +99,7 @@ def paged_attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal ``paged_attention`` of q [T, Hq, D] over caches [blocks, tokens, heads, D] with the prefixes of ``plan`` read once a group.  Any number of
     new tokens a sequence.  Rows of ``out`` behind the last sequence are left as they are; a token without keys gets zeros.  bf16 with heads of
-    64 and 128 runs the kernel; other types and sizes the definition.  Keys and values of pages that lie outside of a sequence may hold anything,
+    64 and 128 runs the kernel, with 16 (D + 2) bytes of workspace for every row and query head; other types and sizes the definition.  Keys and values of pages that lie outside of a sequence may hold anything,
     those of its own new tokens are numbers."""
     shape, pages, device = q.shape, k_cache.shape, q.get_device()
     if len(shape) != 3 or len(pages) != 4 or v_cache.shape != pages or pages[3] != shape[2]:
@@ -112,7 +127,7 @@ def paged_attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         out = q.new_empty(shape)
     elif out.shape != shape or out.dtype != dtype or out.get_device() != device:
         raise ValueError(f"out: {dtype} {tuple(shape)} on {q.device}, not {out.dtype} {tuple(out.shape)} on {out.device}")
-    if device < 0 or dtype is not torch.bfloat16 or D not in HEAD_SIZES or bs < 8 or (128 % bs if bs < 128 else bs % 128):
+    if device < 0 or not has_kernel(dtype, D, bs):
         return _definition(q, k_cache, v_cache, _dense(meta, device), plan, scale, out)
     if T == 0 or plan.tokens == 0 or n == 0:
         return out
@@ -128,12 +143,15 @@ def paged_attention_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         if channel != 1 or head != D or row % 8 or out.data_ptr() % 16:
             out = q.new_empty(shape)
             out.copy_(given)
+    stream = _native.stream_ptr()
+    if stream != plan.stream:
+        plan.table.record_stream(torch.cuda.current_stream())
     # every call has its own results of pieces: calls on two streams, or two graphs, may run at once
     part_rows = 4 * plan.tokens * Hq + plan.blocks * _ROWS
     parts = plan.prefix_lens.new_empty(part_rows * (D + 2))          # of 32 bits each
     rc = _native.lib().b200_attn_shared(_ATTENTION.pack(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), plan.table.data_ptr(), table.data_ptr(), parts.data_ptr(), out.data_ptr(),
-        _native.status_word(plan.prefix_lens.device).data_ptr(), _native.stream_ptr(), q.stride(0), T, NB, table.stride(0), out.stride(0), part_rows,
+        _native.status_word(plan.prefix_lens.device).data_ptr(), stream, q.stride(0), T, NB, table.stride(0), out.stride(0), part_rows,
         strides[0], strides[1], strides[2], scale, bs, table.shape[1], Hq, Hkv, D, plan.blocks, plan.tokens, plan.bases_at, plan.bases))
     _native.check(rc, "attn_shared")
     _native.count_launch(2)
