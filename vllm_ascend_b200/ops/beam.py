@@ -6,6 +6,7 @@ sorts candidates on the host and starts every round with new requests (``LLM.bea
 from __future__ import annotations
 
 import functools
+import math
 import struct
 from ctypes import c_char_p
 from typing import Optional, Sequence
@@ -142,19 +143,24 @@ def _layout(t: torch.Tensor, paged: bool, int4_dim: int) -> tuple:
 
 
 def _check_apart(rows: list) -> None:
-    """Refuses memory that two tensors would move: rows that lie between each other's, as in slices of one buffer, do not overlap."""
+    """Refuses memory that two tensors would move.  Rows may lie between each other's, as in slices of one buffer: places modulo what both
+    distances between rows are multiples of tell, or those modulo the distance of pieces where both have rows of such pieces."""
     ordered = sorted(r for r in rows if r[4] and r[6] * r[3])
     for i, (at, row, run, unit, n, outer, units, _, _) in enumerate(ordered):
-        end = at + (n - 1) * row + (outer - 1) * run + units * unit
-        for at2, row2, run2, unit2, _, outer2, units2, _, _ in ordered[i + 1:]:
-            if at2 >= end:
+        one = units * unit                                     # bytes of a piece
+        span = (outer - 1) * run + one
+        for at2, row2, run2, unit2, n2, outer2, units2, _, _ in ordered[i + 1:]:
+            if at2 >= at + (n - 1) * row + span:
                 break
-            one, two = units * unit, units2 * unit2           # bytes in one piece
-            off = (at2 - at) % row if row else 0
-            apart = row == row2 and (outer - 1) * run + one <= off and off + (outer2 - 1) * run2 + two <= row
-            off %= run or 1
-            if not (apart or row == row2 and outer > 1 and (outer, run) == (outer2, run2) and one <= off and off + two <= run):
-                raise ValueError("two of the tensors share memory")
+            two = units2 * unit2
+            span2 = (outer2 - 1) * run2 + two
+            every = math.gcd(row if n > 1 else 0, row2 if n2 > 1 else 0) or span + span2 + at2 - at
+            off = (at2 - at) % every
+            if off >= span and off + span2 <= every:
+                continue
+            if outer > 1 and (row, run, outer) == (row2, run2, outer2) and one <= off % run and off % run + two <= run:
+                continue
+            raise ValueError("two of the tensors share memory")
 
 
 def beam_states(tensors: Sequence[torch.Tensor], paged: bool = False, int4_dim: int = 0) -> BeamStates:
