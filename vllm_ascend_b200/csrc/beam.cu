@@ -5,14 +5,16 @@
 //
 // Selection reads the logits once.  A block walks a part of a row: every thread keeps a running maximum and the sum of exponentials
 // under it; elements that reach the bound of the k-th best so far go to their warp's list in shared memory.  Within a row totals are
-// ordered as logits are, so the lists need no sum.  The bound begins with the first 4096 elements: the k-th largest of the maxima of
-// slices of them, which k elements or more reach, and not many more where values are in no order.  A warp whose list is full cuts it back to its
-// k best, whose last raises the bound for all.  Keys carry the value and, below it, the place: no two are equal, ties go to the
+// ordered as logits are, so the lists need no sum.  The bound begins with the part's first elements, 32 a thread (16 of 32 bits): the k-th largest of the
+// maxima of slices of them, which k elements or more reach, and not many more where values are in no order.  A warp whose list is full cuts it back to
+// its k best, whose last raises the bound for all.  Keys carry the value and, below it, the place: no two are equal, ties go to the
 // lowest place by themselves, and rows of equal values (masked ones) put nothing behind their first into a list.
-// Bound by HBM for many rows: about six instructions and an exponential an element are 0.6 of what an SM issues at its share of the bytes.
-// A second kernel, a block a group, adds up the sums of the parts, turns its beams' keys into totals and cuts them back in the same way.
+// A second kernel, a block a group, adds up the sums of the parts, turns its beams' keys into totals and takes the best by their places in the lists.
 // Parts' sums are added in 64 bits and totals compared in 64: with thousands of candidates, sums of 32 bits would order near ones
 // by their rounding.
+// Bound by HBM for many rows, while blocks stream: 768 rows of 151936 in bf16 take 91 us, 2.6 TB/s; a block streams its 304 KB for 17 us, two an SM at
+// 5.3 TB/s, takes 3 us for its first elements and their bound, 4 us to put its k best in order, and 768 rows are 2.6 turns of 296 blocks.  Few rows are
+// bound by those beginnings and ends and the second kernel, 5 us: 64 rows 22 us, 4 of 32000 13 us.
 // Reordering: a thread owns 16 bytes of a row for all beams of a group and loads what they become before it stores the first.
 #include "common.cuh"
 
@@ -141,8 +143,8 @@ __device__ int select_best(Key* keys, Key* other, int n, int k, Key* slices, Key
   const int tid = threadIdx.x;
   Key* from = keys;
   // Only k slices reach the bound: a quarter of the elements at most, or where a slice is a thread, its k elements for every 512; values in no order
-  // take one pass.
-  for (bool more = n > max(2 * k, 64); more; more = n > max(3 * k, 256)) {
+  // take one pass.  128 are ranked sooner than thinned out (64 rows of 151936: 22 us, 25 with a pass from 64 on).
+  for (bool more = n > max(2 * k, 128); more; more = n > max(3 * k, 256)) {
     Key top = Key::none();
 #pragma unroll 1
     for (int i = tid; i < n; i += BEAM_THREADS)
@@ -217,22 +219,44 @@ __device__ __forceinline__ void bring(T* to, const T* row, int at, int end) {
     for (int j = 0; j < BEAM_VEC; j++) to[j] = at + j >= 0 && at + j < end ? row[at + j] : T(-INFINITY);
   }
 }
+// Eight elements and the largest of them; of 16 bits two are compared at a time.
 template <typename T>
-__device__ __forceinline__ void take(const T* from, float* x) {
+__device__ __forceinline__ float take(const T* from, float* x) {
   const uint4 a = *reinterpret_cast<const uint4*>(from);
   const uint32_t w[4] = {a.x, a.y, a.z, a.w};
   if constexpr (sizeof(T) == 2) {
+    auto pair = [&](int i) { return *reinterpret_cast<const __nv_bfloat162*>(w + i); };
+    const float2 top = __bfloat1622float2(__hmax2(__hmax2(pair(0), pair(1)), __hmax2(pair(2), pair(3))));
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       x[2 * i] = __uint_as_float(w[i] << 16);
       x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
+    return fmaxf(top.x, top.y);
   } else {
     const uint4 b = *(reinterpret_cast<const uint4*>(from) + 1);
     const uint32_t v[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] = __uint_as_float(w[i]), x[4 + i] = __uint_as_float(v[i]);
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < BEAM_VEC; i++) top = fmaxf(top, x[i]);
+    return top;
   }
+}
+
+// two sums or products of 32 bits at a time
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 y;
+  asm("{\n.reg .b64 p, q;\nmov.b64 p, {%2, %3};\nmov.b64 q, {%4, %5};\nadd.rn.f32x2 p, p, q;\nmov.b64 {%0, %1}, p;\n}"
+      : "=f"(y.x), "=f"(y.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return y;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 y;
+  asm("{\n.reg .b64 p, q;\nmov.b64 p, {%2, %3};\nmov.b64 q, {%4, %5};\nmul.rn.f32x2 p, p, q;\nmov.b64 {%0, %1}, p;\n}"
+      : "=f"(y.x), "=f"(y.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return y;
 }
 
 __device__ __forceinline__ bool is_score(float s) { return s > -INFINITY && s < INFINITY; }
@@ -318,11 +342,8 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
 #pragma unroll
   for (int i = 0; i < STAGES; i++) {
     float x[BEAM_VEC];
-    take(stage + i * BEAM_TILE, x);
-    if (at0 + i * BEAM_TILE < to) {
-#pragma unroll
-      for (int j = 0; j < BEAM_VEC; j++) high = fmaxf(high, x[j]);
-    }
+    const float t = take(stage + i * BEAM_TILE, x);
+    if (at0 + i * BEAM_TILE < to) high = fmaxf(high, t);
   }
   // told apart by their threads; of the bound the value counts, all that equal it reach it
   const RowKey top = slice_bound<RowKey, 32>(RowKey{high > -INFINITY ? ((uint64_t)order32(high) << 32) | (uint32_t)~tid : 0ull}, BEAM_THREADS, a.k, slices, &first_bound);
@@ -342,10 +363,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
     }
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
     float x[BEAM_VEC];
-    take(stage + st * BEAM_TILE, x);
-    float t = x[0];
-#pragma unroll
-    for (int j = 1; j < BEAM_VEC; j++) t = fmaxf(t, x[j]);
+    const float t = take(stage + st * BEAM_TILE, x);
     if (mine < to) {
       if (t > m) {
         s *= beam_exp2((m - t) * kBeamLog2e);      // nothing before the first element that is above -inf
@@ -353,10 +371,13 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
       }
       // differences from the maximum are taken before the factor: a product of the maximum would carry its rounding into every term
       const float under = m == -INFINITY ? 0.f : m;
-      float u[4] = {0.f, 0.f, 0.f, 0.f};
+      float2 u[2] = {};
 #pragma unroll
-      for (int j = 0; j < BEAM_VEC; j++) u[j & 3] += beam_exp2((x[j] - under) * kBeamLog2e);       // a NaN or +inf: NaN
-      s += (u[0] + u[1]) + (u[2] + u[3]);
+      for (int j = 0; j < BEAM_VEC; j += 2) {
+        const float2 d = mul2(add2(make_float2(x[j], x[j + 1]), make_float2(-under, -under)), make_float2(kBeamLog2e, kBeamLog2e));
+        u[j >> 1 & 1] = add2(u[j >> 1 & 1], make_float2(beam_exp2(d.x), beam_exp2(d.y)));       // a NaN or +inf: NaN
+      }
+      s += (u[0].x + u[0].y) + (u[1].x + u[1].y);
     }
     const bool hit = mine < to && (t > reach || (reach > -INFINITY ? t == reach && mine <= place : mine < 2 * a.k));
     if (__any_sync(0xffffffffu, hit)) {
@@ -619,7 +640,8 @@ __device__ __forceinline__ void walk_row(const BeamTensor& t, long run, int widt
 }
 
 // Up to MOST beams: what a thread's 16 bytes of all rows become is loaded before the first is stored.  Blocks walk several positions, so that what it
-// takes to find the sources (three loads one behind the other) shows once: 64 rows of 2.1 MB in 4 layers 174 us with one position a thread.
+// takes to find the sources (three loads one behind the other) shows once: 64 rows of 2.1 MB in 4 layers 113 us (what moves, read and written, at 6.1 TB/s,
+// 0.92 of a copy), 174 with one position a thread.  128 pages of 16 groups in 12 layers 41 us (0.85), 4 pages in 36 layers 15.
 template <int MOST>
 __global__ void __launch_bounds__(256, MOST == 16 ? 2 : 4) reorder_kernel(const ReorderArgs a) {
   __shared__ int from[MOST], to[MOST];

@@ -33,7 +33,7 @@ TILE = 4096
 @functools.lru_cache(maxsize=4096)
 def _parts(rows: int, vocab: int, sms: int) -> tuple[int, int]:
     """(parts, elements of a part) of every row: whole tiles, as many as run at once, two blocks an SM.  A block takes about 8 us to begin and to end
-    and 0.5 us a tile: 64 rows of 151936 in 1, 2, 4, 8, 19 parts 34, 26, 24, 28, 46 us; 768 rows 108, 124, 133, 188, 375."""
+    and 0.5 us a tile: 64 rows of 151936 in 1, 2, 4, 8, 19 parts 34, 25, 24, 28, 46 us; 768 rows 107, 124, 134, 189, 381."""
     tiles = -(-(vocab + 7) // TILE)
     per = -(-tiles // max(1, min(tiles, 2 * sms // rows)))
     return -(-tiles // per), per * TILE
