@@ -359,27 +359,27 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
     if (st == 0) {                                 // the bound, as others have raised it
       least = *(volatile unsigned long long*)&bound;
       reach = least ? unorder32((uint32_t)(least >> 32)) : -INFINITY;
-      place = (uint32_t)least ? (int)~(uint32_t)least : a.vocab;       // equal values count up to there
+      // equal values count up to there
+      place = reach == -INFINITY ? 2 * a.k - 1 : ((uint32_t)least ? (int)~(uint32_t)least : a.vocab);
     }
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
     float x[BEAM_VEC];
     const float t = take(stage + st * BEAM_TILE, x);
-    if (mine < to) {
-      if (t > m) {
-        s *= beam_exp2((m - t) * kBeamLog2e);      // nothing before the first element that is above -inf
-        m = t;
-      }
-      // differences from the maximum are taken before the factor: a product of the maximum would carry its rounding into every term
-      const float under = m == -INFINITY ? 0.f : m;
-      float2 u[2] = {};
+    // No branches: with a warp's 32 maxima, one of them rises in most steps.  The kernel is bound by its instructions.
+    const bool live = mine < to;
+    const float now = live ? fmaxf(m, t) : m;
+    // differences from the maximum are taken before the factor: a product of the maximum would carry its rounding into every term
+    const float under = now == -INFINITY ? 0.f : now;
+    float2 u[2] = {};
 #pragma unroll
-      for (int j = 0; j < BEAM_VEC; j += 2) {
-        const float2 d = mul2(add2(make_float2(x[j], x[j + 1]), make_float2(-under, -under)), make_float2(kBeamLog2e, kBeamLog2e));
-        u[j >> 1 & 1] = add2(u[j >> 1 & 1], make_float2(beam_exp2(d.x), beam_exp2(d.y)));       // a NaN or +inf: NaN
-      }
-      s += (u[0].x + u[0].y) + (u[1].x + u[1].y);
+    for (int j = 0; j < BEAM_VEC; j += 2) {
+      const float2 d = mul2(add2(make_float2(x[j], x[j + 1]), make_float2(-under, -under)), make_float2(kBeamLog2e, kBeamLog2e));
+      u[j >> 1 & 1] = add2(u[j >> 1 & 1], make_float2(beam_exp2(d.x), beam_exp2(d.y)));       // a NaN or +inf: NaN
     }
-    const bool hit = mine < to && (t > reach || (reach > -INFINITY ? t == reach && mine <= place : mine < 2 * a.k));
+    const float all = fmaf(s, beam_exp2(fminf(m - under, 0.f) * kBeamLog2e), (u[0].x + u[0].y) + (u[1].x + u[1].y));       // s is 0 under -inf
+    s = live ? all : s;
+    m = now;
+    const bool hit = live & (t >= reach) & ((t > reach) | (mine <= place));
     if (__any_sync(0xffffffffu, hit)) {
       if (hit) {
         uint32_t which = 0;
