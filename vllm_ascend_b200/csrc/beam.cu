@@ -12,9 +12,9 @@
 // A second kernel, a block a group, adds up the sums of the parts, turns its beams' keys into totals and takes the best by their places in the lists.
 // Parts' sums are added in 64 bits and totals compared in 64: with thousands of candidates, sums of 32 bits would order near ones
 // by their rounding.
-// Bound by HBM for many rows, while blocks stream: 768 rows of 151936 in bf16 take 91 us, 2.6 TB/s; a block streams its 304 KB for 17 us, two an SM at
-// 5.3 TB/s, takes 3 us for its first elements and their bound, 4 us to put its k best in order, and 768 rows are 2.6 turns of 296 blocks.  Few rows are
-// bound by those beginnings and ends and the second kernel, 5 us: 64 rows 22 us, 4 of 32000 13 us.
+// Many rows are bound by the instructions that are issued (three quarters of all places), half of them the walk: 768 rows of 151936 in bf16 take 84 us, 2.8
+// TB/s; 730 of them that are read execute 81000 a row, 48000 in the walk, 16000 where elements reach the bound, the rest before and after.  Few rows are
+// bound by what stands before and behind the walk, 3 and 4 us, and the second kernel, 5: 64 rows 21 us, 4 of 32000 13 us.
 // Reordering: a thread owns 16 bytes of a row for all beams of a group and loads what they become before it stores the first.
 #include "common.cuh"
 
@@ -353,60 +353,66 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
   // ---- all of the part, a warp by itself
   float m = -INFINITY, s = 0.f, reach = 0.f;
   uint64_t least = 0;
-  int place = 0, st = 0;
+  int place = 0;
 #pragma unroll 1
-  for (int mine = at0; mine - tid * BEAM_VEC < to; mine += BEAM_TILE) {
-    if (st == 0) {                                 // the bound, as others have raised it
-      least = *(volatile unsigned long long*)&bound;
-      reach = least ? unorder32((uint32_t)(least >> 32)) : -INFINITY;
-      // equal values count up to there
-      place = reach == -INFINITY ? 2 * a.k - 1 : ((uint32_t)least ? (int)~(uint32_t)least : a.vocab);
-    }
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-    float x[BEAM_VEC];
-    const float t = take(stage + st * BEAM_TILE, x);
-    // No branches: with a warp's 32 maxima, one of them rises in most steps.  The kernel is bound by its instructions.
-    const bool live = mine < to;
-    const float now = live ? fmaxf(m, t) : m;
-    // differences from the maximum are taken before the factor: a product of the maximum would carry its rounding into every term
-    const float under = now == -INFINITY ? 0.f : now;
-    float2 u[2] = {};
+  for (int at = at0; at - tid * BEAM_VEC < to; at += STAGES * BEAM_TILE) {
 #pragma unroll
-    for (int j = 0; j < BEAM_VEC; j += 2) {
-      const float2 d = mul2(add2(make_float2(x[j], x[j + 1]), make_float2(-under, -under)), make_float2(kBeamLog2e, kBeamLog2e));
-      u[j >> 1 & 1] = add2(u[j >> 1 & 1], make_float2(beam_exp2(d.x), beam_exp2(d.y)));       // a NaN or +inf: NaN
-    }
-    const float all = fmaf(s, beam_exp2(fminf(m - under, 0.f) * kBeamLog2e), (u[0].x + u[0].y) + (u[1].x + u[1].y));       // s is 0 under -inf
-    s = live ? all : s;
-    m = now;
-    const bool hit = live & (t >= reach) & ((t > reach) | (mine <= place));
-    if (__any_sync(0xffffffffu, hit)) {
-      if (hit) {
-        uint32_t which = 0;
+    for (int st = 0; st < STAGES; st++) {
+      const int mine = at + st * BEAM_TILE;
+      if (mine - tid * BEAM_VEC >= to) break;
+      if (st == 0) {                                 // the bound, as others have raised it
+        least = *(volatile unsigned long long*)&bound;
+        reach = least ? unorder32((uint32_t)(least >> 32)) : -INFINITY;
+        // equal values count up to there
+        place = reach == -INFINITY ? 2 * a.k - 1 : ((uint32_t)least ? (int)~(uint32_t)least : a.vocab);
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+      float x[BEAM_VEC];
+      const float t = take(stage + st * BEAM_TILE, x);
+      // No branches: with a warp's 32 maxima, one of them rises in most steps.  The kernel is bound by its instructions, about 80 a vector.
+      const bool live = mine < to;
+      const float now = live ? fmaxf(m, t) : m;
+      // differences from the maximum are taken before the factor: a product of the maximum would carry its rounding into every term
+      const float under = now == -INFINITY ? 0.f : now;
+      float2 u[2];
 #pragma unroll
-        for (int j = 0; j < BEAM_VEC; j++) which |= x[j] >= reach ? 1u << j : 0u;
-        while (which) {
-          const int j = __ffs(which) - 1;
-          which &= which - 1;
-          const uint64_t key = key_of((float)stage[st * BEAM_TILE + j], mine + j);
-          if (key != 0 && key >= least) list[atomicAdd(&held[warp], 1)] = key;
-        }
+      for (int j = 0; j < BEAM_VEC; j += 2) {
+        const float2 d = mul2(add2(make_float2(x[j], x[j + 1]), make_float2(-under, -under)), make_float2(kBeamLog2e, kBeamLog2e));
+        const float2 e = make_float2(beam_exp2(d.x), beam_exp2(d.y));          // a NaN or +inf: NaN
+        u[j >> 1 & 1] = j < 4 ? e : add2(u[j >> 1 & 1], e);
       }
-      __syncwarp();
-      const int n = *(volatile int*)&held[warp];
-      if (n > room - 32 * BEAM_VEC) {              // the next vector has room
-        const uint64_t last = cut_back(list, n, a.k);
-        if (lane == 0) {
-          held[warp] = a.k;
-          atomicMax(&bound, (unsigned long long)last);
+      u[0] = add2(u[0], u[1]);
+      const float all = fmaf(s, beam_exp2(fminf(m - under, 0.f) * kBeamLog2e), u[0].x + u[0].y);       // s is 0 under -inf
+      s = live ? all : s;
+      m = now;
+      const bool hit = live & (t >= reach) & ((t > reach) | (mine <= place));
+      if (__any_sync(0xffffffffu, hit)) {
+        if (hit) {
+          uint32_t which = 0;
+#pragma unroll
+          for (int j = 0; j < BEAM_VEC; j++) which |= x[j] >= reach ? 1u << j : 0u;
+          while (which) {
+            const int j = __ffs(which) - 1;
+            which &= which - 1;
+            const uint64_t key = key_of((float)stage[st * BEAM_TILE + j], mine + j);
+            if (key != 0 && key >= least) list[atomicAdd(&held[warp], 1)] = key;
+          }
         }
+        __syncwarp();
+        const int n = *(volatile int*)&held[warp];
+        if (n > room - 32 * BEAM_VEC) {              // the next vector has room
+          const uint64_t last = cut_back(list, n, a.k);
+          if (lane == 0) {
+            held[warp] = a.k;
+            atomicMax(&bound, (unsigned long long)last);
+          }
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      const int next = mine + STAGES * BEAM_TILE;
+      if (next < to) bring(stage + st * BEAM_TILE, x0, next, a.vocab);
+      asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    const int next = mine + STAGES * BEAM_TILE;
-    if (next < to) bring(stage + st * BEAM_TILE, x0, next, a.vocab);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    if (++st == STAGES) st = 0;
   }
   // ---- the block's k best, in the place of the elements
   asm volatile("cp.async.wait_all;" ::: "memory");
