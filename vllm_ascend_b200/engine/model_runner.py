@@ -554,13 +554,12 @@ class ModelRunner:
             attn_state=state, num_decodes=nd, num_decode_tokens=ndt, num_prefills=npf,
             num_input_tokens=Tp)
         if so.shared_groups:
-            firsts = np.full(Bp + 1, B, dtype=np.int32)          # groups behind the last are empty
-            prefixes = np.zeros(Bp, dtype=np.int32)
-            np.cumsum([n for n, _ in so.shared_groups], out=firsts[1:len(so.shared_groups) + 1])
-            firsts[0] = 0
-            prefixes[:len(so.shared_groups)] = [p for _, p in so.shared_groups]
-            self._shared_meta[0, :Bp + 1].copy_(self._to_dev(torch.from_numpy(firsts)))
-            self._shared_meta[1, :Bp].copy_(self._to_dev(torch.from_numpy(prefixes)))
+            n = len(so.shared_groups)
+            groups = np.zeros((2, Bp + 1), dtype=np.int32)
+            groups[0, n:] = B                                    # groups behind the last are empty
+            np.cumsum([width for width, _ in so.shared_groups[:-1]], out=groups[0, 1:n])
+            groups[1, :n] = [prefix for _, prefix in so.shared_groups]
+            self._shared_meta[:, :Bp + 1].copy_(self._to_dev(torch.from_numpy(groups)))
             meta.shared_groups = (self._shared_meta[0, :Bp + 1], self._shared_meta[1, :Bp])
         meta.dcp_interleave = self.dcp_interleave
         if self.dcp_size > 1:
@@ -722,10 +721,15 @@ class ModelRunner:
         return not self.is_cuda or has_kernel(self.kv_dtype, self._attn_layer().D, self.block_size)
 
     def _sharing_pays(self, groups: list) -> bool:
-        """Whether a layer's attention takes less time with prefixes read once: where 256 keys a sequence are not read again.  Behind them every sequence
-        costs a piece of work of its own, which plain decoding splits and feeds better.  32 heads on 8 of 128, us shared (plain): 4 beams over 512 keys
-        12 (13.5), over 4096 16 (21); 64 requests over 128 32 (27), over 256 32 (30), over 512 34 (38); 192 over 128 127 (122), over 512 128 (153)."""
-        return not self.is_cuda or sum((n - 1) * prefix for n, prefix in groups) >= 256 * sum(n for n, _ in groups)
+        """Whether a step takes less time with prefixes read once: where 48 MB of a layer and 256 keys a sequence are not read again.  Plain decoding splits
+        and feeds short work better; every sequence leaves a piece of work behind the prefix, a step has the plan and 60 us more on the host.  32 heads on
+        8 of 128, us of attention, shared (plain): 64 requests over 128 keys 32 (27), over 256 32 (30), over 512 34 (38); 192 over 128 127 (122), over 512
+        128 (153).  Steps of 36 layers: 4 beams over 1500 keys 3852 (3836), 4 prompts of 4 3939 (4078), 8 of 8 over 2000 4828 (6315)."""
+        if not self.is_cuda:
+            return True
+        a = self._attn_layer()
+        keys = sum((n - 1) * prefix for n, prefix in groups) - 256 * sum(n for n, _ in groups)
+        return keys * a.Hkv * a.D * 4 >= 48e6                # has_kernel: 16 bits a channel
 
     def _find_shared(self, so: SchedulerOutput) -> None:
         """Groups of a decode step: those that the caller knows, or all of its sequences where they begin with the same blocks."""
