@@ -170,3 +170,15 @@ def test_engines_that_read_every_prefix_for_itself():
         if kw.get("kv_cache_dtype"):
             cfg.head_dim = 64
         assert not LLM(cfg, device="cpu", max_model_len=64, max_num_seqs=2, disable_cascade_attn=False, **kw).engine.runner.can_share_prefixes()
+
+
+def test_steps_keep_within_their_tokens(monkeypatch):
+    llm = LLM("tiny-qwen", device="cpu", seed=1, block_size=16, max_model_len=128, max_num_seqs=16, max_num_batched_tokens=8)
+    logits, steps = llm.engine.runner.device_logits, []
+    monkeypatch.setattr(llm.engine.runner, "device_logits", lambda so, rows=None: steps.append(so.num_scheduled_tokens) or logits(so, rows))
+    prompts = _prompts(11, 7, 30)
+    found = llm.beam_search(prompts, beam_width=4, max_tokens=5, ignore_eos=True)
+    assert steps and max(steps) <= 8
+    _same(found, LLM("tiny-qwen", device="cpu", seed=1, block_size=16, max_model_len=128, max_num_seqs=16).beam_search(
+        prompts, beam_width=4, max_tokens=5, ignore_eos=True))
+    assert not beam.on_device(llm.engine, prompts, 9, 5)

@@ -23,6 +23,11 @@ def _blocks(engine, prompt: int, width: int, max_tokens: int) -> int:
     return -(-prompt // bs) + 1 + width * (-(-(prompt % bs + max_tokens) // bs) + 1)
 
 
+def _rows(runner) -> int:
+    """Beams that a step holds at most."""
+    return min(runner.max_seqs, runner.max_tokens)
+
+
 def on_device(engine, prompts: list, width: int, max_tokens: int) -> bool:
     """Whether the engine can run these beams itself: one rank that has nothing else to do, no drafts, connectors or adapters, rows and blocks for
     every prompt's beams, as many candidates as the selection takes."""
@@ -34,7 +39,7 @@ def on_device(engine, prompts: list, width: int, max_tokens: int) -> bool:
             or r.dcp_size > 1 or par.tensor_parallel_size > 1:
         return False
     from ..ops.beam import MOST_SELECTED
-    return 2 * width <= MOST_SELECTED and width <= r.max_seqs and bool(prompts) and all(
+    return 2 * width <= MOST_SELECTED and width <= _rows(r) and bool(prompts) and all(
         0 < len(p) and len(p) + max_tokens <= s.cfg.max_model_len and _blocks(engine, len(p), width, max_tokens) <= s.pool.num_free_blocks
         for p in prompts)
 
@@ -63,7 +68,7 @@ class BeamSearch:
         waiting = [_Group(i, p) for i, p in enumerate(prompts)]
         while waiting:
             wave, blocks = [], 0
-            while waiting and (len(wave) + 1) * self.width <= self.runner.max_seqs:
+            while waiting and (len(wave) + 1) * self.width <= _rows(self.runner):
                 blocks += _blocks(self.engine, len(waiting[0].prompt), self.width, self.max_tokens)
                 if wave and blocks > self.scheduler.pool.num_free_blocks:
                     break
