@@ -125,6 +125,7 @@ class ModelRunner:
         self.state_meta = torch.zeros((2, B), dtype=i32, device=device)     # [slot; has_initial_state]
         self._h_sampled2 = [torch.zeros(B, dtype=i64, pin_memory=pin) for _ in range(2)]   # async steps
         self._async_flip = 0
+        self._inputs_copied = torch.cuda.Event() if self.is_cuda else None      # behind the copies out of the host buffers above
         self.share_prefixes = not cfg.disable_cascade_attn      # look for common prefixes in decode batches
         self._shared_meta = torch.zeros((2, B + 1), dtype=i32, device=device)      # [first sequences; prefix lengths] of groups
         self._shared_asked: dict[int, int] = {}                 # capture size -> steps that shared prefixes and had no graph
@@ -439,7 +440,15 @@ class ModelRunner:
     def _prepare_inputs(self, so: SchedulerOutput, pad_to: Optional[int] = None):
         from ..profiler import nvtx_range
         with nvtx_range("prepare_inputs"):
-            return self._prepare_inputs_impl(so, pad_to)
+            # The copies of the step before run behind what was launched ahead of them: steps that nobody waits for (portions of a prompt) would
+            # find the buffers filled for the next one.
+            if self._inputs_copied is not None:
+                self._inputs_copied.synchronize()
+            try:
+                return self._prepare_inputs_impl(so, pad_to)
+            finally:
+                if self._inputs_copied is not None:
+                    self._inputs_copied.record()
 
     def _prepare_inputs_impl(self, so: SchedulerOutput, pad_to: Optional[int] = None):
         reqs = [r for r, _ in so.scheduled]
