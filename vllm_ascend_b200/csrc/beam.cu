@@ -31,18 +31,18 @@ constexpr float kBeamLog2e = 1.4426950408889634f;
 
 struct SelectArgs {
   const void* logits;
-  const float* scores;           // [groups, width]
+  const void* scores;            // [groups, width] of 32 or 64 bits
   uint64_t* keys;                // [rows, parts, k] best first
   int* counts;                   // [rows, parts]
   float* maxima;                 // [rows, parts]
   double* sums;                  // [rows, parts] of exp(x - maximum)
-  float* out_scores;             // [groups, k]
+  void* out_scores;              // [groups, k] of as many
   int* out_parents;
   long* out_tokens;
   int* status;
   cudaStream_t stream;
   long row_stride;
-  int groups, width, vocab, k, parts, per_part, fp32;
+  int groups, width, vocab, k, parts, per_part, fp32, wide;       // wide: scores of 64 bits
 };
 
 // ---------------------------------------------------------------- keys
@@ -259,7 +259,10 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return y;
 }
 
-__device__ __forceinline__ bool is_score(float s) { return s > -INFINITY && s < INFINITY; }
+__device__ __forceinline__ double score_of(const SelectArgs& a, long row) {
+  return a.wide ? ((const double*)a.scores)[row] : (double)((const float*)a.scores)[row];
+}
+__device__ __forceinline__ bool is_score(double s) { return s > -INFINITY && s < INFINITY; }
 
 // A warp's list: room for k keys and more, and for what a vector of its lanes may add.
 __host__ __device__ constexpr int list_room(int k) { return (k + 31) / 32 * 32 + 32 + 32 * BEAM_VEC; }
@@ -315,7 +318,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
   __shared__ double warp_sum[BEAM_WARPS];
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // once all blocks run, groups' may take their places and wait
-  if (!is_score(a.scores[row])) return;            // the beam has ended: the second kernel asks its score first
+  if (!is_score(score_of(a, row))) return;            // the beam has ended: the second kernel asks its score first
   const T* x0 = (const T*)a.logits + (long)row * a.row_stride;
   // vectors lie on 16-byte boundaries of memory, whatever the row's first element does; a vector holds elements [at, at + 8)
   const int shift = (int)(((uintptr_t)x0 & 15) / sizeof(T));
@@ -513,7 +516,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1) select_groups_kernel(const Se
   for (int w = tid >> 5; w < a.width; w += BEAM_WARPS) {          // a warp a beam, a lane a part
     const long row = (long)g * a.width + w;
     double l = __longlong_as_double(0x7ff8000000000000ll);
-    if (is_score(a.scores[row])) {
+    if (is_score(score_of(a, row))) {
       float top = -INFINITY;
       for (int p = lane; p < a.parts; p += 32) top = fmaxf(top, a.maxima[row * a.parts + p]);
       top = warp_reduce_max(top);
@@ -550,7 +553,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1) select_groups_kernel(const Se
       } else if (c < a.counts[slot]) {
         const uint64_t r = a.keys[slot * a.k + c];
         const float x = unorder32((uint32_t)(r >> 32));
-        key = {order64((double)a.scores[row] + ((double)x - l)), ~((uint32_t)(w * a.vocab) + ~(uint32_t)r)};
+        key = {order64(score_of(a, row) + ((double)x - l)), ~((uint32_t)(w * a.vocab) + ~(uint32_t)r)};
       }
       if (key.above(least)) {
         list.keys[atomicAdd(&list.count, 1)] = key;
@@ -569,7 +572,9 @@ __global__ void __launch_bounds__(BEAM_THREADS, 1) select_groups_kernel(const Se
     const GroupKey key = list.keys[i];
     const uint32_t place = ~key.place;
     const long to = (long)g * a.k + i;
-    a.out_scores[to] = (float)unorder64(key.v);
+    const double total = unorder64(key.v);
+    if (a.wide) ((double*)a.out_scores)[to] = total;
+    else ((float*)a.out_scores)[to] = (float)total;
     a.out_parents[to] = (int)(place / (uint32_t)a.vocab);
     a.out_tokens[to] = (long)(place % (uint32_t)a.vocab);
   }

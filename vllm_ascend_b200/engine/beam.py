@@ -87,10 +87,10 @@ class BeamSearch:
     # ------------------------------------------------------------------ rounds
     def _wave(self, groups: list) -> None:
         logits = self._prompts(groups)
-        scores = torch.zeros((len(groups), 1), dtype=torch.float32, device=logits.device)
+        scores = torch.zeros((len(groups), 1), dtype=torch.float64, device=logits.device)
         for round_ in range(self.max_tokens):
             k = min(2 * self.width, scores.shape[1] * self.vocab)
-            totals, parents, tokens = (t.cpu() for t in ops.beam_select(logits, scores, k))
+            totals, parents, tokens = (t.cpu() for t in ops.beam_select(logits, scores, k, torch.float64))
             chosen = [self._choose(g, *(t[i].tolist() for t in (totals, parents, tokens))) for i, g in enumerate(groups)]
             if round_ + 1 < self.max_tokens:
                 going = [(g, p) for g, p in zip(groups, chosen) if p]
@@ -215,7 +215,7 @@ class BeamSearch:
                 if need:
                     r.block_ids.extend(self.scheduler.pool.allocate(need))
         wide = max(len(g.live) for g in groups)
-        scores = np.full((len(groups), wide), -np.inf, dtype=np.float32)
+        scores = np.full((len(groups), wide), -np.inf, dtype=np.float64)
         index, at = np.zeros((len(groups), wide), dtype=np.int64), 0
         for i, g in enumerate(groups):
             scores[i, :len(g.live)] = [c for _, c in g.live]

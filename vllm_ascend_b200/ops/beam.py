@@ -17,7 +17,7 @@ from .. import _native
 from . import reference as ref
 
 # laid out as the source's SelectArgs, BeamTensor and ReorderArgs
-_SELECT = struct.Struct("@11Pq7i")
+_SELECT = struct.Struct("@11Pq8i")
 _TENSOR = struct.Struct("@P4q4i")
 _REORDER = struct.Struct("@6P5i")
 for _name in ("b200_beam_select", "b200_beam_reorder"):
@@ -39,20 +39,24 @@ def _parts(rows: int, vocab: int, sms: int) -> tuple[int, int]:
     return -(-tiles // per), per * TILE
 
 
-def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = None,
+                dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The ``k`` best continuations of every group (default: two for each beam, so that as many as there are beams do not end).
 
-    logits [groups * beams, vocabulary], rows in the order of ``scores``; scores fp32 [groups, beams], the log-probability of each beam so far,
+    logits [groups * beams, vocabulary], rows in the order of ``scores``; scores [groups, beams], the log-probability of each beam so far,
     -inf for beams that ended (their logits are not read).  A continuation's total is its beam's score plus the token's log-probability.
-    Returns totals (fp32), parents (int32, a beam of the group) and tokens (int64), each [groups, k], best first; equal totals come in the order
+    ``dtype``, fp32 or fp64, is the type of scores and totals: totals that become the next step's scores keep what was added up in 64 bits.
+    Returns totals, parents (int32, a beam of the group) and tokens (int64), each [groups, k], best first; equal totals come in the order
     of beams, then tokens.  A row that holds a NaN or +inf, or nothing above -inf, has no distribution: its tokens count as -inf, like masked
     ones.  Sums and totals are held in 64 bits, so the order is that of the exact totals to about 1e-8."""
     if logits.dim() != 2 or scores.dim() != 2 or not logits.is_floating_point():
         raise ValueError(f"logits [groups * beams, vocabulary] and scores [groups, beams], not {logits.dtype} {tuple(logits.shape)} and "
                          f"{tuple(scores.shape)}")
     (rows, vocab), (groups, width), device = logits.shape, scores.shape, logits.get_device()
-    if rows != groups * width or scores.dtype != torch.float32 or scores.get_device() != device:
-        raise ValueError(f"{rows} rows of logits on {logits.device}, scores {scores.dtype} {tuple(scores.shape)} on {scores.device}")
+    if dtype not in (torch.float32, torch.float64):
+        raise ValueError(f"scores and totals of {dtype}: fp32 or fp64")
+    if rows != groups * width or scores.dtype != dtype or scores.get_device() != device:
+        raise ValueError(f"{rows} rows of logits on {logits.device}, scores {scores.dtype} {tuple(scores.shape)} on {scores.device} for totals of {dtype}")
     if width < 1 or width > MOST_BEAMS or vocab < 1 or width * vocab > 2 ** 31 - 1:
         raise ValueError(f"{width} beams over {vocab} tokens: 1 to {MOST_BEAMS} beams, fewer than 2^31 candidates")
     if k is None:
@@ -63,13 +67,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = N
         return ref.beam_select(logits, scores, k)
     if device != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return beam_select(logits, scores, k)
+            return beam_select(logits, scores, k, dtype)
     if logits.dtype not in (torch.bfloat16, torch.float32):
         logits = logits.float()                                 # 64-bit logits round to 32
     if logits.stride(1) != 1 and vocab > 1:
         logits = logits.contiguous()
     scores = scores.contiguous()
-    totals = torch.empty((groups, k), dtype=torch.float32, device=logits.device)
+    totals = torch.empty((groups, k), dtype=dtype, device=logits.device)
     parents = torch.empty((groups, k), dtype=torch.int32, device=logits.device)
     tokens = torch.empty((groups, k), dtype=torch.int64, device=logits.device)
     if groups == 0:
@@ -84,7 +88,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = N
     rc = _native.lib().b200_beam_select(_SELECT.pack(
         logits.data_ptr(), scores.data_ptr(), keys, maxima + slots * 4, maxima, sums, totals.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
         _native.status_word(logits.device).data_ptr(), _native.stream_ptr(), logits.stride(0), groups, width, vocab, k, parts, per,
-        int(logits.dtype == torch.float32)))
+        int(logits.dtype == torch.float32), int(dtype == torch.float64)))
     _native.check(rc, "beam_select")
     _native.count_launch(2)
     return totals, parents, tokens

@@ -537,14 +537,14 @@ def rms_norm_gated(x: torch.Tensor, z: torch.Tensor, w: torch.Tensor, eps: float
 
 # ---------------------------------------------------------------- beam search
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """logits [groups * beams, vocab], scores [groups, beams] -> the k best totals of each group, their beams and tokens."""
+    """logits [groups * beams, vocab], scores [groups, beams] -> the k best totals of each group (of the scores' type), their beams and tokens."""
     (groups, width), vocab = scores.shape, logits.shape[1]
     x = logits.double()
     x = x - torch.logsumexp(x, -1, keepdim=True)                # NaN where a row has no distribution
     total = torch.nan_to_num(scores.double().reshape(-1, 1) + x, nan=-torch.inf, posinf=-torch.inf, neginf=-torch.inf)
     best, at = torch.sort(total.reshape(groups, width * vocab), dim=-1, descending=True, stable=True)
     best, at = best[:, :k], at[:, :k]
-    return best.float(), (at // vocab).to(torch.int32), at % vocab
+    return best.to(scores.dtype), (at // vocab).to(torch.int32), at % vocab
 
 
 def reorder_beams(tensors, rows: torch.Tensor, parents: torch.Tensor, lengths: Optional[torch.Tensor] = None, int4_dim: int = 0) -> None:
