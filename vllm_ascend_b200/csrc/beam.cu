@@ -199,6 +199,38 @@ __device__ int select_best(Key* keys, Key* other, int n, int k, Key* slices, Key
   return min(n, k);
 }
 
+// ---------------------------------------------------------------- exponentials and logarithms in 64 bits
+// e^x for x <= 0 and log x for x >= 1 in 64 bits, by their series: short loops where the library's functions are a few hundred instructions that a
+// kernel of this length waits for.
+__constant__ double kInverseOdd[16] = {1., 1. / 3, 1. / 5, 1. / 7, 1. / 9, 1. / 11, 1. / 13, 1. / 15, 1. / 17, 1. / 19, 1. / 21, 1. / 23,
+                                           1. / 25, 1. / 27, 1. / 29, 1. / 31};
+__constant__ double kInverseFactorial[14] = {1., 1., 1. / 2, 1. / 6, 1. / 24, 1. / 120, 1. / 720, 1. / 5040, 1. / 40320, 1. / 362880, 1. / 3628800,
+                                             1. / 39916800, 1. / 479001600, 1. / 6227020800.};
+template <int TERMS = 13>
+__device__ __forceinline__ double series_exp(double x) {       // e^x = 2^n e^r, |r| <= log(2) / 2; to r^(TERMS + 1) / (TERMS + 1)!
+  if (x < -700.) return 0.;
+  const double n = rint(x * 1.4426950408889634), r = x - n * 0.69314718055994531;
+  double e = kInverseFactorial[TERMS];
+#pragma unroll 1
+  for (int i = TERMS - 1; i >= 0; i--) e = e * r + kInverseFactorial[i];
+  return e * __longlong_as_double((long long)(1023 + (int)n) << 52);
+}
+__device__ __forceinline__ double series_log(double x) {       // log 2^n m = n log 2 + 2 atanh((m - 1) / (m + 1)), m in [0.75, 1.5)
+  const uint64_t b = (uint64_t)__double_as_longlong(x);
+  int n = (int)(b >> 52) - 1023;
+  double m = __longlong_as_double((long long)((b & 0xfffffffffffffull) | 0x3ff0000000000000ull));
+  if (m >= 1.5) m *= 0.5, n++;
+  const double d = m + 1.;
+  double inv = (double)(1.f / (float)d);
+  inv = inv * (2. - d * inv);
+  inv = inv * (2. - d * inv);
+  const double z = (m - 1.) * inv, q = z * z;                  // |z| <= 0.2: sixteen terms are 3e-24
+  double t = 0.;
+#pragma unroll 1
+  for (int i = 15; i >= 0; i--) t = t * q + kInverseOdd[i];
+  return n * 0.69314718055994531 + 2. * z * t;
+}
+
 // ---------------------------------------------------------------- parts of rows
 __device__ __forceinline__ float beam_exp2(float x) {
   float y;
@@ -453,7 +485,9 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < BEAM_WARPS; i++) high = fmaxf(high, warp_max[i]);
-  double sum = m == -INFINITY ? (double)s : (double)s * (double)beam_exp2((m - high) * kBeamLog2e);
+  // in 64 bits: where one element stands above a flat row, all threads have the same distance, and its rounding would not average out (3e-7);
+  // eight terms are off by 2e-10
+  double sum = m == -INFINITY ? (double)s : (double)s * series_exp<8>((double)m - (double)high);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) warp_sum[warp] = sum;
@@ -477,35 +511,6 @@ struct GroupList {
   GroupKey bound;
   int count;
 };
-
-// e^x for x <= 0 and log x for x >= 1 in 64 bits, by their series: short loops where the library's functions are a few hundred instructions that a
-// kernel of this length waits for.
-__constant__ double kInverseOdd[16] = {1., 1. / 3, 1. / 5, 1. / 7, 1. / 9, 1. / 11, 1. / 13, 1. / 15, 1. / 17, 1. / 19, 1. / 21, 1. / 23,
-                                           1. / 25, 1. / 27, 1. / 29, 1. / 31};
-__constant__ double kInverse[14] = {1., 1., 1. / 2, 1. / 3, 1. / 4, 1. / 5, 1. / 6, 1. / 7, 1. / 8, 1. / 9, 1. / 10, 1. / 11, 1. / 12, 1. / 13};
-__device__ __forceinline__ double series_exp(double x) {       // e^x = 2^n e^r, |r| <= log(2) / 2
-  if (x < -700.) return 0.;
-  const double n = rint(x * 1.4426950408889634), r = x - n * 0.69314718055994531;
-  double e = 1.;
-#pragma unroll 1
-  for (int i = 13; i > 0; i--) e = 1. + e * r * kInverse[i];
-  return e * __longlong_as_double((long long)(1023 + (int)n) << 52);
-}
-__device__ __forceinline__ double series_log(double x) {       // log 2^n m = n log 2 + 2 atanh((m - 1) / (m + 1)), m in [0.75, 1.5)
-  const uint64_t b = (uint64_t)__double_as_longlong(x);
-  int n = (int)(b >> 52) - 1023;
-  double m = __longlong_as_double((long long)((b & 0xfffffffffffffull) | 0x3ff0000000000000ull));
-  if (m >= 1.5) m *= 0.5, n++;
-  const double d = m + 1.;
-  double inv = (double)(1.f / (float)d);
-  inv = inv * (2. - d * inv);
-  inv = inv * (2. - d * inv);
-  const double z = (m - 1.) * inv, q = z * z;                  // |z| <= 0.2: sixteen terms are 3e-24
-  double t = 0.;
-#pragma unroll 1
-  for (int i = 15; i >= 0; i--) t = t * q + kInverseOdd[i];
-  return n * 0.69314718055994531 + 2. * z * t;
-}
 
 __global__ void __launch_bounds__(BEAM_THREADS, 1) select_groups_kernel(const SelectArgs a) {
   extern __shared__ __align__(16) uint8_t beam_smem[];
