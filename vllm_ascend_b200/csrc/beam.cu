@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 2) select_rows_kernel(const Sele
   const T* x0 = (const T*)a.logits + (long)row * a.row_stride;
   // vectors lie on 16-byte boundaries of memory, whatever the row's first element does; a vector holds elements [at, at + 8)
   const int shift = (int)(((uintptr_t)x0 & 15) / sizeof(T));
-  const int from = part * a.per_part - shift, to = min(from + a.per_part, a.vocab);
+  const int from = part * a.per_part - shift, to = (int)min((long)from + a.per_part, (long)a.vocab);
   const int room = list_room(a.k);
   constexpr int STAGES = STAGE_BYTES / (BEAM_VEC * (int)sizeof(T));
   T* stage = reinterpret_cast<T*>(beam_smem) + tid * BEAM_VEC;       // [stages][threads][8], a thread's own
@@ -726,8 +726,9 @@ B200_API int b200_beam_select(const b200::SelectArgs* args) {
   const long rows = (long)a.groups * a.width;
   if (a.width < 1 || a.vocab < 1 || a.k < 1 || a.k > BEAM_MOST || (long)a.k > (long)a.width * a.vocab) return 9930;
   if ((long)a.width * a.vocab > 0x7fffffffL || rows * a.parts > 0x7fffffffL || (long)a.width * a.parts * a.k > 0x7fffffffL) return 9931;
-  if (a.parts < 1 || a.per_part < BEAM_VEC || a.per_part % BEAM_VEC || (long)a.parts * a.per_part > 0x7fffffffL - BEAM_TILE ||
-      (long)a.parts * a.per_part < (long)a.vocab + BEAM_VEC - 1)
+  // a walk counts up to eight tiles past a row's end
+  if (a.vocab > 0x7fffffff - 8 * BEAM_TILE || a.parts < 1 || a.per_part < BEAM_VEC || a.per_part % BEAM_VEC ||
+      (long)(a.parts - 1) * a.per_part >= (long)a.vocab + BEAM_VEC - 1 || (long)a.parts * a.per_part < (long)a.vocab + BEAM_VEC - 1)
     return 9932;
   const int row_smem = BEAM_THREADS * STAGE_BYTES + BEAM_WARPS * list_room(a.k) * 8, group_smem = (int)sizeof(GroupList) + a.width * 8;
   if ((long)a.width * a.parts > BEAM_ROOM) return 9933;      // a level of all lists is looked at together

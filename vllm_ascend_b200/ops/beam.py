@@ -28,6 +28,8 @@ MOST_SELECTED = 256
 MOST_BEAMS = 1024
 #: elements of a row that a block takes at a time
 TILE = 4096
+#: tokens of a vocabulary at most: positions of 32 bits count up to eight tiles past its end
+MOST_TOKENS = 2 ** 31 - 1 - 8 * TILE
 
 
 @functools.lru_cache(maxsize=4096)
@@ -58,8 +60,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = N
         raise ValueError(f"scores and totals of {dtype}: fp32 or fp64")
     if rows != groups * width or scores.dtype != dtype or scores.get_device() != device:
         raise ValueError(f"{rows} rows of logits on {logits.device}, scores {scores.dtype} {tuple(scores.shape)} on {scores.device} for totals of {dtype}")
-    if width < 1 or width > MOST_BEAMS or vocab < 1 or width * vocab > 2 ** 31 - 1:
-        raise ValueError(f"{width} beams over {vocab} tokens: 1 to {MOST_BEAMS} beams, fewer than 2^31 candidates")
+    if width < 1 or width > MOST_BEAMS or not 1 <= vocab <= MOST_TOKENS or width * vocab > 2 ** 31 - 1:
+        raise ValueError(f"{width} beams over {vocab} tokens: 1 to {MOST_BEAMS} beams of up to {MOST_TOKENS} tokens, fewer than 2^31 candidates")
     if k is None:
         k = min(2 * width, width * vocab)
     if not 1 <= k <= min(MOST_SELECTED, width * vocab):
