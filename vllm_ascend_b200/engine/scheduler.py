@@ -391,9 +391,13 @@ class Scheduler:
             r.block_ids = blocks
 
     def drop(self, req: Request) -> None:
-        """Forget a request that ``schedule_portions`` or ``fork`` made."""
-        self.abort_request(req.request_id)
-        self.requests.pop(req.request_id, None)
+        """Forget a request that ``reuse``, ``schedule_portions`` or ``fork`` made."""
+        if self.requests.get(req.request_id) is req:
+            self.abort_request(req.request_id)
+            del self.requests[req.request_id]
+        else:                                            # in no step yet: it holds what ``reuse`` found
+            self.free_blocks(req)
+            self._hashes.pop(req.request_id, None)
 
     # ------------------------------------------------------------------ results
     def advance(self, out: SchedulerOutput) -> None:
