@@ -150,24 +150,36 @@ def _layout(t: torch.Tensor, paged: bool, int4_dim: int) -> tuple:
 
 
 def _check_apart(rows: list) -> None:
-    """Refuses memory that two tensors would move.  Rows may lie between each other's, as in slices of one buffer: places modulo what both
-    distances between rows are multiples of tell, or those modulo the distance of pieces where both have rows of such pieces."""
+    """Refuses memory that two tensors would move.  Rows may lie between each other's, as in slices of one buffer."""
     ordered = sorted(r for r in rows if r[4] and r[6] * r[3])
-    for i, (at, row, run, unit, n, outer, units, _, _) in enumerate(ordered):
-        one = units * unit                                     # bytes of a piece
-        span = (outer - 1) * run + one
-        for at2, row2, run2, unit2, n2, outer2, units2, _, _ in ordered[i + 1:]:
-            if at2 >= at + (n - 1) * row + span:
+    for i, a in enumerate(ordered):
+        end = a[0] + (a[4] - 1) * a[1] + (a[5] - 1) * a[2] + a[6] * a[3]
+        for b in ordered[i + 1:]:
+            if b[0] >= end:
                 break
-            two = units2 * unit2
-            span2 = (outer2 - 1) * run2 + two
-            every = math.gcd(row if n > 1 else 0, row2 if n2 > 1 else 0) or span + span2 + at2 - at
-            off = (at2 - at) % every
-            if off >= span and off + span2 <= every:
-                continue
-            if outer > 1 and (row, run, outer) == (row2, run2, outer2) and one <= off % run and off % run + two <= run:
-                continue
-            raise ValueError("two of the tensors share memory")
+            if _meet(a, b):
+                raise ValueError("two of the tensors share memory")
+
+
+def _meet(a: tuple, b: tuple) -> bool:
+    """Whether two layouts share memory, b not in front of a: exactly where rows and pieces are as far apart in both, else also where the places of
+    rows, modulo what both distances between rows are multiples of, do not tell."""
+    at, row, run, unit, n, outer, units, _, _ = a
+    at2, row2, run2, unit2, n2, outer2, units2, _, _ = b
+    one, two, off = units * unit, units2 * unit2, at2 - at               # bytes of a piece
+    span, span2 = (outer - 1) * run + one, (outer2 - 1) * run2 + two
+    if (row == row2 or n == 1 or n2 == 1) and (run == run2 or outer == 1 or outer2 == 1):
+        row, run = (row2 if n == 1 else row) if n * n2 > 1 else 1, (run2 if outer == 1 else run) if outer * outer2 > 1 else 1
+        # rows d apart whose extents meet, then their first pieces that end behind the other's begin
+        for d in range(max(1 - n, (-span2 - off) // row), min(n2 - 1, (span - off) // row) + 1):
+            apart = off + d * row
+            j = max(1 - outer, (-two - apart) // run + 1)
+            if j < outer2 and apart + j * run < one:
+                return True
+        return False
+    every = math.gcd(row if n > 1 else 0, row2 if n2 > 1 else 0) or span + span2 + off
+    off %= every
+    return off < span or off + span2 > every
 
 
 def beam_states(tensors: Sequence[torch.Tensor], paged: bool = False, int4_dim: int = 0) -> BeamStates:
