@@ -666,10 +666,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     scale: float, out: Optional[torch.Tensor] = None, causal: bool = True,
                     window: int = 0) -> torch.Tensor:
     """Attention of every scheduled token over its sequence's paged KV.  With a plan for shared prefixes of these very sequences in ``meta.shared``
-    they are read once a group, where the cache is of the queries' type and there is no window."""
+    they are read once a group, where the cache is of the queries' type, there is no window and, on a GPU, a kernel for it; rows of the block table
+    hold whole sequences either way."""
     plan = getattr(meta, "shared", None)
     if plan is not None and plan.of(meta) and causal and not window and q.dtype == k_cache.dtype == v_cache.dtype and not fixed_sums() \
-            and v_cache.shape == k_cache.shape and (q.shape[1], k_cache.shape[2]) == (plan.heads, plan.kv_heads):
+            and v_cache.shape == k_cache.shape and (q.shape[1], k_cache.shape[2]) == (plan.heads, plan.kv_heads) \
+            and (not q.is_cuda or shared_prefix.has_kernel(q.dtype, k_cache.shape[3], k_cache.shape[1])):
         return paged_attention_shared(q, k_cache, v_cache, meta, plan, scale, out)
     if k_cache.dtype == torch.uint8:
         return paged_attention_int4(q, k_cache, v_cache, meta, scale, out, causal, window)
@@ -991,4 +993,5 @@ from .kv_int4 import alloc_kv_cache_int4, paged_attention_int4, read_kv_int4, wr
 
 # ---------------------------------------------------------------- beam search
 from .beam import BeamStates, beam_select, beam_states, reorder_beams  # noqa: E402,F401
+from . import shared_prefix  # noqa: E402
 from .shared_prefix import SharedPrefixPlan, paged_attention_shared, plan_shared_prefix  # noqa: E402,F401
