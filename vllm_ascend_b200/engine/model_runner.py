@@ -752,10 +752,19 @@ class ModelRunner:
         if so.shared_groups is not None and not (self.can_share_prefixes() and self._sharing_pays(so.shared_groups)):
             so.shared_groups = None
 
-    def _shared_graph(self, gsize: Optional[int]):
-        """Descriptor of the graph for a decode step that shares prefixes; None: it runs eagerly.  A size is captured when it is asked for a third time."""
-        if gsize is None:
+    def _shared_step(self, so: SchedulerOutput, gsize: Optional[int]):
+        """Descriptor of the graph with which a decode step shares its prefixes; None: it replays the plain one of its size, or, where sizes have none, runs
+        eagerly and may share them so."""
+        self._find_shared(so)
+        if not so.shared_groups or gsize is None:
             return None
+        shared = self._shared_graph(gsize)
+        if shared is None:
+            so.shared_groups = None
+        return shared
+
+    def _shared_graph(self, gsize: int):
+        """Descriptor of the graph of a size for steps that share prefixes, captured when it is asked for a third time."""
         key = (gsize, "shared")
         if key not in self.graphs:
             self._shared_asked[gsize] = self._shared_asked.get(gsize, 0) + 1
@@ -836,12 +845,7 @@ class ModelRunner:
         gsize = self._graph_size_for(B) if decode_only else None
         if gsize is not None and self._lora_step_needs_eager(so):
             gsize = None
-        shared = None
-        if decode_only:
-            self._find_shared(so)
-            if so.shared_groups:
-                shared = self._shared_graph(gsize)
-                gsize = gsize if shared is not None else None
+        shared = self._shared_step(so, gsize) if decode_only else None
         meta, T, Tp, sel, sample_reqs = self._prepare_inputs(so, pad_to=gsize)
         t_prep = time.perf_counter()
         if gsize is not None:
@@ -920,10 +924,7 @@ class ModelRunner:
         decode_only = all(n == 1 for _, n in so.scheduled)
         gsize, shared = (self._graph_size_for(len(so.scheduled)), None) if decode_only else (None, None)
         if so.shared_groups:
-            self._find_shared(so)
-            if so.shared_groups:
-                shared = self._shared_graph(gsize)
-                gsize = gsize if shared is not None else None
+            shared = self._shared_step(so, gsize)
         meta, T, Tp, _, _ = self._prepare_inputs(so, pad_to=gsize)
         if gsize is not None:
             hidden = self.graph_wrapper.replay(shared or self.graphs[(gsize, False)])
@@ -1004,12 +1005,7 @@ class ModelRunner:
         gsize = self._graph_size_for(B) if decode_only else None
         if gsize is not None and self._lora_step_needs_eager(so):
             gsize = None
-        shared = None
-        if decode_only:
-            self._find_shared(so)
-            if so.shared_groups:
-                shared = self._shared_graph(gsize)
-                gsize = gsize if shared is not None else None
+        shared = self._shared_step(so, gsize) if decode_only else None
         ev_start = None
         if self._step_timing:
             # device-side account of the step: time between the first and the last GPU operation of
