@@ -672,4 +672,6 @@ class EngineConfig:
     enable_lora: bool = False
     max_loras: int = 4
     max_lora_rank: int = 64
-    disable_cascade_attn: bool = True       # False: decode batches with a common prefix read it once (beam search always may)
+    # False: decode batches read a prefix that all their sequences have in common once (beam search always may): grouped-query attention in bf16
+    # without windows, one GPU, no drafts or adapters.  A batch with one sequence of another prefix is read by sequences.
+    disable_cascade_attn: bool = True

@@ -18,6 +18,7 @@ import torch
 from .. import _native, envs
 from ..config import (CacheConfig, CompilationConfig, EngineConfig, ModelConfig, ParallelConfig,
                       SchedulerConfig, get_model_config)
+from ..logger import logger
 from ..parallel import state as pstate
 from .model_runner import ModelRunner
 from .request import (CompletionOutput, Request, RequestMetrics, RequestOutput, RequestStatus,
@@ -86,6 +87,9 @@ class LLMEngine:
                                      and pc.pipeline_parallel_size == 1
                                      and pc.prefill_context_parallel_size == 1)
         self.runner.capture_graphs()
+        if not cfg.disable_cascade_attn and not self.runner.can_share_prefixes():
+            logger.warning("disable_cascade_attn=False: this engine reads every common prefix for itself (prefixes are shared by grouped-query attention in "
+                           "bf16 without windows, on one GPU, without drafts or adapters)")
         self._req_counter = itertools.count()
         self.eos_token_id: Optional[int] = None
         self.step_times: list[float] = []
