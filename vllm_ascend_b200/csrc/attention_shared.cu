@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const PlanArgs a) {
       b.key_lo = lo;
       b.q_pos0 = group ? ctx : ctx + i * per;
       b.key_hi = group ? hi : min(hi, b.q_pos0 + b.ntok);
-      b.tiles = b.key_hi > lo ? ((b.key_hi + 127) >> 7) - (lo >> 7) : 0;
+      b.tiles = b.key_hi > lo ? (int)(((unsigned)b.key_hi + 127) >> 7) - (lo >> 7) : 0;
       b.weight = b.ntok > per / 2 ? COST_PAIR : COST_TILE;
       b.cum = b.part_row = b.seg0 = b.pad = 0;
       bases[at] = b;
