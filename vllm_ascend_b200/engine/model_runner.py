@@ -440,10 +440,6 @@ class ModelRunner:
     def _prepare_inputs(self, so: SchedulerOutput, pad_to: Optional[int] = None):
         from ..profiler import nvtx_range
         with nvtx_range("prepare_inputs"):
-            # The copies of the step before run behind what was launched ahead of them: steps that nobody waits for (portions of a prompt) would
-            # find the buffers filled for the next one.
-            if self._inputs_copied is not None:
-                self._inputs_copied.synchronize()
             try:
                 return self._prepare_inputs_impl(so, pad_to)
             finally:
@@ -510,6 +506,10 @@ class ModelRunner:
         Bp = pad_to or B
         Tp = T + (Bp - B)                       # padded rows carry one dummy token each
         h = self
+        # The copies of the step before run behind what was launched ahead of them: steps that nobody waits for (portions of a prompt) would find the
+        # buffers filled for the next one.
+        if self._inputs_copied is not None:
+            self._inputs_copied.synchronize()
         h._h_ids[:T] = torch.from_numpy(ids.astype(np.int64))
         h._h_pos[:T] = torch.from_numpy(pos)
         h._h_slot[:T] = torch.from_numpy(slots)
