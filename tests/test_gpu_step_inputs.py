@@ -9,10 +9,10 @@ from vllm_ascend_b200.config import ModelConfig
 pytestmark = pytest.mark.gpu
 
 
-def _llm(**kw):
+def _llm(max_num_batched_tokens=256, **kw):
     cfg = ModelConfig(name="portions", architecture="Qwen3ForCausalLM", vocab_size=2048, hidden_size=256, intermediate_size=512, num_hidden_layers=2,
                       num_attention_heads=4, num_key_value_heads=2, head_dim=64, qk_norm=True, rope_theta=1e6, dtype="float32")
-    return LLM(cfg, device="cuda", max_model_len=2048, max_num_seqs=8, max_num_batched_tokens=256, num_gpu_blocks_override=200, block_size=64,
+    return LLM(cfg, device="cuda", max_model_len=2048, max_num_seqs=8, max_num_batched_tokens=max_num_batched_tokens, num_gpu_blocks_override=200, block_size=64,
                enforce_eager=True, seed=2, **kw)
 
 
@@ -45,6 +45,13 @@ def test_beams_of_prompts_in_many_portions(monkeypatch, caching):
         # a second time from the prefix cache
         outs.append([llm.beam_search(p, beam_width=3, max_tokens=4, ignore_eos=True) for p in (prompts, [q + [5] for q in prompts])])
     assert outs[0] == outs[1]
+
+
+def test_portions_and_whole_prompts_agree():
+    """Six portions and one: the same scores but for roundings of 32 bits (1e-3 of four tokens' log-probabilities, around 8 each)."""
+    prompts = _prompts(1500)
+    found = [_llm(max_num_batched_tokens=n).beam_search(prompts, beam_width=3, max_tokens=4, ignore_eos=True)[0] for n in (256, 2048)]
+    np.testing.assert_allclose(*[[b["cum_logprob"] for b in best] for best in found], atol=1e-3)
 
 
 @pytest.mark.parametrize("asynchronous", [False, True])

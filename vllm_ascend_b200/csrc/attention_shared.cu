@@ -21,9 +21,9 @@
 // Rows of V that no key of the range stands for are zeroed in shared memory where a product would read them (their
 // probabilities are zero, but 0 x NaN is not); scores of such keys are masked whatever they are.
 // All waits are bounded.
-// Bound by HBM for long prefixes: 8 beams over 60000 keys (32 heads on 8 of 128, pages of 128) 56 us, 4.5 TB/s with beginning, end and join, which take
-// 10 us of every call; 16 prompts of 8 beams over 2000 keys 49 us (128 requests read by themselves: 128).  Many requests behind one prompt are bound by
-// their own keys: 192 over 2048 and 900 127 us, 5.5 TB/s.  Few keys are bound by the chain of a block's first tile, its results and the join: 13 us.
+// Bound by HBM for long prefixes: 8 beams over 60000 keys (64 heads on 8 of 128, pages of 128) 57 us, 4.5 TB/s with beginning, end and join, which take
+// 10 us of every call; 16 prompts of 8 beams over 2000 keys, 32 heads on 8, 50 us (128 requests read by themselves: 128).  Many requests behind one prompt are bound by
+// their own keys: 192 over 2048 and 900 130 us, 5.4 TB/s.  Few keys are bound by the chain of a block's first tile, its results and the join: 14 us.
 #include "common.cuh"
 
 #include <mutex>

@@ -10,11 +10,11 @@
 // its k best, whose last raises the bound for all.  Keys carry the value and, below it, the place: no two are equal, ties go to the
 // lowest place by themselves, and rows of equal values (masked ones) put nothing behind their first into a list.
 // A second kernel, a block a group, adds up the sums of the parts, turns its beams' keys into totals and takes the best by their places in the lists.
-// Parts' sums are added in 64 bits and totals compared in 64: with thousands of candidates, sums of 32 bits would order near ones
+// Threads' and parts' sums are joined in 64 bits and totals compared in 64: with thousands of candidates, sums of 32 bits would order near ones
 // by their rounding.
-// Many rows are bound by the instructions that are issued (three quarters of all places), half of them the walk: 768 rows of 151936 in bf16 take 84 us, 2.8
-// TB/s; 730 of them that are read execute 81000 a row, 48000 in the walk, 16000 where elements reach the bound, the rest before and after.  Few rows are
-// bound by what stands before and behind the walk, 3 and 4 us, and the second kernel, 5: 64 rows 21 us, 4 of 32000 13 us.
+// Many rows are bound by the instructions that are issued (three quarters of all places), half of them the walk: 768 rows of 151936 in bf16 take 85 us, 2.8
+// TB/s; 730 of them that are read execute 82000 a row, 48000 in the walk, 16000 where elements reach the bound, the rest before and after.  Few rows are
+// bound by what stands before and behind the walk, 3 and 4 us, and the second kernel, 5: 64 rows 22 us, 4 of 32000 13 us.
 // Reordering: a thread owns 16 bytes of a row for all beams of a group and loads what they become before it stores the first.
 #include "common.cuh"
 

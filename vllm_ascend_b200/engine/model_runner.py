@@ -128,7 +128,7 @@ class ModelRunner:
         self._inputs_copied = torch.cuda.Event() if self.is_cuda else None      # behind the copies out of the host buffers above
         self.share_prefixes = not cfg.disable_cascade_attn      # look for common prefixes in decode batches
         self._shared_meta = torch.zeros((2, B + 1), dtype=i32, device=device)      # [first sequences; prefix lengths] of groups
-        self._shared_asked: dict[int, int] = {}                 # capture size -> steps that shared prefixes and had no graph
+        self._shared_asked: dict[int, int] = {}                 # capture size -> steps that would share prefixes and had no graph
         # ---- CUDA graphs
         self.graphs: dict[tuple, object] = {}     # (capture size, has_lora) -> BatchDescriptor
         self.graph_wrapper = None
